@@ -40,7 +40,8 @@ enum {
   MOERT_E_RANGE = -5     /* token or index out of range (rust/moe-rt/src/gpu_model.rs:255-257) */
 };
 
-typedef enum { MOERT_F32 = 0, MOERT_Q8_0 = 1, MOERT_Q4_0 = 2 } moert_dtype;
+/* MOERT_F16 is a type of rows (moert_rows), not of matrices. */
+typedef enum { MOERT_F32 = 0, MOERT_Q8_0 = 1, MOERT_Q4_0 = 2, MOERT_F16 = 3 } moert_dtype;
 
 /* Model constants; mirrors `Config` (rust/moe-rt/src/model.rs:14-31). */
 typedef struct {
@@ -372,6 +373,101 @@ int moert_attn_decode(const float* q, const uint16_t* k_cache, const uint16_t* v
 int moert_attn_decode_noalloc(const float* q_dev, const uint16_t* k_cache_dev, const uint16_t* v_cache_dev, int heads,
                               int kv_heads, int head_dim, int max_len, int len, float scale, int tiles_per_split,
                               float* out_dev, void* stream);
+
+/* ---------------------------------------------------------------------------------------------------------
+ * 8-bit K/V cache of one layer, in the caller's device buffers (no reference counterpart: the reference's cache, like
+ * moert_model's, is fp16 and as long as the sequence). Rows are appended, attended to and read back; where a cache is
+ * to stay within a budget, attention keeps the weight that each block of it gets and moert_kv8_evict drops the blocks
+ * that got least. Half the bytes of an fp16 cache per position and step.
+ *
+ * What it holds. Positions go in blocks of 32 (MOERT_KV8_BLOCK). A row enters rounded to fp16 (to nearest, ties to
+ * even). When a block of a KV head has its 32 rows, it is coded once, K and V apart: scale = a / 127 in f32, a the
+ * largest magnitude of the block's 32 x head_dim values (1 where a is 0), code = round(x / scale), ties to even, of
+ * the exact quotient; the value it stands for is code * scale. The rows of the block that is not full yet, the tail,
+ * stay in fp16. So the cache does not depend on how its rows were spread over calls. A value that is not finite in
+ * fp16 makes its row (in the tail) or its whole block (once coded) NaN to every position that sees any of it, and to
+ * no other.
+ *
+ * Buffers, all of the device, slots = max_len / 32:
+ *   k_codes, v_codes  u8  [seqs][kv_heads][slots][32 * head_dim]  code + 128. K: [position][element]. V: with
+ *                         U = head_dim / 16, position t and element e at
+ *                         ((e / U * 4 + t % 16 / 4) * U + e % U) * 8 + t % 4 + 4 * (t / 16)
+ *   k_scale, v_scale  f32 [seqs][kv_heads][slots]
+ *   k_tail, v_tail    fp16 [seqs][kv_heads][32 * head_dim], in the orders of the codes
+ *   tail_bad          u32 [seqs][kv_heads]  bit t: row t of the tail is not finite
+ *   table             i32 [seqs][kv_heads][slots]  slot of each block, in order: a permutation of the slots, the
+ *                         blocks in use first (the tail's among them)
+ *   mass              f32 [seqs][kv_heads][slots]  by slot; may be NULL where no call tracks or evicts
+ *   state             i32 [seqs][4]  rows of the sequence, rows dropped for want of room, 0, 0
+ * moert_kv8_clear makes them an empty cache. Lengths are on the device, so that a captured graph of these calls can be
+ * replayed: each replay goes on from the lengths it finds. The buffers may be copied and put back as a whole. Kernels
+ * keep to the buffers whatever table and state hold.
+ *
+ * Limits: head_dim 64 or 128; max_len a multiple of 32, at most 2^20; at most 65535 sequences, 256 KV heads. Calls
+ * take sequences [seq0, seq0 + n_seqs). They enqueue on `stream` (a hipStream_t of the buffers' device, NULL for its
+ * default stream), allocate nothing and do not synchronise, except moert_kv8_lengths. Calls on one cache are ordered
+ * by the caller (one stream, or events); attentions that do not track may overlap, each with a workspace of its own.
+ * ------------------------------------------------------------------------------------------------------- */
+enum { MOERT_KV8_BLOCK = 32 };
+typedef struct {
+  int seqs, kv_heads, head_dim, max_len;
+  uint8_t *k_codes_dev, *v_codes_dev;
+  float *k_scale_dev, *v_scale_dev;
+  uint16_t *k_tail_dev, *v_tail_dev;
+  uint32_t* tail_bad_dev;
+  int* table_dev;
+  float* mass_dev;
+  int* state_dev;
+} moert_kv8;
+
+/* Rows in device memory: element e of head h of position i of the call's sequence s lies at
+ * data[s * seq_stride + i * pos_stride + h * head_stride + e]. Strides are in elements; MOERT_F32 or MOERT_F16, the
+ * pointer aligned to the element. Rows that a call writes must not overlap each other. */
+typedef struct {
+  void* data_dev;
+  int dtype;
+  long long seq_stride, pos_stride, head_stride;
+} moert_rows;
+
+/* Empties the sequences: length 0, blocks in order, no mass. */
+int moert_kv8_clear(const moert_kv8* c, int seq0, int n_seqs, void* stream);
+
+/* Appends n rows of each KV head to every sequence (1 <= n <= max_len). A sequence without room for its n rows stays
+ * as it is; moert_kv8_lengths reports it. */
+int moert_kv8_append(const moert_kv8* c, int seq0, int n_seqs, const moert_rows* k, const moert_rows* v, int n,
+                     void* stream);
+
+/* Bytes of workspace that an attention of n positions of `heads` query heads over n_seqs sequences needs (track: one
+ * that adds to the mass). Nothing in it has to be kept or cleared between calls. */
+int moert_kv8_workspace(const moert_kv8* c, int n_seqs, int heads, int n, int track, size_t* bytes);
+
+/* Attention of n positions over the cache, whose last n rows are theirs (appended before): position i of a sequence of
+ * len rows sees the first len - n + 1 + i of them, and query head h reads KV head h / (heads / kv_heads).
+ * out = sum_t p_t v_t, p = softmax(scale * q . k); a position that sees no row gets 0. q and out are of one type:
+ * scores, weights and sums are f32 for both; with MOERT_F16 the weights enter the second product rounded to fp16, with
+ * MOERT_F32 as the sum of two fp16 (22 bits).
+ * mass_decay in [0, 1] tracks: mass = mass_decay * mass + w for every block in use, w the sum of the block's p over
+ * the n positions and the group's query heads (NaN for what a position sees if it sees a value that is not finite).
+ * A negative mass_decay does not track. ws: moert_kv8_workspace bytes, aligned
+ * to 16. */
+int moert_kv8_attend(const moert_kv8* c, int seq0, int n_seqs, int heads, int n, float scale, const moert_rows* q,
+                     const moert_rows* out, float mass_decay, void* ws_dev, size_t ws_bytes, void* stream);
+
+/* Drops blocks of every sequence that has more than `keep` full ones, until it has `keep`: each KV head keeps its
+ * first `first` and last `last` full blocks (first + last <= keep), and of the others those with the largest mass (the
+ * earlier one among equals; NaN counts as more than any number). The tail stays. What stays keeps its order, and its
+ * codes are not touched: the table's entries move, those of the dropped blocks behind the tail's, and the dropped
+ * blocks' mass becomes 0. */
+int moert_kv8_evict(const moert_kv8* c, int seq0, int n_seqs, int keep, int first, int last, void* stream);
+
+/* The values that the cache holds for positions [pos, pos + n) of every sequence, each KV head's in its own order
+ * after evictions; a negative pos counts from the sequence's end. Positions that a sequence does not have give 0. */
+int moert_kv8_read(const moert_kv8* c, int seq0, int n_seqs, int pos, int n, const moert_rows* k, const moert_rows* v,
+                   void* stream);
+
+/* Lengths of the sequences, once the stream has come to this call (synchronises it; not under capture).
+ * MOERT_E_FULL, with the lengths, where rows were dropped since the sequence was cleared. */
+int moert_kv8_lengths(const moert_kv8* c, int seq0, int n_seqs, int* lengths, void* stream);
 
 /* Achievable HBM bandwidth reference: mean microseconds of one device-to-device streaming copy of `bytes`
  * (multiple of 16) over `iters` launches, each timed by its own dispatch events. No reference counterpart (the

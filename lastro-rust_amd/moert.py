@@ -21,7 +21,7 @@ from typing import List, Optional
 
 import numpy as np
 
-F32, Q8_0, Q4_0 = 0, 1, 2
+F32, Q8_0, Q4_0, F16 = 0, 1, 2, 3  # F16: a type of rows (Kv8), not of matrices
 DTYPE_NAMES = {F32: "f32", Q8_0: "q8_0", Q4_0: "q4_0"}
 
 (K_EMBED, K_QKV, K_ATTN_SPLIT, K_ATTN_COMBINE, K_OPROJ, K_ROUTE_UP, K_EXPERT_DOWN, K_HEAD,
@@ -95,6 +95,17 @@ class moert_model_weights(ctypes.Structure):
                 ("layers", ctypes.POINTER(moert_layer_weights))]
 
 
+class moert_kv8(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int) for n in ("seqs", "kv_heads", "head_dim", "max_len")] + \
+               [(n + "_dev", ctypes.c_void_p) for n in
+                ("k_codes", "v_codes", "k_scale", "v_scale", "k_tail", "v_tail", "tail_bad", "table", "mass", "state")]
+
+
+class moert_rows(ctypes.Structure):
+    _fields_ = [("data_dev", ctypes.c_void_p), ("dtype", ctypes.c_int), ("seq_stride", ctypes.c_longlong),
+                ("pos_stride", ctypes.c_longlong), ("head_stride", ctypes.c_longlong)]
+
+
 _lib = None
 
 
@@ -162,6 +173,13 @@ def lib() -> ctypes.CDLL:
             "moert_rope": (i, [vp, i, i, f, i]),
             "moert_attn_decode": (i, [vp, vp, vp, i, i, i, i, i, f, i, vp]),
             "moert_attn_decode_noalloc": (i, [vp, vp, vp, i, i, i, i, i, f, i, vp, vp]),
+            "moert_kv8_clear": (i, [vp, i, i, vp]),
+            "moert_kv8_append": (i, [vp, i, i, vp, vp, i, vp]),
+            "moert_kv8_workspace": (i, [vp, i, i, i, i, ctypes.POINTER(sz)]),
+            "moert_kv8_attend": (i, [vp, i, i, i, i, f, vp, vp, f, vp, sz, vp]),
+            "moert_kv8_evict": (i, [vp, i, i, i, i, i, vp]),
+            "moert_kv8_read": (i, [vp, i, i, i, i, vp, vp, vp]),
+            "moert_kv8_lengths": (i, [vp, i, i, vp, vp]),
             "moert_exp_device": (i, [vp, vp, i]),
             "moert_copy_probe": (i, [sz, i, ctypes.POINTER(ctypes.c_double)]),
             "moert_read_probe": (i, [sz, i, ctypes.POINTER(ctypes.c_double)]),
@@ -235,7 +253,8 @@ EXPORTED = ["moert_last_error", "moert_device_info", "moert_model_create", "moer
             "moert_block_forward", "moert_block_time", "moert_block_forward_batched",
             "moert_block_experts_in_step", "moert_block_batched_kernel", "moert_block_fault_inject", "moert_block_time_batched", "moert_router_topk", "moert_argmax", "moert_gemv",
             "moert_dequant", "moert_rmsnorm", "moert_rope", "moert_attn_decode", "moert_attn_decode_noalloc",
-            "moert_exp_device",
+            "moert_kv8_clear", "moert_kv8_append", "moert_kv8_workspace", "moert_kv8_attend", "moert_kv8_evict",
+            "moert_kv8_read", "moert_kv8_lengths", "moert_exp_device",
             "moert_copy_probe", "moert_read_probe", "moert_h2d_probe", "moert_quantize", "moert_dtype_bytes", "moert_synth_normal", "moert_synth_quantized",
             "moert_synth_fp16", "moert_config_from_json", "moert_checkpoint_open", "moert_checkpoint_close",
             "moert_checkpoint_tensor", "moert_checkpoint_read_bf16", "moert_checkpoint_load", "moert_host_model_weights",
@@ -854,6 +873,95 @@ def attn_decode_noalloc(q_dev: int, k_dev: int, v_dev: int, heads, kv_heads, max
     check(lib().moert_attn_decode_noalloc(ctypes.c_void_p(q_dev), ctypes.c_void_p(k_dev), ctypes.c_void_p(v_dev),
                                           heads, kv_heads, 64, max_len, length, scale, tiles_per_split,
                                           ctypes.c_void_p(out_dev), ctypes.c_void_p(stream)))
+
+
+# ---- 8-bit K/V cache ---------------------------------------------------------------------------------------------
+KV8_BLOCK = 32  # positions of a block
+
+
+def kv8_shapes(seqs: int, kv_heads: int, head_dim: int, max_len: int) -> dict:
+    """The buffers of an 8-bit K/V cache (moert_kv8): name -> (shape, numpy dtype)."""
+    head, slots = (seqs, kv_heads), max_len // KV8_BLOCK
+    block = (KV8_BLOCK, head_dim)
+    return {"k_codes": (head + (slots,) + block, np.uint8), "v_codes": (head + (slots,) + block, np.uint8),
+            "k_scale": (head + (slots,), np.float32), "v_scale": (head + (slots,), np.float32),
+            "k_tail": (head + block, np.uint16), "v_tail": (head + block, np.uint16),
+            "tail_bad": (head, np.uint32), "table": (head + (slots,), np.int32),
+            "mass": (head + (slots,), np.float32), "state": ((seqs, 4), np.int32)}
+
+
+class Kv8:
+    """8-bit K/V cache of one layer over the caller's device buffers (moert_kv8_*): `buffers` gives the device address
+    of each name of kv8_shapes (mass may be left out where nothing tracks or evicts). Rows, queries and outputs are
+    device addresses too, of `dtype` F32 or F16, laid out [sequence, position, head, element] or with `strides`
+    (elements between sequences, positions and heads). Calls enqueue on `stream` (a hipStream_t address, 0 = default
+    stream) and take sequences [seq0, seq0 + n_seqs), all of them by default."""
+
+    def __init__(self, seqs: int, kv_heads: int, head_dim: int, max_len: int, buffers: dict):
+        names = [n[:-4] for n, _ in moert_kv8._fields_[4:]]
+        unknown = set(buffers) - set(names)
+        if unknown:
+            raise ValueError(f"no such buffers: {sorted(unknown)}")
+        self.seqs, self.kv_heads, self.head_dim, self.max_len = seqs, kv_heads, head_dim, max_len
+        self._c = moert_kv8(seqs, kv_heads, head_dim, max_len, *[buffers.get(n) for n in names])
+        self._p = ctypes.addressof(self._c)
+        self._lib = lib()
+
+    def _n(self, seq0, n_seqs):
+        return self.seqs - seq0 if n_seqs is None else n_seqs
+
+    def _rows(self, at, dtype, strides, n, heads):
+        s, p, h = strides or (n * heads * self.head_dim, heads * self.head_dim, self.head_dim)
+        return moert_rows(at, dtype, s, p, h)
+
+    def clear(self, seq0: int = 0, n_seqs: Optional[int] = None, stream: int = 0) -> None:
+        """Empties the sequences."""
+        check(self._lib.moert_kv8_clear(self._p, seq0, self._n(seq0, n_seqs), stream))
+
+    def append(self, k: int, v: int, n: int, dtype: int = F32, strides: Optional[tuple] = None, seq0: int = 0,
+               n_seqs: Optional[int] = None, stream: int = 0) -> None:
+        """Appends n rows of each KV head to every sequence; one without room for them stays as it is."""
+        kr = self._rows(k, dtype, strides, n, self.kv_heads)
+        vr = self._rows(v, dtype, strides, n, self.kv_heads)
+        check(self._lib.moert_kv8_append(self._p, seq0, self._n(seq0, n_seqs), ctypes.addressof(kr),
+                                         ctypes.addressof(vr), n, stream))
+
+    def workspace(self, heads: int, n: int = 1, n_seqs: Optional[int] = None, track: bool = False) -> int:
+        """Bytes of workspace of an attention of n positions."""
+        b = ctypes.c_size_t(0)
+        check(self._lib.moert_kv8_workspace(self._p, self._n(0, n_seqs), heads, n, int(track), ctypes.byref(b)))
+        return b.value
+
+    def attend(self, q: int, out: int, heads: int, n: int, scale: float, ws: int, ws_bytes: int, dtype: int = F32,
+               q_strides: Optional[tuple] = None, out_strides: Optional[tuple] = None,
+               mass_decay: Optional[float] = None, seq0: int = 0, n_seqs: Optional[int] = None,
+               stream: int = 0) -> None:
+        """Attention of the last n positions of every sequence, each over its row and those before it; with mass_decay
+        the weights that the blocks get are added to the decayed mass."""
+        qr = self._rows(q, dtype, q_strides, n, heads)
+        orow = self._rows(out, dtype, out_strides, n, heads)
+        check(self._lib.moert_kv8_attend(self._p, seq0, self._n(seq0, n_seqs), heads, n, scale, ctypes.addressof(qr),
+                                         ctypes.addressof(orow), -1.0 if mass_decay is None else mass_decay, ws,
+                                         ws_bytes, stream))
+
+    def evict(self, keep: int, first: int = 0, last: int = 0, seq0: int = 0, n_seqs: Optional[int] = None,
+              stream: int = 0) -> None:
+        """Keeps `keep` full blocks of each head: the first `first`, the last `last` and those with the most mass."""
+        check(self._lib.moert_kv8_evict(self._p, seq0, self._n(seq0, n_seqs), keep, first, last, stream))
+
+    def read(self, k: int, v: int, pos: int, n: int, dtype: int = F32, strides: Optional[tuple] = None, seq0: int = 0,
+             n_seqs: Optional[int] = None, stream: int = 0) -> None:
+        """The values held for positions [pos, pos + n) (negative: from each sequence's end), 0 where there are none."""
+        kr = self._rows(k, dtype, strides, n, self.kv_heads)
+        vr = self._rows(v, dtype, strides, n, self.kv_heads)
+        check(self._lib.moert_kv8_read(self._p, seq0, self._n(seq0, n_seqs), pos, n, ctypes.addressof(kr),
+                                       ctypes.addressof(vr), stream))
+
+    def lengths(self, seq0: int = 0, n_seqs: Optional[int] = None, stream: int = 0) -> np.ndarray:
+        """Lengths of the sequences (synchronises the stream); raises E_FULL where rows were dropped."""
+        out = np.empty(max(1, self._n(seq0, n_seqs)), np.int32)
+        check(self._lib.moert_kv8_lengths(self._p, seq0, self._n(seq0, n_seqs), ptr(out), stream))
+        return out
 
 
 def exp_device(x: np.ndarray) -> np.ndarray:
