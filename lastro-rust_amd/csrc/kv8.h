@@ -47,7 +47,7 @@ __device__ __forceinline__ int kv_slot(const Kv8Dev& c, int raw) {
 
 struct KvAttnPlan {
   int splits;         // workgroups of a column tile along the cache, at most
-  size_t parts, lse;  // offsets of the workspace's parts
+  size_t tot, ml, parts, lse;  // offsets of the parts of the workspace
   size_t bytes;
 };
 KvAttnPlan kv8_attn_plan(const Kv8Dev& c, int n_seqs, int heads, int n, bool track);

@@ -1,7 +1,20 @@
-// Attention over the 8-bit K/V cache (kv8.h). A simple form: a wave per position and query head goes through the rows
-// block by block, 32 scores at a time (lane t: row t), with a running maximum and sum; then each lane takes its
-// elements of the output. The weights of the blocks for the mass: log2 of each block's sum by column (a column is one
-// query head at one position), and of the column's whole sum; k_kv8_mass adds them up in order.
+// Attention over the 8-bit K/V cache (kv8.h), on the f16 matrix cores with f32 sums.
+//
+// A column is one query head at one position; the columns of a KV head, position by position, go in tiles of 16, NT of
+// them to a wave. Per block of 32 positions of the cache:
+//   S = K Q^T    MFMA 16x16x32, rows = 16 positions, columns = 16 columns. Codes become fp16 exactly (two bytes become
+//                1024 + byte by one byte permutation, one packed subtraction takes 1152 off). A lane of group
+//                G = lane / 16 reads 16 bytes of K row lane % 16, from element 16 G on.
+//   softmax      u = s scale log2 e in base 2; the running maximum M of u + log2(scale of V) moves only when it has to
+//                (by more than 8), so most blocks cost no exchange between lanes. p = 2^(u + log2 vs - M + 7): the
+//                weights that meet the V codes carry the scale of V, so blocks of any scale add up in one accumulator,
+//                and the largest contribution lies between 2^7 and 2^15, where fp16 has 11 bits down to 2^-21 of it.
+//                The sum of softmax takes p / vs, in f32.
+//   O += V^T P^T MFMA 16x16x32 over the 32 positions: rows = 16 elements, columns = columns. A lane of the S product
+//                holds positions 4 G .. 4 G + 3 of both halves of the block for its column, which is what it has to
+//                hold of P here when the positions of V are taken in that order: v_place lays V out so, and p never
+//                leaves its lane.
+// f32 queries enter as two fp16 (their row scaled by a power of two to below 2^10), f32 outputs take p as two fp16.
 #include "kv8.h"
 #include "launch.h"
 
@@ -9,112 +22,451 @@ namespace moert {
 
 namespace {
 
-constexpr float kLog2e = 1.44269504088896341f;
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+typedef float f4 __attribute__((ext_vector_type(4)));
 
-__device__ __forceinline__ float q_elem(const KvRows& r, long long at) {
+constexpr float kLog2e = 1.44269504088896341f;
+constexpr int kWaves = 4;       // waves of a workgroup, each its share of the blocks
+constexpr int kMinBlocks = 4;   // blocks of a split, at least
+constexpr int kMaxSplits = 64;  // one lane each in the combine
+constexpr float kShift = 7.0f, kSlack = 8.0f;
+
+__device__ __forceinline__ f4 mfma(h8 a, h8 b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+
+// Eight codes + 128 as fp16: 0x64bb is 1024 + bb.
+__device__ __forceinline__ h8 half_codes(uint32_t a, uint32_t b) {
+  union {
+    uint32_t w[4];
+    h2 x[4];
+    h8 v;
+  } r;
+  r.w[0] = __builtin_amdgcn_perm(0x64646464u, a, 0x04010400u);
+  r.w[1] = __builtin_amdgcn_perm(0x64646464u, a, 0x04030402u);
+  r.w[2] = __builtin_amdgcn_perm(0x64646464u, b, 0x04010400u);
+  r.w[3] = __builtin_amdgcn_perm(0x64646464u, b, 0x04030402u);
+  const h2 off = {(_Float16)1152.0f, (_Float16)1152.0f};
+#pragma unroll
+  for (int i = 0; i < 4; i++) r.x[i] -= off;
+  return r.v;
+}
+
+__device__ __forceinline__ float row_f32(const KvRows& r, long long at) {
   return r.f16 ? h2f(gmem((const uint16_t*)r.p)[at]) : gmem((const float*)r.p)[at];
 }
 
-template <int D>
-__global__ __launch_bounds__(64) void k_kv8_simple(Kv8Dev c, KvRows q, KvRows out, int seq0, int heads, int n,
-                                                   float scale, float* __restrict__ lse, float* __restrict__ tot) {
-  __shared__ float Q[D], P[kKvBlock];
-  const int g = heads / c.kvh, lane = threadIdx.x;
-  const int hq = blockIdx.x % heads, i = blockIdx.x / heads, sc = blockIdx.y, s = seq0 + sc, h = hq / g;
-  const int len = kv_len(c, s), sees = len - n + 1 + i;
-  const size_t head = (size_t)s * c.kvh + h;
-  const size_t col = ((size_t)sc * c.kvh + h) * n * g + (size_t)i * g + hq % g;
-  for (int e = lane; e < D; e += 64) Q[e] = q_elem(q, sc * q.seq + i * q.pos + hq * q.head + e);
-  __syncthreads();
-  float m = -1e30f, l = 0.0f, o[D / 64] = {};
-  const uint32_t bad = c.bad[head];
-  for (int b = 0; b * kKvBlock < sees; b++) {
-    const bool tail = b == len / kKvBlock;
-    const size_t slot = head * c.slots + kv_slot(c, c.table[head * c.slots + b]);
-    const float ks = tail ? 1.0f : c.ks[slot], vs = tail ? 1.0f : c.vs[slot];
-    const int t = lane % kKvBlock;
-    const bool in = b * kKvBlock + t < sees;
-    float x = 0.0f;
-    for (int e = 0; e < D; e++) {
-      const float k = tail ? h2f(c.kt[head * kKvBlock * D + t * D + e])
-                           : (float)((int)c.kc[slot * (kKvBlock * D) + t * D + e] - 128);
-      x = __builtin_fmaf(Q[e], k, x);
-    }
-    x = x * (ks * (scale * kLog2e)) + 0.0f * vs;  // a block whose V is not finite has no weights either
-    if (tail && (bad >> t & 1)) x = __int_as_float(0x7fc00000);
-    const float mn = __builtin_fmaxf(m, group_max(in && x == x ? x : -1e30f)), a = __builtin_amdgcn_exp2f(m - mn);
-    const float p = in ? __builtin_amdgcn_exp2f(x - mn) : 0.0f;
-    const float sum = group_sum<32>(p);
-    m = mn;
-    l = __builtin_fmaf(l, a, sum);
-    if (lse && lane == 0) lse[col * c.slots + b] = __builtin_amdgcn_logf(sum) + m;
-    if (lane < kKvBlock) P[t] = p;
-    __syncthreads();
-#pragma unroll
-    for (int j = 0; j < D / 64; j++) {
-      float y = 0.0f;
-      for (int t = 0; t < kKvBlock && b * kKvBlock + t < sees; t++) {
-        const int at = v_place<D>(t, j * 64 + lane);
-        const float v = tail ? h2f(c.vt[head * kKvBlock * D + at])
-                             : (float)((int)c.vc[slot * (kKvBlock * D) + at] - 128);
-        y = __builtin_fmaf(P[t], v, y);
-      }
-      o[j] = __builtin_fmaf(o[j], a, y * vs);
-    }
-    __syncthreads();
-  }
-  for (int j = 0; j < D / 64; j++) {
-    const float y = l == 0.0f ? 0.0f : o[j] / l;
-    const long long at = sc * out.seq + i * out.pos + hq * out.head + j * 64 + lane;
-    if (out.f16) ((uint16_t*)out.p)[at] = f2h(y);
-    else ((float*)out.p)[at] = y;
-  }
-  if (tot && lane == 0) tot[col] = l == 0.0f ? __int_as_float(0x7f800000) : __builtin_amdgcn_logf(l) + m;
+// The part of the cache that a split of a column tile goes through: blocks [lo, hi) of those that the tile's last
+// position sees. `used` splits have any.
+struct Range {
+  int lo, hi, used;
+};
+__device__ __forceinline__ Range range_of(int len, int n, int g, int tile, int width, int splits, int split) {
+  const int last = min((tile + 1) * width - 1, n * g - 1) / g;  // last position of the tile
+  const int sees = max(0, len - n + 1 + last), nb = (sees + kKvBlock - 1) / kKvBlock;
+  const int chunk = max((nb + splits - 1) / splits, kMinBlocks);
+  Range r;
+  r.used = max(1, (nb + chunk - 1) / chunk);
+  r.lo = min(nb, split * chunk);
+  r.hi = min(nb, r.lo + chunk);
+  return r;
 }
 
-// mass = decay * mass + the block's weights, a thread per block.
-__global__ void k_kv8_mass(Kv8Dev c, int seq0, int g, int n, float decay, const float* __restrict__ lse,
-                           const float* __restrict__ tot) {
-  const int sc = blockIdx.z, h = blockIdx.y, s = seq0 + sc, b = blockIdx.x * blockDim.x + threadIdx.x;
-  const int len = kv_len(c, s);
-  if (b * kKvBlock >= len) return;
-  const size_t head = (size_t)s * c.kvh + h, col0 = ((size_t)sc * c.kvh + h) * n * g;
-  float w = 0.0f;
-  for (int i = 0; i < n; i++) {
-    if (b * kKvBlock >= len - n + 1 + i) continue;
-    for (int j = 0; j < g; j++) {
-      const size_t col = col0 + (size_t)i * g + j;
-      w += __builtin_amdgcn_exp2f(lse[col * c.slots + b] - tot[col]);
+struct AttnArgs {
+  Kv8Dev c;
+  KvRows q, out;
+  int seq0, n_seqs, g, n, splits, tiles;
+  float kf;       // |scale| log2 e
+  uint32_t sign;  // of the scale
+  float* part;    // [sequence, KV head, column][split][D]
+  float2* ml;     // [sequence, KV head, column][split]: M - 7, sum
+  float* tot;     // [sequence, KV head, column]: log2 of the whole sum, +inf where nothing is seen
+  float* lse;     // [sequence, KV head][block][column]: log2 of the block's sum
+};
+
+template <int D, bool F16, int NT, bool TRACK>
+__global__ __launch_bounds__(kWaves * 64) void k_kv8_attend(AttnArgs a) {
+  constexpr int KS = D / 32, U = D / 16, CH = D / 64, W = 16 * NT;
+  constexpr int PF = 2;  // blocks in flight
+  __shared__ __align__(16) float Os[kWaves][16][D + 4];
+  __shared__ float2 Ms[kWaves][16];
+  const Kv8Dev& c = a.c;
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int col16 = lane & 15, G = lane >> 4;
+  // the tiles that read the same blocks run on the same XCD (workgroups go round them in turn)
+  const int id = blockIdx.x, unit = id / 8 / a.tiles * 8 + id % 8, tile = id / 8 % a.tiles;
+  if (unit >= a.n_seqs * c.kvh * a.splits) return;
+  const int split = unit % a.splits, hs = unit / a.splits, h = hs % c.kvh, sc = hs / c.kvh, s = a.seq0 + sc;
+  const int len = kv_len(c, s), cols = a.n * a.g;
+  const Range rg = range_of(len, a.n, a.g, tile, W, a.splits, split);
+  if (split >= rg.used) return;
+  const size_t head = (size_t)s * c.kvh + h;
+  const size_t col0 = (size_t)hs * cols;  // of the workspace's columns
+
+  // queries and the rows that each column sees
+  h8 qh[NT][KS], ql[NT][F16 ? 1 : KS];
+  float kf[NT];
+  int sees[NT];
+#pragma unroll
+  for (int t = 0; t < NT; t++) {
+    const int col = tile * W + t * 16 + col16, cc = min(col, cols - 1), i = cc / a.g;
+    sees[t] = len - a.n + 1 + i;
+    const long long at = sc * a.q.seq + i * a.q.pos + (long long)(h * a.g + cc % a.g) * a.q.head;
+    float x[KS][8];
+#pragma unroll
+    for (int k = 0; k < KS; k++)
+#pragma unroll
+      for (int j = 0; j < 8; j++)
+        x[k][j] = __uint_as_float(__float_as_uint(row_f32(a.q, at + (k >> 1) * 64 + G * 16 + (k & 1) * 8 + j)) ^ a.sign);
+    kf[t] = a.kf;
+    if constexpr (!F16) {
+      float m = 0.0f;
+#pragma unroll
+      for (int k = 0; k < KS; k++)
+#pragma unroll
+        for (int j = 0; j < 8; j++) m = __builtin_fmaxf(m, __builtin_fabsf(x[k][j]));
+      m = max_stage<16>(m);
+      m = max_stage<32>(m);
+      const int e = m > 0.0f && m < __int_as_float(0x7f800000) ? __builtin_amdgcn_frexp_expf(m) : 0;
+      // 2^(10 - e) in two factors: either alone could leave the type
+      const int e1 = (10 - e) / 2, e2 = 10 - e - e1;
+#pragma unroll
+      for (int k = 0; k < KS; k++)
+#pragma unroll
+        for (int j = 0; j < 8; j++) x[k][j] = __builtin_amdgcn_ldexpf(__builtin_amdgcn_ldexpf(x[k][j], e1), e2);
+      kf[t] = __builtin_amdgcn_ldexpf(a.kf, e - 10);
+    }
+#pragma unroll
+    for (int k = 0; k < KS; k++)
+#pragma unroll
+      for (int j = 0; j < 8; j++) {
+        const _Float16 hi = (_Float16)x[k][j];
+        qh[t][k][j] = hi;
+        if constexpr (!F16) ql[t][k][j] = (_Float16)(x[k][j] - (float)hi);
+      }
+  }
+  const int sees0 = len - a.n + 1 + min(tile * W, cols - 1) / a.g;  // the least of the tile
+
+  float M[NT], l[NT];
+  f4 O[NT][U];
+#pragma unroll
+  for (int t = 0; t < NT; t++) {
+    M[t] = -1e30f;
+    l[t] = 0.0f;
+#pragma unroll
+    for (int u = 0; u < U; u++) O[t][u] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+  }
+
+  // One block: kop(half, k), vop(u) give the operands, bad the poisoned rows of the tail.
+  auto block = [&](auto kop, auto vop, float ks, float lvs, float ivs, int b, uint32_t bad) {
+    f4 S[NT][2];
+#pragma unroll
+    for (int x = 0; x < 2; x++) {
+#pragma unroll
+      for (int t = 0; t < NT; t++) S[t][x] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int k = 0; k < KS; k++) {
+        const h8 ka = kop(x, k);
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
+          S[t][x] = mfma(ka, qh[t][k], S[t][x]);
+          if constexpr (!F16) S[t][x] = mfma(ka, ql[t][k], S[t][x]);
+        }
+      }
+    }
+    const bool whole = sees0 >= (b + 1) * kKvBlock;  // every column sees all of it
+    float mx[NT];
+    bool move = false;
+#pragma unroll
+    for (int t = 0; t < NT; t++) {
+      const float f = kf[t] * ks;
+      mx[t] = __int_as_float(0xff800000);
+#pragma unroll
+      for (int x = 0; x < 2; x++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          S[t][x][i] *= f;
+          const int row = x * 16 + G * 4 + i;
+          if (!whole) {
+            if (bad >> row & 1) S[t][x][i] = __int_as_float(0x7fc00000);
+            if (b * kKvBlock + row >= sees[t]) S[t][x][i] = __int_as_float(0xff800000);
+          }
+          mx[t] = __builtin_fmaxf(mx[t], S[t][x][i]);
+        }
+      move |= mx[t] + lvs > M[t] + kSlack;
+    }
+    if (__any(move)) {
+#pragma unroll
+      for (int t = 0; t < NT; t++) {
+        const float y = max_stage<32>(max_stage<16>(mx[t])) + lvs;
+        const float mn = y > M[t] ? y : M[t], al = __builtin_amdgcn_exp2f(M[t] - mn);
+        M[t] = mn;
+        l[t] *= al;
+#pragma unroll
+        for (int u = 0; u < U; u++)
+#pragma unroll
+          for (int i = 0; i < 4; i++) O[t][u][i] *= al;
+      }
+    }
+    h8 ph[NT], pl[F16 ? 1 : NT];
+#pragma unroll
+    for (int t = 0; t < NT; t++) {
+      const float c0 = lvs - M[t] + kShift;
+      float sum = 0.0f;
+#pragma unroll
+      for (int x = 0; x < 2; x++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          const float p = __builtin_amdgcn_exp2f(S[t][x][i] + c0);
+          sum += p;
+          const _Float16 hi = (_Float16)p;
+          ph[t][x * 4 + i] = hi;
+          if constexpr (!F16) pl[t][x * 4 + i] = (_Float16)(p - (float)hi);
+        }
+      l[t] = __builtin_fmaf(sum, ivs, l[t]);
+      if constexpr (TRACK) {
+        sum = sum + partner<16>(sum);
+        sum = sum + partner<32>(sum);
+        const int col = tile * W + t * 16 + col16;
+        if (G == 0 && col < cols)
+          a.lse[((size_t)hs * c.slots + b) * cols + col] = __builtin_amdgcn_logf(sum) + (M[t] - kShift - lvs);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      const h8 va = vop(u);
+#pragma unroll
+      for (int t = 0; t < NT; t++) {
+        O[t][u] = mfma(va, ph[t], O[t][u]);
+        if constexpr (!F16) O[t][u] = mfma(va, pl[t], O[t][u]);
+      }
+    }
+  };
+
+  const int full = min(rg.hi, len / kKvBlock);  // blocks that are coded
+  for (int base = rg.lo + w; base < full; base += 64 * kWaves) {
+    // lane x: slot and scales of this wave's x-th block from here
+    const int mine = base + lane * kWaves;
+    const size_t sl = head * c.slots + (mine < full ? kv_slot(c, c.table[head * c.slots + mine]) : 0);
+    const int slot_l = (int)(sl - head * c.slots);
+    // a V that is not finite makes the scores NaN, not the scale: columns that see none of the block are masked there
+    const float vs_r = c.vs[sl], vs_l = vs_r == vs_r ? vs_r : 1.0f, ks_l = vs_r == vs_r ? c.ks[sl] : vs_r;
+    const float lvs_l = __builtin_amdgcn_logf(vs_l), ivs_l = 1.0f / vs_l;
+    const int count = min(64, (full - base + kWaves - 1) / kWaves);
+    uint4 kb[PF][2 * CH], vb[PF][2 * CH];
+    auto fetch = [&](int p, int x) {
+      const int slot = __builtin_amdgcn_readlane(slot_l, min(x, count - 1));
+      const size_t at = (head * c.slots + slot) * (size_t)(kKvBlock * D);
+      const uint8_t* kp = c.kc + at + col16 * D + G * 16;
+      const uint8_t* vp = c.vc + at + (col16 * 4 + G) * (U * 8);
+#pragma unroll
+      for (int y = 0; y < 2; y++)
+#pragma unroll
+        for (int z = 0; z < CH; z++) {
+          kb[p][y * CH + z] = gload_u4(kp + y * 16 * D + z * 64);
+          vb[p][y * CH + z] = gload_u4(vp + (y * CH + z) * 16);
+        }
+    };
+#pragma unroll
+    for (int p = 0; p < PF; p++) fetch(p, p);
+    for (int x = 0; x < count; x += PF) {
+#pragma unroll
+      for (int p = 0; p < PF; p++) {
+        if (x + p < count) {
+          auto kop = [&](int y, int k) {
+            const uint4 v = kb[p][y * CH + (k >> 1)];
+            return k & 1 ? half_codes(v.z, v.w) : half_codes(v.x, v.y);
+          };
+          auto vop = [&](int u) {
+            const uint4 v = vb[p][u >> 1];
+            return u & 1 ? half_codes(v.z, v.w) : half_codes(v.x, v.y);
+          };
+          block(kop, vop, __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(ks_l), x + p)),
+                __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(lvs_l), x + p)),
+                __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(ivs_l), x + p)),
+                base + (x + p) * kWaves, 0u);
+        }
+        fetch(p, x + p + PF);
+      }
     }
   }
+  if (rg.hi > full && (full - rg.lo) % kWaves == w) {  // the tail, in fp16
+    const int r = len % kKvBlock;
+    const uint32_t bad = c.bad[head], use = ~bad & ((1u << r) - 1u);
+    const uint16_t* kt = c.kt + head * kKvBlock * D;
+    const uint16_t* vt = c.vt + head * kKvBlock * D;
+    auto kop = [&](int y, int k) {
+      return *reinterpret_cast<const h8*>(kt + (y * 16 + col16) * D + (k >> 1) * 64 + G * 16 + (k & 1) * 8);
+    };
+    auto vop = [&](int u) {
+      h8 v = *reinterpret_cast<const h8*>(vt + ((col16 * 4 + G) * U + u) * 8);
+#pragma unroll
+      for (int j = 0; j < 8; j++)  // what no row has written, or poison, must not meet a weight of 0
+        v[j] = use >> (G * 4 + (j & 3) + 16 * (j >> 2)) & 1 ? v[j] : (_Float16)0.0f;
+      return v;
+    };
+    block(kop, vop, 1.0f, 0.0f, 1.0f, full, bad);
+  }
+
+  // the waves' shares, tile by tile
+#pragma unroll
+  for (int t = 0; t < NT; t++) {
+    float lt = l[t] + partner<16>(l[t]);
+    lt = lt + partner<32>(lt);
+    if (t) __syncthreads();
+    if (G == 0) Ms[w][col16] = make_float2(M[t], lt);
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+#pragma unroll
+      for (int u = 0; u < U; u += 4)
+        *reinterpret_cast<f4*>(&Os[w][col16][(G * 4 + i) * U + u]) =
+            f4{O[t][u][i], O[t][u + 1][i], O[t][u + 2][i], O[t][u + 3][i]};
+    __syncthreads();
+    const int cl = threadIdx.x >> 4, e0 = (threadIdx.x & 15) * U, col = tile * W + t * 16 + cl;
+    if (col < cols) {
+      float m = Ms[0][cl].x;
+#pragma unroll
+      for (int x = 1; x < kWaves; x++) m = __builtin_fmaxf(m, Ms[x][cl].x);
+      float sum = 0.0f, o[U] = {};
+#pragma unroll
+      for (int x = 0; x < kWaves; x++) {
+        const float al = __builtin_amdgcn_exp2f(Ms[x][cl].x - m);
+        sum = __builtin_fmaf(Ms[x][cl].y, al, sum);
+#pragma unroll
+        for (int e = 0; e < U; e++) o[e] = __builtin_fmaf(Os[x][cl][e0 + e], al, o[e]);
+      }
+      const size_t wc = col0 + col;
+      if (rg.used == 1) {
+        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+        const long long at = sc * a.out.seq + (long long)(col / a.g) * a.out.pos +
+                             (long long)(h * a.g + col % a.g) * a.out.head + e0;
+#pragma unroll
+        for (int e = 0; e < U; e++) {
+          if constexpr (F16) ((uint16_t*)a.out.p)[at + e] = f2h(o[e] * inv);
+          else ((float*)a.out.p)[at + e] = o[e] * inv;
+        }
+        if (TRACK && e0 == 0)
+          a.tot[wc] = sum == 0.0f ? __int_as_float(0x7f800000) : __builtin_amdgcn_logf(sum) + (m - kShift);
+      } else {
+        float* po = a.part + (wc * a.splits + split) * D + e0;
+#pragma unroll
+        for (int e = 0; e < U; e++) po[e] = o[e];
+        if (e0 == 0) a.ml[wc * a.splits + split] = make_float2(m, sum);
+      }
+    }
+  }
+}
+
+// The splits' shares of a column: a workgroup per column, lane x of each wave holds split x's maximum and sum, the waves
+// take every fourth split's sums.
+template <int D, bool F16, bool TRACK>
+__global__ __launch_bounds__(256) void k_kv8_combine(AttnArgs a, int width) {
+  constexpr int E = D / 64;
+  __shared__ float Os[4][D];
+  const Kv8Dev& c = a.c;
+  const int cols = a.n * a.g, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const size_t wc = blockIdx.x;
+  const int col = (int)(wc % cols), hs = (int)(wc / cols), h = hs % c.kvh, sc = hs / c.kvh;
+  const Range rg = range_of(kv_len(c, a.seq0 + sc), a.n, a.g, col / width, width, a.splits, 0);
+  if (rg.used == 1) return;
+  const bool in = lane < rg.used;
+  const float2 x = in ? a.ml[wc * a.splits + lane] : make_float2(-3e38f, 0.0f);
+  const float m = group_max(x.x), al = in ? __builtin_amdgcn_exp2f(x.x - m) : 0.0f, sum = group_sum(x.y * al);
+  float o[E] = {};
+  for (int j = w; j < rg.used; j += 4) {
+    const float aj = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(al), j));
+    const float* po = a.part + (wc * a.splits + j) * D;
+#pragma unroll
+    for (int e = 0; e < E; e++) o[e] = __builtin_fmaf(po[e * 64 + lane], aj, o[e]);
+  }
+#pragma unroll
+  for (int e = 0; e < E; e++) Os[w][e * 64 + lane] = o[e];
+  __syncthreads();
+  if (threadIdx.x < D) {
+    const float y = ((Os[0][threadIdx.x] + Os[1][threadIdx.x]) + (Os[2][threadIdx.x] + Os[3][threadIdx.x])) *
+                    (sum == 0.0f ? 0.0f : 1.0f / sum);
+    const long long at = sc * a.out.seq + (long long)(col / a.g) * a.out.pos +
+                         (long long)(h * a.g + col % a.g) * a.out.head + threadIdx.x;
+    if constexpr (F16) ((uint16_t*)a.out.p)[at] = f2h(y);
+    else ((float*)a.out.p)[at] = y;
+  }
+  if (TRACK && threadIdx.x == 0)
+    a.tot[wc] = sum == 0.0f ? __int_as_float(0x7f800000) : __builtin_amdgcn_logf(sum) + (m - kShift);
+}
+
+// mass = decay * mass + the block's weights, a thread per block, columns in order.
+__global__ __launch_bounds__(256) void k_kv8_mass(AttnArgs a, float decay) {
+  const Kv8Dev& c = a.c;
+  const int sc = blockIdx.z, h = blockIdx.y, s = a.seq0 + sc, b = blockIdx.x * blockDim.x + threadIdx.x;
+  const int len = kv_len(c, s), cols = a.n * a.g;
+  if (b * kKvBlock >= len) return;
+  const size_t head = (size_t)s * c.kvh + h, hs = (size_t)sc * c.kvh + h;
+  const int i0 = max(0, b * kKvBlock - (len - a.n));  // the first position that sees any of the block
+  const float* lse = a.lse + (hs * c.slots + b) * cols;
+  const float* tot = a.tot + hs * cols;
+  float w = 0.0f;
+  for (int col = i0 * a.g; col < cols; col++) w += __builtin_amdgcn_exp2f(lse[col] - tot[col]);
   float* m = c.mass + head * c.slots + kv_slot(c, c.table[head * c.slots + b]);
   *m = __builtin_fmaf(decay, *m, w);
 }
+
+// Tiles of 16 columns of a wave.
+int tile_count(int cols, int d) { return cols <= 16 ? 1 : cols <= 32 || d == 128 ? 2 : 4; }
 
 }  // namespace
 
 KvAttnPlan kv8_attn_plan(const Kv8Dev& c, int n_seqs, int heads, int n, bool track) {
   KvAttnPlan p;
+  const int cols1 = heads / c.kvh * n, nt = tile_count(cols1, c.d), tiles = (cols1 + 16 * nt - 1) / (16 * nt);
   const size_t cols = (size_t)n_seqs * heads * n;
-  p.splits = 1;
-  p.parts = 0;
-  p.lse = (cols * 4 + 255) / 256 * 256;
+  const long long units = (long long)n_seqs * c.kvh * tiles;
+  const int most = (c.slots + kMinBlocks - 1) / kMinBlocks;
+  long long s = (1024 + units - 1) / units;
+  s = s < 1 ? 1 : s > kMaxSplits ? kMaxSplits : s;
+  p.splits = (int)(s > most ? most : s);
+  auto up = [](size_t x) { return (x + 255) / 256 * 256; };
+  p.tot = 0;
+  p.ml = up(cols * 4);
+  p.parts = p.ml + (p.splits > 1 ? up(cols * p.splits * 8) : 0);
+  p.lse = p.parts + (p.splits > 1 ? up(cols * p.splits * c.d * 4) : 0);
   p.bytes = p.lse + (track ? cols * c.slots * 4 : 0);
   return p;
 }
+
+namespace {
+
+template <int D, bool F16, bool TRACK>
+hipError_t attend(hipStream_t s, AttnArgs a, float decay) {
+  const int cols = a.n * a.g, nt = tile_count(cols, D), width = 16 * nt;
+  a.tiles = (cols + width - 1) / width;
+  const long long units = (long long)a.n_seqs * a.c.kvh * a.splits;
+  const long long grid = (units + 7) / 8 * 8 * a.tiles;
+  if (grid > 0x7fffffff) return hipErrorInvalidValue;
+  if (nt == 1) klaunch(k_kv8_attend<D, F16, 1, TRACK>, (unsigned)grid, kWaves * 64, 0, s, a);
+  else if (nt == 2) klaunch(k_kv8_attend<D, F16, 2, TRACK>, (unsigned)grid, kWaves * 64, 0, s, a);
+  else if constexpr (D == 64) klaunch(k_kv8_attend<D, F16, 4, TRACK>, (unsigned)grid, kWaves * 64, 0, s, a);
+  if (a.splits > 1)
+    klaunch(k_kv8_combine<D, F16, TRACK>, (unsigned)((size_t)a.n_seqs * a.c.kvh * cols), 256, 0, s, a, width);
+  if (TRACK)
+    klaunch(k_kv8_mass, dim3((a.c.slots + 255) / 256, a.c.kvh, a.n_seqs), 256, 0, s, a, decay);
+  return hipGetLastError();
+}
+
+}  // namespace
 
 hipError_t launch_kv8_attend(hipStream_t s, const Kv8Dev& c, int seq0, int n_seqs, int heads, int n, float scale,
                              KvRows q, KvRows out, float decay, void* ws) {
   const bool track = decay >= 0.0f;
   const KvAttnPlan p = kv8_attn_plan(c, n_seqs, heads, n, track);
-  float* tot = track ? (float*)ws : nullptr;
-  float* lse = track ? (float*)((char*)ws + p.lse) : nullptr;
-  if (c.d == 64) klaunch(k_kv8_simple<64>, dim3(n * heads, n_seqs), 64, 0, s, c, q, out, seq0, heads, n, scale, lse, tot);
-  else klaunch(k_kv8_simple<128>, dim3(n * heads, n_seqs), 64, 0, s, c, q, out, seq0, heads, n, scale, lse, tot);
-  if (track)
-    klaunch(k_kv8_mass, dim3((c.slots + 255) / 256, c.kvh, n_seqs), 256, 0, s, c, seq0, heads / c.kvh, n, decay, lse,
-            tot);
-  return hipGetLastError();
+  char* w = (char*)ws;
+  AttnArgs a{c, q, out, seq0, n_seqs, heads / c.kvh, n, p.splits, 1, __builtin_fabsf(scale) * kLog2e,
+             scale < 0.0f ? 0x80000000u : 0u, (float*)(w + p.parts), (float2*)(w + p.ml), (float*)(w + p.tot),
+             track ? (float*)(w + p.lse) : nullptr};
+#define ATT(DD, FF) \
+  if (c.d == DD && q.f16 == FF) return track ? attend<DD, FF, true>(s, a, decay) : attend<DD, FF, false>(s, a, decay);
+  ATT(64, 0) ATT(64, 1) ATT(128, 0) ATT(128, 1)
+#undef ATT
+  return hipErrorInvalidValue;
 }
 
 }  // namespace moert
