@@ -8,7 +8,7 @@
 namespace moert {
 
 constexpr int kKvBlock = 32;  // positions of a block
-enum { KV_LEN = 0, KV_DROPPED = 1, KV_STATE = 4 };  // words of a sequence's state
+enum { KV_LEN = 0, KV_DROPPED = 1, KV_ARRIVED = 2, KV_STATE = 4 };  // words of a sequence's state
 
 struct Kv8Dev {
   int seqs, kvh, d, slots, max_len;

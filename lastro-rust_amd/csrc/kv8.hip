@@ -10,128 +10,154 @@ int set_error(int code, const char* fmt, ...);
 
 namespace {
 
-// Rows t < 32 of one block, K or V, as fp16 in LDS: two elements apart from row to row more than the row has, so that
-// a column's elements lie in different banks.
-template <int D>
-struct BlockLds {
-  uint16_t x[kKvBlock][D + 2];
-};
-
-__device__ __forceinline__ uint16_t row_elem(const KvRows& r, long long at) {
-  return r.f16 ? gmem((const uint16_t*)r.p)[at] : f2h(gmem((const float*)r.p)[at]);
+// Eight elements of a row as fp16 bits. vec: the rows' strides and pointer allow 16-byte loads.
+__device__ __forceinline__ uint4 row_halves(const KvRows& r, long long at, bool vec) {
+  uint32_t w[4];
+  if (r.f16) {
+    const uint16_t* p = (const uint16_t*)r.p + at;
+    if (vec) return gload_u4(p);
+#pragma unroll
+    for (int i = 0; i < 4; i++) w[i] = (uint32_t)gmem(p)[2 * i] | (uint32_t)gmem(p)[2 * i + 1] << 16;
+  } else {
+    const float* p = (const float*)r.p + at;
+    float x[8];
+    if (vec) {
+      const float4 a = gload_f4(p), b = gload_f4(p + 4);
+      x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; i++) x[i] = gmem(p)[i];
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++) w[i] = (uint32_t)f2h(x[2 * i]) | (uint32_t)f2h(x[2 * i + 1]) << 16;
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
 // round(x / s), ties to even, of the exact quotient. x * inv is off by less than one step near a tie; the residual
 // x - q s (one fma) decides: next to a tie it is a multiple of ulp(s) / 2 below s, so it is exact there.
-__device__ __forceinline__ int code_of(float x, float s, float inv) {
+__device__ __forceinline__ uint32_t code_of(float x, float s, float inv) {
   float q = __builtin_rintf(x * inv);
   const float r = __builtin_fmaf(-q, s, x), h = 0.5f * s;
-  if (r > h || (r == h && ((int)q & 1))) q += 1.0f;
-  else if (r < -h || (r == -h && ((int)q & 1))) q -= 1.0f;
-  return (int)q;
+  const bool odd = (int)q & 1;
+  q += r > h || (r == h && odd) ? 1.0f : r < -h || (r == -h && odd) ? -1.0f : 0.0f;
+  return (uint32_t)((int)q + 128) & 255u;
 }
 
-// Codes the 32 rows in `b` (one wave, K or V) into `codes` and returns the scale.
-template <int D, bool V>
-__device__ float code_block(const BlockLds<D>& b, int lane, uint8_t* codes) {
-  int top = 0;
-  for (int i = lane; i < kKvBlock * D; i += 64) top = max(top, b.x[i / D][i % D] & 0x7fff);
+// Largest magnitude of eight fp16, as bits.
+__device__ __forceinline__ int top_of(uint4 x) {
+  const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+  int m = 0;
 #pragma unroll
-  for (int m = 32; m; m >>= 1) top = max(top, __shfl_xor(top, m));
-  const float a = h2f((uint16_t)top);
-  const bool bad = top >= 0x7c00;
-  const float s = bad ? __int_as_float(0x7fc00000) : top ? a / 127.0f : 1.0f, inv = 1.0f / s;
-  for (int i = lane; i < kKvBlock * D / 8; i += 64) {  // 8 codes, one store
-    uint32_t w[2] = {0x80808080u, 0x80808080u};
-    if (!bad) {
-#pragma unroll
-      for (int j = 0; j < 8; j++) {
-        // V: i = (r * 4 + g) * U + u, element r U + u, positions 4 g + j and 16 + 4 g + j
-        constexpr int U = D / 16;
-        const int t = V ? i / U % 4 * 4 + (j & 3) + 16 * (j >> 2) : i * 8 / D;
-        const int e = V ? i / (4 * U) * U + i % U : i * 8 % D + j;
-        const uint32_t q = (uint32_t)(code_of(h2f(b.x[t][e]), s, inv) + 128) & 255u;
-        w[j >> 2] = (w[j >> 2] & ~(255u << (8 * (j & 3)))) | q << (8 * (j & 3));
-      }
-    }
-    *reinterpret_cast<uint2*>(codes + (size_t)i * 8) = make_uint2(w[0], w[1]);
-  }
-  return s;
+  for (int i = 0; i < 4; i++) m = max(m, max((int)(w[i] & 0x7fffu), (int)(w[i] >> 16 & 0x7fffu)));
+  return m;
 }
 
-// One wave's share of an append: block `b` (0: the one that the tail began) of one head; for block 0 also what is left
-// over as the new tail, so that the rows of the old one are read before the new ones are written. K and V one after
-// the other through the wave's LDS.
-template <int D>
-__device__ void append_block(const Kv8Dev& c, const KvRows& k, const KvRows& v, int s, int sc, int h, int b, int n,
-                             int len, BlockLds<D>& lds) {
-  const int lane = threadIdx.x & 63;
-  const int r = len % kKvBlock, whole = (r + n) / kKvBlock;
-  const size_t head = (size_t)s * c.kvh + h;
-  if (b >= whole && b > 0) return;
-  int slot = 0;
-  if (b < whole) slot = kv_slot(c, c.table[head * c.slots + len / kKvBlock + b]);
-  uint32_t bad = whole ? 0u : c.bad[head];
-#pragma unroll 1
-  for (int p = 0; p < 2; p++) {
-    const KvRows& in = p ? v : k;
-    uint16_t* tail = (p ? c.vt : c.kt) + head * kKvBlock * D;
-    const long long base = sc * in.seq + h * in.head;
-    if (b < whole) {
-      for (int i = lane; i < kKvBlock * D; i += 64) {
-        const int t = i / D, e = i % D, row = b * kKvBlock - r + t;  // row of the call; below 0: of the tail
-        lds.x[t][e] = row >= 0 ? row_elem(in, base + row * in.pos + e) : tail[p ? v_place<D>(t, e) : i];
-      }
-      wave_lds_sync();
-      uint8_t* codes = (p ? c.vc : c.kc) + (head * c.slots + slot) * (size_t)(kKvBlock * D);
-      const float sc2 = p ? code_block<D, true>(lds, lane, codes) : code_block<D, false>(lds, lane, codes);
-      if (lane == 0) (p ? c.vs : c.ks)[head * c.slots + slot] = sc2;
-      wave_lds_sync();
-    }
-    if (b == 0) {  // rows [t0, t1) of the tail that is there after the call
-      const int t0 = whole ? 0 : r, t1 = whole ? (r + n) % kKvBlock : r + n;
-      for (int t = t0; t < t1; t++) {
-        const int row = whole * kKvBlock - r + t;
-        bool off = false;
-        for (int e = lane; e < D; e += 64) {
-          const uint16_t x = row_elem(in, base + row * in.pos + e);
-          tail[p ? v_place<D>(t, e) : t * D + e] = x;
-          off |= (x & 0x7fff) >= 0x7c00;
-        }
-        bad = p == 0 ? bad & ~(1u << t) : bad;
-        if (__ballot(off)) bad |= 1u << t;
-      }
-    }
-  }
-  if (b == 0 && lane == 0) c.bad[head] = bad;
-}
+constexpr int kAppendThreads = 256;
 
-// n = 1: a workgroup per sequence, its waves the heads; the length moves on behind the last of them.
+// A workgroup per block and KV head: its first half codes K, the other V, 8 elements of a row to a thread at a time, in
+// registers. V goes through LDS to its own order. The workgroup of block 0, the one that the old tail began, also
+// writes the new tail, once the old one's rows have been read. arrive: the last workgroup of a sequence to get there
+// moves its length on (few of them: the counter's additions come one after the other); otherwise k_kv8_advance does.
 template <int D>
-__global__ __launch_bounds__(512) void k_kv8_append_one(Kv8Dev c, KvRows k, KvRows v, int seq0) {
-  __shared__ BlockLds<D> lds[8];
-  const int sc = blockIdx.x, s = seq0 + sc, w = threadIdx.x >> 6, W = blockDim.x >> 6;
+__global__ __launch_bounds__(kAppendThreads) void k_kv8_append(Kv8Dev c, KvRows k, KvRows v, int seq0, int n,
+                                                               int blocks, int vec, int arrive) {
+  constexpr int C = D / 32, R = D / 8, U = D / 16;  // a thread's chunks of 8, a row's, elements of a run of V
+  __shared__ __align__(16) uint16_t lds[kKvBlock][D + 8];
+  __shared__ int tops[4];
+  __shared__ uint32_t bad_rows;
+  const int b = blockIdx.x % blocks, h = blockIdx.x / blocks, sc = blockIdx.y, s = seq0 + sc;
+  const int p = threadIdx.x >> 7, x = threadIdx.x & 127;
   const int len = kv_len(c, s);
-  if (len + 1 > c.max_len) {
-    if (threadIdx.x == 0) c.state[(size_t)s * KV_STATE + KV_DROPPED] += 1;
+  int* state = c.state + (size_t)s * KV_STATE;
+  if (len + n > c.max_len) {
+    if (arrive && blockIdx.x == 0 && threadIdx.x == 0) state[KV_DROPPED] += n;
     return;
   }
-  for (int h = w; h < c.kvh; h += W) append_block<D>(c, k, v, s, sc, h, 0, 1, len, lds[w]);
-  __syncthreads();
-  if (threadIdx.x == 0) c.state[(size_t)s * KV_STATE + KV_LEN] = len + 1;
-}
-
-// n > 1: a wave per block and head; k_kv8_advance follows.
-template <int D>
-__global__ __launch_bounds__(256) void k_kv8_append(Kv8Dev c, KvRows k, KvRows v, int seq0, int n, int blocks) {
-  __shared__ BlockLds<D> lds[4];
-  const int w = threadIdx.x >> 6;
-  const long long u = (long long)blockIdx.x * 4 + w;
-  const int b = (int)(u % blocks), h = (int)(u / blocks), sc = blockIdx.y;
-  if (h >= c.kvh) return;
-  const int len = kv_len(c, seq0 + sc);
-  if (len + n > c.max_len) return;
-  append_block<D>(c, k, v, seq0 + sc, sc, h, b, n, len, lds[w]);
+  const int r = len % kKvBlock, whole = (r + n) / kKvBlock;
+  const size_t head = (size_t)s * c.kvh + h;
+  const KvRows in = p ? v : k;
+  const bool wide = vec >> p & 1;
+  uint16_t* tail = (p ? c.vt : c.kt) + head * kKvBlock * D;
+  const long long base = sc * in.seq + h * in.head;
+  if (b < whole) {
+    const size_t slot = head * c.slots + kv_slot(c, c.table[head * c.slots + len / kKvBlock + b]);
+    uint4 q[C];
+    int top = 0;
+#pragma unroll
+    for (int j = 0; j < C; j++) {
+      const int t = (x + 128 * j) / R, e = (x + 128 * j) % R * 8, row = b * kKvBlock - r + t;
+      if (row >= 0) {
+        q[j] = row_halves(in, base + row * in.pos + e, wide);
+      } else if (p == 0) {
+        q[j] = gload_u4(tail + t * D + e);
+      } else {
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+          w[i] = (uint32_t)tail[v_place<D>(t, e + 2 * i)] | (uint32_t)tail[v_place<D>(t, e + 2 * i + 1)] << 16;
+        q[j] = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+      top = max(top, top_of(q[j]));
+      if (p) *reinterpret_cast<uint4*>(&lds[t][e]) = q[j];
+    }
+    top = max(top, partner<1>(top));
+    top = max(top, partner<2>(top));
+    top = max(top, partner<4>(top));
+    top = max(top, partner<8>(top));
+    top = max(top, partner<16>(top));
+    top = max(top, partner<32>(top));
+    if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = top;
+    __syncthreads();
+    top = max(tops[2 * p], tops[2 * p + 1]);
+    const bool bad = top >= 0x7c00;
+    const float sc8 = bad ? __int_as_float(0x7fc00000) : top ? h2f((uint16_t)top) / 127.0f : 1.0f, inv = 1.0f / sc8;
+    uint8_t* codes = (p ? c.vc : c.kc) + slot * (size_t)(kKvBlock * D);
+#pragma unroll
+    for (int j = 0; j < C; j++) {
+      const int i = x + 128 * j;
+      const uint32_t w[4] = {q[j].x, q[j].y, q[j].z, q[j].w};
+      uint32_t o[2] = {0u, 0u};
+#pragma unroll
+      for (int y = 0; y < 8; y++) {
+        // V: run i is ((element / U) * 4 + group) * U + element % U
+        const uint16_t a = p ? lds[i / U % 4 * 4 + (y & 3) + 16 * (y >> 2)][i / (4 * U) * U + i % U]
+                             : (uint16_t)(w[y >> 1] >> (16 * (y & 1)));
+        o[y >> 2] |= (bad ? 128u : code_of(h2f(a), sc8, inv)) << (8 * (y & 3));
+      }
+      *reinterpret_cast<uint2*>(codes + i * 8) = make_uint2(o[0], o[1]);
+    }
+    if (x == 0) (p ? c.vs : c.ks)[slot] = sc8;
+  }
+  if (b == 0) {  // rows [t0, t1) of the tail that is there after the call
+    const int t0 = whole ? 0 : r, t1 = whole ? (r + n) % kKvBlock : r + n;
+    if (threadIdx.x == 0) bad_rows = 0u;
+    __syncthreads();
+    for (int i = x; i < (t1 - t0) * R; i += 128) {
+      const int t = t0 + i / R, e = i % R * 8, row = whole * kKvBlock - r + t;
+      const uint4 y = row_halves(in, base + row * in.pos + e, wide);
+      if (p == 0) {
+        *reinterpret_cast<uint4*>(tail + t * D + e) = y;
+      } else {
+        const uint32_t w[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+        for (int z = 0; z < 8; z++) tail[v_place<D>(t, e + z)] = (uint16_t)(w[z >> 1] >> (16 * (z & 1)));
+      }
+      if (top_of(y) >= 0x7c00) atomicOr(&bad_rows, 1u << t);
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      const uint32_t before = whole ? 0u : c.bad[head] & ((1u << r) - 1u);
+      c.bad[head] = before | bad_rows;
+    }
+  }
+  if (arrive) {
+    __syncthreads();  // every wave has read the length
+    if (threadIdx.x == 0 && atomicAdd(&state[KV_ARRIVED], 1) == (int)gridDim.x - 1) {
+      state[KV_LEN] = len + n;
+      state[KV_ARRIVED] = 0;
+    }
+  }
 }
 
 __global__ void k_kv8_advance(Kv8Dev c, int seq0, int n_seqs, int n) {
@@ -155,31 +181,72 @@ __global__ void k_kv8_clear(Kv8Dev c, int seq0) {
   if (i < KV_STATE) c.state[(size_t)s * KV_STATE + i] = 0;
 }
 
-// A workgroup per block of the positions asked for (aligned as the call's, not as the cache's) and head.
+// A workgroup per block of the cache and head, its first half K, the other V; the codes go through LDS, where V comes
+// back to rows, and out 8 elements of a row at a time. Positions that are not there give 0: their blocks lie before
+// the sequence's first one or behind its last.
 template <int D>
-__global__ __launch_bounds__(256) void k_kv8_read(Kv8Dev c, KvRows k, KvRows v, int seq0, int pos, int n) {
+__global__ __launch_bounds__(256) void k_kv8_read(Kv8Dev c, KvRows k, KvRows v, int seq0, int pos, int n, int vec) {
+  constexpr int C = D / 32, R = D / 8, U = D / 16;
+  __shared__ __align__(16) float lds[2][kKvBlock][D + 4];
   const int sc = blockIdx.z, h = blockIdx.y, s = seq0 + sc, len = kv_len(c, s);
   const size_t head = (size_t)s * c.kvh + h;
-  const int first = pos < 0 ? len + pos : pos;
-  for (int i = threadIdx.x; i < kKvBlock * D; i += blockDim.x) {
-    const int row = blockIdx.x * kKvBlock + i / D, e = i % D;
-    if (row >= n) break;
-    const int at = first + row, b = at / kKvBlock, t = at % kKvBlock;
-    const bool in = at >= 0 && at < len, tail = in && b == len / kKvBlock;
-    size_t slot = 0;
-    if (in && !tail) slot = head * c.slots + kv_slot(c, c.table[head * c.slots + b]);
+  const int first = pos < 0 ? len + pos : pos;           // position of the call's row 0
+  const int b = (first - (first & 31)) / kKvBlock + (int)blockIdx.x;  // whole numbers below 0 too
+  const int p = threadIdx.x >> 7, x = threadIdx.x & 127;
+  const bool tail = b == len / kKvBlock, in = b >= 0 && b * kKvBlock < len;
+  if (in && !tail) {
+    const size_t slot = head * c.slots + kv_slot(c, c.table[head * c.slots + b]);
+    const float sc8 = (p ? c.vs : c.ks)[slot];
+    const uint8_t* codes = (p ? c.vc : c.kc) + slot * (size_t)(kKvBlock * D);
 #pragma unroll
-    for (int p = 0; p < 2; p++) {
-      const KvRows& out = p ? v : k;
-      float x = 0.0f;
-      if (in) {
-        const int place = p ? v_place<D>(t, e) : t * D + e;
-        if (tail) x = h2f((p ? c.vt : c.kt)[head * kKvBlock * D + place]);
-        else x = (float)((int)(p ? c.vc : c.kc)[slot * (kKvBlock * D) + place] - 128) * (p ? c.vs : c.ks)[slot];
+    for (int j = 0; j < C; j++) {
+      const int i = x + 128 * j;
+      const uint2 w = gload_u2(codes + i * 8);
+#pragma unroll
+      for (int y = 0; y < 8; y++) {
+        const float z = (float)((int)((y < 4 ? w.x : w.y) >> (8 * (y & 3)) & 255u) - 128) * sc8;
+        if (p) lds[1][i / U % 4 * 4 + (y & 3) + 16 * (y >> 2)][i / (4 * U) * U + i % U] = z;
+        else lds[0][i / R][i % R * 8 + y] = z;
       }
-      const long long o = sc * out.seq + row * out.pos + h * out.head + e;
-      if (out.f16) ((uint16_t*)out.p)[o] = f2h(x);
-      else ((float*)out.p)[o] = x;
+    }
+  } else if (in) {
+    const uint16_t* t16 = (p ? c.vt : c.kt) + head * kKvBlock * D;
+    for (int i = x; i < kKvBlock * D; i += 128) {
+      const int t = i / D, e = i % D;
+      lds[p][t][e] = h2f(t16[p ? v_place<D>(t, e) : i]);
+    }
+  }
+  __syncthreads();
+  const KvRows out = p ? v : k;
+#pragma unroll
+  for (int j = 0; j < C; j++) {
+    const int t = (x + 128 * j) / R, e = (x + 128 * j) % R * 8, at = b * kKvBlock + t, row = at - first;
+    if (row < 0 || row >= n) continue;
+    const bool there = at >= 0 && at < len;
+    float y[8];
+#pragma unroll
+    for (int z = 0; z < 8; z++) y[z] = there ? lds[p][t][e + z] : 0.0f;
+    const long long o = sc * out.seq + row * out.pos + h * out.head + e;
+    if (out.f16) {
+      uint16_t* d = (uint16_t*)out.p + o;
+      uint32_t w[4];
+#pragma unroll
+      for (int z = 0; z < 4; z++) w[z] = (uint32_t)f2h(y[2 * z]) | (uint32_t)f2h(y[2 * z + 1]) << 16;
+      if (vec >> p & 1) {
+        *reinterpret_cast<uint4*>(d) = make_uint4(w[0], w[1], w[2], w[3]);
+      } else {
+#pragma unroll
+        for (int z = 0; z < 8; z++) d[z] = (uint16_t)(w[z >> 1] >> (16 * (z & 1)));
+      }
+    } else {
+      float* d = (float*)out.p + o;
+      if (vec >> p & 1) {
+        *reinterpret_cast<float4*>(d) = make_float4(y[0], y[1], y[2], y[3]);
+        *reinterpret_cast<float4*>(d + 4) = make_float4(y[4], y[5], y[6], y[7]);
+      } else {
+#pragma unroll
+        for (int z = 0; z < 8; z++) d[z] = y[z];
+      }
     }
   }
 }
@@ -220,7 +287,9 @@ __device__ int block_prefix(int v, int* waves, int* total) {
 // found 8 bits at a time by counting; among blocks of that key the earlier stay.
 template <int KPT>
 __global__ __launch_bounds__(kEvictThreads) void k_kv8_evict(Kv8Dev c, int seq0, int keep, int first, int last) {
-  __shared__ int hist[256], waves[kEvictThreads / 64], pick[2];
+  __shared__ __align__(16) int hist[256];
+  __shared__ int waves[kEvictThreads / 64], pick[2];
+  const int lane = threadIdx.x & 63;
   const int s = seq0 + blockIdx.x / c.kvh, len = kv_len(c, s), nb = len / kKvBlock;
   if (nb <= keep) return;
   const size_t base = ((size_t)s * c.kvh + blockIdx.x % c.kvh) * c.slots;
@@ -245,11 +314,24 @@ __global__ __launch_bounds__(kEvictThreads) void k_kv8_evict(Kv8Dev c, int seq0,
         atomicAdd(&hist[key[j] >> sh & 255u], 1);
     }
     __syncthreads();
-    if (threadIdx.x == 0) {
-      int x = 255, above = 0;
-      while (above + hist[x] < left) above += hist[x--];
-      pick[0] = x;
-      pick[1] = above;
+    if (threadIdx.x < 64) {  // lane x: bins 255 - 4 x and the three below
+      const int4 q = *reinterpret_cast<const int4*>(&hist[252 - 4 * lane]);
+      const int v[4] = {q.w, q.z, q.y, q.x}, mine = q.x + q.y + q.z + q.w;
+      int above = mine;
+#pragma unroll
+      for (int m = 1; m < 64; m <<= 1) {
+        const int y = __shfl_up(above, m);
+        if (lane >= m) above += y;
+      }
+      above -= mine;  // keys in the bins above this lane's
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        if (above < left && above + v[j] >= left) {  // true of one bin
+          pick[0] = 255 - 4 * lane - j;
+          pick[1] = above;
+        }
+        above += v[j];
+      }
     }
     __syncthreads();
     pre |= (uint32_t)pick[0] << sh;
@@ -285,14 +367,14 @@ __global__ __launch_bounds__(kEvictThreads) void k_kv8_evict(Kv8Dev c, int seq0,
     to += stays[j] ? 1 : 0;
     gone += stays[j] ? 0 : 1;
   }
-  if (tail && threadIdx.x == 0) c.table[base + keep] = tail_slot;
-}
-
-__global__ void k_kv8_shorten(Kv8Dev c, int seq0, int n_seqs, int keep) {
-  const int i = blockIdx.x * blockDim.x + threadIdx.x;
-  if (i >= n_seqs) return;
-  const int len = kv_len(c, seq0 + i);
-  if (len / kKvBlock > keep) c.state[(size_t)(seq0 + i) * KV_STATE + KV_LEN] = keep * kKvBlock + len % kKvBlock;
+  if (threadIdx.x == 0) {
+    if (tail) c.table[base + keep] = tail_slot;
+    int* state = c.state + (size_t)s * KV_STATE;  // every thread has read the length: the last head shortens it
+    if (atomicAdd(&state[KV_ARRIVED], 1) == c.kvh - 1) {
+      state[KV_LEN] = keep * kKvBlock + len % kKvBlock;
+      state[KV_ARRIVED] = 0;
+    }
+  }
 }
 
 }  // namespace
@@ -302,35 +384,36 @@ hipError_t launch_kv8_clear(hipStream_t s, const Kv8Dev& c, int seq0, int n_seqs
   return hipGetLastError();
 }
 
+// Whether rows can be moved 16 bytes at a time.
+static int wide(const KvRows& r) {
+  const int m = r.f16 ? 8 : 4;
+  return (uintptr_t)r.p % 16 == 0 && r.seq % m == 0 && r.pos % m == 0 && r.head % m == 0;
+}
+
 hipError_t launch_kv8_append(hipStream_t s, const Kv8Dev& c, int seq0, int n_seqs, KvRows k, KvRows v, int n) {
-  if (n == 1) {
-    const int threads = 64 * (c.kvh < 8 ? c.kvh : 8);
-    if (c.d == 64) klaunch(k_kv8_append_one<64>, n_seqs, threads, 0, s, c, k, v, seq0);
-    else klaunch(k_kv8_append_one<128>, n_seqs, threads, 0, s, c, k, v, seq0);
-    return hipGetLastError();
-  }
-  const int blocks = (kKvBlock - 1 + n) / kKvBlock;
-  const dim3 grid((unsigned)(((long long)blocks * c.kvh + 3) / 4), n_seqs);
-  if (c.d == 64) klaunch(k_kv8_append<64>, grid, 256, 0, s, c, k, v, seq0, n, blocks);
-  else klaunch(k_kv8_append<128>, grid, 256, 0, s, c, k, v, seq0, n, blocks);
-  klaunch(k_kv8_advance, (n_seqs + 63) / 64, 64, 0, s, c, seq0, n_seqs, n);
+  const int blocks = (kKvBlock - 1 + n) / kKvBlock, vec = wide(k) | wide(v) << 1;
+  const int arrive = blocks * c.kvh <= 64;
+  const dim3 grid(blocks * c.kvh, n_seqs);
+  if (c.d == 64) klaunch(k_kv8_append<64>, grid, kAppendThreads, 0, s, c, k, v, seq0, n, blocks, vec, arrive);
+  else klaunch(k_kv8_append<128>, grid, kAppendThreads, 0, s, c, k, v, seq0, n, blocks, vec, arrive);
+  if (!arrive) klaunch(k_kv8_advance, (n_seqs + 63) / 64, 64, 0, s, c, seq0, n_seqs, n);
   return hipGetLastError();
 }
 
 hipError_t launch_kv8_read(hipStream_t s, const Kv8Dev& c, int seq0, int n_seqs, int pos, int n, KvRows k, KvRows v) {
-  const dim3 grid((n + kKvBlock - 1) / kKvBlock, c.kvh, n_seqs);
-  if (c.d == 64) klaunch(k_kv8_read<64>, grid, 256, 0, s, c, k, v, seq0, pos, n);
-  else klaunch(k_kv8_read<128>, grid, 256, 0, s, c, k, v, seq0, pos, n);
+  const dim3 grid((n + 2 * kKvBlock - 2) / kKvBlock, c.kvh, n_seqs);
+  const int vec = wide(k) | wide(v) << 1;
+  if (c.d == 64) klaunch(k_kv8_read<64>, grid, 256, 0, s, c, k, v, seq0, pos, n, vec);
+  else klaunch(k_kv8_read<128>, grid, 256, 0, s, c, k, v, seq0, pos, n, vec);
   return hipGetLastError();
 }
 
 hipError_t launch_kv8_evict(hipStream_t s, const Kv8Dev& c, int seq0, int n_seqs, int keep, int first, int last) {
   const int grid = n_seqs * c.kvh;
-#define EVICT(K)                                                                               \
-  if (c.slots <= K * kEvictThreads) {                                                          \
-    klaunch(k_kv8_evict<K>, grid, kEvictThreads, 0, s, c, seq0, keep, first, last);            \
-    klaunch(k_kv8_shorten, (n_seqs + 63) / 64, 64, 0, s, c, seq0, n_seqs, keep);               \
-    return hipGetLastError();                                                                  \
+#define EVICT(K)                                                                    \
+  if (c.slots <= K * kEvictThreads) {                                               \
+    klaunch(k_kv8_evict<K>, grid, kEvictThreads, 0, s, c, seq0, keep, first, last); \
+    return hipGetLastError();                                                       \
   }
   EVICT(1) EVICT(2) EVICT(4) EVICT(8) EVICT(16) EVICT(32)
 #undef EVICT

@@ -394,18 +394,21 @@ __global__ __launch_bounds__(256) void k_kv8_combine(AttnArgs a, int width) {
     a.tot[wc] = sum == 0.0f ? __int_as_float(0x7f800000) : __builtin_amdgcn_logf(sum) + (m - kShift);
 }
 
-// mass = decay * mass + the block's weights, a thread per block, columns in order.
-__global__ __launch_bounds__(256) void k_kv8_mass(AttnArgs a, float decay) {
+// mass = decay * mass + the block's weights: P lanes to a block, each with every P-th column, joined pairwise.
+__global__ __launch_bounds__(256) void k_kv8_mass(AttnArgs a, float decay, int P) {
   const Kv8Dev& c = a.c;
-  const int sc = blockIdx.z, h = blockIdx.y, s = a.seq0 + sc, b = blockIdx.x * blockDim.x + threadIdx.x;
+  const int sc = blockIdx.z, h = blockIdx.y, s = a.seq0 + sc, x = threadIdx.x % P;
+  const int b = blockIdx.x * (256 / P) + threadIdx.x / P;
   const int len = kv_len(c, s), cols = a.n * a.g;
-  if (b * kKvBlock >= len) return;
+  if (b * kKvBlock >= len) return;  // all P lanes
   const size_t head = (size_t)s * c.kvh + h, hs = (size_t)sc * c.kvh + h;
   const int i0 = max(0, b * kKvBlock - (len - a.n));  // the first position that sees any of the block
   const float* lse = a.lse + (hs * c.slots + b) * cols;
   const float* tot = a.tot + hs * cols;
   float w = 0.0f;
-  for (int col = i0 * a.g; col < cols; col++) w += __builtin_amdgcn_exp2f(lse[col] - tot[col]);
+  for (int col = i0 * a.g + x; col < cols; col += P) w += __builtin_amdgcn_exp2f(lse[col] - tot[col]);
+  for (int m = P / 2; m; m >>= 1) w += __shfl_xor(w, m);
+  if (x) return;
   float* m = c.mass + head * c.slots + kv_slot(c, c.table[head * c.slots + b]);
   *m = __builtin_fmaf(decay, *m, w);
 }
@@ -447,8 +450,11 @@ hipError_t attend(hipStream_t s, AttnArgs a, float decay) {
   else if constexpr (D == 64) klaunch(k_kv8_attend<D, F16, 4, TRACK>, (unsigned)grid, kWaves * 64, 0, s, a);
   if (a.splits > 1)
     klaunch(k_kv8_combine<D, F16, TRACK>, (unsigned)((size_t)a.n_seqs * a.c.kvh * cols), 256, 0, s, a, width);
-  if (TRACK)
-    klaunch(k_kv8_mass, dim3((a.c.slots + 255) / 256, a.c.kvh, a.n_seqs), 256, 0, s, a, decay);
+  if (TRACK) {
+    int P = 1;
+    while (P < cols && P < 64) P *= 2;
+    klaunch(k_kv8_mass, dim3((a.c.slots * P + 255) / 256, a.c.kvh, a.n_seqs), 256, 0, s, a, decay, P);
+  }
   return hipGetLastError();
 }
 
