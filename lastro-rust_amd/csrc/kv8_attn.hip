@@ -15,6 +15,8 @@
 //                hold of P here when the positions of V are taken in that order: v_place lays V out so, and p never
 //                leaves its lane.
 // f32 queries enter as two fp16 (their row scaled by a power of two to below 2^10), f32 outputs take p as two fp16.
+#include <type_traits>
+
 #include "kv8.h"
 #include "launch.h"
 
@@ -29,7 +31,6 @@ typedef float f4 __attribute__((ext_vector_type(4)));
 
 constexpr float kLog2e = 1.44269504088896341f;
 constexpr int kWaves = 4;       // waves of a workgroup, each its share of the blocks
-constexpr int kMinBlocks = 4;   // blocks of a split, at least
 constexpr int kMaxSplits = 64;  // one lane each in the combine
 constexpr float kShift = 7.0f, kSlack = 8.0f;
 
@@ -56,20 +57,14 @@ __device__ __forceinline__ float row_f32(const KvRows& r, long long at) {
   return r.f16 ? h2f(gmem((const uint16_t*)r.p)[at]) : gmem((const float*)r.p)[at];
 }
 
-// The part of the cache that a split of a column tile goes through: blocks [lo, hi) of those that the tile's last
-// position sees. `used` splits have any.
-struct Range {
-  int lo, hi, used;
-};
-__device__ __forceinline__ Range range_of(int len, int n, int g, int tile, int width, int splits, int split) {
+// Blocks that a column tile's last position sees, and the splits of it that have any: split x's waves take blocks
+// x kWaves + wave, then every (splits kWaves)-th, so where a wave begins does not wait for the length.
+__device__ __forceinline__ int blocks_seen(int len, int n, int g, int tile, int width) {
   const int last = min((tile + 1) * width - 1, n * g - 1) / g;  // last position of the tile
-  const int sees = max(0, len - n + 1 + last), nb = (sees + kKvBlock - 1) / kKvBlock;
-  const int chunk = max((nb + splits - 1) / splits, kMinBlocks);
-  Range r;
-  r.used = max(1, (nb + chunk - 1) / chunk);
-  r.lo = min(nb, split * chunk);
-  r.hi = min(nb, r.lo + chunk);
-  return r;
+  return (max(0, len - n + 1 + last) + kKvBlock - 1) / kKvBlock;
+}
+__device__ __forceinline__ int splits_used(int blocks, int splits) {
+  return max(1, min(splits, (blocks + kWaves - 1) / kWaves));
 }
 
 struct AttnArgs {
@@ -84,8 +79,8 @@ struct AttnArgs {
   float* lse;     // [sequence, KV head][block][column]: log2 of the block's sum
 };
 
-template <int D, bool F16, int NT, bool TRACK>
-__global__ __launch_bounds__(kWaves * 64) void k_kv8_attend(AttnArgs a) {
+template <int D, bool F16, int NT, bool TRACK, int MINW = NT == 1 ? (D == 64 ? 4 : 2) : 2>
+__global__ __launch_bounds__(kWaves * 64, MINW) void k_kv8_attend(AttnArgs a) {
   constexpr int KS = D / 32, U = D / 16, CH = D / 64, W = 16 * NT;
   constexpr int PF = 2;  // blocks in flight
   __shared__ __align__(16) float Os[kWaves][16][D + 4];
@@ -97,10 +92,13 @@ __global__ __launch_bounds__(kWaves * 64) void k_kv8_attend(AttnArgs a) {
   const int id = blockIdx.x, unit = id / 8 / a.tiles * 8 + id % 8, tile = id / 8 % a.tiles;
   if (unit >= a.n_seqs * c.kvh * a.splits) return;
   const int split = unit % a.splits, hs = unit / a.splits, h = hs % c.kvh, sc = hs / c.kvh, s = a.seq0 + sc;
-  const int len = kv_len(c, s), cols = a.n * a.g;
-  const Range rg = range_of(len, a.n, a.g, tile, W, a.splits, split);
-  if (split >= rg.used) return;
   const size_t head = (size_t)s * c.kvh + h;
+  const int b0 = split * kWaves + w, step = a.splits * kWaves;  // this wave's first block, and on to the next
+  const int* table = c.table + head * c.slots;
+  int raw = table[min(b0 + lane * step, c.slots - 1)];  // lane x: the slot of this wave's x-th block
+  const int len = kv_len(c, s), cols = a.n * a.g;
+  const int seen = blocks_seen(len, a.n, a.g, tile, W), used = splits_used(seen, a.splits);
+  if (split >= used) return;
   const size_t col0 = (size_t)hs * cols;  // of the workspace's columns
 
   // queries and the rows that each column sees
@@ -157,8 +155,14 @@ __global__ __launch_bounds__(kWaves * 64) void k_kv8_attend(AttnArgs a) {
     for (int u = 0; u < U; u++) O[t][u] = f4{0.0f, 0.0f, 0.0f, 0.0f};
   }
 
-  // One block: kop(half, k), vop(u) give the operands, bad the poisoned rows of the tail.
-  auto block = [&](auto kop, auto vop, float ks, float lvs, float ivs, int b, uint32_t bad) {
+  bool far = false;  // some column's M is beyond 2^16
+  h8 ones;
+#pragma unroll
+  for (int j = 0; j < 8; j++) ones[j] = (_Float16)1.0f;
+  // One block: kop(half, k), vop(u) give the operands. masked: some column does not see all of it (S is a finite -3e38
+  // there, so that a scale of 0 makes no NaN of it), or `bad` names poisoned rows, of the tail.
+  auto block = [&](auto masked, auto kop, auto vop, float ks, float lvs, float ivs, int b, uint32_t bad) {
+    constexpr bool MASKED = decltype(masked)::value;
     f4 S[NT][2];
 #pragma unroll
     for (int x = 0; x < 2; x++) {
@@ -174,33 +178,35 @@ __global__ __launch_bounds__(kWaves * 64) void k_kv8_attend(AttnArgs a) {
         }
       }
     }
-    const bool whole = sees0 >= (b + 1) * kKvBlock;  // every column sees all of it
-    float mx[NT];
+    if constexpr (MASKED) {
+#pragma unroll
+      for (int t = 0; t < NT; t++)
+#pragma unroll
+        for (int x = 0; x < 2; x++)
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            const int row = x * 16 + G * 4 + i;
+            if (bad >> row & 1) S[t][x][i] = __int_as_float(0x7fc00000);
+            if (b * kKvBlock + row >= sees[t]) S[t][x][i] = -3e38f;
+          }
+    }
+    float f[NT], mx[NT];
     bool move = false;
 #pragma unroll
     for (int t = 0; t < NT; t++) {
-      const float f = kf[t] * ks;
-      mx[t] = __int_as_float(0xff800000);
+      f[t] = kf[t] * ks;
+      mx[t] = S[t][0][0];  // NaN only where all are
 #pragma unroll
-      for (int x = 0; x < 2; x++)
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-          S[t][x][i] *= f;
-          const int row = x * 16 + G * 4 + i;
-          if (!whole) {
-            if (bad >> row & 1) S[t][x][i] = __int_as_float(0x7fc00000);
-            if (b * kKvBlock + row >= sees[t]) S[t][x][i] = __int_as_float(0xff800000);
-          }
-          mx[t] = __builtin_fmaxf(mx[t], S[t][x][i]);
-        }
-      move |= mx[t] + lvs > M[t] + kSlack;
+      for (int x = 1; x < 8; x++) mx[t] = __builtin_fmaxf(mx[t], S[t][x >> 2][x & 3]);
+      move |= __builtin_fmaf(mx[t], f[t], lvs) > M[t] + kSlack;
     }
     if (__any(move)) {
 #pragma unroll
       for (int t = 0; t < NT; t++) {
-        const float y = max_stage<32>(max_stage<16>(mx[t])) + lvs;
+        const float y = max_stage<32>(max_stage<16>(mx[t])) * f[t] + lvs;
         const float mn = y > M[t] ? y : M[t], al = __builtin_amdgcn_exp2f(M[t] - mn);
         M[t] = mn;
+        far |= __any(__builtin_fabsf(mn) > 65536.0f && mn != -1e30f);
         l[t] *= al;
 #pragma unroll
         for (int u = 0; u < U; u++)
@@ -208,29 +214,38 @@ __global__ __launch_bounds__(kWaves * 64) void k_kv8_attend(AttnArgs a) {
           for (int i = 0; i < 4; i++) O[t][u][i] *= al;
       }
     }
+    if (far) {  // M is rounded by more than p allows: the same rounding for the scores
+#pragma unroll
+      for (int t = 0; t < NT; t++) {
+#pragma unroll
+        for (int x = 0; x < 8; x++) S[t][x >> 2][x & 3] *= f[t];
+        f[t] = 1.0f;
+      }
+    }
     h8 ph[NT], pl[F16 ? 1 : NT];
 #pragma unroll
     for (int t = 0; t < NT; t++) {
       const float c0 = lvs - M[t] + kShift;
-      float sum = 0.0f;
+      float p[8];
 #pragma unroll
-      for (int x = 0; x < 2; x++)
+      for (int x = 0; x < 8; x++) p[x] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[t][x >> 2][x & 3], f[t], c0));
+      if constexpr (MASKED) {
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-          const float p = __builtin_amdgcn_exp2f(S[t][x][i] + c0);
-          sum += p;
-          const _Float16 hi = (_Float16)p;
-          ph[t][x * 4 + i] = hi;
-          if constexpr (!F16) pl[t][x * 4 + i] = (_Float16)(p - (float)hi);
-        }
-      l[t] = __builtin_fmaf(sum, ivs, l[t]);
-      if constexpr (TRACK) {
-        sum = sum + partner<16>(sum);
-        sum = sum + partner<32>(sum);
-        const int col = tile * W + t * 16 + col16;
-        if (G == 0 && col < cols)
-          a.lse[((size_t)hs * c.slots + b) * cols + col] = __builtin_amdgcn_logf(sum) + (M[t] - kShift - lvs);
+        for (int x = 0; x < 8; x++)
+          if (b * kKvBlock + (x >> 2) * 16 + G * 4 + (x & 3) >= sees[t]) p[x] = 0.0f;
       }
+#pragma unroll
+      for (int x = 0; x < 8; x++) {
+        ph[t][x] = (_Float16)p[x];
+        if constexpr (!F16) pl[t][x] = (_Float16)(p[x] - (float)ph[t][x]);
+      }
+    }
+    // the sums over the block's positions, in every lane of the column
+    f4 sum[NT];
+#pragma unroll
+    for (int t = 0; t < NT; t++) {
+      sum[t] = mfma(ones, ph[t], f4{0.0f, 0.0f, 0.0f, 0.0f});
+      if constexpr (!F16) sum[t] = mfma(ones, pl[t], sum[t]);
     }
 #pragma unroll
     for (int u = 0; u < U; u++) {
@@ -241,18 +256,31 @@ __global__ __launch_bounds__(kWaves * 64) void k_kv8_attend(AttnArgs a) {
         if constexpr (!F16) O[t][u] = mfma(va, pl[t], O[t][u]);
       }
     }
+#pragma unroll
+    for (int t = 0; t < NT; t++) l[t] = __builtin_fmaf(sum[t][0], ivs, l[t]);
+    if constexpr (TRACK) {  // lane group t writes tile t's
+      float y = sum[0][0], m = M[0];
+#pragma unroll
+      for (int t = 1; t < NT; t++) {
+        y = G == t ? sum[t][0] : y;
+        m = G == t ? M[t] : m;
+      }
+      const int col = tile * W + lane;
+      if (lane < W && col < cols)
+        a.lse[((size_t)hs * c.slots + b) * cols + col] = __builtin_amdgcn_logf(y) + (m - kShift - lvs);
+    }
   };
 
-  const int full = min(rg.hi, len / kKvBlock);  // blocks that are coded
-  for (int base = rg.lo + w; base < full; base += 64 * kWaves) {
+  const int full = min(seen, len / kKvBlock);  // blocks that are coded
+  for (int base = b0; base < full; base += 64 * step) {
     // lane x: slot and scales of this wave's x-th block from here
-    const int mine = base + lane * kWaves;
-    const size_t sl = head * c.slots + (mine < full ? kv_slot(c, c.table[head * c.slots + mine]) : 0);
-    const int slot_l = (int)(sl - head * c.slots);
+    if (base != b0) raw = table[min(base + lane * step, c.slots - 1)];
+    const int slot_l = kv_slot(c, raw);
+    const size_t sl = head * c.slots + slot_l;
     // a V that is not finite makes the scores NaN, not the scale: columns that see none of the block are masked there
     const float vs_r = c.vs[sl], vs_l = vs_r == vs_r ? vs_r : 1.0f, ks_l = vs_r == vs_r ? c.ks[sl] : vs_r;
     const float lvs_l = __builtin_amdgcn_logf(vs_l), ivs_l = 1.0f / vs_l;
-    const int count = min(64, (full - base + kWaves - 1) / kWaves);
+    const int count = min(64, (full - base + step - 1) / step);
     uint4 kb[PF][2 * CH], vb[PF][2 * CH];
     auto fetch = [&](int p, int x) {
       const int slot = __builtin_amdgcn_readlane(slot_l, min(x, count - 1));
@@ -267,30 +295,38 @@ __global__ __launch_bounds__(kWaves * 64) void k_kv8_attend(AttnArgs a) {
           vb[p][y * CH + z] = gload_u4(vp + (y * CH + z) * 16);
         }
     };
+    auto run = [&](auto masked, int p, int x) {
+      auto kop = [&](int y, int k) {
+        const uint4 v = kb[p][y * CH + (k >> 1)];
+        return k & 1 ? half_codes(v.z, v.w) : half_codes(v.x, v.y);
+      };
+      auto vop = [&](int u) {
+        const uint4 v = vb[p][u >> 1];
+        return u & 1 ? half_codes(v.z, v.w) : half_codes(v.x, v.y);
+      };
+      block(masked, kop, vop, __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(ks_l), x)),
+            __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(lvs_l), x)),
+            __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(ivs_l), x)), base + x * step, 0u);
+    };
+    // the blocks that every column sees all of, and those that some see a part of
+    const int whole = max(0, min(count, (sees0 / kKvBlock - base + step - 1) / step));
+    if (whole) {
 #pragma unroll
-    for (int p = 0; p < PF; p++) fetch(p, p);
-    for (int x = 0; x < count; x += PF) {
+      for (int p = 0; p < PF; p++) fetch(p, p);
+      for (int x = 0; x < whole; x += PF) {
 #pragma unroll
-      for (int p = 0; p < PF; p++) {
-        if (x + p < count) {
-          auto kop = [&](int y, int k) {
-            const uint4 v = kb[p][y * CH + (k >> 1)];
-            return k & 1 ? half_codes(v.z, v.w) : half_codes(v.x, v.y);
-          };
-          auto vop = [&](int u) {
-            const uint4 v = vb[p][u >> 1];
-            return u & 1 ? half_codes(v.z, v.w) : half_codes(v.x, v.y);
-          };
-          block(kop, vop, __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(ks_l), x + p)),
-                __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(lvs_l), x + p)),
-                __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(ivs_l), x + p)),
-                base + (x + p) * kWaves, 0u);
+        for (int p = 0; p < PF; p++) {
+          if (x + p < whole) run(std::false_type(), p, x + p);
+          fetch(p, x + p + PF);
         }
-        fetch(p, x + p + PF);
       }
     }
+    for (int x = whole; x < count; x++) {
+      fetch(0, x);
+      run(std::true_type(), 0, x);
+    }
   }
-  if (rg.hi > full && (full - rg.lo) % kWaves == w) {  // the tail, in fp16
+  if (seen > full && full % step == b0) {  // the tail, in fp16
     const int r = len % kKvBlock;
     const uint32_t bad = c.bad[head], use = ~bad & ((1u << r) - 1u);
     const uint16_t* kt = c.kt + head * kKvBlock * D;
@@ -305,16 +341,14 @@ __global__ __launch_bounds__(kWaves * 64) void k_kv8_attend(AttnArgs a) {
         v[j] = use >> (G * 4 + (j & 3) + 16 * (j >> 2)) & 1 ? v[j] : (_Float16)0.0f;
       return v;
     };
-    block(kop, vop, 1.0f, 0.0f, 1.0f, full, bad);
+    block(std::true_type(), kop, vop, 1.0f, 0.0f, 1.0f, full, bad);
   }
 
   // the waves' shares, tile by tile
 #pragma unroll
   for (int t = 0; t < NT; t++) {
-    float lt = l[t] + partner<16>(l[t]);
-    lt = lt + partner<32>(lt);
     if (t) __syncthreads();
-    if (G == 0) Ms[w][col16] = make_float2(M[t], lt);
+    if (G == 0) Ms[w][col16] = make_float2(M[t], l[t]);
 #pragma unroll
     for (int i = 0; i < 4; i++)
 #pragma unroll
@@ -336,7 +370,7 @@ __global__ __launch_bounds__(kWaves * 64) void k_kv8_attend(AttnArgs a) {
         for (int e = 0; e < U; e++) o[e] = __builtin_fmaf(Os[x][cl][e0 + e], al, o[e]);
       }
       const size_t wc = col0 + col;
-      if (rg.used == 1) {
+      if (used == 1) {
         const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
         const long long at = sc * a.out.seq + (long long)(col / a.g) * a.out.pos +
                              (long long)(h * a.g + col % a.g) * a.out.head + e0;
@@ -367,13 +401,14 @@ __global__ __launch_bounds__(256) void k_kv8_combine(AttnArgs a, int width) {
   const int cols = a.n * a.g, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   const size_t wc = blockIdx.x;
   const int col = (int)(wc % cols), hs = (int)(wc / cols), h = hs % c.kvh, sc = hs / c.kvh;
-  const Range rg = range_of(kv_len(c, a.seq0 + sc), a.n, a.g, col / width, width, a.splits, 0);
-  if (rg.used == 1) return;
-  const bool in = lane < rg.used;
-  const float2 x = in ? a.ml[wc * a.splits + lane] : make_float2(-3e38f, 0.0f);
+  float2 x = a.ml[wc * a.splits + min(lane, a.splits - 1)];
+  const int used = splits_used(blocks_seen(kv_len(c, a.seq0 + sc), a.n, a.g, col / width, width), a.splits);
+  if (used == 1) return;
+  const bool in = lane < used;
+  if (!in) x = make_float2(-3e38f, 0.0f);
   const float m = group_max(x.x), al = in ? __builtin_amdgcn_exp2f(x.x - m) : 0.0f, sum = group_sum(x.y * al);
   float o[E] = {};
-  for (int j = w; j < rg.used; j += 4) {
+  for (int j = w; j < used; j += 4) {
     const float aj = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(al), j));
     const float* po = a.part + (wc * a.splits + j) * D;
 #pragma unroll
@@ -423,7 +458,7 @@ KvAttnPlan kv8_attn_plan(const Kv8Dev& c, int n_seqs, int heads, int n, bool tra
   const int cols1 = heads / c.kvh * n, nt = tile_count(cols1, c.d), tiles = (cols1 + 16 * nt - 1) / (16 * nt);
   const size_t cols = (size_t)n_seqs * heads * n;
   const long long units = (long long)n_seqs * c.kvh * tiles;
-  const int most = (c.slots + kMinBlocks - 1) / kMinBlocks;
+  const int most = (c.slots + kWaves - 1) / kWaves;
   long long s = (1024 + units - 1) / units;
   s = s < 1 ? 1 : s > kMaxSplits ? kMaxSplits : s;
   p.splits = (int)(s > most ? most : s);
