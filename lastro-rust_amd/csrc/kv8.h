@@ -28,6 +28,12 @@ struct KvRows {
   long long seq, pos, head;
 };
 
+// Whether rows can be moved 16 bytes at a time.
+inline int wide_rows(const KvRows& r) {
+  const int m = r.f16 ? 8 : 4;
+  return (uintptr_t)r.p % 16 == 0 && r.seq % m == 0 && r.pos % m == 0 && r.head % m == 0;
+}
+
 // Place of position t, element e in a block of V: what one lane multiplies at once, 8 positions of U = d / 16
 // elements, is one run of bytes (k_kv8_attend says which lane).
 template <int D>

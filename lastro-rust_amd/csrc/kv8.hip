@@ -384,14 +384,8 @@ hipError_t launch_kv8_clear(hipStream_t s, const Kv8Dev& c, int seq0, int n_seqs
   return hipGetLastError();
 }
 
-// Whether rows can be moved 16 bytes at a time.
-static int wide(const KvRows& r) {
-  const int m = r.f16 ? 8 : 4;
-  return (uintptr_t)r.p % 16 == 0 && r.seq % m == 0 && r.pos % m == 0 && r.head % m == 0;
-}
-
 hipError_t launch_kv8_append(hipStream_t s, const Kv8Dev& c, int seq0, int n_seqs, KvRows k, KvRows v, int n) {
-  const int blocks = (kKvBlock - 1 + n) / kKvBlock, vec = wide(k) | wide(v) << 1;
+  const int blocks = (kKvBlock - 1 + n) / kKvBlock, vec = wide_rows(k) | wide_rows(v) << 1;
   const int arrive = blocks * c.kvh <= 64;
   const dim3 grid(blocks * c.kvh, n_seqs);
   if (c.d == 64) klaunch(k_kv8_append<64>, grid, kAppendThreads, 0, s, c, k, v, seq0, n, blocks, vec, arrive);
@@ -402,7 +396,7 @@ hipError_t launch_kv8_append(hipStream_t s, const Kv8Dev& c, int seq0, int n_seq
 
 hipError_t launch_kv8_read(hipStream_t s, const Kv8Dev& c, int seq0, int n_seqs, int pos, int n, KvRows k, KvRows v) {
   const dim3 grid((n + 2 * kKvBlock - 2) / kKvBlock, c.kvh, n_seqs);
-  const int vec = wide(k) | wide(v) << 1;
+  const int vec = wide_rows(k) | wide_rows(v) << 1;
   if (c.d == 64) klaunch(k_kv8_read<64>, grid, 256, 0, s, c, k, v, seq0, pos, n, vec);
   else klaunch(k_kv8_read<128>, grid, 256, 0, s, c, k, v, seq0, pos, n, vec);
   return hipGetLastError();

@@ -34,6 +34,17 @@ constexpr int kWaves = 4;       // waves of a workgroup, each its share of the b
 constexpr int kMaxSplits = 64;  // one lane each in the combine
 constexpr float kShift = 7.0f, kSlack = 8.0f;
 
+// a + the value of a's lane 16 (32) away, in both of them.
+__device__ __forceinline__ float add16(float a) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(a), __float_as_uint(a), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+// Lanes 0 .. 31: a + a's lane 32 on; lanes 32 .. 63: the same of b.
+__device__ __forceinline__ float add32(float a, float b) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(a), __float_as_uint(b), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
 __device__ __forceinline__ f4 mfma(h8 a, h8 b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 
 // Eight codes + 128 as fp16: 0x64bb is 1024 + bb.
@@ -53,8 +64,55 @@ __device__ __forceinline__ h8 half_codes(uint32_t a, uint32_t b) {
   return r.v;
 }
 
-__device__ __forceinline__ float row_f32(const KvRows& r, long long at) {
-  return r.f16 ? h2f(gmem((const uint16_t*)r.p)[at]) : gmem((const float*)r.p)[at];
+// Eight elements of a row. wide: the rows' pointer and strides allow 16-byte loads.
+template <bool F16>
+__device__ __forceinline__ void load8(const KvRows& r, long long at, bool wide, float* x) {
+  if constexpr (F16) {
+    const uint16_t* p = (const uint16_t*)r.p + at;
+    if (wide) {
+      const uint4 v = gload_u4(p);
+      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int j = 0; j < 8; j++) x[j] = h2f((uint16_t)(w[j >> 1] >> (16 * (j & 1))));
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; j++) x[j] = h2f(gmem(p)[j]);
+    }
+  } else {
+    const float* p = (const float*)r.p + at;
+    if (wide) {
+      const float4 u = gload_f4(p), v = gload_f4(p + 4);
+      x[0] = u.x, x[1] = u.y, x[2] = u.z, x[3] = u.w, x[4] = v.x, x[5] = v.y, x[6] = v.z, x[7] = v.w;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; j++) x[j] = gmem(p)[j];
+    }
+  }
+}
+
+// N elements (a multiple of 4) of a row of the output.
+template <int N, bool F16>
+__device__ __forceinline__ void store_out(const KvRows& r, long long at, bool wide, const float* x) {
+  if constexpr (F16) {
+    uint16_t* p = (uint16_t*)r.p + at;
+    uint32_t w[N / 2];
+#pragma unroll
+    for (int j = 0; j < N / 2; j++) w[j] = (uint32_t)f2h(x[2 * j]) | (uint32_t)f2h(x[2 * j + 1]) << 16;
+    if (wide) {
+#pragma unroll
+      for (int j = 0; j < N / 4; j++) *reinterpret_cast<uint2*>(p + 4 * j) = make_uint2(w[2 * j], w[2 * j + 1]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < N; j++) p[j] = (uint16_t)(w[j >> 1] >> (16 * (j & 1)));
+    }
+  } else {
+    float* p = (float*)r.p + at;
+#pragma unroll
+    for (int j = 0; j < N; j += 4) {
+      if (wide) *reinterpret_cast<f4*>(p + j) = f4{x[j], x[j + 1], x[j + 2], x[j + 3]};
+      else p[j] = x[j], p[j + 1] = x[j + 1], p[j + 2] = x[j + 2], p[j + 3] = x[j + 3];
+    }
+  }
 }
 
 // Blocks that a column tile's last position sees, and the splits of it that have any: split x's waves take blocks
@@ -71,6 +129,7 @@ struct AttnArgs {
   Kv8Dev c;
   KvRows q, out;
   int seq0, n_seqs, g, n, splits, tiles;
+  int vec;        // bit 0: q can be loaded 16 bytes at a time, bit 1: out can be stored so
   float kf;       // |scale| log2 e
   uint32_t sign;  // of the scale
   float* part;    // [sequence, KV head, column][split][D]
@@ -79,10 +138,14 @@ struct AttnArgs {
   float* lse;     // [sequence, KV head][block][column]: log2 of the block's sum
 };
 
-template <int D, bool F16, int NT, bool TRACK, int MINW = NT == 1 ? (D == 64 ? 4 : 2) : 2>
+template <int D, bool F16, int NT, bool TRACK, int MINW = NT == 1 && D == 64 ? 4 : 2>
 __global__ __launch_bounds__(kWaves * 64, MINW) void k_kv8_attend(AttnArgs a) {
   constexpr int KS = D / 32, U = D / 16, CH = D / 64, W = 16 * NT;
   constexpr int PF = 2;  // blocks in flight
+  // Sums of weights come from the matrix cores, which have time to spare: of the two halves of f32's, or of the rounded
+  // weights, whose error is far below an fp16 output's. The blocks' weights are f32 in any case: there the vector unit
+  // adds up a lane's eight, and lanes are joined for the block's sum and at the end.
+  constexpr bool VSUM = F16 && TRACK;
   __shared__ __align__(16) float Os[kWaves][16][D + 4];
   __shared__ float2 Ms[kWaves][16];
   const Kv8Dev& c = a.c;
@@ -112,10 +175,11 @@ __global__ __launch_bounds__(kWaves * 64, MINW) void k_kv8_attend(AttnArgs a) {
     const long long at = sc * a.q.seq + i * a.q.pos + (long long)(h * a.g + cc % a.g) * a.q.head;
     float x[KS][8];
 #pragma unroll
-    for (int k = 0; k < KS; k++)
+    for (int k = 0; k < KS; k++) {
+      load8<F16>(a.q, at + (k >> 1) * 64 + G * 16 + (k & 1) * 8, a.vec & 1, x[k]);
 #pragma unroll
-      for (int j = 0; j < 8; j++)
-        x[k][j] = __uint_as_float(__float_as_uint(row_f32(a.q, at + (k >> 1) * 64 + G * 16 + (k & 1) * 8 + j)) ^ a.sign);
+      for (int j = 0; j < 8; j++) x[k][j] = __uint_as_float(__float_as_uint(x[k][j]) ^ a.sign);
+    }
     kf[t] = a.kf;
     if constexpr (!F16) {
       float m = 0.0f;
@@ -223,6 +287,7 @@ __global__ __launch_bounds__(kWaves * 64, MINW) void k_kv8_attend(AttnArgs a) {
       }
     }
     h8 ph[NT], pl[F16 ? 1 : NT];
+    float part[NT];
 #pragma unroll
     for (int t = 0; t < NT; t++) {
       const float c0 = lvs - M[t] + kShift;
@@ -234,18 +299,20 @@ __global__ __launch_bounds__(kWaves * 64, MINW) void k_kv8_attend(AttnArgs a) {
         for (int x = 0; x < 8; x++)
           if (b * kKvBlock + (x >> 2) * 16 + G * 4 + (x & 3) >= sees[t]) p[x] = 0.0f;
       }
+      if constexpr (VSUM) part[t] = ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
 #pragma unroll
       for (int x = 0; x < 8; x++) {
         ph[t][x] = (_Float16)p[x];
         if constexpr (!F16) pl[t][x] = (_Float16)(p[x] - (float)ph[t][x]);
       }
     }
-    // the sums over the block's positions, in every lane of the column
     f4 sum[NT];
+    if constexpr (!VSUM) {
 #pragma unroll
-    for (int t = 0; t < NT; t++) {
-      sum[t] = mfma(ones, ph[t], f4{0.0f, 0.0f, 0.0f, 0.0f});
-      if constexpr (!F16) sum[t] = mfma(ones, pl[t], sum[t]);
+      for (int t = 0; t < NT; t++) {
+        sum[t] = mfma(ones, ph[t], f4{0.0f, 0.0f, 0.0f, 0.0f});
+        if constexpr (!F16) sum[t] = mfma(ones, pl[t], sum[t]);
+      }
     }
 #pragma unroll
     for (int u = 0; u < U; u++) {
@@ -257,16 +324,13 @@ __global__ __launch_bounds__(kWaves * 64, MINW) void k_kv8_attend(AttnArgs a) {
       }
     }
 #pragma unroll
-    for (int t = 0; t < NT; t++) l[t] = __builtin_fmaf(sum[t][0], ivs, l[t]);
-    if constexpr (TRACK) {  // lane group t writes tile t's
-      float y = sum[0][0], m = M[0];
-#pragma unroll
-      for (int t = 1; t < NT; t++) {
-        y = G == t ? sum[t][0] : y;
-        m = G == t ? M[t] : m;
-      }
-      const int col = tile * W + lane;
-      if (lane < W && col < cols)
+    for (int t = 0; t < NT; t++) l[t] = __builtin_fmaf(VSUM ? part[t] : sum[t][0], ivs, l[t]);
+    if constexpr (TRACK) {  // lanes of group 0 write tile 0's, those of group 2 tile 1's
+      static_assert(NT <= 2, "");
+      const float y = VSUM ? add16(add32(part[0], part[NT - 1])) : G >= 2 ? sum[NT - 1][0] : sum[0][0];
+      const float m = G >= 2 ? M[NT - 1] : M[0];
+      const int col = tile * W + (G >> 1) * 16 + col16;
+      if ((NT == 2 ? !(G & 1) : G == 0) && col < cols)
         a.lse[((size_t)hs * c.slots + b) * cols + col] = __builtin_amdgcn_logf(y) + (m - kShift - lvs);
     }
   };
@@ -347,8 +411,9 @@ __global__ __launch_bounds__(kWaves * 64, MINW) void k_kv8_attend(AttnArgs a) {
   // the waves' shares, tile by tile
 #pragma unroll
   for (int t = 0; t < NT; t++) {
+    const float lt = VSUM ? add16(add32(l[t], l[t])) : l[t];
     if (t) __syncthreads();
-    if (G == 0) Ms[w][col16] = make_float2(M[t], l[t]);
+    if (G == 0) Ms[w][col16] = make_float2(M[t], lt);
 #pragma unroll
     for (int i = 0; i < 4; i++)
 #pragma unroll
@@ -375,31 +440,30 @@ __global__ __launch_bounds__(kWaves * 64, MINW) void k_kv8_attend(AttnArgs a) {
         const long long at = sc * a.out.seq + (long long)(col / a.g) * a.out.pos +
                              (long long)(h * a.g + col % a.g) * a.out.head + e0;
 #pragma unroll
-        for (int e = 0; e < U; e++) {
-          if constexpr (F16) ((uint16_t*)a.out.p)[at + e] = f2h(o[e] * inv);
-          else ((float*)a.out.p)[at + e] = o[e] * inv;
-        }
+        for (int e = 0; e < U; e++) o[e] *= inv;
+        store_out<U, F16>(a.out, at, a.vec & 2, o);
         if (TRACK && e0 == 0)
           a.tot[wc] = sum == 0.0f ? __int_as_float(0x7f800000) : __builtin_amdgcn_logf(sum) + (m - kShift);
       } else {
         float* po = a.part + (wc * a.splits + split) * D + e0;
 #pragma unroll
-        for (int e = 0; e < U; e++) po[e] = o[e];
+        for (int e = 0; e < U; e += 4) *reinterpret_cast<f4*>(po + e) = f4{o[e], o[e + 1], o[e + 2], o[e + 3]};
         if (e0 == 0) a.ml[wc * a.splits + split] = make_float2(m, sum);
       }
     }
   }
 }
 
-// The splits' shares of a column: a workgroup per column, lane x of each wave holds split x's maximum and sum, the waves
-// take every fourth split's sums.
-template <int D, bool F16, bool TRACK>
+// The splits' shares of a column: C waves to a column, 4 / C columns to a workgroup. Lane x of each wave holds split x's
+// maximum and sum; the waves take every C-th split's products. Many splits go to four waves, whose loads overlap.
+template <int D, bool F16, bool TRACK, int C>
 __global__ __launch_bounds__(256) void k_kv8_combine(AttnArgs a, int width) {
   constexpr int E = D / 64;
   __shared__ float Os[4][D];
   const Kv8Dev& c = a.c;
-  const int cols = a.n * a.g, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  const size_t wc = blockIdx.x;
+  const int cols = a.n * a.g, lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const long long wc = (long long)blockIdx.x * (4 / C) + w / C;
+  if (wc >= (long long)a.n_seqs * c.kvh * cols) return;  // C = 4: no column is left out
   const int col = (int)(wc % cols), hs = (int)(wc / cols), h = hs % c.kvh, sc = hs / c.kvh;
   float2 x = a.ml[wc * a.splits + min(lane, a.splits - 1)];
   const int used = splits_used(blocks_seen(kv_len(c, a.seq0 + sc), a.n, a.g, col / width, width), a.splits);
@@ -408,24 +472,38 @@ __global__ __launch_bounds__(256) void k_kv8_combine(AttnArgs a, int width) {
   if (!in) x = make_float2(-3e38f, 0.0f);
   const float m = group_max(x.x), al = in ? __builtin_amdgcn_exp2f(x.x - m) : 0.0f, sum = group_sum(x.y * al);
   float o[E] = {};
-  for (int j = w; j < used; j += 4) {
-    const float aj = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(al), j));
-    const float* po = a.part + (wc * a.splits + j) * D;
+  const float* po = a.part + wc * a.splits * D + lane;
+  for (int j0 = w % C; j0 < used; j0 += 4 * C) {  // four loads in flight; past the last split its own, at weight 0
+    float y[4][E];
 #pragma unroll
-    for (int e = 0; e < E; e++) o[e] = __builtin_fmaf(po[e * 64 + lane], aj, o[e]);
-  }
+    for (int j = 0; j < 4; j++)
 #pragma unroll
-  for (int e = 0; e < E; e++) Os[w][e * 64 + lane] = o[e];
-  __syncthreads();
-  if (threadIdx.x < D) {
-    const float y = ((Os[0][threadIdx.x] + Os[1][threadIdx.x]) + (Os[2][threadIdx.x] + Os[3][threadIdx.x])) *
-                    (sum == 0.0f ? 0.0f : 1.0f / sum);
-    const long long at = sc * a.out.seq + (long long)(col / a.g) * a.out.pos +
-                         (long long)(h * a.g + col % a.g) * a.out.head + threadIdx.x;
-    if constexpr (F16) ((uint16_t*)a.out.p)[at] = f2h(y);
-    else ((float*)a.out.p)[at] = y;
+      for (int e = 0; e < E; e++) y[j][e] = po[(size_t)min(j0 + j * C, used - 1) * D + e * 64];
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      const float aj = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(al), min(j0 + j * C, used - 1)));
+#pragma unroll
+      for (int e = 0; e < E; e++) o[e] = __builtin_fmaf(y[j][e], j0 + j * C < used ? aj : 0.0f, o[e]);
+    }
   }
-  if (TRACK && threadIdx.x == 0)
+  if constexpr (C == 4) {
+#pragma unroll
+    for (int e = 0; e < E; e++) Os[w][e * 64 + lane] = o[e];
+    __syncthreads();
+    if (w) return;
+#pragma unroll
+    for (int e = 0; e < E; e++)
+      o[e] = (o[e] + Os[1][e * 64 + lane]) + (Os[2][e * 64 + lane] + Os[3][e * 64 + lane]);
+  }
+  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+  const long long at = sc * a.out.seq + (long long)(col / a.g) * a.out.pos +
+                       (long long)(h * a.g + col % a.g) * a.out.head + lane;
+#pragma unroll
+  for (int e = 0; e < E; e++) {
+    if constexpr (F16) ((uint16_t*)a.out.p)[at + e * 64] = f2h(o[e] * inv);
+    else ((float*)a.out.p)[at + e * 64] = o[e] * inv;
+  }
+  if (TRACK && lane == 0)
     a.tot[wc] = sum == 0.0f ? __int_as_float(0x7f800000) : __builtin_amdgcn_logf(sum) + (m - kShift);
 }
 
@@ -448,20 +526,22 @@ __global__ __launch_bounds__(256) void k_kv8_mass(AttnArgs a, float decay, int P
   *m = __builtin_fmaf(decay, *m, w);
 }
 
-// Tiles of 16 columns of a wave.
-int tile_count(int cols, int d) { return cols <= 16 ? 1 : cols <= 32 || d == 128 ? 2 : 4; }
+int tile_count(int cols) { return cols <= 16 ? 1 : 2; }  // tiles of 16 columns of a wave
 
 }  // namespace
 
 KvAttnPlan kv8_attn_plan(const Kv8Dev& c, int n_seqs, int heads, int n, bool track) {
   KvAttnPlan p;
-  const int cols1 = heads / c.kvh * n, nt = tile_count(cols1, c.d), tiles = (cols1 + 16 * nt - 1) / (16 * nt);
+  const int cols1 = heads / c.kvh * n, nt = tile_count(cols1), tiles = (cols1 + 16 * nt - 1) / (16 * nt);
   const size_t cols = (size_t)n_seqs * heads * n;
   const long long units = (long long)n_seqs * c.kvh * tiles;
-  const int most = (c.slots + kWaves - 1) / kWaves;
-  long long s = (1024 + units - 1) / units;
-  s = s < 1 ? 1 : s > kMaxSplits ? kMaxSplits : s;
-  p.splits = (int)(s > most ? most : s);
+  // Splits cost a second launch and the partials' way through memory: one workgroup for each of 256 compute units, and
+  // more (up to 1024, four to a unit) only while a wave keeps 16 blocks of a full cache; never fewer than 3 a wave.
+  const int cap = c.slots / (kWaves * 3);
+  long long s = 256 / units > 1 ? 256 / units : 1;
+  while (2 * s * units <= 1024 && c.slots / (2 * s * kWaves) >= 16) s *= 2;
+  s = s < cap ? s : cap;
+  p.splits = (int)(s < 1 ? 1 : s > kMaxSplits ? kMaxSplits : s);
   auto up = [](size_t x) { return (x + 255) / 256 * 256; };
   p.tot = 0;
   p.ml = up(cols * 4);
@@ -475,16 +555,16 @@ namespace {
 
 template <int D, bool F16, bool TRACK>
 hipError_t attend(hipStream_t s, AttnArgs a, float decay) {
-  const int cols = a.n * a.g, nt = tile_count(cols, D), width = 16 * nt;
+  const int cols = a.n * a.g, nt = tile_count(cols), width = 16 * nt;
   a.tiles = (cols + width - 1) / width;
   const long long units = (long long)a.n_seqs * a.c.kvh * a.splits;
   const long long grid = (units + 7) / 8 * 8 * a.tiles;
   if (grid > 0x7fffffff) return hipErrorInvalidValue;
   if (nt == 1) klaunch(k_kv8_attend<D, F16, 1, TRACK>, (unsigned)grid, kWaves * 64, 0, s, a);
-  else if (nt == 2) klaunch(k_kv8_attend<D, F16, 2, TRACK>, (unsigned)grid, kWaves * 64, 0, s, a);
-  else if constexpr (D == 64) klaunch(k_kv8_attend<D, F16, 4, TRACK>, (unsigned)grid, kWaves * 64, 0, s, a);
-  if (a.splits > 1)
-    klaunch(k_kv8_combine<D, F16, TRACK>, (unsigned)((size_t)a.n_seqs * a.c.kvh * cols), 256, 0, s, a, width);
+  else klaunch(k_kv8_attend<D, F16, 2, TRACK>, (unsigned)grid, kWaves * 64, 0, s, a);
+  const long long all = (long long)a.n_seqs * a.c.kvh * cols;
+  if (a.splits > 8) klaunch(k_kv8_combine<D, F16, TRACK, 4>, (unsigned)all, 256, 0, s, a, width);
+  else if (a.splits > 1) klaunch(k_kv8_combine<D, F16, TRACK, 1>, (unsigned)((all + 3) / 4), 256, 0, s, a, width);
   if (TRACK) {
     int P = 1;
     while (P < cols && P < 64) P *= 2;
@@ -500,7 +580,7 @@ hipError_t launch_kv8_attend(hipStream_t s, const Kv8Dev& c, int seq0, int n_seq
   const bool track = decay >= 0.0f;
   const KvAttnPlan p = kv8_attn_plan(c, n_seqs, heads, n, track);
   char* w = (char*)ws;
-  AttnArgs a{c, q, out, seq0, n_seqs, heads / c.kvh, n, p.splits, 1, __builtin_fabsf(scale) * kLog2e,
+  AttnArgs a{c, q, out, seq0, n_seqs, heads / c.kvh, n, p.splits, 1, wide_rows(q) | wide_rows(out) << 1, __builtin_fabsf(scale) * kLog2e,
              scale < 0.0f ? 0x80000000u : 0u, (float*)(w + p.parts), (float2*)(w + p.ml), (float*)(w + p.tot),
              track ? (float*)(w + p.lse) : nullptr};
 #define ATT(DD, FF) \
