@@ -138,10 +138,16 @@ struct AttnArgs {
   float* lse;     // [sequence, KV head][block][column]: log2 of the block's sum
 };
 
-template <int D, bool F16, int NT, bool TRACK, int MINW = NT == 1 && D == 64 ? 4 : 2>
-__global__ __launch_bounds__(kWaves * 64, MINW) void k_kv8_attend(AttnArgs a) {
+// log2 of a column's whole sum; +inf, which no weight survives, where it sees nothing.
+__device__ __forceinline__ float total_of(float m, float sum) {
+  return sum == 0.0f ? __int_as_float(0x7f800000) : __builtin_amdgcn_logf(sum) + (m - kShift);
+}
+
+// STREAM: the codes are loaded with the non-temporal hint.
+template <int D, bool F16, int NT, bool TRACK, bool STREAM>
+__global__ __launch_bounds__(kWaves * 64, NT == 1 && D == 64 ? 4 : 2) void k_kv8_attend(AttnArgs a) {
   constexpr int KS = D / 32, U = D / 16, CH = D / 64, W = 16 * NT;
-  constexpr int PF = 2;  // blocks in flight
+  constexpr int PF = NT == 1 ? 2 : 1;  // blocks in flight: with two tiles the other waves cover the loads
   // Sums of weights come from the matrix cores, which have time to spare: of the two halves of f32's, or of the rounded
   // weights, whose error is far below an fp16 output's. The blocks' weights are f32 in any case: there the vector unit
   // adds up a lane's eight, and lanes are joined for the block's sum and at the end.
@@ -355,8 +361,8 @@ __global__ __launch_bounds__(kWaves * 64, MINW) void k_kv8_attend(AttnArgs a) {
       for (int y = 0; y < 2; y++)
 #pragma unroll
         for (int z = 0; z < CH; z++) {
-          kb[p][y * CH + z] = gload_u4(kp + y * 16 * D + z * 64);
-          vb[p][y * CH + z] = gload_u4(vp + (y * CH + z) * 16);
+          kb[p][y * CH + z] = STREAM ? gload_u4_nt(kp + y * 16 * D + z * 64) : gload_u4(kp + y * 16 * D + z * 64);
+          vb[p][y * CH + z] = STREAM ? gload_u4_nt(vp + (y * CH + z) * 16) : gload_u4(vp + (y * CH + z) * 16);
         }
     };
     auto run = [&](auto masked, int p, int x) {
@@ -442,8 +448,7 @@ __global__ __launch_bounds__(kWaves * 64, MINW) void k_kv8_attend(AttnArgs a) {
 #pragma unroll
         for (int e = 0; e < U; e++) o[e] *= inv;
         store_out<U, F16>(a.out, at, a.vec & 2, o);
-        if (TRACK && e0 == 0)
-          a.tot[wc] = sum == 0.0f ? __int_as_float(0x7f800000) : __builtin_amdgcn_logf(sum) + (m - kShift);
+        if (TRACK && e0 == 0) a.tot[wc] = total_of(m, sum);
       } else {
         float* po = a.part + (wc * a.splits + split) * D + e0;
 #pragma unroll
@@ -454,23 +459,30 @@ __global__ __launch_bounds__(kWaves * 64, MINW) void k_kv8_attend(AttnArgs a) {
   }
 }
 
-// The splits' shares of a column: C waves to a column, 4 / C columns to a workgroup. Lane x of each wave holds split x's
-// maximum and sum; the waves take every C-th split's products. Many splits go to four waves, whose loads overlap.
+// A column's maximum and sum over its splits, lane x holding split x's, and the factor of split x's products.
+__device__ __forceinline__ void column_sum(const AttnArgs& a, long long wc, int used, int lane, float* m, float* al,
+                                           float* sum) {
+  const float2 x = a.ml[wc * a.splits + min(lane, a.splits - 1)];
+  const bool in = lane < used;
+  *m = group_max(in ? x.x : -3e38f);
+  *al = in ? __builtin_amdgcn_exp2f(x.x - *m) : 0.0f;
+  *sum = group_sum(in ? x.y * *al : 0.0f);
+}
+
+// The splits' shares of a column: C waves to a column, 4 / C columns to a workgroup. The waves take every C-th split's
+// products. Many splits go to four waves, whose loads overlap.
 template <int D, bool F16, bool TRACK, int C>
-__global__ __launch_bounds__(256) void k_kv8_combine(AttnArgs a, int width) {
+__device__ __forceinline__ void combine_column(const AttnArgs& a, int width, int block, float (*Os)[D]) {
   constexpr int E = D / 64;
-  __shared__ float Os[4][D];
   const Kv8Dev& c = a.c;
   const int cols = a.n * a.g, lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const long long wc = (long long)blockIdx.x * (4 / C) + w / C;
+  const long long wc = (long long)block * (4 / C) + w / C;
   if (wc >= (long long)a.n_seqs * c.kvh * cols) return;  // C = 4: no column is left out
   const int col = (int)(wc % cols), hs = (int)(wc / cols), h = hs % c.kvh, sc = hs / c.kvh;
-  float2 x = a.ml[wc * a.splits + min(lane, a.splits - 1)];
   const int used = splits_used(blocks_seen(kv_len(c, a.seq0 + sc), a.n, a.g, col / width, width), a.splits);
+  float m, al, sum;
+  column_sum(a, wc, used, lane, &m, &al, &sum);
   if (used == 1) return;
-  const bool in = lane < used;
-  if (!in) x = make_float2(-3e38f, 0.0f);
-  const float m = group_max(x.x), al = in ? __builtin_amdgcn_exp2f(x.x - m) : 0.0f, sum = group_sum(x.y * al);
   float o[E] = {};
   const float* po = a.part + wc * a.splits * D + lane;
   for (int j0 = w % C; j0 < used; j0 += 4 * C) {  // four loads in flight; past the last split its own, at weight 0
@@ -503,27 +515,57 @@ __global__ __launch_bounds__(256) void k_kv8_combine(AttnArgs a, int width) {
     if constexpr (F16) ((uint16_t*)a.out.p)[at + e * 64] = f2h(o[e] * inv);
     else ((float*)a.out.p)[at + e * 64] = o[e] * inv;
   }
-  if (TRACK && lane == 0)
-    a.tot[wc] = sum == 0.0f ? __int_as_float(0x7f800000) : __builtin_amdgcn_logf(sum) + (m - kShift);
+  if (TRACK && lane == 0) a.tot[wc] = total_of(m, sum);
+}
+
+template <int D, bool F16, bool TRACK, int C>
+__global__ __launch_bounds__(256) void k_kv8_combine(AttnArgs a, int width) {
+  __shared__ float Os[4][D];
+  combine_column<D, F16, TRACK, C>(a, width, blockIdx.x, Os);
 }
 
 // mass = decay * mass + the block's weights: P lanes to a block, each with every P-th column, joined pairwise.
-__global__ __launch_bounds__(256) void k_kv8_mass(AttnArgs a, float decay, int P) {
+__device__ __forceinline__ void mass_block(const AttnArgs& a, int hs, int b, int x, int P, float decay,
+                                           const float* tot) {
   const Kv8Dev& c = a.c;
-  const int sc = blockIdx.z, h = blockIdx.y, s = a.seq0 + sc, x = threadIdx.x % P;
-  const int b = blockIdx.x * (256 / P) + threadIdx.x / P;
-  const int len = kv_len(c, s), cols = a.n * a.g;
+  const int h = hs % c.kvh, s = a.seq0 + hs / c.kvh, len = kv_len(c, s), cols = a.n * a.g;
   if (b * kKvBlock >= len) return;  // all P lanes
-  const size_t head = (size_t)s * c.kvh + h, hs = (size_t)sc * c.kvh + h;
+  const size_t head = (size_t)s * c.kvh + h;
   const int i0 = max(0, b * kKvBlock - (len - a.n));  // the first position that sees any of the block
-  const float* lse = a.lse + (hs * c.slots + b) * cols;
-  const float* tot = a.tot + hs * cols;
+  const float* lse = a.lse + ((size_t)hs * c.slots + b) * cols;
   float w = 0.0f;
   for (int col = i0 * a.g + x; col < cols; col += P) w += __builtin_amdgcn_exp2f(lse[col] - tot[col]);
   for (int m = P / 2; m; m >>= 1) w += __shfl_xor(w, m);
   if (x) return;
   float* m = c.mass + head * c.slots + kv_slot(c, c.table[head * c.slots + b]);
   *m = __builtin_fmaf(decay, *m, w);
+}
+
+__global__ __launch_bounds__(256) void k_kv8_mass(AttnArgs a, float decay, int P) {
+  const int hs = blockIdx.z * a.c.kvh + blockIdx.y;
+  mass_block(a, hs, blockIdx.x * (256 / P) + threadIdx.x / P, threadIdx.x % P, P, decay,
+             a.tot + (size_t)hs * a.n * a.g);
+}
+
+// Combine and masses of one tile of columns in one launch: the first workgroups combine, the others, per KV head, form
+// the columns' sums from the splits' again instead of waiting for them.
+template <int D, bool F16, int C>
+__global__ __launch_bounds__(256) void k_kv8_finish(AttnArgs a, int width, int combines, int per_head, float decay,
+                                                    int P) {
+  __shared__ float Os[4][D], tot[16];
+  if ((int)blockIdx.x < combines) {
+    combine_column<D, F16, false, C>(a, width, blockIdx.x, Os);
+    return;
+  }
+  const int x = blockIdx.x - combines, hs = x / per_head, lane = threadIdx.x & 63, cols = a.n * a.g;
+  const int used = splits_used(blocks_seen(kv_len(a.c, a.seq0 + hs / a.c.kvh), a.n, a.g, 0, width), a.splits);
+  for (int col = threadIdx.x >> 6; col < cols; col += 4) {
+    float m, al, sum;
+    column_sum(a, (long long)hs * cols + col, used, lane, &m, &al, &sum);
+    if (lane == 0) tot[col] = used == 1 ? a.tot[(size_t)hs * cols + col] : total_of(m, sum);
+  }
+  __syncthreads();
+  mass_block(a, hs, x % per_head * (256 / P) + threadIdx.x / P, threadIdx.x % P, P, decay, tot);
 }
 
 int tile_count(int cols) { return cols <= 16 ? 1 : 2; }  // tiles of 16 columns of a wave
@@ -560,16 +602,28 @@ hipError_t attend(hipStream_t s, AttnArgs a, float decay) {
   const long long units = (long long)a.n_seqs * a.c.kvh * a.splits;
   const long long grid = (units + 7) / 8 * 8 * a.tiles;
   if (grid > 0x7fffffff) return hipErrorInvalidValue;
-  if (nt == 1) klaunch(k_kv8_attend<D, F16, 1, TRACK>, (unsigned)grid, kWaves * 64, 0, s, a);
-  else klaunch(k_kv8_attend<D, F16, 2, TRACK>, (unsigned)grid, kWaves * 64, 0, s, a);
+  // A cache that can outgrow the 256 MB last-level cache is streamed past the others: 124 -> 119 us for 565 MB of eight
+  // sequences in 839 MB; in smaller ones the hint costs what a step finds there of the last (26.6 -> 32.3 us for 68 MB).
+  const bool stream = nt == 1 && 2ll * a.n_seqs * a.c.kvh * a.c.max_len * D > 256ll << 20;
+  if (stream) klaunch(k_kv8_attend<D, F16, 1, TRACK, true>, (unsigned)grid, kWaves * 64, 0, s, a);
+  else if (nt == 1) klaunch(k_kv8_attend<D, F16, 1, TRACK, false>, (unsigned)grid, kWaves * 64, 0, s, a);
+  else klaunch(k_kv8_attend<D, F16, 2, TRACK, false>, (unsigned)grid, kWaves * 64, 0, s, a);
   const long long all = (long long)a.n_seqs * a.c.kvh * cols;
+  int P = 1;
+  while (P < cols && P < 64) P *= 2;
+  const int per_head = (a.c.slots * P + 255) / 256;
+  if (TRACK && a.splits > 1 && cols <= 16) {
+    const int C = a.splits > 8 ? 4 : 1, combines = (int)((all * C + 3) / 4);
+    const long long both = combines + (long long)a.n_seqs * a.c.kvh * per_head;
+    if (both <= 0x7fffffff) {
+      if (C == 4) klaunch(k_kv8_finish<D, F16, 4>, (unsigned)both, 256, 0, s, a, width, combines, per_head, decay, P);
+      else klaunch(k_kv8_finish<D, F16, 1>, (unsigned)both, 256, 0, s, a, width, combines, per_head, decay, P);
+      return hipGetLastError();
+    }
+  }
   if (a.splits > 8) klaunch(k_kv8_combine<D, F16, TRACK, 4>, (unsigned)all, 256, 0, s, a, width);
   else if (a.splits > 1) klaunch(k_kv8_combine<D, F16, TRACK, 1>, (unsigned)((all + 3) / 4), 256, 0, s, a, width);
-  if (TRACK) {
-    int P = 1;
-    while (P < cols && P < 64) P *= 2;
-    klaunch(k_kv8_mass, dim3((a.c.slots * P + 255) / 256, a.c.kvh, a.n_seqs), 256, 0, s, a, decay, P);
-  }
+  if (TRACK) klaunch(k_kv8_mass, dim3(per_head, a.c.kvh, a.n_seqs), 256, 0, s, a, decay, P);
   return hipGetLastError();
 }
 

@@ -15,6 +15,7 @@ import ctypes
 import json
 import math
 import os
+import struct
 import time
 from dataclasses import dataclass, field
 from typing import List, Optional
@@ -101,9 +102,7 @@ class moert_kv8(ctypes.Structure):
                 ("k_codes", "v_codes", "k_scale", "v_scale", "k_tail", "v_tail", "tail_bad", "table", "mass", "state")]
 
 
-class moert_rows(ctypes.Structure):
-    _fields_ = [("data_dev", ctypes.c_void_p), ("dtype", ctypes.c_int), ("seq_stride", ctypes.c_longlong),
-                ("pos_stride", ctypes.c_longlong), ("head_stride", ctypes.c_longlong)]
+_ROWS = struct.Struct("@Piqqq")  # moert_rows: address, dtype, strides; packing one takes a third of a Structure's time
 
 
 _lib = None
@@ -912,7 +911,7 @@ class Kv8:
 
     def _rows(self, at, dtype, strides, n, heads):
         s, p, h = strides or (n * heads * self.head_dim, heads * self.head_dim, self.head_dim)
-        return moert_rows(at, dtype, s, p, h)
+        return _ROWS.pack(at or 0, dtype, s, p, h)
 
     def clear(self, seq0: int = 0, n_seqs: Optional[int] = None, stream: int = 0) -> None:
         """Empties the sequences."""
@@ -923,8 +922,7 @@ class Kv8:
         """Appends n rows of each KV head to every sequence; one without room for them stays as it is."""
         kr = self._rows(k, dtype, strides, n, self.kv_heads)
         vr = self._rows(v, dtype, strides, n, self.kv_heads)
-        check(self._lib.moert_kv8_append(self._p, seq0, self._n(seq0, n_seqs), ctypes.addressof(kr),
-                                         ctypes.addressof(vr), n, stream))
+        check(self._lib.moert_kv8_append(self._p, seq0, self._n(seq0, n_seqs), kr, vr, n, stream))
 
     def workspace(self, heads: int, n: int = 1, n_seqs: Optional[int] = None, track: bool = False) -> int:
         """Bytes of workspace of an attention of n positions."""
@@ -940,8 +938,8 @@ class Kv8:
         the weights that the blocks get are added to the decayed mass."""
         qr = self._rows(q, dtype, q_strides, n, heads)
         orow = self._rows(out, dtype, out_strides, n, heads)
-        check(self._lib.moert_kv8_attend(self._p, seq0, self._n(seq0, n_seqs), heads, n, scale, ctypes.addressof(qr),
-                                         ctypes.addressof(orow), -1.0 if mass_decay is None else mass_decay, ws,
+        check(self._lib.moert_kv8_attend(self._p, seq0, self._n(seq0, n_seqs), heads, n, scale, qr, orow,
+                                         -1.0 if mass_decay is None else mass_decay, ws,
                                          ws_bytes, stream))
 
     def evict(self, keep: int, first: int = 0, last: int = 0, seq0: int = 0, n_seqs: Optional[int] = None,
@@ -954,8 +952,7 @@ class Kv8:
         """The values held for positions [pos, pos + n) (negative: from each sequence's end), 0 where there are none."""
         kr = self._rows(k, dtype, strides, n, self.kv_heads)
         vr = self._rows(v, dtype, strides, n, self.kv_heads)
-        check(self._lib.moert_kv8_read(self._p, seq0, self._n(seq0, n_seqs), pos, n, ctypes.addressof(kr),
-                                       ctypes.addressof(vr), stream))
+        check(self._lib.moert_kv8_read(self._p, seq0, self._n(seq0, n_seqs), pos, n, kr, vr, stream))
 
     def lengths(self, seq0: int = 0, n_seqs: Optional[int] = None, stream: int = 0) -> np.ndarray:
         """Lengths of the sequences (synchronises the stream); raises E_FULL where rows were dropped."""

@@ -1,6 +1,5 @@
 """The 8-bit K/V cache without a device: every refusal comes before anything is launched, the buffers' shapes, the
 layout of a block of V, and the definition that the GPU tests compare with (tests/kv8_util.py) against plain facts."""
-import ctypes
 import math
 
 import numpy as np
@@ -107,10 +106,10 @@ def test_bad_attentions_are_refused():
         need = c.workspace(4, 3, track=track)
         assert need > 0
         refused(lambda: CALLS["attend"](c, n=3, mass_decay=1.0 if track else None, ws_bytes=need - 1), "workspace")
-    rows = moert.moert_rows(0x20000, moert.F32, 256, 256, 64)
-    half = moert.moert_rows(0x20000, moert.F16, 256, 256, 64)
+    rows = c._rows(0x20000, moert.F32, None, 1, 4)
+    half = c._rows(0x20000, moert.F16, None, 1, 4)
     refused(lambda: moert.check(moert.lib().moert_kv8_attend(
-        c._p, 0, 2, 4, 1, 0.125, ctypes.addressof(rows), ctypes.addressof(half), -1.0, 0x30000, 1 << 30, None)), "dtype")
+        c._p, 0, 2, 4, 1, 0.125, rows, half, -1.0, 0x30000, 1 << 30, None)), "dtype")
     big = cache(seqs=65535, max_len=1 << 20)
     refused(lambda: big.workspace(64, 1 << 12), "sequences")
     with pytest.raises(moert.MoertError):
