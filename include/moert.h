@@ -403,8 +403,8 @@ int moert_attn_decode_noalloc(const float* q_dev, const uint16_t* k_cache_dev, c
  * replayed: each replay goes on from the lengths it finds. The buffers may be copied and put back as a whole. Kernels
  * keep to the buffers whatever table and state hold.
  *
- * Limits: head_dim 64 or 128; max_len a multiple of 32, at most 2^20; at most 65535 sequences, 256 KV heads. Calls
- * take sequences [seq0, seq0 + n_seqs). They enqueue on `stream` (a hipStream_t of the buffers' device, NULL for its
+ * Limits: head_dim 64 or 128; max_len a multiple of 32, at most 2^20; at most 65535 sequences, 256 KV heads, 64 query
+ * heads to each, and 2^28 query heads x positions x sequences in one attention. Calls take sequences [seq0, seq0 + n_seqs). They enqueue on `stream` (a hipStream_t of the buffers' device, NULL for its
  * default stream), allocate nothing and do not synchronise, except moert_kv8_lengths. Calls on one cache are ordered
  * by the caller (one stream, or events); attentions that do not track may overlap, each with a workspace of its own.
  * ------------------------------------------------------------------------------------------------------- */
@@ -437,8 +437,8 @@ int moert_kv8_clear(const moert_kv8* c, int seq0, int n_seqs, void* stream);
 int moert_kv8_append(const moert_kv8* c, int seq0, int n_seqs, const moert_rows* k, const moert_rows* v, int n,
                      void* stream);
 
-/* Bytes of workspace that an attention of n positions of `heads` query heads over n_seqs sequences needs (track: one
- * that adds to the mass). Nothing in it has to be kept or cleared between calls. */
+/* Bytes of workspace for attentions of at most n positions of `heads` query heads over at most n_seqs sequences (track:
+ * ones that add to the mass among them). Nothing in it has to be kept or cleared between calls. */
 int moert_kv8_workspace(const moert_kv8* c, int n_seqs, int heads, int n, int track, size_t* bytes);
 
 /* Attention of n positions over the cache, whose last n rows are theirs (appended before): position i of a sequence of

@@ -34,14 +34,29 @@ __device__ __forceinline__ uint4 row_halves(const KvRows& r, long long at, bool 
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// round(x / s), ties to even, of the exact quotient. x * inv is off by less than one step near a tie; the residual
-// x - q s (one fma) decides: next to a tie it is a multiple of ulp(s) / 2 below s, so it is exact there.
-__device__ __forceinline__ uint32_t code_of(float x, float s, float inv) {
-  float q = __builtin_rintf(x * inv);
-  const float r = __builtin_fmaf(-q, s, x), h = 0.5f * s;
-  const bool odd = (int)q & 1;
-  q += r > h || (r == h && odd) ? 1.0f : r < -h || (r == -h && odd) ? -1.0f : 0.0f;
-  return (uint32_t)((int)q + 128) & 255u;
+// round(x / s) + 128 of eight fp16 as bytes, ties to even, of the exact quotients. q = round(x * inv) is off by less
+// than one, next to a tie; there the residual x - q s (one fma) is a multiple of ulp(s) / 2 below s, so it is exact and
+// tells: below s / 2, q is right, and that is all that nearly every wave has to look at.
+__device__ __forceinline__ uint2 codes_of(const uint16_t* x, float s, float inv) {
+  const float h = 0.5f * s;
+  float q[8], r[8], most = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 8; i++) {
+    q[i] = __builtin_rintf(h2f(x[i]) * inv);
+    r[i] = __builtin_fmaf(-q[i], s, h2f(x[i]));
+    most = __builtin_fmaxf(most, __builtin_fabsf(r[i]));
+  }
+  if (__any(most >= h)) {
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      const float d = __builtin_fabsf(r[i]);
+      q[i] += d > h || (d == h && ((int)q[i] & 1)) ? __builtin_copysignf(1.0f, r[i]) : 0.0f;
+    }
+  }
+  uint32_t o[2] = {0u, 0u};
+#pragma unroll
+  for (int i = 0; i < 8; i++) o[i >> 2] = __builtin_amdgcn_cvt_pk_u8_f32(q[i] + 128.0f, i & 3, o[i >> 2]);
+  return make_uint2(o[0], o[1]);
 }
 
 // Largest magnitude of eight fp16, as bits.
@@ -87,19 +102,28 @@ __global__ __launch_bounds__(kAppendThreads) void k_kv8_append(Kv8Dev c, KvRows 
 #pragma unroll
     for (int j = 0; j < C; j++) {
       const int t = (x + 128 * j) / R, e = (x + 128 * j) % R * 8, row = b * kKvBlock - r + t;
-      if (row >= 0) {
-        q[j] = row_halves(in, base + row * in.pos + e, wide);
-      } else if (p == 0) {
-        q[j] = gload_u4(tail + t * D + e);
-      } else {
-        uint32_t w[4];
-#pragma unroll
-        for (int i = 0; i < 4; i++)
-          w[i] = (uint32_t)tail[v_place<D>(t, e + 2 * i)] | (uint32_t)tail[v_place<D>(t, e + 2 * i + 1)] << 16;
-        q[j] = make_uint4(w[0], w[1], w[2], w[3]);
-      }
+      if (row >= 0) q[j] = row_halves(in, base + row * in.pos + e, wide);
+      else if (p == 0) q[j] = gload_u4(tail + t * D + e);
+      else continue;
       top = max(top, top_of(q[j]));
       if (p) *reinterpret_cast<uint4*>(&lds[t][e]) = q[j];
+    }
+    if (p && b == 0 && r) {  // V's old tail, a run of 8 positions of an element at a time
+#pragma unroll
+      for (int j = 0; j < C; j++) {
+        const int i = x + 128 * j, t = i / U % 4 * 4, e = i / (4 * U) * U + i % U;
+        const uint4 y = gload_u4(tail + i * 8);
+        const uint32_t w[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+        for (int z = 0; z < 8; z++) {
+          const int tz = t + (z & 3) + 16 * (z >> 2);
+          const uint16_t a = (uint16_t)(w[z >> 1] >> (16 * (z & 1)));
+          if (tz < r) {
+            lds[tz][e] = a;
+            top = max(top, a & 0x7fff);
+          }
+        }
+      }
     }
     top = max(top, partner<1>(top));
     top = max(top, partner<2>(top));
@@ -111,23 +135,21 @@ __global__ __launch_bounds__(kAppendThreads) void k_kv8_append(Kv8Dev c, KvRows 
     __syncthreads();
     top = max(tops[2 * p], tops[2 * p + 1]);
     const bool bad = top >= 0x7c00;
-    const float sc8 = bad ? __int_as_float(0x7fc00000) : top ? h2f((uint16_t)top) / 127.0f : 1.0f, inv = 1.0f / sc8;
+    const float sc8 = top && !bad ? h2f((uint16_t)top) / 127.0f : 1.0f, inv = 1.0f / sc8;
     uint8_t* codes = (p ? c.vc : c.kc) + slot * (size_t)(kKvBlock * D);
 #pragma unroll
     for (int j = 0; j < C; j++) {
       const int i = x + 128 * j;
       const uint32_t w[4] = {q[j].x, q[j].y, q[j].z, q[j].w};
-      uint32_t o[2] = {0u, 0u};
+      uint16_t a[8];
 #pragma unroll
-      for (int y = 0; y < 8; y++) {
-        // V: run i is ((element / U) * 4 + group) * U + element % U
-        const uint16_t a = p ? lds[i / U % 4 * 4 + (y & 3) + 16 * (y >> 2)][i / (4 * U) * U + i % U]
-                             : (uint16_t)(w[y >> 1] >> (16 * (y & 1)));
-        o[y >> 2] |= (bad ? 128u : code_of(h2f(a), sc8, inv)) << (8 * (y & 3));
-      }
-      *reinterpret_cast<uint2*>(codes + i * 8) = make_uint2(o[0], o[1]);
+      for (int y = 0; y < 8; y++)  // V: run i is ((element / U) * 4 + group) * U + element % U
+        a[y] = p ? lds[i / U % 4 * 4 + (y & 3) + 16 * (y >> 2)][i / (4 * U) * U + i % U]
+                 : (uint16_t)(w[y >> 1] >> (16 * (y & 1)));
+      const uint2 o = codes_of(a, sc8, inv);
+      *reinterpret_cast<uint2*>(codes + i * 8) = bad ? make_uint2(0x80808080u, 0x80808080u) : o;
     }
-    if (x == 0) (p ? c.vs : c.ks)[slot] = sc8;
+    if (x == 0) (p ? c.vs : c.ks)[slot] = bad ? __int_as_float(0x7fc00000) : sc8;
   }
   if (b == 0) {  // rows [t0, t1) of the tail that is there after the call
     const int t0 = whole ? 0 : r, t1 = whole ? (r + n) % kKvBlock : r + n;
@@ -211,9 +233,17 @@ __global__ __launch_bounds__(256) void k_kv8_read(Kv8Dev c, KvRows k, KvRows v, 
     }
   } else if (in) {
     const uint16_t* t16 = (p ? c.vt : c.kt) + head * kKvBlock * D;
-    for (int i = x; i < kKvBlock * D; i += 128) {
-      const int t = i / D, e = i % D;
-      lds[p][t][e] = h2f(t16[p ? v_place<D>(t, e) : i]);
+#pragma unroll
+    for (int j = 0; j < C; j++) {
+      const int i = x + 128 * j;
+      const uint4 q = gload_u4(t16 + i * 8);
+      const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+      for (int y = 0; y < 8; y++) {
+        const float z = h2f((uint16_t)(w[y >> 1] >> (16 * (y & 1))));
+        if (p) lds[1][i / U % 4 * 4 + (y & 3) + 16 * (y >> 2)][i / (4 * U) * U + i % U] = z;
+        else lds[0][i / R][i % R * 8 + y] = z;
+      }
     }
   }
   __syncthreads();
@@ -284,12 +314,12 @@ __device__ int block_prefix(int v, int* waves, int* total) {
 
 // A workgroup per head. Thread i holds blocks i KPT .. i KPT + KPT - 1 (their table entries and mass keys, in
 // registers, so the table can be rewritten in place once all have been read). The key of the last block that stays is
-// found 8 bits at a time by counting; among blocks of that key the earlier stay.
+// found by counting, 11, 11 and 10 bits at a time (the first take masses apart by a fifth, so that few counts meet in
+// one bin: 13.8 us with 8 bits four times, 12.1 so, 4062 blocks of 128 heads); among blocks of that key the earlier stay.
 template <int KPT>
 __global__ __launch_bounds__(kEvictThreads) void k_kv8_evict(Kv8Dev c, int seq0, int keep, int first, int last) {
-  __shared__ __align__(16) int hist[256];
+  __shared__ __align__(16) int hist[2048];
   __shared__ int waves[kEvictThreads / 64], pick[2];
-  const int lane = threadIdx.x & 63;
   const int s = seq0 + blockIdx.x / c.kvh, len = kv_len(c, s), nb = len / kKvBlock;
   if (nb <= keep) return;
   const size_t base = ((size_t)s * c.kvh + blockIdx.x % c.kvh) * c.slots;
@@ -304,48 +334,39 @@ __global__ __launch_bounds__(kEvictThreads) void k_kv8_evict(Kv8Dev c, int seq0,
   }
   int left = keep - first - last;  // blocks that stay of those that may leave
   uint32_t pre = 0;                // bits of the key of the last that stays, from the top
-  for (int sh = 24; sh >= 0 && left > 0; sh -= 8) {
-    if (threadIdx.x < 256) hist[threadIdx.x] = 0;
+#pragma unroll
+  for (int pass = 0; pass < 3; pass++) {
+    if (left <= 0) break;  // the same for all
+    const int sh = pass == 0 ? 21 : pass == 1 ? 10 : 0, bins = pass == 2 ? 1024 : 2048;
+    hist[threadIdx.x] = 0;
+    hist[threadIdx.x + kEvictThreads] = 0;
     __syncthreads();
 #pragma unroll
     for (int j = 0; j < KPT; j++) {
       const int i = i0 + j;
-      if (i >= first && i < nb - last && (sh == 24 || key[j] >> (sh + 8) == pre >> (sh + 8)))
-        atomicAdd(&hist[key[j] >> sh & 255u], 1);
+      if (i >= first && i < nb - last && (pass == 0 || (key[j] ^ pre) >> (sh + (pass == 1 ? 11 : 10)) == 0))
+        atomicAdd(&hist[key[j] >> sh & (bins - 1)], 1);
     }
     __syncthreads();
-    if (threadIdx.x < 64) {  // lane x: bins 255 - 4 x and the three below
-      const int4 q = *reinterpret_cast<const int4*>(&hist[252 - 4 * lane]);
-      const int v[4] = {q.w, q.z, q.y, q.x}, mine = q.x + q.y + q.z + q.w;
-      int above = mine;
-#pragma unroll
-      for (int m = 1; m < 64; m <<= 1) {
-        const int y = __shfl_up(above, m);
-        if (lane >= m) above += y;
-      }
-      above -= mine;  // keys in the bins above this lane's
-#pragma unroll
-      for (int j = 0; j < 4; j++) {
-        if (above < left && above + v[j] >= left) {  // true of one bin
-          pick[0] = 255 - 4 * lane - j;
-          pick[1] = above;
-        }
-        above += v[j];
-      }
-    }
+    const int hi = 2047 - 2 * (int)threadIdx.x;  // this thread's bins: hi and hi - 1
+    const int2 v = *reinterpret_cast<const int2*>(&hist[hi - 1]);
+    int total, above = block_prefix(v.x + v.y, waves, &total);  // keys in the bins above them
+    if (above < left && above + v.y >= left) pick[0] = hi, pick[1] = above;
+    above += v.y;
+    if (above < left && above + v.x >= left) pick[0] = hi - 1, pick[1] = above;
     __syncthreads();
     pre |= (uint32_t)pick[0] << sh;
     left -= pick[1];
   }
   // `left` blocks of key `pre` stay, and all above it
   bool may[KPT], stays[KPT];
-  int same = 0, total;
+  int same = 0;
 #pragma unroll
   for (int j = 0; j < KPT; j++) {
     may[j] = i0 + j >= first && i0 + j < nb - last;
     same += may[j] && left > 0 && key[j] == pre ? 1 : 0;
   }
-  int before = block_prefix(same, waves, &total), stay = 0;
+  int total, before = block_prefix(same, waves, &total), stay = 0;
 #pragma unroll
   for (int j = 0; j < KPT; j++) {
     const bool eq = may[j] && left > 0 && key[j] == pre;
@@ -386,7 +407,7 @@ hipError_t launch_kv8_clear(hipStream_t s, const Kv8Dev& c, int seq0, int n_seqs
 
 hipError_t launch_kv8_append(hipStream_t s, const Kv8Dev& c, int seq0, int n_seqs, KvRows k, KvRows v, int n) {
   const int blocks = (kKvBlock - 1 + n) / kKvBlock, vec = wide_rows(k) | wide_rows(v) << 1;
-  const int arrive = blocks * c.kvh <= 64;
+  const int arrive = blocks * c.kvh <= 256;
   const dim3 grid(blocks * c.kvh, n_seqs);
   if (c.d == 64) klaunch(k_kv8_append<64>, grid, kAppendThreads, 0, s, c, k, v, seq0, n, blocks, vec, arrive);
   else klaunch(k_kv8_append<128>, grid, kAppendThreads, 0, s, c, k, v, seq0, n, blocks, vec, arrive);

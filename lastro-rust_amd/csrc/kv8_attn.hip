@@ -170,6 +170,42 @@ __global__ __launch_bounds__(kWaves * 64, NT == 1 && D == 64 ? 4 : 2) void k_kv8
   if (split >= used) return;
   const size_t col0 = (size_t)hs * cols;  // of the workspace's columns
 
+  // The wave's blocks, 64 at a time, lane x holding the x-th one's slot and scales. The first are asked for before the
+  // queries are looked at.
+  const int full = min(seen, len / kKvBlock);  // blocks that are coded
+  int slot_l = 0, count = 0;
+  float ks_l = 0.0f, lvs_l = 0.0f, ivs_l = 0.0f;
+  uint4 kb[PF][2 * CH], vb[PF][2 * CH];
+  auto batch = [&](int base) {
+    if (base != b0) raw = table[min(base + lane * step, c.slots - 1)];
+    slot_l = kv_slot(c, raw);
+    const size_t sl = head * c.slots + slot_l;
+    // a V that is not finite makes the scores NaN, not the scale: columns that see none of the block are masked there
+    const float vs_r = c.vs[sl], ks_r = c.ks[sl], vs_l = vs_r == vs_r ? vs_r : 1.0f;
+    ks_l = vs_r == vs_r ? ks_r : vs_r;
+    lvs_l = __builtin_amdgcn_logf(vs_l);
+    ivs_l = 1.0f / vs_l;
+    count = min(64, (full - base + step - 1) / step);
+  };
+  auto fetch = [&](int p, int x) {
+    const int slot = __builtin_amdgcn_readlane(slot_l, min(x, count - 1));
+    const size_t at = (head * c.slots + slot) * (size_t)(kKvBlock * D);
+    const uint8_t* kp = c.kc + at + col16 * D + G * 16;
+    const uint8_t* vp = c.vc + at + (col16 * 4 + G) * (U * 8);
+#pragma unroll
+    for (int y = 0; y < 2; y++)
+#pragma unroll
+      for (int z = 0; z < CH; z++) {
+        kb[p][y * CH + z] = STREAM ? gload_u4_nt(kp + y * 16 * D + z * 64) : gload_u4(kp + y * 16 * D + z * 64);
+        vb[p][y * CH + z] = STREAM ? gload_u4_nt(vp + (y * CH + z) * 16) : gload_u4(vp + (y * CH + z) * 16);
+      }
+  };
+  if (b0 < full) {
+    batch(b0);
+#pragma unroll
+    for (int p = 0; p < PF; p++) fetch(p, p);
+  }
+
   // queries and the rows that each column sees
   h8 qh[NT][KS], ql[NT][F16 ? 1 : KS];
   float kf[NT];
@@ -341,30 +377,12 @@ __global__ __launch_bounds__(kWaves * 64, NT == 1 && D == 64 ? 4 : 2) void k_kv8
     }
   };
 
-  const int full = min(seen, len / kKvBlock);  // blocks that are coded
   for (int base = b0; base < full; base += 64 * step) {
-    // lane x: slot and scales of this wave's x-th block from here
-    if (base != b0) raw = table[min(base + lane * step, c.slots - 1)];
-    const int slot_l = kv_slot(c, raw);
-    const size_t sl = head * c.slots + slot_l;
-    // a V that is not finite makes the scores NaN, not the scale: columns that see none of the block are masked there
-    const float vs_r = c.vs[sl], vs_l = vs_r == vs_r ? vs_r : 1.0f, ks_l = vs_r == vs_r ? c.ks[sl] : vs_r;
-    const float lvs_l = __builtin_amdgcn_logf(vs_l), ivs_l = 1.0f / vs_l;
-    const int count = min(64, (full - base + step - 1) / step);
-    uint4 kb[PF][2 * CH], vb[PF][2 * CH];
-    auto fetch = [&](int p, int x) {
-      const int slot = __builtin_amdgcn_readlane(slot_l, min(x, count - 1));
-      const size_t at = (head * c.slots + slot) * (size_t)(kKvBlock * D);
-      const uint8_t* kp = c.kc + at + col16 * D + G * 16;
-      const uint8_t* vp = c.vc + at + (col16 * 4 + G) * (U * 8);
+    if (base != b0) {
+      batch(base);
 #pragma unroll
-      for (int y = 0; y < 2; y++)
-#pragma unroll
-        for (int z = 0; z < CH; z++) {
-          kb[p][y * CH + z] = STREAM ? gload_u4_nt(kp + y * 16 * D + z * 64) : gload_u4(kp + y * 16 * D + z * 64);
-          vb[p][y * CH + z] = STREAM ? gload_u4_nt(vp + (y * CH + z) * 16) : gload_u4(vp + (y * CH + z) * 16);
-        }
-    };
+      for (int p = 0; p < PF; p++) fetch(p, p);
+    }
     auto run = [&](auto masked, int p, int x) {
       auto kop = [&](int y, int k) {
         const uint4 v = kb[p][y * CH + (k >> 1)];
@@ -380,19 +398,15 @@ __global__ __launch_bounds__(kWaves * 64, NT == 1 && D == 64 ? 4 : 2) void k_kv8
     };
     // the blocks that every column sees all of, and those that some see a part of
     const int whole = max(0, min(count, (sees0 / kKvBlock - base + step - 1) / step));
-    if (whole) {
+    for (int x = 0; x < whole; x += PF) {
 #pragma unroll
-      for (int p = 0; p < PF; p++) fetch(p, p);
-      for (int x = 0; x < whole; x += PF) {
-#pragma unroll
-        for (int p = 0; p < PF; p++) {
-          if (x + p < whole) run(std::false_type(), p, x + p);
-          fetch(p, x + p + PF);
-        }
+      for (int p = 0; p < PF; p++) {
+        if (x + p < whole) run(std::false_type(), p, x + p);
+        fetch(p, x + p + PF);
       }
     }
     for (int x = whole; x < count; x++) {
-      fetch(0, x);
+      if (x) fetch(0, x);
       run(std::true_type(), 0, x);
     }
   }
@@ -534,7 +548,16 @@ __device__ __forceinline__ void mass_block(const AttnArgs& a, int hs, int b, int
   const int i0 = max(0, b * kKvBlock - (len - a.n));  // the first position that sees any of the block
   const float* lse = a.lse + ((size_t)hs * c.slots + b) * cols;
   float w = 0.0f;
-  for (int col = i0 * a.g + x; col < cols; col += P) w += __builtin_amdgcn_exp2f(lse[col] - tot[col]);
+  for (int col = i0 * a.g + x; col < cols; col += 4 * P) {  // four loads in flight; past the last column its own, for 0
+    float y[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      const int at = min(col + j * P, cols - 1);
+      y[j] = lse[at] - tot[at];
+    }
+#pragma unroll
+    for (int j = 0; j < 4; j++) w += col + j * P < cols ? __builtin_amdgcn_exp2f(y[j]) : 0.0f;
+  }
   for (int m = P / 2; m; m >>= 1) w += __shfl_xor(w, m);
   if (x) return;
   float* m = c.mass + head * c.slots + kv_slot(c, c.table[head * c.slots + b]);
@@ -578,17 +601,21 @@ KvAttnPlan kv8_attn_plan(const Kv8Dev& c, int n_seqs, int heads, int n, bool tra
   const size_t cols = (size_t)n_seqs * heads * n;
   const long long units = (long long)n_seqs * c.kvh * tiles;
   // Splits cost a second launch and the partials' way through memory: one workgroup for each of 256 compute units, and
-  // more (up to 1024, four to a unit) only while a wave keeps 16 blocks of a full cache; never fewer than 3 a wave.
-  const int cap = c.slots / (kWaves * 3);
+  // more (up to 1024, four to a unit) only while a wave keeps 16 blocks of a full cache; never fewer than 3 a wave. With
+  // 1024 workgroups wherever they could be had, sixteen sequences of wide heads took 37 us for 25, 300 positions after
+  // 1000 in f32 77 for 19; with 256 at most, eight sequences of up to 100003 take 173 for 115.
+  const int cap = c.slots / (kWaves * 3), most = cap < 1 ? 1 : cap > kMaxSplits ? kMaxSplits : cap;
   long long s = 256 / units > 1 ? 256 / units : 1;
   while (2 * s * units <= 1024 && c.slots / (2 * s * kWaves) >= 16) s *= 2;
-  s = s < cap ? s : cap;
-  p.splits = (int)(s < 1 ? 1 : s > kMaxSplits ? kMaxSplits : s);
+  p.splits = (int)(s < most ? s : most);
+  // Sizes that grow with every argument, so that a workspace does for all smaller calls: splits * units is at most 1024,
+  // a unit at most 32 columns.
+  const size_t shares = most > 1 ? (cols * most < 32768 ? cols * most : 32768) : 0;
   auto up = [](size_t x) { return (x + 255) / 256 * 256; };
   p.tot = 0;
   p.ml = up(cols * 4);
-  p.parts = p.ml + (p.splits > 1 ? up(cols * p.splits * 8) : 0);
-  p.lse = p.parts + (p.splits > 1 ? up(cols * p.splits * c.d * 4) : 0);
+  p.parts = p.ml + up(shares * 8);
+  p.lse = p.parts + up(shares * c.d * 4);
   p.bytes = p.lse + (track ? cols * c.slots * 4 : 0);
   return p;
 }

@@ -183,3 +183,17 @@ def test_the_definition_of_evictions():
     assert c.len(0) == 5 * 32 + 7
     c.evict(9, 0, 0)
     assert c.len(0) == 5 * 32 + 7
+
+
+def test_a_workspace_does_for_every_smaller_attention():
+    rng = np.random.default_rng(6)
+    for _ in range(300):
+        seqs, kv_heads, group = int(rng.integers(1, 40)), int(rng.integers(1, 9)), int(rng.integers(1, 9))
+        c = cache(seqs=seqs, kv_heads=kv_heads, head_dim=int(rng.choice([64, 128])),
+                  max_len=32 * int(2 ** rng.uniform(0, 12)))
+        n = int(rng.integers(1, c.max_len + 1))
+        a, b = int(rng.integers(1, seqs + 1)), int(rng.integers(1, n + 1))
+        heads = kv_heads * group
+        for track in (False, True):
+            assert c.workspace(heads, b, n_seqs=a, track=track) <= c.workspace(heads, n, n_seqs=seqs, track=track)
+            assert c.workspace(heads, b, n_seqs=a) <= c.workspace(heads, b, n_seqs=a, track=True)
