@@ -403,8 +403,9 @@ int moert_attn_decode_noalloc(const float* q_dev, const uint16_t* k_cache_dev, c
  * replayed: each replay goes on from the lengths it finds. The buffers may be copied and put back as a whole. Kernels
  * keep to the buffers whatever table and state hold.
  *
- * Limits: head_dim 64 or 128; max_len a multiple of 32, at most 2^20; at most 65535 sequences, 256 KV heads, 64 query
- * heads to each, and 2^28 query heads x positions x sequences in one attention. Calls take sequences [seq0, seq0 + n_seqs). They enqueue on `stream` (a hipStream_t of the buffers' device, NULL for its
+ * Limits: head_dim 64 or 128; max_len a multiple of 32, at most 2^20; at most 65535 sequences, 256 KV heads and 2^20
+ * KV heads of all sequences together, 64 query heads to a KV head, and 2^27 query heads x positions x sequences in one
+ * attention. Calls take sequences [seq0, seq0 + n_seqs). They enqueue on `stream` (a hipStream_t of the buffers' device, NULL for its
  * default stream), allocate nothing and do not synchronise, except moert_kv8_lengths. Calls on one cache are ordered
  * by the caller (one stream, or events); attentions that do not track may overlap, each with a workspace of its own.
  * ------------------------------------------------------------------------------------------------------- */

@@ -465,7 +465,8 @@ constexpr int kKvMaxLen = 1 << 20, kKvMaxSeqs = 65535, kKvMaxHeads = 256;
 int view(const char* what, const moert_kv8* c, int seq0, int n_seqs, bool mass, Kv8Dev* d) {
   KV_CFG(c, "%s: null cache", what);
   KV_CFG(c->seqs >= 1 && c->seqs <= kKvMaxSeqs && c->kv_heads >= 1 && c->kv_heads <= kKvMaxHeads &&
-             (c->head_dim == 64 || c->head_dim == 128) && c->max_len >= kKvBlock && c->max_len % kKvBlock == 0 &&
+             (long long)c->seqs * c->kv_heads <= 1 << 20 && (c->head_dim == 64 || c->head_dim == 128) &&
+             c->max_len >= kKvBlock && c->max_len % kKvBlock == 0 &&
              c->max_len <= kKvMaxLen,
          "%s: %d sequences, %d KV heads of %d, max_len %d", what, c->seqs, c->kv_heads, c->head_dim, c->max_len);
   KV_CFG(c->k_codes_dev && c->v_codes_dev && c->k_scale_dev && c->v_scale_dev && c->k_tail_dev && c->v_tail_dev &&
@@ -598,7 +599,7 @@ static int attend_shape(const char* what, const Kv8Dev& d, int n_seqs, int heads
   KV_CFG(heads >= 1 && heads % d.kvh == 0 && heads / d.kvh <= 64, "%s: %d query heads over %d KV heads", what, heads,
          d.kvh);
   KV_CFG(n >= 1 && n <= d.max_len, "%s: %d positions, max_len %d", what, n, d.max_len);
-  KV_CFG((long long)n_seqs * heads * n <= 1 << 28, "%s: %d sequences x %d positions x %d heads", what, n_seqs, n, heads);
+  KV_CFG((long long)n_seqs * heads * n <= 1 << 27, "%s: %d sequences x %d positions x %d heads", what, n_seqs, n, heads);
   return MOERT_OK;
 }
 

@@ -270,6 +270,7 @@ __global__ __launch_bounds__(kWaves * 64, NT == 1 && D == 64 ? 4 : 2) void k_kv8
   auto block = [&](auto masked, auto kop, auto vop, float ks, float lvs, float ivs, int b, uint32_t bad) {
     constexpr bool MASKED = decltype(masked)::value;
     f4 S[NT][2];
+    if constexpr (NT > 1) __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int x = 0; x < 2; x++) {
 #pragma unroll
@@ -296,6 +297,7 @@ __global__ __launch_bounds__(kWaves * 64, NT == 1 && D == 64 ? 4 : 2) void k_kv8
             if (b * kKvBlock + row >= sees[t]) S[t][x][i] = -3e38f;
           }
     }
+    if constexpr (NT > 1) __builtin_amdgcn_s_setprio(0);
     float f[NT], mx[NT];
     bool move = false;
 #pragma unroll
@@ -349,6 +351,7 @@ __global__ __launch_bounds__(kWaves * 64, NT == 1 && D == 64 ? 4 : 2) void k_kv8
       }
     }
     f4 sum[NT];
+    if constexpr (NT > 1) __builtin_amdgcn_s_setprio(1);
     if constexpr (!VSUM) {
 #pragma unroll
       for (int t = 0; t < NT; t++) {
@@ -365,6 +368,7 @@ __global__ __launch_bounds__(kWaves * 64, NT == 1 && D == 64 ? 4 : 2) void k_kv8
         if constexpr (!F16) O[t][u] = mfma(va, pl[t], O[t][u]);
       }
     }
+    if constexpr (NT > 1) __builtin_amdgcn_s_setprio(0);
 #pragma unroll
     for (int t = 0; t < NT; t++) l[t] = __builtin_fmaf(VSUM ? part[t] : sum[t][0], ivs, l[t]);
     if constexpr (TRACK) {  // lanes of group 0 write tile 0's, those of group 2 tile 1's
@@ -574,7 +578,7 @@ __global__ __launch_bounds__(256) void k_kv8_mass(AttnArgs a, float decay, int P
 // the columns' sums from the splits' again instead of waiting for them.
 template <int D, bool F16, int C>
 __global__ __launch_bounds__(256) void k_kv8_finish(AttnArgs a, int width, int combines, int per_head, float decay,
-                                                    int P) {
+                                                    int P) {  // per_head: workgroups for the masses of a head
   __shared__ float Os[4][D], tot[16];
   if ((int)blockIdx.x < combines) {
     combine_column<D, F16, false, C>(a, width, blockIdx.x, Os);
@@ -628,7 +632,6 @@ hipError_t attend(hipStream_t s, AttnArgs a, float decay) {
   a.tiles = (cols + width - 1) / width;
   const long long units = (long long)a.n_seqs * a.c.kvh * a.splits;
   const long long grid = (units + 7) / 8 * 8 * a.tiles;
-  if (grid > 0x7fffffff) return hipErrorInvalidValue;
   // A cache that can outgrow the 256 MB last-level cache is streamed past the others: 124 -> 119 us for 565 MB of eight
   // sequences in 839 MB; in smaller ones the hint costs what a step finds there of the last (26.6 -> 32.3 us for 68 MB).
   const bool stream = nt == 1 && 2ll * a.n_seqs * a.c.kvh * a.c.max_len * D > 256ll << 20;
@@ -640,13 +643,13 @@ hipError_t attend(hipStream_t s, AttnArgs a, float decay) {
   while (P < cols && P < 64) P *= 2;
   const int per_head = (a.c.slots * P + 255) / 256;
   if (TRACK && a.splits > 1 && cols <= 16) {
+    // splits mean fewer than 1024 heads: the grid stays small. (A fifth as many workgroups, each with more blocks of a
+    // head, took 11.6 us for 9.4: the blocks' loads wait for each other.)
     const int C = a.splits > 8 ? 4 : 1, combines = (int)((all * C + 3) / 4);
-    const long long both = combines + (long long)a.n_seqs * a.c.kvh * per_head;
-    if (both <= 0x7fffffff) {
-      if (C == 4) klaunch(k_kv8_finish<D, F16, 4>, (unsigned)both, 256, 0, s, a, width, combines, per_head, decay, P);
-      else klaunch(k_kv8_finish<D, F16, 1>, (unsigned)both, 256, 0, s, a, width, combines, per_head, decay, P);
-      return hipGetLastError();
-    }
+    const unsigned both = (unsigned)(combines + all / cols * per_head);
+    if (C == 4) klaunch(k_kv8_finish<D, F16, 4>, both, 256, 0, s, a, width, combines, per_head, decay, P);
+    else klaunch(k_kv8_finish<D, F16, 1>, both, 256, 0, s, a, width, combines, per_head, decay, P);
+    return hipGetLastError();
   }
   if (a.splits > 8) klaunch(k_kv8_combine<D, F16, TRACK, 4>, (unsigned)all, 256, 0, s, a, width);
   else if (a.splits > 1) klaunch(k_kv8_combine<D, F16, TRACK, 1>, (unsigned)((all + 3) / 4), 256, 0, s, a, width);

@@ -218,13 +218,14 @@ class Device:
     """A cache in device buffers, beside moert.Kv8: uploads, workspaces, what the buffers hold as the definition's."""
 
     def __init__(self, hip, seqs, kv_heads, d, max_len, fill=True):
+        """fill: with random bytes, as whatever was there before; without, large buffers stay as they come."""
         self.hip, self.d = hip, d
         self.shapes = moert.kv8_shapes(seqs, kv_heads, d, max_len)
         rng = np.random.default_rng(5)
         self.at = {}
         for name, (shape, dtype) in self.shapes.items():  # whatever was there before: clear makes it a cache
             n = int(np.prod(shape)) * np.dtype(dtype).itemsize
-            self.at[name] = hip.upload(rng.integers(0, 256, n, dtype=np.uint8) if fill else np.zeros(n, np.uint8))
+            self.at[name] = hip.upload(rng.integers(0, 256, n, dtype=np.uint8)) if fill else hip.alloc(n)
         self.c = moert.Kv8(seqs, kv_heads, d, max_len, self.at)
         self.c.clear()
         self.ws = {}

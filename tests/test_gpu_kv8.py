@@ -238,6 +238,65 @@ def test_long_contexts_in_many_splits(hip, n):
         check_attend(dev, ref, normal(rng, 1, n, 6, 64, scale=3.0), 0.125, dtype, decay=1.0)
 
 
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("dtype", [moert.F32, moert.F16])
+def test_one_long_sequence_among_many(hip, d, dtype):
+    """128 sequences, most of a few rows or none, one of 9001: no splits, and more blocks to a wave than one of its
+    rounds of 64 holds."""
+    S, H, g = 128, 8, 2
+    dev, ref = ku.Device(hip, S, H, d, 9216, fill=False), ku.Cache(S, H, d, 9216)
+    rng = np.random.default_rng(21)
+    for s, m in ((5, 9001), (0, 1), (17, 33), (64, 64), (127, 300)):
+        k, v = normal(rng, 1, m, H, d), normal(rng, 1, m, H, d)
+        dev.append(k, v, seq0=s)
+        ref.append(k, v, s)
+    q = normal(rng, S, 1, H * g, d, scale=2.0)
+    got = check_attend(dev, ref, q, d ** -0.5, dtype, decay=1.0)
+    assert not got[[1, 2, 100]].any()
+    got = check_attend(dev, ref, q, d ** -0.5, dtype)
+    assert got[5].all()
+
+
+def test_offsets_beyond_32_bits(hip):
+    """Five sequences of 2^20 positions and 1 GiB of K codes each, the last one's blocks in its last slots."""
+    S, H, d, max_len = 5, 8, 128, 1 << 20
+    dev, ref = ku.Device(hip, S, H, d, max_len, fill=False), ku.Cache(S, H, d, max_len)
+    table = dev.array("table")
+    dev.set("table", table[:, :, ::-1].copy())
+    rng = np.random.default_rng(22)
+    for m in (150, 1, 60, 200):
+        k, v = normal(rng, 1, m, H, d), normal(rng, 1, m, H, d)
+        dev.append(k, v, seq0=4)
+        ref.append(k, v, 4)
+        for dtype in (moert.F32, moert.F16):
+            check_attend(dev, ref, normal(rng, 1, 1, H * 2, d), 0.1, dtype, decay=1.0, seq0=4)
+    check_attend(dev, ref, normal(rng, 1, 5, H * 8, d), 0.1, moert.F16, decay=1.0, seq0=4)
+    dev.c.evict(6, first=1, last=1, seq0=4)
+    ref.evict(6, 1, 1, 4, 1)
+    assert dev.c.lengths().tolist() == [0, 0, 0, 0, 6 * 32 + 411 % 32]
+    check_attend(dev, ref, normal(rng, 1, 3, H * 2, d), 0.1, decay=1.0, seq0=4)
+    k, v = normal(rng, 1, 40, H, d), normal(rng, 1, 40, H, d)
+    dev.append(k, v, seq0=4)
+    ref.append(k, v, 4)
+    shape = (1, 240, H, d)
+    at = [hip.alloc(int(np.prod(shape)) * 4) for _ in range(2)]
+    dev.c.read(at[0], at[1], 0, 240, seq0=4, n_seqs=1)
+    hip.sync()
+    for x, want in zip(at, ref.read(4, 0, 240)):
+        assert np.array_equal(hip.get(x, shape, np.float32)[0], want.astype(np.float32))
+
+
+def test_a_scale_of_zero_weighs_every_row_alike(hip):
+    dev, ref = both(hip, 1, 2, 64, 256)
+    rng = np.random.default_rng(23)
+    r = normal(rng, 2, 1, 203, 2, 64)
+    dev.append(r[0], r[1])
+    ref.append(r[0], r[1])
+    for n in (1, 40):
+        for dtype in (moert.F32, moert.F16):
+            check_attend(dev, ref, normal(rng, 1, n, 4, 64), 0.0, dtype, decay=1.0)
+
+
 def test_scales_far_apart(hip):
     """Blocks of V whose scales differ by 2^30, with the attention on the small ones: sums keep what the type holds.
     Queries from 2^-60 to 2^60 beside keys that make ordinary scores."""
@@ -466,6 +525,43 @@ def test_a_captured_step_replays_from_the_lengths_it_finds(hip):
     with pytest.raises(moert.MoertError) as e:
         hip.capture(stream, lambda: one.c.lengths(stream=stream))
     assert e.value.code == moert.E_CONFIG
+
+
+def test_two_graphs_of_one_cache_and_workspace(hip):
+    """A graph that appends and attends with five positions and one that only attends with masses, sharing the
+    workspace, replayed in turn on one stream; against the same calls made one by one."""
+    rng = np.random.default_rng(20)
+    S, H, g, d, max_len, n = 2, 2, 4, 64, 512, 5
+    one, two = (ku.Device(hip, S, H, d, max_len) for _ in range(2))
+    stream = hip.stream()
+    k, v, q = (hip.alloc(S * n * x * d * 2) for x in (H, H, H * g))
+    size = one.c.workspace(H * g, n, track=True)
+    ws = hip.alloc(size)
+    outs = [[hip.alloc(S * n * H * g * d * 2) for _ in range(2)] for _ in range(2)]
+
+    def chunk(dev, o, s):
+        dev.c.append(k, v, n, dtype=moert.F16, stream=s)
+        dev.c.attend(q, o[0], H * g, n, 0.125, ws, size, dtype=moert.F16, stream=s)
+
+    def last(dev, o, s):
+        dev.c.attend(q, o[1], H * g, 1, 0.125, ws, size, dtype=moert.F16, mass_decay=0.5, stream=s)
+
+    hip.sync()
+    graphs = [hip.capture(stream, lambda: f(one, outs[0], stream)) for f in (chunk, last)]
+    for i in range(30):
+        for at, heads in ((k, H), (v, H), (q, H * g)):
+            hip.put(at, normal(rng, S, n, heads, d).astype(np.float16))
+        for graph in graphs:
+            hip.launch(graph, stream)
+        hip.sync()
+        chunk(two, outs[1], 0)
+        last(two, outs[1], 0)
+        hip.sync()
+        for j, m in ((0, n), (1, 1)):
+            a, b = (hip.get(o[j], (S, m, H * g, d), np.float16) for o in outs)
+            assert np.array_equal(a, b) and a.any(), (i, j)
+    assert np.array_equal(one.array("mass"), two.array("mass"))
+    assert one.c.lengths().tolist() == [150, 150]
 
 
 def test_attentions_on_two_streams(hip):

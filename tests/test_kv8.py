@@ -40,7 +40,7 @@ def refused(call, what):
 @pytest.mark.parametrize("name", sorted(CALLS))
 def test_bad_caches_are_refused(name):
     call = CALLS[name]
-    for bad in (dict(seqs=0), dict(seqs=65536), dict(kv_heads=0), dict(kv_heads=257), dict(head_dim=32),
+    for bad in (dict(seqs=0), dict(seqs=65536), dict(kv_heads=0), dict(kv_heads=257), dict(seqs=8192, kv_heads=129), dict(head_dim=32),
                 dict(head_dim=96), dict(max_len=0), dict(max_len=95), dict(max_len=(1 << 20) + 32)):
         refused(lambda: call(cache(**bad), seq0=0, n_seqs=1), "kv8_" + name)
     for buf in ("k_codes", "v_codes", "k_scale", "v_scale", "k_tail", "v_tail", "tail_bad", "table", "state"):
