@@ -174,18 +174,21 @@ __global__ __launch_bounds__(kWaves * 64, NT == 1 && D == 64 ? 4 : 2) void k_kv8
   // queries are looked at.
   const int full = min(seen, len / kKvBlock);  // blocks that are coded
   int slot_l = 0, count = 0;
-  float ks_l = 0.0f, lvs_l = 0.0f, ivs_l = 0.0f;
+  float ks_l = 0.0f, vs_l = 0.0f, lvs_l = 0.0f, ivs_l = 0.0f;
   uint4 kb[PF][2 * CH], vb[PF][2 * CH];
-  auto batch = [&](int base) {
+  auto batch = [&](int base) {  // scales() follows, behind the loads of the first blocks
     if (base != b0) raw = table[min(base + lane * step, c.slots - 1)];
     slot_l = kv_slot(c, raw);
     const size_t sl = head * c.slots + slot_l;
+    vs_l = gmem(c.vs)[sl];
+    ks_l = gmem(c.ks)[sl];
+    count = min(64, (full - base + step - 1) / step);
+  };
+  auto scales = [&]() {
     // a V that is not finite makes the scores NaN, not the scale: columns that see none of the block are masked there
-    const float vs_r = c.vs[sl], ks_r = c.ks[sl], vs_l = vs_r == vs_r ? vs_r : 1.0f;
-    ks_l = vs_r == vs_r ? ks_r : vs_r;
+    if (vs_l != vs_l) ks_l = vs_l, vs_l = 1.0f;
     lvs_l = __builtin_amdgcn_logf(vs_l);
     ivs_l = 1.0f / vs_l;
-    count = min(64, (full - base + step - 1) / step);
   };
   auto fetch = [&](int p, int x) {
     const int slot = __builtin_amdgcn_readlane(slot_l, min(x, count - 1));
@@ -204,6 +207,7 @@ __global__ __launch_bounds__(kWaves * 64, NT == 1 && D == 64 ? 4 : 2) void k_kv8
     batch(b0);
 #pragma unroll
     for (int p = 0; p < PF; p++) fetch(p, p);
+    __builtin_amdgcn_sched_barrier(0);
   }
 
   // queries and the rows that each column sees
@@ -387,6 +391,7 @@ __global__ __launch_bounds__(kWaves * 64, NT == 1 && D == 64 ? 4 : 2) void k_kv8
 #pragma unroll
       for (int p = 0; p < PF; p++) fetch(p, p);
     }
+    scales();
     auto run = [&](auto masked, int p, int x) {
       auto kop = [&](int y, int k) {
         const uint4 v = kb[p][y * CH + (k >> 1)];
