@@ -15,6 +15,19 @@
 //                hold of P here when the positions of V are taken in that order: v_place lays V out so, and p never
 //                leaves its lane.
 // f32 queries enter as two fp16 (their row scaled by a power of two to below 2^10), f32 outputs take p as two fp16.
+//
+// The waves of a workgroup take the blocks of their tile in turn and join in LDS; where the tiles are too few for the
+// device, several workgroups share a tile (splits) and a second launch joins them. For eviction each block's sum goes
+// out as log2 by column, which needs no final maximum, and a pass over them adds up the weights in a fixed order.
+//
+// What bounds it, measured on one MI355X (3B shape: 8 KV heads of 64, 3 query heads each):
+//   one position   the cache's bytes: 134 MB of one sequence in 27 us (5.0 TB/s), 565 MB of eight in 115 us (4.9; blocks
+//                  in any order; a streaming read of 512 MiB reaches 5.7). Short caches: launches (5.7 us for 100 rows).
+//   many           the vector unit: a block of two tiles is 16 or 18 MFMAs of 16 cycles beside some 170 vector
+//                  instructions, 64 of them the conversion of the codes, 16 exps at a quarter of the rate. 1000
+//                  positions after 16001: 101 GFLOP in about 180 us in fp16. Tiles to a wave, whole call: one 311, two 206,
+//                  three 215 and four 260 us (fewer waves to overlap the two units); 2, 4 or 8 waves to a workgroup: 282,
+//                  206, 243. The matrix instructions first (s_setprio): 206 -> 197.
 #include <type_traits>
 
 #include "kv8.h"
