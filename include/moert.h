@@ -444,7 +444,8 @@ int moert_kv8_workspace(const moert_kv8* c, int n_seqs, int heads, int n, int tr
 
 /* Attention of n positions over the cache, whose last n rows are theirs (appended before): position i of a sequence of
  * len rows sees the first len - n + 1 + i of them, and query head h reads KV head h / (heads / kv_heads).
- * out = sum_t p_t v_t, p = softmax(scale * q . k); a position that sees no row gets 0. q and out are of one type:
+ * out = sum_t p_t v_t, p = softmax(scale * q . k); a position that sees no row gets 0, a query row that is not finite
+ * NaN. q and out are of one type:
  * scores, weights and sums are f32 for both; with MOERT_F16 the weights enter the second product rounded to fp16, with
  * MOERT_F32 as the sum of two fp16 (22 bits).
  * mass_decay in [0, 1] tracks: mass = mass_decay * mass + w for every block in use, w the sum of the block's p over

@@ -206,8 +206,8 @@ __global__ void k_kv8_clear(Kv8Dev c, int seq0) {
 }
 
 // A workgroup per block of the cache and head, its first half K, the other V; the codes go through LDS, where V comes
-// back to rows, and out 8 elements of a row at a time (100 MB in 22 us; byte by byte without LDS 55). Positions that are not there give 0: their blocks lie before
-// the sequence's first one or behind its last.
+// back to rows, and out 8 elements of a row at a time (100 MB in 22 us; byte by byte without LDS 55). Positions that
+// are not there give 0: their blocks lie before the sequence's first one or behind its last.
 template <int D>
 __global__ __launch_bounds__(256) void k_kv8_read(Kv8Dev c, KvRows k, KvRows v, int seq0, int pos, int n, int vec) {
   constexpr int C = D / 32, R = D / 8, U = D / 16;
@@ -580,6 +580,7 @@ int moert_kv8_read(const moert_kv8* c, int seq0, int n_seqs, int pos, int n, con
          n, pos, d.max_len);
   KV_TRY(rows("kv8_read", k, n_seqs, n, d.kvh, d.d, true, &kr));
   KV_TRY(rows("kv8_read", v, n_seqs, n, d.kvh, d.d, true, &vr));
+  KV_CFG(k->data_dev != v->data_dev, "kv8_read: K and V to one address");
   OnDevice on;
   KV_TRY(on.enter("kv8_read", d.kc));
   KV_HIP(launch_kv8_read((hipStream_t)stream, d, seq0, n_seqs, pos, n, kr, vr));

@@ -151,10 +151,12 @@ struct AttnArgs {
   float* lse;     // [sequence, KV head][block][column]: log2 of the block's sum
 };
 
-// log2 of a column's whole sum; +inf, which no weight survives, where it sees nothing.
-__device__ __forceinline__ float total_of(float m, float sum) {
-  return sum == 0.0f ? __int_as_float(0x7f800000) : __builtin_amdgcn_logf(sum) + (m - kShift);
+// log2 of a column's whole sum; +inf, which no weight survives, where it sees nothing. (A sum of 0 of rows that are
+// seen, scores beyond f32, becomes NaN here and in the output.)
+__device__ __forceinline__ float total_of(float m, float sum, bool none) {
+  return none ? __int_as_float(0x7f800000) : __builtin_amdgcn_logf(sum) + (m - kShift);
 }
+__device__ __forceinline__ bool sees_none(int len, int n, int g, int col) { return len - n + 1 + col / g <= 0; }
 
 // STREAM: the codes are loaded with the non-temporal hint.
 template <int D, bool F16, int NT, bool TRACK, bool STREAM>
@@ -237,7 +239,10 @@ __global__ __launch_bounds__(kWaves * 64, NT == 1 && D == 64 ? 4 : 2) void k_kv8
     for (int k = 0; k < KS; k++) {
       load8<F16>(a.q, at + (k >> 1) * 64 + G * 16 + (k & 1) * 8, a.vec & 1, x[k]);
 #pragma unroll
-      for (int j = 0; j < 8; j++) x[k][j] = __uint_as_float(__float_as_uint(x[k][j]) ^ a.sign);
+      for (int j = 0; j < 8; j++) {
+        x[k][j] = __uint_as_float(__float_as_uint(x[k][j]) ^ a.sign);
+        if constexpr (F16) x[k][j] += x[k][j] - x[k][j];  // inf to NaN, as the difference of f32's halves makes it
+      }
     }
     kf[t] = a.kf;
     if constexpr (!F16) {
@@ -478,13 +483,14 @@ __global__ __launch_bounds__(kWaves * 64, NT == 1 && D == 64 ? 4 : 2) void k_kv8
       }
       const size_t wc = col0 + col;
       if (used == 1) {
-        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+        const bool none = sees_none(len, a.n, a.g, col);
+        const float inv = none ? 0.0f : 1.0f / sum;
         const long long at = sc * a.out.seq + (long long)(col / a.g) * a.out.pos +
                              (long long)(h * a.g + col % a.g) * a.out.head + e0;
 #pragma unroll
         for (int e = 0; e < U; e++) o[e] *= inv;
         store_out<U, F16>(a.out, at, a.vec & 2, o);
-        if (TRACK && e0 == 0) a.tot[wc] = total_of(m, sum);
+        if (TRACK && e0 == 0) a.tot[wc] = total_of(m, sum, none);
       } else {
         float* po = a.part + (wc * a.splits + split) * D + e0;
 #pragma unroll
@@ -515,7 +521,7 @@ __device__ __forceinline__ void combine_column(const AttnArgs& a, int width, int
   const long long wc = (long long)block * (4 / C) + w / C;
   if (wc >= (long long)a.n_seqs * c.kvh * cols) return;  // C = 4: no column is left out
   const int col = (int)(wc % cols), hs = (int)(wc / cols), h = hs % c.kvh, sc = hs / c.kvh;
-  const int used = splits_used(blocks_seen(kv_len(c, a.seq0 + sc), a.n, a.g, col / width, width), a.splits);
+  const int len = kv_len(c, a.seq0 + sc), used = splits_used(blocks_seen(len, a.n, a.g, col / width, width), a.splits);
   float m, al, sum;
   column_sum(a, wc, used, lane, &m, &al, &sum);
   if (used == 1) return;
@@ -543,7 +549,8 @@ __device__ __forceinline__ void combine_column(const AttnArgs& a, int width, int
     for (int e = 0; e < E; e++)
       o[e] = (o[e] + Os[1][e * 64 + lane]) + (Os[2][e * 64 + lane] + Os[3][e * 64 + lane]);
   }
-  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+  const bool none = sees_none(len, a.n, a.g, col);
+  const float inv = none ? 0.0f : 1.0f / sum;
   const long long at = sc * a.out.seq + (long long)(col / a.g) * a.out.pos +
                        (long long)(h * a.g + col % a.g) * a.out.head + lane;
 #pragma unroll
@@ -551,7 +558,7 @@ __device__ __forceinline__ void combine_column(const AttnArgs& a, int width, int
     if constexpr (F16) ((uint16_t*)a.out.p)[at + e * 64] = f2h(o[e] * inv);
     else ((float*)a.out.p)[at + e * 64] = o[e] * inv;
   }
-  if (TRACK && lane == 0) a.tot[wc] = total_of(m, sum);
+  if (TRACK && lane == 0) a.tot[wc] = total_of(m, sum, none);
 }
 
 template <int D, bool F16, bool TRACK, int C>
@@ -603,11 +610,11 @@ __global__ __launch_bounds__(256) void k_kv8_finish(AttnArgs a, int width, int c
     return;
   }
   const int x = blockIdx.x - combines, hs = x / per_head, lane = threadIdx.x & 63, cols = a.n * a.g;
-  const int used = splits_used(blocks_seen(kv_len(a.c, a.seq0 + hs / a.c.kvh), a.n, a.g, 0, width), a.splits);
+  const int len = kv_len(a.c, a.seq0 + hs / a.c.kvh), used = splits_used(blocks_seen(len, a.n, a.g, 0, width), a.splits);
   for (int col = threadIdx.x >> 6; col < cols; col += 4) {
     float m, al, sum;
     column_sum(a, (long long)hs * cols + col, used, lane, &m, &al, &sum);
-    if (lane == 0) tot[col] = used == 1 ? a.tot[(size_t)hs * cols + col] : total_of(m, sum);
+    if (lane == 0) tot[col] = used == 1 ? a.tot[(size_t)hs * cols + col] : total_of(m, sum, sees_none(len, a.n, a.g, col));
   }
   __syncthreads();
   mass_block(a, hs, x % per_head * (256 / P) + threadIdx.x / P, threadIdx.x % P, P, decay, tot);

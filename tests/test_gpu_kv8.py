@@ -336,21 +336,38 @@ def test_poison_reaches_what_sees_it_and_nothing_else(hip, dtype):
                 assert np.array_equal(np.isnan(k[0]), np.isnan(wk)) and np.array_equal(np.isnan(v[0]), np.isnan(wv))
 
 
-def test_queries_that_are_not_finite(hip):
-    """NaN and inf in one query head's row: that row is NaN, the others are what they were."""
-    dev, ref = both(hip, 1, 2, 64, 128)
+@pytest.mark.parametrize("dtype", [moert.F32, moert.F16])
+def test_queries_that_are_not_finite(hip, dtype):
+    """NaN and inf in one query head's row: that row is NaN, the others are what they were; also where every score is
+    -inf, of one row and of many, with and without splits."""
     rng = np.random.default_rng(12)
-    r = normal(rng, 2, 1, 77, 2, 64)
-    dev.append(r[0], r[1])
-    q = normal(rng, 1, 3, 6, 64)
-    want = dev.attend(q, 0.125)
-    bad = q.copy()
-    bad[0, 1, 2, 5], bad[0, 2, 4, 0] = np.nan, np.inf
-    got = dev.attend(bad, 0.125)
-    assert np.isnan(got[0, 1, 2]).all() and np.isnan(got[0, 2, 4]).all()
-    hit = np.zeros((1, 3, 6), bool)
-    hit[0, 1, 2] = hit[0, 2, 4] = True
-    assert np.array_equal(got[~hit], want[~hit])
+    for length, max_len in ((77, 128), (1, 128), (64, 128), (1000, 16384)):
+        dev = ku.Device(hip, 1, 2, 64, max_len)
+        r = normal(rng, 2, 1, length, 2, 64)
+        r[0, :, :, :, 5] = -np.abs(r[0, :, :, :, 5]) - 1.0
+        dev.append(r[0], r[1])
+        for n in (1, 3):
+            q = normal(rng, 1, n, 6, 64)
+            want = dev.attend(q, 0.125, dtype)
+            bad = q.copy()
+            bad[0, 0, 2, 5], bad[0, n - 1, 4, 5], bad[0, n - 1, 1, 0] = np.nan, np.inf, -np.inf
+            got = dev.attend(bad, 0.125, dtype)
+            hit = np.zeros((1, n, 6), bool)
+            hit[0, 0, 2] = hit[0, n - 1, 4] = hit[0, n - 1, 1] = True
+            seen = np.broadcast_to((length - n + 1 + np.arange(n) > 0)[None, :, None], hit.shape)
+            assert np.isnan(got[hit & seen]).all() and not got[hit & ~seen].any(), (length, n)
+            assert np.array_equal(got[~hit], want[~hit]), (length, n)
+
+
+def test_scores_beyond_f32_are_not_zero_outputs(hip):
+    """Every score -1e42: NaN, as f32 softmax has it, not the 0 of a position that sees nothing."""
+    dev = ku.Device(hip, 1, 1, 64, 128)
+    k = np.full((1, 40, 1, 64), -1e4, np.float32)
+    dev.append(k, k)
+    q = np.full((1, 2, 1, 64), 1e37, np.float32)
+    assert np.isnan(dev.attend(q, 1.0)).all()
+    dev.attend(q, 1.0, decay=1.0)
+    assert np.isnan(dev.mass(0, 0, 2)).all()
 
 
 @pytest.mark.parametrize("d", [64, 128])

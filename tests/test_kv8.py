@@ -25,7 +25,7 @@ CALLS = {
     "attend": lambda c, **kw: c.attend(**{**dict(q=0x20000, out=0x20000, heads=4, n=1, scale=0.125, ws=0x30000,
                                                  ws_bytes=1 << 30), **kw}),
     "evict": lambda c, **kw: c.evict(**{**dict(keep=2), **kw}),
-    "read": lambda c, **kw: c.read(**{**dict(k=0x20000, v=0x20000, pos=0, n=1), **kw}),
+    "read": lambda c, **kw: c.read(**{**dict(k=0x20000, v=0x28000, pos=0, n=1), **kw}),
     "lengths": lambda c, **kw: c.lengths(**kw),
 }
 
@@ -78,6 +78,7 @@ def test_bad_rows_are_refused():
             refused(lambda: CALLS[name](c, dtype=dtype), "dtype")
     for pos, n in ((0, 0), (0, -3), (0, 97), (96, 1), (-97, 1)):
         refused(lambda: CALLS["read"](c, pos=pos, n=n), "positions")
+    refused(lambda: CALLS["read"](c, v=0x20000), "one address")
     # rows to be written must not overlap, in whatever order the axes lie
     for strides in ((0, 128, 64), (256, 128, 63), (256, 64, 64), (127, 128, 64), (64, 128, 64), (-256, 128, 64)):
         refused(lambda: CALLS["read"](c, n=2, strides=strides), "overlap")
