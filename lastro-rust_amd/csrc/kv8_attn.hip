@@ -512,32 +512,36 @@ __device__ __forceinline__ void column_sum(const AttnArgs& a, long long wc, int 
 }
 
 // The splits' shares of a column: C waves to a column, 4 / C columns to a workgroup. The waves take every C-th split's
-// products. Many splits go to four waves, whose loads overlap.
+// products, all of them asked for at once and before the factors are known: the splits that a short sequence leaves
+// unused lie in the workspace too, and are not looked at. Bound by latency: 2.7 us behind a short attention (3.4 with
+// four loads at a time behind the factors), 4.9 behind one of 134 MB, as any launch there.
 template <int D, bool F16, bool TRACK, int C>
 __device__ __forceinline__ void combine_column(const AttnArgs& a, int width, int block, float (*Os)[D]) {
-  constexpr int E = D / 64;
+  constexpr int E = D / 64, N = C == 4 ? kMaxSplits / 4 : 8;  // a wave's splits, at most
   const Kv8Dev& c = a.c;
   const int cols = a.n * a.g, lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const long long wc = (long long)block * (4 / C) + w / C;
   if (wc >= (long long)a.n_seqs * c.kvh * cols) return;  // C = 4: no column is left out
   const int col = (int)(wc % cols), hs = (int)(wc / cols), h = hs % c.kvh, sc = hs / c.kvh;
+  const float* po = a.part + wc * a.splits * D + lane;
+  float y[N][E];
+#pragma unroll
+  for (int j = 0; j < N; j++)
+#pragma unroll
+    for (int e = 0; e < E; e++)
+      if (w % C + j * C < a.splits) y[j][e] = gmem(po)[(size_t)(w % C + j * C) * D + e * 64];
   const int len = kv_len(c, a.seq0 + sc), used = splits_used(blocks_seen(len, a.n, a.g, col / width, width), a.splits);
   float m, al, sum;
   column_sum(a, wc, used, lane, &m, &al, &sum);
   if (used == 1) return;
   float o[E] = {};
-  const float* po = a.part + wc * a.splits * D + lane;
-  for (int j0 = w % C; j0 < used; j0 += 4 * C) {  // four loads in flight; past the last split its own, at weight 0
-    float y[4][E];
 #pragma unroll
-    for (int j = 0; j < 4; j++)
+  for (int j = 0; j < N; j++) {
+    const int split = w % C + j * C;
+    if (split < used) {
+      const float aj = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(al), split));
 #pragma unroll
-      for (int e = 0; e < E; e++) y[j][e] = po[(size_t)min(j0 + j * C, used - 1) * D + e * 64];
-#pragma unroll
-    for (int j = 0; j < 4; j++) {
-      const float aj = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(al), min(j0 + j * C, used - 1)));
-#pragma unroll
-      for (int e = 0; e < E; e++) o[e] = __builtin_fmaf(y[j][e], j0 + j * C < used ? aj : 0.0f, o[e]);
+      for (int e = 0; e < E; e++) o[e] = __builtin_fmaf(y[j][e], aj, o[e]);
     }
   }
   if constexpr (C == 4) {
@@ -610,14 +614,27 @@ __global__ __launch_bounds__(256) void k_kv8_finish(AttnArgs a, int width, int c
     return;
   }
   const int x = blockIdx.x - combines, hs = x / per_head, lane = threadIdx.x & 63, cols = a.n * a.g;
-  const int len = kv_len(a.c, a.seq0 + hs / a.c.kvh), used = splits_used(blocks_seen(len, a.n, a.g, 0, width), a.splits);
-  for (int col = threadIdx.x >> 6; col < cols; col += 4) {
+  // lane `col` of a block's P holds its column; all that does not wait for the sums is asked for first
+  const Kv8Dev& c = a.c;
+  const int h = hs % c.kvh, s = a.seq0 + hs / c.kvh, col = threadIdx.x % P;
+  const int b = min(x % per_head * (256 / P) + (int)threadIdx.x / P, c.slots - 1);
+  const size_t head = (size_t)s * c.kvh + h;
+  const float lse = gmem(a.lse)[((size_t)hs * c.slots + b) * cols + min(col, cols - 1)];
+  float* mass = c.mass + head * c.slots + kv_slot(c, gmem(c.table)[head * c.slots + b]);
+  const float old = gmem(mass)[0];
+  const int len = kv_len(c, s), used = splits_used(blocks_seen(len, a.n, a.g, 0, width), a.splits);
+  for (int i = threadIdx.x >> 6; i < cols; i += 4) {
     float m, al, sum;
-    column_sum(a, (long long)hs * cols + col, used, lane, &m, &al, &sum);
-    if (lane == 0) tot[col] = used == 1 ? a.tot[(size_t)hs * cols + col] : total_of(m, sum, sees_none(len, a.n, a.g, col));
+    column_sum(a, (long long)hs * cols + i, used, lane, &m, &al, &sum);
+    if (lane == 0)
+      tot[i] = used == 1 ? a.tot[(size_t)hs * cols + i] : total_of(m, sum, sees_none(len, a.n, a.g, i));
   }
   __syncthreads();
-  mass_block(a, hs, x % per_head * (256 / P) + threadIdx.x / P, threadIdx.x % P, P, decay, tot);
+  // a column's position sees some of the block, and the block is the last thread group's own (the index is clamped)
+  const bool mine = x % per_head * (256 / P) + (int)threadIdx.x / P == b && b * kKvBlock < len;
+  float w = col < cols && b * kKvBlock < len - a.n + 1 + col / a.g ? __builtin_amdgcn_exp2f(lse - tot[col]) : 0.0f;
+  for (int m = P / 2; m; m >>= 1) w += __shfl_xor(w, m);
+  if (mine && col == 0) *mass = __builtin_fmaf(decay, old, w);
 }
 
 int tile_count(int cols) { return cols <= 16 ? 1 : 2; }  // tiles of 16 columns of a wave
@@ -669,7 +686,7 @@ hipError_t attend(hipStream_t s, AttnArgs a, float decay) {
   const int per_head = (a.c.slots * P + 255) / 256;
   if (TRACK && a.splits > 1 && cols <= 16) {
     // splits mean fewer than 1024 heads: the grid stays small. (A fifth as many workgroups, each with more blocks of a
-    // head, took 11.6 us for 9.4: the blocks' loads wait for each other.)
+    // head, took 11.6 us for 9.2: the blocks' loads wait for each other.)
     const int C = a.splits > 8 ? 4 : 1, combines = (int)((all * C + 3) / 4);
     const unsigned both = (unsigned)(combines + all / cols * per_head);
     if (C == 4) klaunch(k_kv8_finish<D, F16, 4>, both, 256, 0, s, a, width, combines, per_head, decay, P);

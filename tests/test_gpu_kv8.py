@@ -425,7 +425,7 @@ def set_masses(dev, ref, masses):
     dev.set("mass", m)
 
 
-@pytest.mark.parametrize("max_len,lens", [(320, (7, 64, 300)), (65536, (40000, 33000)), (2 ** 18, (2 ** 18 - 5,))])
+@pytest.mark.parametrize("max_len,lens", [(320, (7, 64, 300)), (16384, (8256, 8191, 8259)), (65536, (40000, 33000)), (2 ** 18, (2 ** 18 - 5,))])
 def test_evictions(hip, max_len, lens):
     """Masses with ties, zeros, infinities and NaN; budgets from 0 to more than there is; what stays is as it was."""
     S = len(lens)
