@@ -162,7 +162,14 @@ __device__ __forceinline__ bool sees_none(int len, int n, int g, int col) { retu
 template <int D, bool F16, int NT, bool TRACK, bool STREAM>
 __global__ __launch_bounds__(kWaves * 64, NT == 1 && D == 64 ? 4 : 2) void k_kv8_attend(AttnArgs a) {
   constexpr int KS = D / 32, U = D / 16, CH = D / 64, W = 16 * NT;
-  constexpr int PF = NT == 1 ? 2 : 1;  // blocks in flight: with two tiles the other waves cover the loads
+  // Which 16 elements a product of V has as its rows is free. A load of 16 bytes a lane takes 1 KB of V in a row, whole
+  // cache lines: RP of the runs' rows, U / 2 pieces of each. (Two loads that each took half of every line asked the L2
+  // for 1.8 times the bytes: 115 us where this takes 108, 565 MB.) So row i of product u is element elem(u, i).
+  constexpr int RP = 16 / (U / 2);
+  auto elem = [](int u, int i) { return (u / 2 * RP + i % RP) * U + 2 * (i / RP) + u % 2; };
+  // blocks in flight: with two tiles, or the 8 KB blocks of wide heads, the other waves cover the loads (sixteen
+  // sequences of wide heads 31.4 us a pass for 32.9, one sequence of 131000 positions of narrow ones 36.6 for 35.4)
+  constexpr int PF = NT == 1 && D == 64 ? 2 : 1;
   // Sums of weights come from the matrix cores, which have time to spare: of the two halves of f32's, or of the rounded
   // weights, whose error is far below an fp16 output's. The blocks' weights are f32 in any case: there the vector unit
   // adds up a lane's eight, and lanes are joined for the block's sum and at the end.
@@ -209,14 +216,14 @@ __global__ __launch_bounds__(kWaves * 64, NT == 1 && D == 64 ? 4 : 2) void k_kv8
     const int slot = __builtin_amdgcn_readlane(slot_l, min(x, count - 1));
     const size_t at = (head * c.slots + slot) * (size_t)(kKvBlock * D);
     const uint8_t* kp = c.kc + at + col16 * D + G * 16;
-    const uint8_t* vp = c.vc + at + (col16 * 4 + G) * (U * 8);
+    const uint8_t* vp = c.vc + at + (col16 % RP * 4 + G) * (U * 8) + col16 / RP * 16;
 #pragma unroll
     for (int y = 0; y < 2; y++)
 #pragma unroll
-      for (int z = 0; z < CH; z++) {
+      for (int z = 0; z < CH; z++)
         kb[p][y * CH + z] = STREAM ? gload_u4_nt(kp + y * 16 * D + z * 64) : gload_u4(kp + y * 16 * D + z * 64);
-        vb[p][y * CH + z] = STREAM ? gload_u4_nt(vp + (y * CH + z) * 16) : gload_u4(vp + (y * CH + z) * 16);
-      }
+#pragma unroll
+    for (int y = 0; y < 2 * CH; y++) vb[p][y] = STREAM ? gload_u4_nt(vp + y * 1024) : gload_u4(vp + y * 1024);
   };
   if (b0 < full) {
     batch(b0);
@@ -446,7 +453,7 @@ __global__ __launch_bounds__(kWaves * 64, NT == 1 && D == 64 ? 4 : 2) void k_kv8
       return *reinterpret_cast<const h8*>(kt + (y * 16 + col16) * D + (k >> 1) * 64 + G * 16 + (k & 1) * 8);
     };
     auto vop = [&](int u) {
-      h8 v = *reinterpret_cast<const h8*>(vt + ((col16 * 4 + G) * U + u) * 8);
+      h8 v = *reinterpret_cast<const h8*>(vt + ((elem(u, col16) / U * 4 + G) * U + elem(u, col16) % U) * 8);
 #pragma unroll
       for (int j = 0; j < 8; j++)  // what no row has written, or poison, must not meet a weight of 0
         v[j] = use >> (G * 4 + (j & 3) + 16 * (j >> 2)) & 1 ? v[j] : (_Float16)0.0f;
@@ -464,9 +471,8 @@ __global__ __launch_bounds__(kWaves * 64, NT == 1 && D == 64 ? 4 : 2) void k_kv8
 #pragma unroll
     for (int i = 0; i < 4; i++)
 #pragma unroll
-      for (int u = 0; u < U; u += 4)
-        *reinterpret_cast<f4*>(&Os[w][col16][(G * 4 + i) * U + u]) =
-            f4{O[t][u][i], O[t][u + 1][i], O[t][u + 2][i], O[t][u + 3][i]};
+      for (int u = 0; u < U; u += 2)
+        *reinterpret_cast<float2*>(&Os[w][col16][elem(u, G * 4 + i)]) = make_float2(O[t][u][i], O[t][u + 1][i]);
     __syncthreads();
     const int cl = threadIdx.x >> 4, e0 = (threadIdx.x & 15) * U, col = tile * W + t * 16 + cl;
     if (col < cols) {
@@ -674,9 +680,10 @@ hipError_t attend(hipStream_t s, AttnArgs a, float decay) {
   a.tiles = (cols + width - 1) / width;
   const long long units = (long long)a.n_seqs * a.c.kvh * a.splits;
   const long long grid = (units + 7) / 8 * 8 * a.tiles;
-  // A cache that can outgrow the 256 MB last-level cache is streamed past the others: 124 -> 119 us for 565 MB of eight
-  // sequences in 839 MB; in smaller ones the hint costs what a step finds there of the last (26.6 -> 32.3 us for 68 MB).
-  const bool stream = nt == 1 && 2ll * a.n_seqs * a.c.kvh * a.c.max_len * D > 256ll << 20;
+  // A layer's cache of 96 MB and more is streamed past the others: three of them outgrow the 256 MB last-level cache, and
+  // a model has more. 565 MB of eight sequences 138 -> 125 us a pass, 134 MB of one 35.4 -> 32.5; where three caches
+  // still fit (68 MB in use of 134 each), a pass loses what it would find there, 32.9 -> 34.1.
+  const bool stream = nt == 1 && 2ll * a.n_seqs * a.c.kvh * a.c.max_len * D >= 96ll << 20;
   if (stream) klaunch(k_kv8_attend<D, F16, 1, TRACK, true>, (unsigned)grid, kWaves * 64, 0, s, a);
   else if (nt == 1) klaunch(k_kv8_attend<D, F16, 1, TRACK, false>, (unsigned)grid, kWaves * 64, 0, s, a);
   else klaunch(k_kv8_attend<D, F16, 2, TRACK, false>, (unsigned)grid, kWaves * 64, 0, s, a);
