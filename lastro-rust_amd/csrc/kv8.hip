@@ -291,9 +291,8 @@ __device__ __forceinline__ uint32_t mass_key(float m) {
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 
-constexpr int kEvictThreads = 1024;
-
-// Sum over the workgroup's threads before this one, and all of them.
+// Sum over the workgroup's T threads before this one, and all of them.
+template <int T>
 __device__ int block_prefix(int v, int* waves, int* total) {
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   int x = v;
@@ -306,7 +305,8 @@ __device__ int block_prefix(int v, int* waves, int* total) {
   if (lane == 63) waves[w] = x;
   __syncthreads();
   int before = 0, all = 0;
-  for (int i = 0; i < kEvictThreads / 64; i++) {
+#pragma unroll
+  for (int i = 0; i < T / 64; i++) {
     before += i < w ? waves[i] : 0;
     all += waves[i];
   }
@@ -318,10 +318,11 @@ __device__ int block_prefix(int v, int* waves, int* total) {
 // registers, so the table can be rewritten in place once all have been read). The key of the last block that stays is
 // found by counting, 11, 11 and 10 bits at a time (the first take masses apart by a fifth, so that few counts meet in
 // one bin: 13.8 us with 8 bits four times, 12.1 so, 4062 blocks of 128 heads); among blocks of that key the earlier stay.
-template <int KPT>
-__global__ __launch_bounds__(kEvictThreads) void k_kv8_evict(Kv8Dev c, int seq0, int keep, int first, int last) {
+template <int T, int KPT>
+__global__ __launch_bounds__(T) void k_kv8_evict(Kv8Dev c, int seq0, int keep, int first, int last) {
   __shared__ __align__(16) int hist[2048];
-  __shared__ int waves[kEvictThreads / 64], pick[2];
+  constexpr int B = 2048 / T;  // bins of a thread
+  __shared__ int waves[T / 64], pick[2];
   const int s = seq0 + blockIdx.x / c.kvh, len = kv_len(c, s), nb = len / kKvBlock;
   if (nb <= keep) return;
   const size_t base = ((size_t)s * c.kvh + blockIdx.x % c.kvh) * c.slots;
@@ -340,8 +341,8 @@ __global__ __launch_bounds__(kEvictThreads) void k_kv8_evict(Kv8Dev c, int seq0,
   for (int pass = 0; pass < 3; pass++) {
     if (left <= 0) break;  // the same for all
     const int sh = pass == 0 ? 21 : pass == 1 ? 10 : 0, bins = pass == 2 ? 1024 : 2048;
-    hist[threadIdx.x] = 0;
-    hist[threadIdx.x + kEvictThreads] = 0;
+#pragma unroll
+    for (int j = 0; j < B; j++) hist[threadIdx.x + j * T] = 0;
     __syncthreads();
 #pragma unroll
     for (int j = 0; j < KPT; j++) {
@@ -350,12 +351,16 @@ __global__ __launch_bounds__(kEvictThreads) void k_kv8_evict(Kv8Dev c, int seq0,
         atomicAdd(&hist[key[j] >> sh & (bins - 1)], 1);
     }
     __syncthreads();
-    const int hi = 2047 - 2 * (int)threadIdx.x;  // this thread's bins: hi and hi - 1
-    const int2 v = *reinterpret_cast<const int2*>(&hist[hi - 1]);
-    int total, above = block_prefix(v.x + v.y, waves, &total);  // keys in the bins above them
-    if (above < left && above + v.y >= left) pick[0] = hi, pick[1] = above;
-    above += v.y;
-    if (above < left && above + v.x >= left) pick[0] = hi - 1, pick[1] = above;
+    const int top = 2047 - B * (int)threadIdx.x;  // this thread's bins: top and the B - 1 below
+    int v[B], mine = 0, total;
+#pragma unroll
+    for (int j = 0; j < B; j++) mine += v[j] = hist[top - j];
+    int above = block_prefix<T>(mine, waves, &total);  // keys in the bins above them
+#pragma unroll
+    for (int j = 0; j < B; j++) {
+      if (above < left && above + v[j] >= left) pick[0] = top - j, pick[1] = above;
+      above += v[j];
+    }
     __syncthreads();
     pre |= (uint32_t)pick[0] << sh;
     left -= pick[1];
@@ -368,7 +373,7 @@ __global__ __launch_bounds__(kEvictThreads) void k_kv8_evict(Kv8Dev c, int seq0,
     may[j] = i0 + j >= first && i0 + j < nb - last;
     same += may[j] && left > 0 && key[j] == pre ? 1 : 0;
   }
-  int total, before = block_prefix(same, waves, &total), stay = 0;
+  int total, before = block_prefix<T>(same, waves, &total), stay = 0;
 #pragma unroll
   for (int j = 0; j < KPT; j++) {
     const bool eq = may[j] && left > 0 && key[j] == pre;
@@ -376,7 +381,7 @@ __global__ __launch_bounds__(kEvictThreads) void k_kv8_evict(Kv8Dev c, int seq0,
     before += eq ? 1 : 0;
     stay += stays[j] ? 1 : 0;
   }
-  int to = block_prefix(stay, waves, &total);
+  int to = block_prefix<T>(stay, waves, &total);
   const bool tail = len % kKvBlock != 0;
   const int tail_slot = tail && threadIdx.x == 0 ? c.table[base + nb] : 0;
   int gone = keep + (tail ? 1 : 0) + min(i0, nb) - to;  // place of this thread's first block that leaves
@@ -427,12 +432,14 @@ hipError_t launch_kv8_read(hipStream_t s, const Kv8Dev& c, int seq0, int n_seqs,
 
 hipError_t launch_kv8_evict(hipStream_t s, const Kv8Dev& c, int seq0, int n_seqs, int keep, int first, int last) {
   const int grid = n_seqs * c.kvh;
-#define EVICT(K)                                                                    \
-  if (c.slots <= K * kEvictThreads) {                                               \
-    klaunch(k_kv8_evict<K>, grid, kEvictThreads, 0, s, c, seq0, keep, first, last); \
-    return hipGetLastError();                                                       \
+  // Short tables take fewer threads, whose barriers cost less (7.7 us for 8.7 with 1024, 144 slots, 7.9 for 8.9 with 512);
+  // long ones as many as there are: fewer, with more keys each, are slower (130000 positions: 14.2 us, 15.8 with 512).
+#define EVICT(T, K)                                                        \
+  if (c.slots <= K * T) {                                                  \
+    klaunch(k_kv8_evict<T, K>, grid, T, 0, s, c, seq0, keep, first, last); \
+    return hipGetLastError();                                              \
   }
-  EVICT(1) EVICT(2) EVICT(4) EVICT(8) EVICT(16) EVICT(32)
+  EVICT(256, 1) EVICT(512, 1) EVICT(1024, 1) EVICT(1024, 2) EVICT(1024, 4) EVICT(1024, 8) EVICT(1024, 16) EVICT(1024, 32)
 #undef EVICT
   return hipErrorInvalidValue;
 }

@@ -425,7 +425,9 @@ def set_masses(dev, ref, masses):
     dev.set("mass", m)
 
 
-@pytest.mark.parametrize("max_len,lens", [(320, (7, 64, 300)), (16384, (8256, 8191, 8259)), (65536, (40000, 33000)), (2 ** 18, (2 ** 18 - 5,))])
+@pytest.mark.parametrize("max_len,lens", [(320, (7, 64, 300)), (16384, (8256, 8191, 8259)), (2 ** 15, (30000,)),
+                                          (65536, (40000, 33000)), (2 ** 17, (130001,)), (2 ** 18, (2 ** 18 - 5,)),
+                                          (2 ** 20, (2 ** 20 - 3,))])
 def test_evictions(hip, max_len, lens):
     """Masses with ties, zeros, infinities and NaN; budgets from 0 to more than there is; what stays is as it was."""
     S = len(lens)
@@ -438,7 +440,7 @@ def test_evictions(hip, max_len, lens):
             keep, first, last = keep * 113, first * 5, last * 7
         for kind in ("spread", "equal", "odd"):
             print(f"[case] lengths {lens}, keep {keep}, first {first}, last {last}, {kind}", flush=True)
-            dev, ref = both(hip, S, H, 64, max_len)
+            dev, ref = ku.Device(hip, S, H, 64, max_len, fill=few), ku.Cache(S, H, 64, max_len)
             for s, n in enumerate(lens):
                 r = normal(rng, 2, 1, n if few else 64 + n % 32, H, 64)
                 dev.append(r[0], r[1], seq0=s)
@@ -474,7 +476,8 @@ def test_evictions(hip, max_len, lens):
                 for h in range(H):
                     stay = [where[s][h][id(x)] for x in ref.blocks[s][h]]
                     tail = [full0[s]] if r else []
-                    gone = [b for b in range(full0[s]) if b not in set(stay)]
+                    kept = set(stay)
+                    gone = [b for b in range(full0[s]) if b not in kept]
                     rest = list(range(full0[s] + len(tail), max_len // B))
                     assert table[s, h].tolist() == table0[s, h][stay + tail + gone + rest].tolist(), (s, h)
                     want = mass0[s, h].copy()
