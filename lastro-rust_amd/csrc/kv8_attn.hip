@@ -21,7 +21,7 @@
 // out as log2 by column, which needs no final maximum, and a pass over them adds up the weights in a fixed order.
 //
 // What bounds it, measured on one MI355X (3B shape: 8 KV heads of 64, 3 query heads each):
-//   one position   the cache's bytes: 134 MB of one sequence in 27 us (5.0 TB/s), 565 MB of eight in 115 us (4.9; blocks
+//   one position   the cache's bytes: 134 MB of one sequence in 25 us (5.3 TB/s), 565 MB of eight in 108 us (5.2; blocks
 //                  in any order; a streaming read of 512 MiB reaches 5.7). Short caches: launches (5.7 us for 100 rows).
 //   many           the vector unit: a block of two tiles is 16 or 18 MFMAs of 16 cycles beside some 170 vector
 //                  instructions, 64 of them the conversion of the codes, 16 exps at a quarter of the rate. 1000
