@@ -103,6 +103,10 @@ __device__ __forceinline__ void load8(const KvRows& r, long long at, bool wide, 
   }
 }
 
+// An output is a mean of values of at most 65504. Weights rounded to fp16 beside a sum that is not make it up to 2^-11
+// more, and fp16 would have no number for it.
+__device__ __forceinline__ float in_f16(float x) { return x > 65504.0f ? 65504.0f : x < -65504.0f ? -65504.0f : x; }
+
 // N elements (a multiple of 4) of a row of the output.
 template <int N, bool F16>
 __device__ __forceinline__ void store_out(const KvRows& r, long long at, bool wide, const float* x) {
@@ -494,7 +498,7 @@ __global__ __launch_bounds__(kWaves * 64, NT == 1 && D == 64 ? 4 : 2) void k_kv8
         const long long at = sc * a.out.seq + (long long)(col / a.g) * a.out.pos +
                              (long long)(h * a.g + col % a.g) * a.out.head + e0;
 #pragma unroll
-        for (int e = 0; e < U; e++) o[e] *= inv;
+        for (int e = 0; e < U; e++) o[e] = VSUM ? in_f16(o[e] * inv) : o[e] * inv;
         store_out<U, F16>(a.out, at, a.vec & 2, o);
         if (TRACK && e0 == 0) a.tot[wc] = total_of(m, sum, none);
       } else {
@@ -565,7 +569,7 @@ __device__ __forceinline__ void combine_column(const AttnArgs& a, int width, int
                        (long long)(h * a.g + col % a.g) * a.out.head + lane;
 #pragma unroll
   for (int e = 0; e < E; e++) {
-    if constexpr (F16) ((uint16_t*)a.out.p)[at + e * 64] = f2h(o[e] * inv);
+    if constexpr (F16) ((uint16_t*)a.out.p)[at + e * 64] = f2h(in_f16(o[e] * inv));
     else ((float*)a.out.p)[at + e * 64] = o[e] * inv;
   }
   if (TRACK && lane == 0) a.tot[wc] = total_of(m, sum, none);

@@ -370,6 +370,25 @@ def test_scores_beyond_f32_are_not_zero_outputs(hip):
     assert np.isnan(dev.mass(0, 0, 2)).all()
 
 
+@pytest.mark.parametrize("decay", [None, 0.5])
+@pytest.mark.parametrize("max_len", [384, 8192])
+def test_the_largest_values_stay_finite(hip, max_len, decay):
+    """V of fp16's largest magnitude and, in all rows that count, weights whose rounding to fp16 has one sign: 64 heads
+    whose scores lie 1 .. 7.3 (in base 2) above the rows that set each wave's maximum. An output is off by half a step
+    of its weights at most, and the exact one, +-65504, is the type's last number: nothing becomes infinite."""
+    d, rows = 64, 384
+    dev, ref = both(hip, 1, 1, d, max_len)
+    k, v = np.zeros((1, rows, 1, d)), np.full((1, rows, 1, d), 65504.0)
+    k[:, rows // 2:, :, 0] = 1.0  # the first blocks, every wave's first, score 0
+    v[..., 1::2] = -65504.0
+    dev.append(k, v)
+    ref.append(k, v)
+    q = np.zeros((1, 1, 64, d))
+    q[..., 0] = 0.7 + np.arange(64) / 14.5
+    out = check_attend(dev, ref, q.astype(np.float16), 1.0, dtype=moert.F16, decay=decay)
+    assert np.isfinite(out).all()
+
+
 @pytest.mark.parametrize("d", [64, 128])
 @pytest.mark.parametrize("dtype", [moert.F32, moert.F16])
 def test_reads(hip, d, dtype):
