@@ -46,6 +46,7 @@ constexpr float kLog2e = 1.44269504088896341f;
 constexpr int kWaves = 4;       // waves of a workgroup, each its share of the blocks
 constexpr int kMaxSplits = 64;  // one lane each in the combine
 constexpr float kShift = 7.0f, kSlack = 8.0f;
+constexpr float kNone = -3.4e38f;  // maximum of what has no score yet; finite, so that differences with it are
 
 // a + the value of a's lane 16 (32) away, in both of them.
 __device__ __forceinline__ float add16(float a) {
@@ -288,7 +289,7 @@ __global__ __launch_bounds__(kWaves * 64, NT == 1 && D == 64 ? 4 : 2) void k_kv8
   f4 O[NT][U];
 #pragma unroll
   for (int t = 0; t < NT; t++) {
-    M[t] = -1e30f;
+    M[t] = kNone;
     l[t] = 0.0f;
 #pragma unroll
     for (int u = 0; u < U; u++) O[t][u] = f4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -298,8 +299,8 @@ __global__ __launch_bounds__(kWaves * 64, NT == 1 && D == 64 ? 4 : 2) void k_kv8
   h8 ones;
 #pragma unroll
   for (int j = 0; j < 8; j++) ones[j] = (_Float16)1.0f;
-  // One block: kop(half, k), vop(u) give the operands. masked: some column does not see all of it (S is a finite -3e38
-  // there, so that a scale of 0 makes no NaN of it), or `bad` names poisoned rows, of the tail.
+  // One block: kop(half, k), vop(u) give the operands. masked: some column does not see all of it (S is -inf there,
+  // which moves no maximum; NaN with a scale of 0, which moves none either), or `bad` names poisoned rows, of the tail.
   auto block = [&](auto masked, auto kop, auto vop, float ks, float lvs, float ivs, int b, uint32_t bad) {
     constexpr bool MASKED = decltype(masked)::value;
     f4 S[NT][2];
@@ -327,7 +328,7 @@ __global__ __launch_bounds__(kWaves * 64, NT == 1 && D == 64 ? 4 : 2) void k_kv8
           for (int i = 0; i < 4; i++) {
             const int row = x * 16 + G * 4 + i;
             if (bad >> row & 1) S[t][x][i] = __int_as_float(0x7fc00000);
-            if (b * kKvBlock + row >= sees[t]) S[t][x][i] = -3e38f;
+            if (b * kKvBlock + row >= sees[t]) S[t][x][i] = -__builtin_inff();
           }
     }
     if constexpr (NT > 1) __builtin_amdgcn_s_setprio(0);
@@ -347,7 +348,7 @@ __global__ __launch_bounds__(kWaves * 64, NT == 1 && D == 64 ? 4 : 2) void k_kv8
         const float y = max_stage<32>(max_stage<16>(mx[t])) * f[t] + lvs;
         const float mn = y > M[t] ? y : M[t], al = __builtin_amdgcn_exp2f(M[t] - mn);
         M[t] = mn;
-        far |= __any(__builtin_fabsf(mn) > 65536.0f && mn != -1e30f);
+        far |= __any(__builtin_fabsf(mn) > 65536.0f && mn != kNone);
         l[t] *= al;
 #pragma unroll
         for (int u = 0; u < U; u++)
@@ -516,7 +517,7 @@ __device__ __forceinline__ void column_sum(const AttnArgs& a, long long wc, int 
                                            float* sum) {
   const float2 x = a.ml[wc * a.splits + min(lane, a.splits - 1)];
   const bool in = lane < used;
-  *m = group_max(in ? x.x : -3e38f);
+  *m = group_max(in ? x.x : kNone);
   *al = in ? __builtin_amdgcn_exp2f(x.x - *m) : 0.0f;
   *sum = group_sum(in ? x.y * *al : 0.0f);
 }

@@ -389,6 +389,30 @@ def test_the_largest_values_stay_finite(hip, max_len, decay):
     assert np.isfinite(out).all()
 
 
+@pytest.mark.parametrize("n", [1, 9])
+def test_scores_near_f32s_lowest(hip, n):
+    """Scores of about -1e36, apart by 1e34 and more: all the weight is on the least negative one that is seen."""
+    rng = np.random.default_rng(23)
+    d, rows = 64, 700
+    dev, ref = both(hip, 1, 2, d, 1024)
+    k, v = np.zeros((1, rows, 2, d)), normal(rng, 1, rows, 2, d)
+    k[..., 0] = 127.0  # of a scale of 1 in every block
+    for h in range(2):
+        k[0, 40 + 300 * h, h, 0] = 100.0
+    dev.append(k, v)
+    ref.append(k, v)
+    q = np.zeros((1, n, 4, d), np.float32)
+    q[..., 0] = -1e34
+    out = dev.attend(q, 1.0, decay=0.0)
+    for h in range(2):
+        want = ref.rows(0, h)[1][40 + 300 * h]
+        for a in (2 * h, 2 * h + 1):
+            # weights of one row, a code and a scale: three roundings of 2^-24
+            assert np.abs(out[0, :, a] - want).max() <= 4 * 2.0 ** -24 * np.abs(want).max()
+        mass = dev.mass(0, h, -(-rows // 32))
+        assert mass[(40 + 300 * h) // 32] == 2 * n and mass.sum() == 2 * n
+
+
 @pytest.mark.parametrize("d", [64, 128])
 @pytest.mark.parametrize("dtype", [moert.F32, moert.F16])
 def test_reads(hip, d, dtype):
