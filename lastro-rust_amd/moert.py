@@ -955,9 +955,15 @@ class Kv8:
         check(self._lib.moert_kv8_read(self._p, seq0, self._n(seq0, n_seqs), pos, n, kr, vr, stream))
 
     def lengths(self, seq0: int = 0, n_seqs: Optional[int] = None, stream: int = 0) -> np.ndarray:
-        """Lengths of the sequences (synchronises the stream); raises E_FULL where rows were dropped."""
+        """Lengths of the sequences (synchronises the stream); raises E_FULL, with the lengths in the error's `lengths`,
+        where rows were dropped."""
         out = np.empty(max(1, self._n(seq0, n_seqs)), np.int32)
-        check(self._lib.moert_kv8_lengths(self._p, seq0, self._n(seq0, n_seqs), ptr(out), stream))
+        try:
+            check(self._lib.moert_kv8_lengths(self._p, seq0, self._n(seq0, n_seqs), ptr(out), stream))
+        except MoertError as e:
+            if e.code == E_FULL:
+                e.lengths = out
+            raise
         return out
 
 

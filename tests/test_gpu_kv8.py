@@ -452,6 +452,17 @@ def test_appends_without_room_leave_the_sequence(hip):
         dev.c.lengths(1, 1)
 
 
+def test_lengths_come_with_the_report_of_dropped_rows(hip):
+    dev, _ = both(hip, 3, 1, 64, 64)
+    x = np.ones((1, 40, 1, 64))
+    dev.append(x, x, seq0=1)
+    dev.append(x, x, seq0=1)
+    dev.append(x[:, :7], x[:, :7], seq0=2)
+    with pytest.raises(moert.MoertError) as e:
+        dev.c.lengths()
+    assert e.value.code == moert.E_FULL and e.value.lengths.tolist() == [0, 40, 7]
+
+
 def set_masses(dev, ref, masses):
     """masses(s, h, blocks) -> f32 of every block in use, set on both sides."""
     m = dev.array("mass")
