@@ -159,7 +159,7 @@ struct AttnArgs {
 // log2 of a column's whole sum; +inf, which no weight survives, where it sees nothing. (A sum of 0 of rows that are
 // seen, scores beyond f32, becomes NaN here and in the output.)
 __device__ __forceinline__ float total_of(float m, float sum, bool none) {
-  return none ? __int_as_float(0x7f800000) : __builtin_amdgcn_logf(sum) + (m - kShift);
+  return none ? __int_as_float(0x7f800000) : __builtin_amdgcn_logf(sum) + m;
 }
 __device__ __forceinline__ bool sees_none(int len, int n, int g, int col) { return len - n + 1 + col / g <= 0; }
 
@@ -285,7 +285,7 @@ __global__ __launch_bounds__(kWaves * 64, NT == 1 && D == 64 ? 4 : 2) void k_kv8
   }
   const int sees0 = len - a.n + 1 + min(tile * W, cols - 1) / a.g;  // the least of the tile
 
-  float M[NT], l[NT];
+  float M[NT], l[NT];  // M: the maximum less 7, so that the weights below are 2^7 times those to it
   f4 O[NT][U];
 #pragma unroll
   for (int t = 0; t < NT; t++) {
@@ -296,6 +296,8 @@ __global__ __launch_bounds__(kWaves * 64, NT == 1 && D == 64 ? 4 : 2) void k_kv8
   }
 
   bool far = false;  // some column's M is beyond 2^16
+  float none = -__builtin_inff();  // opaque, so that eight maxima with it are four instructions
+  asm("" : "+s"(none));
   h8 ones;
 #pragma unroll
   for (int j = 0; j < 8; j++) ones[j] = (_Float16)1.0f;
@@ -337,15 +339,15 @@ __global__ __launch_bounds__(kWaves * 64, NT == 1 && D == 64 ? 4 : 2) void k_kv8
 #pragma unroll
     for (int t = 0; t < NT; t++) {
       f[t] = kf[t] * ks;
-      mx[t] = S[t][0][0];  // NaN only where all are
+      mx[t] = none;
 #pragma unroll
-      for (int x = 1; x < 8; x++) mx[t] = __builtin_fmaxf(mx[t], S[t][x >> 2][x & 3]);
-      move |= __builtin_fmaf(mx[t], f[t], lvs) > M[t] + kSlack;
+      for (int x = 0; x < 8; x++) mx[t] = __builtin_fmaxf(mx[t], S[t][x >> 2][x & 3]);
+      move |= __builtin_fmaf(mx[t], f[t], lvs) > M[t] + (kShift + kSlack);
     }
     if (__any(move)) {
 #pragma unroll
       for (int t = 0; t < NT; t++) {
-        const float y = max_stage<32>(max_stage<16>(mx[t])) * f[t] + lvs;
+        const float y = max_stage<32>(max_stage<16>(mx[t])) * f[t] + lvs - kShift;
         const float mn = y > M[t] ? y : M[t], al = __builtin_amdgcn_exp2f(M[t] - mn);
         M[t] = mn;
         far |= __any(__builtin_fabsf(mn) > 65536.0f && mn != kNone);
@@ -368,7 +370,7 @@ __global__ __launch_bounds__(kWaves * 64, NT == 1 && D == 64 ? 4 : 2) void k_kv8
     float part[NT];
 #pragma unroll
     for (int t = 0; t < NT; t++) {
-      const float c0 = lvs - M[t] + kShift;
+      const float c0 = lvs - M[t];
       float p[8];
 #pragma unroll
       for (int x = 0; x < 8; x++) p[x] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[t][x >> 2][x & 3], f[t], c0));
@@ -411,7 +413,7 @@ __global__ __launch_bounds__(kWaves * 64, NT == 1 && D == 64 ? 4 : 2) void k_kv8
       const float m = G >= 2 ? M[NT - 1] : M[0];
       const int col = tile * W + (G >> 1) * 16 + col16;
       if ((NT == 2 ? !(G & 1) : G == 0) && col < cols)
-        a.lse[((size_t)hs * c.slots + b) * cols + col] = __builtin_amdgcn_logf(y) + (m - kShift - lvs);
+        a.lse[((size_t)hs * c.slots + b) * cols + col] = __builtin_amdgcn_logf(y) + (m - lvs);
     }
   };
 
