@@ -175,6 +175,10 @@ __global__ __launch_bounds__(kWaves * 64, NT == 1 && D == 64 ? 4 : 2) void k_kv8
   // blocks in flight: with two tiles, or the 8 KB blocks of wide heads, the other waves cover the loads (sixteen
   // sequences of wide heads 31.4 us a pass for 32.9, one sequence of 131000 positions of narrow ones 36.6 for 35.4)
   constexpr int PF = NT == 1 && D == 64 ? 2 : 1;
+  // One block in flight: the next one's K is asked for once this one's scores are there, not behind its products of V
+  // (sixteen sequences of wide heads 34.2 -> 32.9 us a pass, 1000 positions after 16001 191 -> 189). With two in flight
+  // that is late already (131000 positions 33.0 -> 34.3).
+  constexpr bool EARLY = PF == 1;
   // Sums of weights come from the matrix cores, which have time to spare: of the two halves of f32's, or of the rounded
   // weights, whose error is far below an fp16 output's. The blocks' weights are f32 in any case: there the vector unit
   // adds up a lane's eight, and lanes are joined for the block's sum and at the end.
@@ -217,18 +221,26 @@ __global__ __launch_bounds__(kWaves * 64, NT == 1 && D == 64 ? 4 : 2) void k_kv8
     lvs_l = __builtin_amdgcn_logf(vs_l);
     ivs_l = 1.0f / vs_l;
   };
-  auto fetch = [&](int p, int x) {
+  auto fetch_k = [&](int p, int x) {
     const int slot = __builtin_amdgcn_readlane(slot_l, min(x, count - 1));
     const size_t at = (head * c.slots + slot) * (size_t)(kKvBlock * D);
     const uint8_t* kp = c.kc + at + col16 * D + G * 16;
-    const uint8_t* vp = c.vc + at + (col16 % RP * 4 + G) * (U * 8) + col16 / RP * 16;
 #pragma unroll
     for (int y = 0; y < 2; y++)
 #pragma unroll
       for (int z = 0; z < CH; z++)
         kb[p][y * CH + z] = STREAM ? gload_u4_nt(kp + y * 16 * D + z * 64) : gload_u4(kp + y * 16 * D + z * 64);
+  };
+  auto fetch_v = [&](int p, int x) {
+    const int slot = __builtin_amdgcn_readlane(slot_l, min(x, count - 1));
+    const size_t at = (head * c.slots + slot) * (size_t)(kKvBlock * D);
+    const uint8_t* vp = c.vc + at + (col16 % RP * 4 + G) * (U * 8) + col16 / RP * 16;
 #pragma unroll
     for (int y = 0; y < 2 * CH; y++) vb[p][y] = STREAM ? gload_u4_nt(vp + y * 1024) : gload_u4(vp + y * 1024);
+  };
+  auto fetch = [&](int p, int x) {
+    fetch_k(p, x);
+    fetch_v(p, x);
   };
   if (b0 < full) {
     batch(b0);
@@ -301,9 +313,9 @@ __global__ __launch_bounds__(kWaves * 64, NT == 1 && D == 64 ? 4 : 2) void k_kv8
   h8 ones;
 #pragma unroll
   for (int j = 0; j < 8; j++) ones[j] = (_Float16)1.0f;
-  // One block: kop(half, k), vop(u) give the operands. masked: some column does not see all of it (S is -inf there,
+  // One block: kop(half, k), vop(u) give the operands, then() runs behind the scores. masked: some column does not see all of it (S is -inf there,
   // which moves no maximum; NaN with a scale of 0, which moves none either), or `bad` names poisoned rows, of the tail.
-  auto block = [&](auto masked, auto kop, auto vop, float ks, float lvs, float ivs, int b, uint32_t bad) {
+  auto block = [&](auto masked, auto kop, auto vop, auto then, float ks, float lvs, float ivs, int b, uint32_t bad) {
     constexpr bool MASKED = decltype(masked)::value;
     f4 S[NT][2];
     if constexpr (NT > 1) __builtin_amdgcn_s_setprio(1);
@@ -334,6 +346,7 @@ __global__ __launch_bounds__(kWaves * 64, NT == 1 && D == 64 ? 4 : 2) void k_kv8
           }
     }
     if constexpr (NT > 1) __builtin_amdgcn_s_setprio(0);
+    then();
     float f[NT], mx[NT];
     bool move = false;
 #pragma unroll
@@ -424,7 +437,7 @@ __global__ __launch_bounds__(kWaves * 64, NT == 1 && D == 64 ? 4 : 2) void k_kv8
       for (int p = 0; p < PF; p++) fetch(p, p);
     }
     scales();
-    auto run = [&](auto masked, int p, int x) {
+    auto run = [&](auto masked, int p, int x, auto then) {
       auto kop = [&](int y, int k) {
         const uint4 v = kb[p][y * CH + (k >> 1)];
         return k & 1 ? half_codes(v.z, v.w) : half_codes(v.x, v.y);
@@ -433,7 +446,7 @@ __global__ __launch_bounds__(kWaves * 64, NT == 1 && D == 64 ? 4 : 2) void k_kv8
         const uint4 v = vb[p][u >> 1];
         return u & 1 ? half_codes(v.z, v.w) : half_codes(v.x, v.y);
       };
-      block(masked, kop, vop, __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(ks_l), x)),
+      block(masked, kop, vop, then, __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(ks_l), x)),
             __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(lvs_l), x)),
             __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(ivs_l), x)), base + x * step, 0u);
     };
@@ -442,13 +455,14 @@ __global__ __launch_bounds__(kWaves * 64, NT == 1 && D == 64 ? 4 : 2) void k_kv8
     for (int x = 0; x < whole; x += PF) {
 #pragma unroll
       for (int p = 0; p < PF; p++) {
-        if (x + p < whole) run(std::false_type(), p, x + p);
-        fetch(p, x + p + PF);
+        if (x + p < whole) run(std::false_type(), p, x + p, [&]() { if constexpr (EARLY) fetch_k(p, x + p + PF); });
+        if constexpr (EARLY) fetch_v(p, x + p + PF);
+        else fetch(p, x + p + PF);
       }
     }
     for (int x = whole; x < count; x++) {
       if (x) fetch(0, x);
-      run(std::true_type(), 0, x);
+      run(std::true_type(), 0, x, []() {});
     }
   }
   if (seen > full && full % step == b0) {  // the tail, in fp16
@@ -466,7 +480,7 @@ __global__ __launch_bounds__(kWaves * 64, NT == 1 && D == 64 ? 4 : 2) void k_kv8
         v[j] = use >> (G * 4 + (j & 3) + 16 * (j >> 2)) & 1 ? v[j] : (_Float16)0.0f;
       return v;
     };
-    block(std::true_type(), kop, vop, 1.0f, 0.0f, 1.0f, full, bad);
+    block(std::true_type(), kop, vop, []() {}, 1.0f, 0.0f, 1.0f, full, bad);
   }
 
   // the waves' shares, tile by tile
