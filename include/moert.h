@@ -405,9 +405,10 @@ int moert_attn_decode_noalloc(const float* q_dev, const uint16_t* k_cache_dev, c
  *
  * Limits: head_dim 64 or 128; max_len a multiple of 32, at most 2^20; at most 65535 sequences, 256 KV heads and 2^20
  * KV heads of all sequences together, 64 query heads to a KV head, and 2^27 query heads x positions x sequences in one
- * attention. Calls take sequences [seq0, seq0 + n_seqs). They enqueue on `stream` (a hipStream_t of the buffers' device, NULL for its
- * default stream), allocate nothing and do not synchronise, except moert_kv8_lengths. Calls on one cache are ordered
- * by the caller (one stream, or events); attentions that do not track may overlap, each with a workspace of its own.
+ * attention. Calls take sequences [seq0, seq0 + n_seqs). They enqueue on `stream` (a hipStream_t of the buffers'
+ * device, NULL for its default stream), allocate nothing and do not synchronise, except moert_kv8_lengths. Calls on one
+ * cache are ordered by the caller (one stream, or events); attentions that do not track may overlap, each with a
+ * workspace of its own.
  * ------------------------------------------------------------------------------------------------------- */
 enum { MOERT_KV8_BLOCK = 32 };
 typedef struct {
@@ -445,13 +446,12 @@ int moert_kv8_workspace(const moert_kv8* c, int n_seqs, int heads, int n, int tr
 /* Attention of n positions over the cache, whose last n rows are theirs (appended before): position i of a sequence of
  * len rows sees the first len - n + 1 + i of them, and query head h reads KV head h / (heads / kv_heads).
  * out = sum_t p_t v_t, p = softmax(scale * q . k); a position that sees no row gets 0, a query row that is not finite
- * NaN. q and out are of one type:
- * scores, weights and sums are f32 for both; with MOERT_F16 the weights enter the second product rounded to fp16, with
- * MOERT_F32 as the sum of two fp16 (22 bits).
+ * NaN. q and out are of one type: scores, weights and sums are f32 for both, a weight as good as its score, an f32 (of
+ * scores of 10^5, to 1 in 100); with MOERT_F16 the weights enter the second product rounded to fp16, with MOERT_F32 as
+ * the sum of two fp16 (22 bits).
  * mass_decay in [0, 1] tracks: mass = mass_decay * mass + w for every block in use, w the sum of the block's p over
  * the n positions and the group's query heads (NaN for what a position sees if it sees a value that is not finite).
- * A negative mass_decay does not track. ws: moert_kv8_workspace bytes, aligned
- * to 16. */
+ * A negative mass_decay does not track. ws: moert_kv8_workspace bytes, aligned to 16. */
 int moert_kv8_attend(const moert_kv8* c, int seq0, int n_seqs, int heads, int n, float scale, const moert_rows* q,
                      const moert_rows* out, float mass_decay, void* ws_dev, size_t ws_bytes, void* stream);
 

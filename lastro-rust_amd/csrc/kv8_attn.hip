@@ -21,11 +21,11 @@
 // out as log2 by column, which needs no final maximum, and a pass over them adds up the weights in a fixed order.
 //
 // What bounds it, measured on one MI355X (3B shape: 8 KV heads of 64, 3 query heads each):
-//   one position   the cache's bytes: 134 MB of one sequence in 25 us (5.3 TB/s), 565 MB of eight in 108 us (5.2; blocks
+//   one position   the cache's bytes: 134 MB of one sequence in 25 us (5.3 TB/s), 565 MB of eight in 109 us (5.2; blocks
 //                  in any order; a streaming read of 512 MiB reaches 5.7). Short caches: launches (5.7 us for 100 rows).
-//   many           the vector unit: a block of two tiles is 16 or 18 MFMAs of 16 cycles beside some 170 vector
+//   many           the vector unit: a block of two tiles is 16 or 18 MFMAs of 16 cycles beside some 145 vector
 //                  instructions, 64 of them the conversion of the codes, 16 exps at a quarter of the rate. 1000
-//                  positions after 16001: 101 GFLOP in about 180 us in fp16. Tiles to a wave, whole call: one 311, two 206,
+//                  positions after 16001: 101 GFLOP in about 172 us in fp16. Tiles to a wave, whole call: one 311, two 206,
 //                  three 215 and four 260 us (fewer waves to overlap the two units); 2, 4 or 8 waves to a workgroup: 282,
 //                  206, 243. The matrix instructions first (s_setprio): 206 -> 197.
 #include <type_traits>
@@ -734,8 +734,8 @@ hipError_t launch_kv8_attend(hipStream_t s, const Kv8Dev& c, int seq0, int n_seq
   const bool track = decay >= 0.0f;
   const KvAttnPlan p = kv8_attn_plan(c, n_seqs, heads, n, track);
   char* w = (char*)ws;
-  AttnArgs a{c, q, out, seq0, n_seqs, heads / c.kvh, n, p.splits, 1, wide_rows(q) | wide_rows(out) << 1, __builtin_fabsf(scale) * kLog2e,
-             scale < 0.0f ? 0x80000000u : 0u, (float*)(w + p.parts), (float2*)(w + p.ml), (float*)(w + p.tot),
+  AttnArgs a{c, q, out, seq0, n_seqs, heads / c.kvh, n, p.splits, 1, wide_rows(q) | wide_rows(out) << 1,
+             __builtin_fabsf(scale) * kLog2e, scale < 0.0f ? 0x80000000u : 0u, (float*)(w + p.parts), (float2*)(w + p.ml), (float*)(w + p.tot),
              track ? (float*)(w + p.lse) : nullptr};
 #define ATT(DD, FF) \
   if (c.d == DD && q.f16 == FF) return track ? attend<DD, FF, true>(s, a, decay) : attend<DD, FF, false>(s, a, decay);
