@@ -8,8 +8,12 @@
 //   softmax      u = s scale log2 e in base 2; the running maximum M of u + log2(scale of V) moves only when it has to
 //                (by more than 8), so most blocks cost no exchange between lanes. p = 2^(u + log2 vs - M + 7): the
 //                weights that meet the V codes carry the scale of V, so blocks of any scale add up in one accumulator,
-//                and the largest contribution lies between 2^7 and 2^15, where fp16 has 11 bits down to 2^-21 of it.
-//                The sum of softmax takes p / vs, in f32.
+//                and the largest contribution lies between 2^7 and 2^15, where fp16 has 11 bits down to 2^-21 of it and
+//                stops at 2^-32. The sum of softmax and the blocks' weights take p / vs in f32, before p is rounded.
+//                A block whose scale of V lies more than 2^8 below that of one that has moved M (zeros have scale 1)
+//                would have its p below that, however much softmax weight it has: its p, and O for the time of its
+//                products, are taken 2^k2 times as large, which brings its largest p to 2^6 or above. So the rounding
+//                of a weight is off by its last bit or by 2^-24 of the column's largest weight.
 //   O += V^T P^T MFMA 16x16x32 over the 32 positions: rows = 16 elements, columns = columns. A lane of the S product
 //                holds positions 4 G .. 4 G + 3 of both halves of the block for its column, which is what it has to
 //                hold of P here when the positions of V are taken in that order: v_place lays V out so, and p never
@@ -46,6 +50,8 @@ constexpr float kLog2e = 1.44269504088896341f;
 constexpr int kWaves = 4;       // waves of a workgroup, each its share of the blocks
 constexpr int kMaxSplits = 64;  // one lane each in the combine
 constexpr float kShift = 7.0f, kSlack = 8.0f;
+constexpr float kApart = 8.0f;    // log2 of how far a block's scale of V may lie below one that M follows
+constexpr float kMostUp = 60.0f;  // O is a sum of at most 2^20 products below 2^22, so it stays in range 2^60 times
 constexpr float kNone = -3.4e38f;  // maximum of what has no score yet; finite, so that differences with it are
 
 // a + the value of a's lane 16 (32) away, in both of them.
@@ -179,10 +185,6 @@ __global__ __launch_bounds__(kWaves * 64, NT == 1 && D == 64 ? 4 : 2) void k_kv8
   // (sixteen sequences of wide heads 34.2 -> 32.9 us a pass, 1000 positions after 16001 191 -> 189). With two in flight
   // that is late already (131000 positions 33.0 -> 34.3).
   constexpr bool EARLY = PF == 1;
-  // Sums of weights come from the matrix cores, which have time to spare: of the two halves of f32's, or of the rounded
-  // weights, whose error is far below an fp16 output's. The blocks' weights are f32 in any case: there the vector unit
-  // adds up a lane's eight, and lanes are joined for the block's sum and at the end.
-  constexpr bool VSUM = F16 && TRACK;
   __shared__ __align__(16) float Os[kWaves][16][D + 4];
   __shared__ float2 Ms[kWaves][16];
   const Kv8Dev& c = a.c;
@@ -297,7 +299,7 @@ __global__ __launch_bounds__(kWaves * 64, NT == 1 && D == 64 ? 4 : 2) void k_kv8
   }
   const int sees0 = len - a.n + 1 + min(tile * W, cols - 1) / a.g;  // the least of the tile
 
-  float M[NT], l[NT];  // M: the maximum less 7, so that the weights below are 2^7 times those to it
+  float M[NT], l[NT];  // M: the maximum less 7, so that the weights below are 2^7 times those to it; l: a lane's own sum
   f4 O[NT][U];
 #pragma unroll
   for (int t = 0; t < NT; t++) {
@@ -307,12 +309,10 @@ __global__ __launch_bounds__(kWaves * 64, NT == 1 && D == 64 ? 4 : 2) void k_kv8
     for (int u = 0; u < U; u++) O[t][u] = f4{0.0f, 0.0f, 0.0f, 0.0f};
   }
 
-  bool far = false;  // some column's M is beyond 2^16
+  bool far = false;    // some column's M is beyond 2^16
+  float vref = kNone;  // the largest log2 of a scale of V that came with a move of M
   float none = -__builtin_inff();  // opaque, so that eight maxima with it are four instructions
   asm("" : "+s"(none));
-  h8 ones;
-#pragma unroll
-  for (int j = 0; j < 8; j++) ones[j] = (_Float16)1.0f;
   // One block: kop(half, k), vop(u) give the operands, then() runs behind the scores. masked: some column does not see all of it (S is -inf there,
   // which moves no maximum; NaN with a scale of 0, which moves none either), or `bad` names poisoned rows, of the tail.
   auto block = [&](auto masked, auto kop, auto vop, auto then, float ks, float lvs, float ivs, int b, uint32_t bad) {
@@ -358,6 +358,7 @@ __global__ __launch_bounds__(kWaves * 64, NT == 1 && D == 64 ? 4 : 2) void k_kv8
       move |= __builtin_fmaf(mx[t], f[t], lvs) > M[t] + (kShift + kSlack);
     }
     if (__any(move)) {
+      vref = __builtin_fmaxf(vref, lvs);
 #pragma unroll
       for (int t = 0; t < NT; t++) {
         const float y = max_stage<32>(max_stage<16>(mx[t])) * f[t] + lvs - kShift;
@@ -369,6 +370,21 @@ __global__ __launch_bounds__(kWaves * 64, NT == 1 && D == 64 ? 4 : 2) void k_kv8
         for (int u = 0; u < U; u++)
 #pragma unroll
           for (int i = 0; i < 4; i++) O[t][u][i] *= al;
+      }
+    }
+    const bool apart = lvs < vref - kApart;  // the same for the wave
+    float k2[NT];                            // p is 2^k2 times what M makes it, and O with it
+#pragma unroll
+    for (int t = 0; t < NT; t++) k2[t] = 0.0f;
+    if (apart) {
+#pragma unroll
+      for (int t = 0; t < NT; t++) {
+        const float y = max_stage<32>(max_stage<16>(mx[t])) * f[t] + lvs - kShift;
+        k2[t] = __builtin_fminf(__builtin_fmaxf(__builtin_floorf(M[t] - y), 0.0f), kMostUp);  // of NaN 0
+#pragma unroll
+        for (int u = 0; u < U; u++)
+#pragma unroll
+          for (int i = 0; i < 4; i++) O[t][u][i] = __builtin_amdgcn_ldexpf(O[t][u][i], (int)k2[t]);
       }
     }
     if (far) {  // M is rounded by more than p allows: the same rounding for the scores
@@ -383,7 +399,7 @@ __global__ __launch_bounds__(kWaves * 64, NT == 1 && D == 64 ? 4 : 2) void k_kv8
     float part[NT];
 #pragma unroll
     for (int t = 0; t < NT; t++) {
-      const float c0 = lvs - M[t];
+      const float c0 = lvs - M[t] + k2[t];
       float p[8];
 #pragma unroll
       for (int x = 0; x < 8; x++) p[x] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[t][x >> 2][x & 3], f[t], c0));
@@ -392,22 +408,14 @@ __global__ __launch_bounds__(kWaves * 64, NT == 1 && D == 64 ? 4 : 2) void k_kv8
         for (int x = 0; x < 8; x++)
           if (b * kKvBlock + (x >> 2) * 16 + G * 4 + (x & 3) >= sees[t]) p[x] = 0.0f;
       }
-      if constexpr (VSUM) part[t] = ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+      part[t] = ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
 #pragma unroll
       for (int x = 0; x < 8; x++) {
         ph[t][x] = (_Float16)p[x];
         if constexpr (!F16) pl[t][x] = (_Float16)(p[x] - (float)ph[t][x]);
       }
     }
-    f4 sum[NT];
     if constexpr (NT > 1) __builtin_amdgcn_s_setprio(1);
-    if constexpr (!VSUM) {
-#pragma unroll
-      for (int t = 0; t < NT; t++) {
-        sum[t] = mfma(ones, ph[t], f4{0.0f, 0.0f, 0.0f, 0.0f});
-        if constexpr (!F16) sum[t] = mfma(ones, pl[t], sum[t]);
-      }
-    }
 #pragma unroll
     for (int u = 0; u < U; u++) {
       const h8 va = vop(u);
@@ -418,11 +426,21 @@ __global__ __launch_bounds__(kWaves * 64, NT == 1 && D == 64 ? 4 : 2) void k_kv8
       }
     }
     if constexpr (NT > 1) __builtin_amdgcn_s_setprio(0);
+    if (apart) {
 #pragma unroll
-    for (int t = 0; t < NT; t++) l[t] = __builtin_fmaf(VSUM ? part[t] : sum[t][0], ivs, l[t]);
+      for (int t = 0; t < NT; t++) {
+        part[t] = __builtin_amdgcn_ldexpf(part[t], -(int)k2[t]);
+#pragma unroll
+        for (int u = 0; u < U; u++)
+#pragma unroll
+          for (int i = 0; i < 4; i++) O[t][u][i] = __builtin_amdgcn_ldexpf(O[t][u][i], -(int)k2[t]);
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < NT; t++) l[t] = __builtin_fmaf(part[t], ivs, l[t]);
     if constexpr (TRACK) {  // lanes of group 0 write tile 0's, those of group 2 tile 1's
       static_assert(NT <= 2, "");
-      const float y = VSUM ? add16(add32(part[0], part[NT - 1])) : G >= 2 ? sum[NT - 1][0] : sum[0][0];
+      const float y = add16(add32(part[0], part[NT - 1]));
       const float m = G >= 2 ? M[NT - 1] : M[0];
       const int col = tile * W + (G >> 1) * 16 + col16;
       if ((NT == 2 ? !(G & 1) : G == 0) && col < cols)
@@ -486,7 +504,7 @@ __global__ __launch_bounds__(kWaves * 64, NT == 1 && D == 64 ? 4 : 2) void k_kv8
   // the waves' shares, tile by tile
 #pragma unroll
   for (int t = 0; t < NT; t++) {
-    const float lt = VSUM ? add16(add32(l[t], l[t])) : l[t];
+    const float lt = add16(add32(l[t], l[t]));
     if (t) __syncthreads();
     if (G == 0) Ms[w][col16] = make_float2(M[t], lt);
 #pragma unroll
@@ -515,7 +533,7 @@ __global__ __launch_bounds__(kWaves * 64, NT == 1 && D == 64 ? 4 : 2) void k_kv8
         const long long at = sc * a.out.seq + (long long)(col / a.g) * a.out.pos +
                              (long long)(h * a.g + col % a.g) * a.out.head + e0;
 #pragma unroll
-        for (int e = 0; e < U; e++) o[e] = VSUM ? in_f16(o[e] * inv) : o[e] * inv;
+        for (int e = 0; e < U; e++) o[e] = F16 ? in_f16(o[e] * inv) : o[e] * inv;
         store_out<U, F16>(a.out, at, a.vec & 2, o);
         if (TRACK && e0 == 0) a.tot[wc] = total_of(m, sum, none);
       } else {

@@ -681,3 +681,95 @@ def test_a_broken_table_stays_inside_the_buffers(hip):
         got = dev.attend(q, 0.125, decay=1.0)
         assert np.isfinite(got).all() and got.any() == (length > 0)
         dev.c.evict(1)
+
+
+def weights_bound(ref, q, scale, f16):
+    """How far an output may be from the 64-bit one, element by element, whatever the scales of V: e, the relative error
+    of a weight in f32, is out_bound's. The weights of the second product are rounded by 2^-11 (F16) or 2^-21 (F32) of
+    themselves. Below that an fp16 has a step of 2^-24, an error of 2^-25, where the largest contribution to its column
+    so far, weight x scale of V, is at 2^7 or above: 2^-32 of it, over the block's own scale; and where the scale of a
+    block lies more than 2^8 below that of a contribution that set the maximum, its weights are taken relative to their
+    own largest: 2^-32 of the largest weight. So an error never passes 2^-24 of the largest weight."""
+    N, n, heads, d = q.shape
+    g = heads // ref.H
+    off = np.zeros(q.shape)
+    for i in range(N):
+        L = ref.len(i)
+        for h in range(ref.H):
+            k, v, _ = ref.rows(i, h)
+            vs = np.repeat([np.float64(b[3]) for b in ref.blocks[i][h]] + [1.0], B)[:L]
+            for j in range(n):
+                m = L - n + 1 + j
+                for a in range(h * g, h * g + g):
+                    x = q[i, j, a].astype(np.float64)
+                    mag = abs(scale) * (np.abs(k[:m]) @ np.abs(x)).max()
+                    sc = scale * (k[:m] @ x)
+                    p = np.exp(sc - sc.max())
+                    p /= p.sum()
+                    e = 2 * mag * ((d + 8) * 2.0 ** -23 + 2.0 ** -22) + (1.5 * np.abs(sc).max() + 32) * 2.0 ** -22 + \
+                        (64 + 4 * -(-m // B)) * 2.0 ** -23
+                    floor = np.minimum(2.0 ** -24 * p.max(), 2.0 ** -32 * (p * vs[:m]).max() / vs[:m])
+                    floor = np.maximum(floor, 2.0 ** -32 * p.max())
+                    off[i, j, a] = (e + (2.0 ** -11 if f16 else 2.0 ** -21)) * (p @ np.abs(v[:m])) + floor @ np.abs(v[:m])
+                    if f16:
+                        off[i, j, a] += 2.0 ** -11 * np.abs(p @ v[:m]) + 2.0 ** -24
+    return off
+
+
+def scaled_v(kind, rng, rows, kv_heads, d):
+    """V whose blocks differ by scale, the large ones first."""
+    v, b = normal(rng, 1, rows, kv_heads, d), np.arange(rows)[None, :, None, None] // B
+    if kind == "falling":  # by 2^2 from block to block, 2^8 from one of a wave's to its next, 2^37 in all
+        return v * 2.0 ** np.maximum(13.0 - 2 * b, -24.0)
+    if kind == "large first":
+        return v * np.where(b < 4, 1e4, 1e-6)
+    if kind == "zeros first":
+        return v * np.where(b < 5, 0.0, 1e-4)
+    if kind == "zeros between":
+        return v * np.where(b % 3 == 1, 0.0, 1e-2)
+    assert kind == "by element"  # the first blocks hold element 0 alone, the others all but it
+    e = np.arange(d) == 0
+    return np.where(b < 4, np.where(e, 1e4, 0.0), np.where(e, 0.0, 1e-3)) * v
+
+
+@pytest.mark.parametrize("kind", ["falling", "large first", "zeros first", "zeros between", "by element"])
+@pytest.mark.parametrize("d,n", [(64, 1), (64, 30), (128, 1), (128, 30)])
+@pytest.mark.parametrize("dtype", [moert.F32, moert.F16])
+def test_scales_of_v_that_fall(hip, dtype, d, n, kind):
+    """A wave's blocks with ever smaller V, and blocks of zeros before others: every row keeps its share of the sum of
+    softmax and of its block's weight, and outputs do not depend on whether the weights are kept."""
+    rng = np.random.default_rng(24)
+    rows = 500  # blocks 0, 4, 8, 12 are one wave's
+    dev, ref = both(hip, 1, 2, d, 512)
+    k, v = normal(rng, 1, rows, 2, d), scaled_v(kind, rng, rows, 2, d)
+    dev.append(k, v)
+    ref.append(k, v)
+    for size in (0.5, 4.0):
+        q = normal(rng, 1, n, 6, d, scale=size).astype(np.float16 if dtype == moert.F16 else np.float32)
+        off = weights_bound(ref, q, d ** -0.5, dtype == moert.F16)
+        want = ref.attend(q, d ** -0.5)
+        plain = dev.attend(q, d ** -0.5, dtype)
+        kept = check_attend(dev, ref, q, d ** -0.5, dtype, decay=1.0)
+        for got in (plain, kept):
+            worst = np.abs(got.astype(np.float64) - want) / off
+            assert (worst <= 1).all(), f"{size}: {worst.max()} of its bound"
+        same = np.array_equal(plain.astype(np.float64), kept)
+        assert same, size
+
+
+@pytest.mark.parametrize("dtype", [moert.F32, moert.F16])
+@pytest.mark.parametrize("n", [1, 12])
+def test_zero_rows_before_a_long_sequence(hip, dtype, n):
+    """A padded prompt: 1000 rows of zeros in K and V, then small V, in many splits."""
+    rng = np.random.default_rng(25)
+    dev, ref = both(hip, 1, 2, 64, 16384)
+    k, v = normal(rng, 1, 9001, 2, 64), normal(rng, 1, 9001, 2, 64, scale=1e-4)
+    k[:, :1000], v[:, :1000] = 0.0, 0.0
+    dev.append(k, v)
+    ref.append(k, v)
+    q = normal(rng, 1, n, 6, 64).astype(np.float16 if dtype == moert.F16 else np.float32)
+    off, want = weights_bound(ref, q, 0.125, dtype == moert.F16), ref.attend(q, 0.125)
+    for decay in (None, 1.0):
+        got = check_attend(dev, ref, q, 0.125, dtype, decay=decay)
+        worst = np.abs(got.astype(np.float64) - want) / off
+        assert (worst <= 1).all(), f"{worst.max()} of its bound"
