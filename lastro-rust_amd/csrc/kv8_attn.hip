@@ -190,9 +190,12 @@ __global__ __launch_bounds__(kWaves * 64, NT == 1 && D == 64 ? 4 : 2) void k_kv8
   const Kv8Dev& c = a.c;
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col16 = lane & 15, G = lane >> 4;
-  // the tiles that read the same blocks run on the same XCD (workgroups go round them in turn)
-  const int id = blockIdx.x, unit = id / 8 / a.tiles * 8 + id % 8, tile = id / 8 % a.tiles;
-  if (unit >= a.n_seqs * c.kvh * a.splits) return;
+  // the tiles that read the same blocks run on the same XCD (workgroups go round them in turn), where there are enough
+  // units for all of them; fewer than 8 take turns, and none stands for a unit that is not there
+  const int id = blockIdx.x, units = a.n_seqs * c.kvh * a.splits;
+  const int unit = units < 8 ? id % units : id / 8 / a.tiles * 8 + id % 8;
+  const int tile = units < 8 ? id / units : id / 8 % a.tiles;
+  if (unit >= units) return;
   const int split = unit % a.splits, hs = unit / a.splits, h = hs % c.kvh, sc = hs / c.kvh, s = a.seq0 + sc;
   const size_t head = (size_t)s * c.kvh + h;
   const int b0 = split * kWaves + w, step = a.splits * kWaves;  // this wave's first block, and on to the next
@@ -718,7 +721,7 @@ hipError_t attend(hipStream_t s, AttnArgs a, float decay) {
   const int cols = a.n * a.g, nt = tile_count(cols), width = 16 * nt;
   a.tiles = (cols + width - 1) / width;
   const long long units = (long long)a.n_seqs * a.c.kvh * a.splits;
-  const long long grid = (units + 7) / 8 * 8 * a.tiles;
+  const long long grid = (units < 8 ? units : (units + 7) / 8 * 8) * a.tiles;  // below 2^23 (256 threads each: 2^31)
   // A layer's cache of 96 MB and more is streamed past the others: three of them outgrow the 256 MB last-level cache, and
   // a model has more. 565 MB of eight sequences 138 -> 125 us a pass, 134 MB of one 35.4 -> 32.5; where three caches
   // still fit (68 MB in use of 134 each), a pass loses what it would find there, 32.9 -> 34.1.
