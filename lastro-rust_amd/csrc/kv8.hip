@@ -418,6 +418,7 @@ hipError_t launch_kv8_append(hipStream_t s, const Kv8Dev& c, int seq0, int n_seq
   const dim3 grid(blocks * c.kvh, n_seqs);
   if (c.d == 64) klaunch(k_kv8_append<64>, grid, kAppendThreads, 0, s, c, k, v, seq0, n, blocks, vec, arrive);
   else klaunch(k_kv8_append<128>, grid, kAppendThreads, 0, s, c, k, v, seq0, n, blocks, vec, arrive);
+  if (const hipError_t e = hipGetLastError()) return e;  // no rows, no length
   if (!arrive) klaunch(k_kv8_advance, (n_seqs + 63) / 64, 64, 0, s, c, seq0, n_seqs, n);
   return hipGetLastError();
 }

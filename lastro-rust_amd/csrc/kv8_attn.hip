@@ -729,6 +729,8 @@ hipError_t attend(hipStream_t s, AttnArgs a, float decay) {
   if (stream) klaunch(k_kv8_attend<D, F16, 1, TRACK, true>, (unsigned)grid, kWaves * 64, 0, s, a);
   else if (nt == 1) klaunch(k_kv8_attend<D, F16, 1, TRACK, false>, (unsigned)grid, kWaves * 64, 0, s, a);
   else klaunch(k_kv8_attend<D, F16, 2, TRACK, false>, (unsigned)grid, kWaves * 64, 0, s, a);
+  // what follows reads the workspace that this launch writes, and the masses are the caller's
+  if (const hipError_t e = hipGetLastError()) return e;
   const long long all = (long long)a.n_seqs * a.c.kvh * cols;
   int P = 1;
   while (P < cols && P < 64) P *= 2;
@@ -744,6 +746,7 @@ hipError_t attend(hipStream_t s, AttnArgs a, float decay) {
   }
   if (a.splits > 8) klaunch(k_kv8_combine<D, F16, TRACK, 4>, (unsigned)all, 256, 0, s, a, width);
   else if (a.splits > 1) klaunch(k_kv8_combine<D, F16, TRACK, 1>, (unsigned)((all + 3) / 4), 256, 0, s, a, width);
+  if (const hipError_t e = hipGetLastError()) return e;
   if (TRACK) klaunch(k_kv8_mass, dim3(per_head, a.c.kvh, a.n_seqs), 256, 0, s, a, decay, P);
   return hipGetLastError();
 }
