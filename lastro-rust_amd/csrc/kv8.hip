@@ -525,13 +525,15 @@ int rows(const char* what, const moert_rows* r, int n_seqs, int n, int heads, in
   return MOERT_OK;
 }
 
-// Makes the buffers' device the current one while the call lasts.
+// Makes the buffers' device the current one while the call lasts. An error that an earlier call of the caller's has
+// left in the thread is dropped: the launchers ask for the last error, and it would pass for a launch's.
 class OnDevice {
  public:
   ~OnDevice() {
     if (back_ >= 0) (void)hipSetDevice(back_);
   }
   int enter(const char* what, const void* p) {
+    (void)hipGetLastError();
     hipPointerAttribute_t a;
     if (hipPointerGetAttributes(&a, p) != hipSuccess) {
       (void)hipGetLastError();  // an address that the runtime does not know is no device error

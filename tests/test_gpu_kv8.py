@@ -773,3 +773,18 @@ def test_zero_rows_before_a_long_sequence(hip, dtype, n):
         got = check_attend(dev, ref, q, 0.125, dtype, decay=decay)
         worst = np.abs(got.astype(np.float64) - want) / off
         assert (worst <= 1).all(), f"{worst.max()} of its bound"
+
+
+def test_an_error_the_caller_has_dealt_with_fails_no_call(hip):
+    dev, ref = both(hip, 1, 2, 64, 128)
+    rng = np.random.default_rng(26)
+    r = normal(rng, 2, 1, 70, 2, 64)
+    at = [hip.upload(x) for x in r]
+    assert hip.rt.hipSetDevice(4096) != 0  # no such device: the thread's last error
+    dev.c.append(at[0], at[1], 70)
+    ref.append(r[0], r[1])
+    ku.assert_holds(dev, ref)
+    q = normal(rng, 1, 1, 4, 64)
+    dev.workspace(4, 1, 1, True)
+    assert hip.rt.hipSetDevice(4096) != 0
+    check_attend(dev, ref, q, 0.125, decay=1.0)

@@ -145,3 +145,10 @@ def test_grids_stay_below_32_bits_of_threads(launches):
         assert got[0] == 0 and kinds(got)[0] == "attend", (c, got)
         for name, x, y, z, threads in got[1]:
             assert x * threads < 1 << 32 and y < 1 << 16 and z < 1 << 16, (c, name, x, y, z)
+
+
+def test_an_error_of_an_earlier_call_is_not_the_launchs(launches):
+    """The runtime keeps a thread's last error until it is asked for. One that the caller has dealt with (an allocation
+    that did not fit, say) makes no call fail, and leaves none half done."""
+    for (c, want), got in zip(FORMS, launches([dict(c, stale=2) for c, _ in FORMS])):
+        assert got[0] == 0 and kinds(got) == want, (c, got)
