@@ -398,7 +398,7 @@ int moert_attn_decode_noalloc(const float* q_dev, const uint16_t* k_cache_dev, c
  *   table             i32 [seqs][kv_heads][slots]  slot of each block, in order: a permutation of the slots, the
  *                         blocks in use first (the tail's among them)
  *   mass              f32 [seqs][kv_heads][slots]  by slot; may be NULL where no call tracks or evicts
- *   state             i32 [seqs][4]  rows of the sequence, rows dropped for want of room, 0, 0
+ *   state             i32 [seqs][4]  rows of the sequence, rows dropped for want of room (2^31 - 1: or more), 0, 0
  * moert_kv8_clear makes them an empty cache. Lengths are on the device, so that a captured graph of these calls can be
  * replayed: each replay goes on from the lengths it finds. The buffers may be copied and put back as a whole. Kernels
  * keep to the buffers whatever table and state hold.

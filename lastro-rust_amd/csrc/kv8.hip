@@ -68,6 +68,12 @@ __device__ __forceinline__ int top_of(uint4 x) {
   return m;
 }
 
+// Counts rows that found no room, up to the type's largest number: no count of them comes back to 0, which is none.
+__device__ __forceinline__ void count_dropped(int* state, int n) {
+  const int had = state[KV_DROPPED];
+  state[KV_DROPPED] = had > 0x7fffffff - n ? 0x7fffffff : had + n;
+}
+
 constexpr int kAppendThreads = 256;
 
 // A workgroup per block and KV head: its first half codes K, the other V, 8 elements of a row to a thread at a time, in
@@ -88,7 +94,7 @@ __global__ __launch_bounds__(kAppendThreads) void k_kv8_append(Kv8Dev c, KvRows 
   const int len = kv_len(c, s);
   int* state = c.state + (size_t)s * KV_STATE;
   if (len + n > c.max_len) {
-    if (arrive && blockIdx.x == 0 && threadIdx.x == 0) state[KV_DROPPED] += n;
+    if (arrive && blockIdx.x == 0 && threadIdx.x == 0) count_dropped(state, n);
     return;
   }
   const int r = len % kKvBlock, whole = (r + n) / kKvBlock;
@@ -189,7 +195,7 @@ __global__ void k_kv8_advance(Kv8Dev c, int seq0, int n_seqs, int n) {
   if (i >= n_seqs) return;
   const int len = kv_len(c, seq0 + i);
   int* st = c.state + (size_t)(seq0 + i) * KV_STATE;
-  if (len + n > c.max_len) st[KV_DROPPED] += n;
+  if (len + n > c.max_len) count_dropped(st, n);
   else st[KV_LEN] = len + n;
 }
 

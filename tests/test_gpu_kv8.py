@@ -788,3 +788,22 @@ def test_an_error_the_caller_has_dealt_with_fails_no_call(hip):
     dev.workspace(4, 1, 1, True)
     assert hip.rt.hipSetDevice(4096) != 0
     check_attend(dev, ref, q, 0.125, decay=1.0)
+
+
+@pytest.mark.parametrize("n", [40, 3000])
+def test_dropped_rows_are_never_counted_back_to_none(hip, n):
+    """Two appends without room, behind 2^31 - 100 dropped rows: the count stays at the largest number."""
+    max_len = 32 * (n // 32 + 1)
+    dev, _ = both(hip, 1, 8, 64, max_len)
+    x = np.ones((1, n, 8, 64))
+    dev.append(x, x)
+    state = dev.array("state")
+    state[0, 1] = 2 ** 31 - 100
+    dev.set("state", state)
+    for _ in range(2):
+        dev.append(np.ones((1, max_len, 8, 64)), np.ones((1, max_len, 8, 64)))
+    dev.append(x, x)
+    assert dev.array("state")[0].tolist() == [n, 2 ** 31 - 1, 0, 0]
+    with pytest.raises(moert.MoertError) as e:
+        dev.c.lengths()
+    assert e.value.code == moert.E_FULL and e.value.lengths.tolist() == [n]
