@@ -807,3 +807,43 @@ def test_dropped_rows_are_never_counted_back_to_none(hip, n):
     with pytest.raises(moert.MoertError) as e:
         dev.c.lengths()
     assert e.value.code == moert.E_FULL and e.value.lengths.tolist() == [n]
+
+
+@pytest.mark.parametrize("d,dtype", [(64, moert.F32), (128, moert.F16)])
+def test_broken_tables_and_lengths_change_nothing_outside_the_buffers(hip, d, dtype):
+    """The cache's arrays in one allocation with known bytes before, between and behind them; entries outside the slots
+    and lengths outside the cache, met by every call that reads or writes through them."""
+    S, H, max_len, guard = 2, 2, 256, 8192
+    dev = ku.Device(hip, S, H, d, max_len)
+    place, size = {}, guard
+    for name, (shape, kind) in dev.shapes.items():
+        place[name] = size
+        size += -(-int(np.prod(shape)) * np.dtype(kind).itemsize // 16) * 16 + guard
+    memory = np.full(size, 0xA5, np.uint8)
+    base = hip.upload(memory)
+    dev.at = {name: base + x for name, x in place.items()}
+    dev.c = moert.Kv8(S, H, d, max_len, dev.at)
+    dev.c.clear()
+    outside = np.ones(size, bool)
+    for name, (shape, kind) in dev.shapes.items():
+        outside[place[name]:place[name] + int(np.prod(shape)) * np.dtype(kind).itemsize] = False
+    rng = np.random.default_rng(27)
+    slots = max_len // B
+    broken = np.array([-1, slots, 2 ** 31 - 1, -2 ** 31, slots + 1, -2, 3, 2 ** 20], np.int64)
+    for length in (0, 40, 200, -5, max_len + 1, 2 ** 30, 2 ** 31 - 1, -2 ** 31):
+        print(f"[case] length {length}", flush=True)
+        for rows in (1, 33, 128):
+            state = np.zeros((S, 4), np.int32)
+            state[:, 0] = length
+            dev.set("state", state)
+            dev.set("table", np.stack([np.stack([rng.permutation(broken) for _ in range(H)]) for _ in range(S)]))
+            dev.append(normal(rng, S, rows, H, d), normal(rng, S, rows, H, d), dtype)
+            for n in (1, 20):
+                dev.attend(normal(rng, S, n, 3 * H, d), 0.125, dtype, decay=0.5)
+            dev.read(-100, 256, dtype)
+            dev.c.evict(1, first=1)
+            dev.attend(normal(rng, S, 1, 3 * H, d), 0.125, dtype)
+            hip.sync()
+            now = hip.get(base, (size,), np.uint8)
+            changed = np.flatnonzero(outside & (now != 0xA5))
+            assert changed.size == 0, (length, rows, changed[:4])
