@@ -440,7 +440,9 @@ int moert_kv8_append(const moert_kv8* c, int seq0, int n_seqs, const moert_rows*
                      void* stream);
 
 /* Bytes of workspace for attentions of at most n positions of `heads` query heads over at most n_seqs sequences (track:
- * ones that add to the mass among them). Nothing in it has to be kept or cleared between calls. */
+ * ones that add to the mass among them). Nothing in it has to be kept or cleared between calls. Tracking takes 4 bytes
+ * per position, query head and block of max_len (393 MB for 1000 positions of 24 heads at max_len 131072): a long prompt
+ * that tracks is appended and attended to in parts, whose masses, with a decay of 1, add up to the same. */
 int moert_kv8_workspace(const moert_kv8* c, int n_seqs, int heads, int n, int track, size_t* bytes);
 
 /* Attention of n positions over the cache, whose last n rows are theirs (appended before): position i of a sequence of
@@ -452,7 +454,7 @@ int moert_kv8_workspace(const moert_kv8* c, int n_seqs, int heads, int n, int tr
  * scales of V. Outputs do not depend on whether the call tracks.
  * mass_decay in [0, 1] tracks: mass = mass_decay * mass + w for every block in use, w the sum of the block's p over
  * the n positions and the group's query heads (NaN for what a position sees if it sees a value that is not finite).
- * A negative mass_decay does not track. ws: moert_kv8_workspace bytes, aligned to 16. */
+ * A negative mass_decay does not track. out may be q itself, with the same strides; otherwise they do not overlap. ws: moert_kv8_workspace bytes, aligned to 16. */
 int moert_kv8_attend(const moert_kv8* c, int seq0, int n_seqs, int heads, int n, float scale, const moert_rows* q,
                      const moert_rows* out, float mass_decay, void* ws_dev, size_t ws_bytes, void* stream);
 

@@ -847,3 +847,24 @@ def test_broken_tables_and_lengths_change_nothing_outside_the_buffers(hip, d, dt
             now = hip.get(base, (size,), np.uint8)
             changed = np.flatnonzero(outside & (now != 0xA5))
             assert changed.size == 0, (length, rows, changed[:4])
+
+
+@pytest.mark.parametrize("max_len", [256, 16384])
+@pytest.mark.parametrize("dtype", [moert.F32, moert.F16])
+def test_outputs_in_place_of_the_queries(hip, dtype, max_len):
+    """out = q, of the same strides: every row of q is read before its output is written, with and without splits."""
+    rng = np.random.default_rng(28)
+    t = np.float32 if dtype == moert.F32 else np.float16
+    dev = ku.Device(hip, 2, 2, 64, max_len)
+    r = normal(rng, 2, 2, max_len // 2 + 7, 2, 64)
+    dev.append(r[0], r[1])
+    for n in (1, 3, 70):
+        q = normal(rng, 2, n, 6, 64).astype(t)
+        for decay in (None, 1.0):
+            want = dev.attend(q, 0.125, dtype, decay)
+            at = hip.upload(q)
+            ws, size = dev.workspace(6, n, 2, decay is not None)
+            dev.c.attend(at, at, 6, n, 0.125, ws, size, dtype=dtype, mass_decay=decay)
+            hip.sync()
+            same = np.array_equal(hip.get(at, q.shape, t), want)
+            assert same, (n, decay)
