@@ -18,7 +18,10 @@
 //                holds positions 4 G .. 4 G + 3 of both halves of the block for its column, which is what it has to
 //                hold of P here when the positions of V are taken in that order: v_place lays V out so, and p never
 //                leaves its lane.
-// f32 queries enter as two fp16 (their row scaled by a power of two to below 2^10), f32 outputs take p as two fp16.
+// f32 queries enter as two fp16 (their row scaled by a power of two to below 2^10). p is taken as two fp16 for f32 outputs,
+// and for fp16 ones of a single tile, where that is free (step after 131000 positions 32.9 us, of eight sequences 125 ->
+// 125.2) and brings them from 2.2-2.4e-4 off to the 2.0-2.2e-4 of their own rounding. Wider ones round p once: bound by the
+// vector unit, 1000 positions after 16001 would take 245 us for 194, to be 2.1e-4 off for 2.4e-4.
 //
 // The waves of a workgroup take the blocks of their tile in turn and join in LDS; where the tiles are too few for the
 // device, several workgroups share a tile (splits) and a second launch joins them. For eviction each block's sum goes
@@ -174,6 +177,7 @@ __device__ __forceinline__ bool sees_none(int len, int n, int g, int col) { retu
 template <int D, bool F16, int NT, bool TRACK, bool STREAM>
 __global__ __launch_bounds__(kWaves * 64, NT == 1 && D == 64 ? 4 : 2) void k_kv8_attend(AttnArgs a) {
   constexpr int KS = D / 32, U = D / 16, CH = D / 64, W = 16 * NT;
+  constexpr bool LO = !F16 || NT == 1;  // p as two fp16
   // Which 16 elements a product of V has as its rows is free. A load of 16 bytes a lane takes 1 KB of V in a row, whole
   // cache lines: RP of the runs' rows, U / 2 pieces of each. (Two loads that each took half of every line asked the L2
   // for 1.8 times the bytes: 115 us where this takes 108, 565 MB.) So row i of product u is element elem(u, i).
@@ -400,7 +404,7 @@ __global__ __launch_bounds__(kWaves * 64, NT == 1 && D == 64 ? 4 : 2) void k_kv8
         f[t] = 1.0f;
       }
     }
-    h8 ph[NT], pl[F16 ? 1 : NT];
+    h8 ph[NT], pl[LO ? NT : 1];
     float part[NT];
 #pragma unroll
     for (int t = 0; t < NT; t++) {
@@ -417,7 +421,7 @@ __global__ __launch_bounds__(kWaves * 64, NT == 1 && D == 64 ? 4 : 2) void k_kv8
 #pragma unroll
       for (int x = 0; x < 8; x++) {
         ph[t][x] = (_Float16)p[x];
-        if constexpr (!F16) pl[t][x] = (_Float16)(p[x] - (float)ph[t][x]);
+        if constexpr (LO) pl[t][x] = (_Float16)(p[x] - (float)ph[t][x]);
       }
     }
     if constexpr (NT > 1) __builtin_amdgcn_s_setprio(1);
@@ -427,7 +431,7 @@ __global__ __launch_bounds__(kWaves * 64, NT == 1 && D == 64 ? 4 : 2) void k_kv8
 #pragma unroll
       for (int t = 0; t < NT; t++) {
         O[t][u] = mfma(va, ph[t], O[t][u]);
-        if constexpr (!F16) O[t][u] = mfma(va, pl[t], O[t][u]);
+        if constexpr (LO) O[t][u] = mfma(va, pl[t], O[t][u]);
       }
     }
     if constexpr (NT > 1) __builtin_amdgcn_s_setprio(0);

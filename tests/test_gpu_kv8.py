@@ -868,3 +868,25 @@ def test_outputs_in_place_of_the_queries(hip, dtype, max_len):
             hip.sync()
             same = np.array_equal(hip.get(at, q.shape, t), want)
             assert same, (n, decay)
+
+
+@pytest.mark.parametrize("d,heads,n", [(64, 16, 1), (64, 3, 5), (128, 8, 2), (128, 5, 1)])
+@pytest.mark.parametrize("max_len", [1024, 16384])
+def test_fp16_outputs_of_few_rows_are_off_by_their_own_rounding(hip, d, heads, n, max_len):
+    """At most 16 query rows of a KV head: the weights keep 22 bits, as with f32, and the output is rounded once. All
+    rows that count have one weight, so that roundings of weights would add up, whatever part of a step they take."""
+    rng = np.random.default_rng(29)
+    rows = 999
+    dev, ref = both(hip, 1, 1, d, max_len)
+    k, v = np.zeros((1, rows, 1, d)), np.broadcast_to(rng.uniform(1.0, 2.0, d), (1, rows, 1, d))
+    k[:, rows // 2:, :, 0] = 1.0  # each wave's first block has score 0
+    dev.append(k, v)
+    ref.append(k, v)
+    q = np.zeros((1, n, heads, d), np.float16)
+    q[..., 0] = (0.7 + np.arange(n * heads) / 14.5).reshape(n, heads)
+    want = ref.attend(q, 1.0)
+    # half a step of the output: the steps of [1, 2) are 2^-10, those of [1/2, 1) half of that
+    off = weights_bound(ref, q, 1.0, False) + np.where(np.abs(want) < 1.0, 2.0 ** -12, 2.0 ** -11)
+    for decay in (None, 1.0):
+        worst = np.abs(dev.attend(q, 1.0, moert.F16, decay).astype(np.float64) - want) / off
+        assert (worst <= 1).all(), f"{worst.max()} of its bound"
