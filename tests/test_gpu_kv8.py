@@ -890,3 +890,20 @@ def test_fp16_outputs_of_few_rows_are_off_by_their_own_rounding(hip, d, heads, n
     for decay in (None, 1.0):
         worst = np.abs(dev.attend(q, 1.0, moert.F16, decay).astype(np.float64) - want) / off
         assert (worst <= 1).all(), f"{worst.max()} of its bound"
+
+
+def test_k_and_v_of_different_types(hip):
+    """Each of the rows of a call has its own type and strides."""
+    rng = np.random.default_rng(30)
+    dev, ref = both(hip, 1, 2, 64, 128)
+    k, v = normal(rng, 1, 77, 2, 64), normal(rng, 1, 77, 2, 64).astype(np.float16)
+    lib, c = moert.lib(), dev.c
+    rows = lambda at, dtype: c._rows(at, dtype, None, 77, 2)
+    moert.check(lib.moert_kv8_append(c._p, 0, 1, rows(hip.upload(k), moert.F32), rows(hip.upload(v), moert.F16), 77, None))
+    ref.append(k, v)
+    ku.assert_holds(dev, ref)
+    out = [hip.upload(np.full((77, 2, 64), 7.0, t)) for t in (np.float16, np.float32)]
+    moert.check(lib.moert_kv8_read(c._p, 0, 1, 0, 77, rows(out[0], moert.F16), rows(out[1], moert.F32), None))
+    hip.sync()
+    for at, t, want in zip(out, (np.float16, np.float32), ref.read(0, 0, 77)):
+        assert np.array_equal(hip.get(at, want.shape, t), want.astype(np.float32).astype(t))
