@@ -13,7 +13,9 @@
 //                A block whose scale of V lies more than 2^8 below that of one that has moved M (zeros have scale 1)
 //                would have its p below that, however much softmax weight it has: its p, and O for the time of its
 //                products, are taken 2^k2 times as large, which brings its largest p to 2^6 or above. So the rounding
-//                of a weight is off by its last bit or by 2^-24 of the column's largest weight.
+//                of a weight is off by its last bit or by 2^-24 of the column's largest weight. Beyond 2^16, where u
+//                in f32 rounds the scales away, M follows u alone and every block is taken so: equal scores stay equal
+//                weights, and no p leaves fp16 (M and the scales in one sum made it 2^17 and more from u of 2^24 on).
 //   O += V^T P^T MFMA 16x16x32 over the 32 positions: rows = 16 elements, columns = columns. A lane of the S product
 //                holds positions 4 G .. 4 G + 3 of both halves of the block for its column, which is what it has to
 //                hold of P here when the positions of V are taken in that order: v_place lays V out so, and p never
@@ -55,6 +57,7 @@ constexpr int kWaves = 4;       // waves of a workgroup, each its share of the b
 constexpr int kMaxSplits = 64;  // one lane each in the combine
 constexpr float kShift = 7.0f, kSlack = 8.0f;
 constexpr float kApart = 8.0f;    // log2 of how far a block's scale of V may lie below one that M follows
+constexpr float kFarL = 9.0f - kShift;  // L beside scores beyond 2^16: no scale of V is above 2^9.02 (65504 / 127)
 constexpr float kMostUp = 60.0f;  // O is a sum of at most 2^20 products below 2^22, so it stays in range 2^60 times
 constexpr float kNone = -3.4e38f;  // maximum of what has no score yet; finite, so that differences with it are
 
@@ -161,7 +164,7 @@ struct AttnArgs {
   float kf;       // |scale| log2 e
   uint32_t sign;  // of the scale
   float* part;    // [sequence, KV head, column][split][D]
-  float2* ml;     // [sequence, KV head, column][split]: M - 7, sum
+  float2* ml;     // [sequence, KV head, column][split]: M + L, sum
   float* tot;     // [sequence, KV head, column]: log2 of the whole sum, +inf where nothing is seen
   float* lse;     // [sequence, KV head][block][column]: log2 of the block's sum
 };
@@ -308,17 +311,20 @@ __global__ __launch_bounds__(kWaves * 64, NT == 1 && D == 64 ? 4 : 2) void k_kv8
   }
   const int sees0 = len - a.n + 1 + min(tile * W, cols - 1) / a.g;  // the least of the tile
 
-  float M[NT], l[NT];  // M: the maximum less 7, so that the weights below are 2^7 times those to it; l: a lane's own sum
+  // M + L: the maximum less 7, so that the weights below are 2^7 times those to it; M its part of a score, L of a scale
+  // of V, which large scores would round away. l: a lane's own sum
+  float M[NT], L[NT], l[NT];
   f4 O[NT][U];
 #pragma unroll
   for (int t = 0; t < NT; t++) {
     M[t] = kNone;
-    l[t] = 0.0f;
+    L[t] = l[t] = 0.0f;
 #pragma unroll
     for (int u = 0; u < U; u++) O[t][u] = f4{0.0f, 0.0f, 0.0f, 0.0f};
   }
 
-  bool far = false;    // some column's M is beyond 2^16
+  bool far = false;    // some column's M is, or has been, beyond 2^16
+  float limit = kShift + kSlack;  // how far beyond M + L a contribution moves it
   float vref = kNone;  // the largest log2 of a scale of V that came with a move of M
   float none = -__builtin_inff();  // opaque, so that eight maxima with it are four instructions
   asm("" : "+s"(none));
@@ -356,7 +362,7 @@ __global__ __launch_bounds__(kWaves * 64, NT == 1 && D == 64 ? 4 : 2) void k_kv8
     }
     if constexpr (NT > 1) __builtin_amdgcn_s_setprio(0);
     then();
-    float f[NT], mx[NT];
+    float f[NT], mx[NT], d[NT];
     bool move = false;
 #pragma unroll
     for (int t = 0; t < NT; t++) {
@@ -364,16 +370,27 @@ __global__ __launch_bounds__(kWaves * 64, NT == 1 && D == 64 ? 4 : 2) void k_kv8
       mx[t] = none;
 #pragma unroll
       for (int x = 0; x < 8; x++) mx[t] = __builtin_fmaxf(mx[t], S[t][x >> 2][x & 3]);
-      move |= __builtin_fmaf(mx[t], f[t], lvs) > M[t] + (kShift + kSlack);
+      d[t] = lvs - L[t];
+      move |= __builtin_fmaf(mx[t], f[t], d[t] - M[t]) > limit;
     }
     if (__any(move)) {
       vref = __builtin_fmaxf(vref, lvs);
+      float y[NT];
 #pragma unroll
       for (int t = 0; t < NT; t++) {
-        const float y = max_stage<32>(max_stage<16>(mx[t])) * f[t] + lvs - kShift;
-        const float mn = y > M[t] ? y : M[t], al = __builtin_amdgcn_exp2f(M[t] - mn);
+        y[t] = max_stage<32>(max_stage<16>(mx[t])) * f[t];
+        far |= __any(__builtin_fabsf(y[t]) > 65536.0f && y[t] > kNone);
+      }
+      if (far) limit = none;  // -inf: from here on every block comes here, and M follows the scores alone
+#pragma unroll
+      for (int t = 0; t < NT; t++) {
+        const float yl = far ? kFarL : lvs - kShift;
+        const bool up = (y[t] - M[t]) + (yl - L[t]) > 0.0f;
+        const float mn = up ? y[t] : M[t], ln = up ? yl : L[t];
+        const float al = __builtin_amdgcn_exp2f((M[t] - mn) + (L[t] - ln));
         M[t] = mn;
-        far |= __any(__builtin_fabsf(mn) > 65536.0f && mn != kNone);
+        L[t] = ln;
+        d[t] = lvs - ln;
         l[t] *= al;
 #pragma unroll
         for (int u = 0; u < U; u++)
@@ -381,37 +398,42 @@ __global__ __launch_bounds__(kWaves * 64, NT == 1 && D == 64 ? 4 : 2) void k_kv8
           for (int i = 0; i < 4; i++) O[t][u][i] *= al;
       }
     }
-    const bool apart = lvs < vref - kApart;  // the same for the wave
+    const bool apart = far || lvs < vref - kApart;  // the same for the wave
     float k2[NT];                            // p is 2^k2 times what M makes it, and O with it
 #pragma unroll
     for (int t = 0; t < NT; t++) k2[t] = 0.0f;
     if (apart) {
 #pragma unroll
       for (int t = 0; t < NT; t++) {
-        const float y = max_stage<32>(max_stage<16>(mx[t])) * f[t] + lvs - kShift;
-        k2[t] = __builtin_fminf(__builtin_fmaxf(__builtin_floorf(M[t] - y), 0.0f), kMostUp);  // of NaN 0
+        const float y = max_stage<32>(max_stage<16>(mx[t])) * f[t];
+        k2[t] = __builtin_floorf((M[t] - y) - (d[t] - kShift));
+        k2[t] = __builtin_fminf(__builtin_fmaxf(k2[t], 0.0f), kMostUp);  // of NaN 0
+        d[t] += k2[t];
 #pragma unroll
         for (int u = 0; u < U; u++)
 #pragma unroll
           for (int i = 0; i < 4; i++) O[t][u][i] = __builtin_amdgcn_ldexpf(O[t][u][i], (int)k2[t]);
       }
     }
-    if (far) {  // M is rounded by more than p allows: the same rounding for the scores
+    float c0[NT];
+#pragma unroll
+    for (int t = 0; t < NT; t++) c0[t] = d[t] - M[t];
+    if (far) {  // M is rounded by more than p allows: the same rounding for the scores, and their difference first
 #pragma unroll
       for (int t = 0; t < NT; t++) {
 #pragma unroll
-        for (int x = 0; x < 8; x++) S[t][x >> 2][x & 3] *= f[t];
+        for (int x = 0; x < 8; x++) S[t][x >> 2][x & 3] = S[t][x >> 2][x & 3] * f[t] - M[t];
         f[t] = 1.0f;
+        c0[t] = d[t];
       }
     }
     h8 ph[NT], pl[LO ? NT : 1];
     float part[NT];
 #pragma unroll
     for (int t = 0; t < NT; t++) {
-      const float c0 = lvs - M[t] + k2[t];
       float p[8];
 #pragma unroll
-      for (int x = 0; x < 8; x++) p[x] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[t][x >> 2][x & 3], f[t], c0));
+      for (int x = 0; x < 8; x++) p[x] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[t][x >> 2][x & 3], f[t], c0[t]));
       if constexpr (MASKED) {
 #pragma unroll
         for (int x = 0; x < 8; x++)
@@ -450,10 +472,10 @@ __global__ __launch_bounds__(kWaves * 64, NT == 1 && D == 64 ? 4 : 2) void k_kv8
     if constexpr (TRACK) {  // lanes of group 0 write tile 0's, those of group 2 tile 1's
       static_assert(NT <= 2, "");
       const float y = add16(add32(part[0], part[NT - 1]));
-      const float m = G >= 2 ? M[NT - 1] : M[0];
+      const float m = G >= 2 ? M[NT - 1] : M[0], ml = G >= 2 ? L[NT - 1] : L[0];
       const int col = tile * W + (G >> 1) * 16 + col16;
       if ((NT == 2 ? !(G & 1) : G == 0) && col < cols)
-        a.lse[((size_t)hs * c.slots + b) * cols + col] = __builtin_amdgcn_logf(y) + (m - lvs);
+        a.lse[((size_t)hs * c.slots + b) * cols + col] = __builtin_amdgcn_logf(y) + (ml - lvs) + m;
     }
   };
 
@@ -515,7 +537,7 @@ __global__ __launch_bounds__(kWaves * 64, NT == 1 && D == 64 ? 4 : 2) void k_kv8
   for (int t = 0; t < NT; t++) {
     const float lt = add16(add32(l[t], l[t]));
     if (t) __syncthreads();
-    if (G == 0) Ms[w][col16] = make_float2(M[t], lt);
+    if (G == 0) Ms[w][col16] = make_float2(M[t] + L[t], lt);
 #pragma unroll
     for (int i = 0; i < 4; i++)
 #pragma unroll
@@ -625,6 +647,9 @@ __global__ __launch_bounds__(256) void k_kv8_combine(AttnArgs a, int width) {
   combine_column<D, F16, TRACK, C>(a, width, blockIdx.x, Os);
 }
 
+// A block's weight for a column, at most 1 however far scores beyond 2^16 have rounded the two logarithms; NaN stays.
+__device__ __forceinline__ float weight_of(float x) { return __builtin_amdgcn_exp2f(x > 0.0f ? 0.0f : x); }
+
 // mass = decay * mass + the block's weights: P lanes to a block, each with every P-th column, joined pairwise.
 __device__ __forceinline__ void mass_block(const AttnArgs& a, int hs, int b, int x, int P, float decay,
                                            const float* tot) {
@@ -643,7 +668,7 @@ __device__ __forceinline__ void mass_block(const AttnArgs& a, int hs, int b, int
       y[j] = lse[at] - tot[at];
     }
 #pragma unroll
-    for (int j = 0; j < 4; j++) w += col + j * P < cols ? __builtin_amdgcn_exp2f(y[j]) : 0.0f;
+    for (int j = 0; j < 4; j++) w += col + j * P < cols ? weight_of(y[j]) : 0.0f;
   }
   for (int m = P / 2; m; m >>= 1) w += __shfl_xor(w, m);
   if (x) return;
@@ -686,7 +711,7 @@ __global__ __launch_bounds__(256) void k_kv8_finish(AttnArgs a, int width, int c
   __syncthreads();
   // a column's position sees some of the block, and the block is the last thread group's own (the index is clamped)
   const bool mine = x % per_head * (256 / P) + (int)threadIdx.x / P == b && b * kKvBlock < len;
-  float w = col < cols && b * kKvBlock < len - a.n + 1 + col / a.g ? __builtin_amdgcn_exp2f(lse - tot[col]) : 0.0f;
+  float w = col < cols && b * kKvBlock < len - a.n + 1 + col / a.g ? weight_of(lse - tot[col]) : 0.0f;
   for (int m = P / 2; m; m >>= 1) w += __shfl_xor(w, m);
   if (mine && col == 0) *mass = __builtin_fmaf(decay, old, w);
 }

@@ -907,3 +907,52 @@ def test_k_and_v_of_different_types(hip):
     hip.sync()
     for at, t, want in zip(out, (np.float16, np.float32), ref.read(0, 0, 77)):
         assert np.array_equal(hip.get(at, want.shape, t), want.astype(np.float32).astype(t))
+
+
+@pytest.mark.parametrize("max_len,n", [(768, 1), (768, 20), (16384, 1), (16384, 12)])
+@pytest.mark.parametrize("dtype", [moert.F32, moert.F16])
+def test_scores_of_any_size(hip, dtype, max_len, n):
+    """Scores of 10^4 to 10^30, far beyond the steps of exponents: all the weight on one row, or shared by every 37th in
+    equal parts, whatever the scales of V of their blocks."""
+    rng = np.random.default_rng(31)
+    d, rows = 64, 700
+    b = np.arange(rows)[None, :, None, None] // B
+    for kind, v_scale in (("ordinary", 1.0), ("small", 1e-3), ("rising", 2.0 ** (b % 7 * 3 - 10.0)), ("large", 1e4)):
+        v = normal(rng, 1, rows, 2, d) * v_scale
+        for every in (rows, 37):
+            k = np.zeros((1, rows, 2, d), np.float32)
+            k[..., 0], k[..., 1] = rng.integers(20, 100, (1, rows, 2)), 127.0  # a scale of 1 in every block
+            k[0, 20::every, :, 0] = 127.0
+            dev, ref = both(hip, 1, 2, d, max_len)
+            dev.append(k, v)
+            ref.append(k, v)
+            at = np.arange(20, rows, every)
+            for size in (1e4, 1e5, 1e6, 1e7, 3e7, 1e8, 3e8, 1e9, 4e9, 1e10, 1e12, 1e30):
+                for sign in (1.0, -1.0):
+                    q = np.zeros((1, n, 4, d), np.float32)
+                    q[..., 0] = 16.0
+                    if sign < 0:  # every score below 0, the same ones apart
+                        q[..., 1] = -32.0
+                    scale = size / (16.0 * 127.0)
+                    for decay in (None, 0.0):
+                        out = dev.attend(q.astype(np.float16) if dtype == moert.F16 else q, scale, dtype, decay)
+                        for h in range(2):
+                            x = ref.rows(0, h)[1]
+                            for i in range(n):
+                                w = at[at < rows - n + 1 + i]
+                                want = x[w].mean(0)
+                                # a weight: 22 bits or (F16, two tiles) 11, exp2 of an argument below 64 to 2^-21; sums and
+                                # products in f32, 32 roundings at most; an fp16 output rounded once more
+                                few = dtype == moert.F32 or 2 * n <= 16
+                                rel = 2.0 ** -20 if few else 2.0 ** -11
+                                if size * 1.4427 <= 2 ** 16:  # exponents of 2 round as the scores do, 4 times at most
+                                    rel += 4 * 2.0 ** -24 * size
+                                off = rel * np.abs(x[w]).mean(0) + 2.0 ** -24 * np.abs(x[w]).max()
+                                if dtype == moert.F16:
+                                    off = off + 2.0 ** -11 * np.abs(want) + 2.0 ** -25
+                                for a in (2 * h, 2 * h + 1):
+                                    worst = np.abs(out[0, i, a].astype(np.float64) - want) / off
+                                    assert (worst <= 1).all(), (kind, every, size, sign, i, a, float(worst.max()))
+                        if decay is not None:
+                            mass = np.stack([dev.mass(0, h, -(-rows // B)) for h in range(2)])
+                            assert np.isfinite(mass).all() and (mass >= 0).all() and (mass <= 2 * n).all(), (kind, size)
