@@ -449,10 +449,10 @@ int moert_kv8_workspace(const moert_kv8* c, int n_seqs, int heads, int n, int tr
  * len rows sees the first len - n + 1 + i of them, and query head h reads KV head h / (heads / kv_heads).
  * out = sum_t p_t v_t, p = softmax(scale * q . k); a position that sees no row gets 0, a query row that is not finite
  * NaN. q and out are of one type: scores, weights and sums are f32 for both, a weight as good as its score, an f32 (of
- * scores of 10^5, to 1 in 100); outputs are finite as long as scores are. The weights enter the second product as the
- * sum of two fp16 (22 bits), with MOERT_F16 and more than 16 query rows of a KV head (n * heads / kv_heads) rounded to
- * fp16, each rounding off by its last bit or 2^-24 of the row's largest weight, whatever the scales of V. Outputs do
- * not depend on whether the call tracks.
+ * scores of 10^5, to 1 in 100); outputs are finite as long as head_dim * |scale| * max|q| * max|k| is below 10^38. The
+ * weights enter the second product as the sum of two fp16 (22 bits), with MOERT_F16 and more than 16 query rows of a KV
+ * head (n * heads / kv_heads) rounded to fp16, each rounding off by its last bit or 2^-24 of the row's largest weight,
+ * whatever the scales of V. Outputs do not depend on whether the call tracks.
  * mass_decay in [0, 1] tracks: mass = mass_decay * mass + w for every block in use, w the sum of the block's p over
  * the n positions and the group's query heads (NaN for what a position sees if it sees a value that is not finite).
  * A negative mass_decay does not track. out may be q itself, with the same strides; otherwise they do not overlap.

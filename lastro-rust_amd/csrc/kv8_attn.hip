@@ -38,6 +38,8 @@
 //                  in 25%, 2.4 waves are on a SIMD. The whole call is 189 us, with one tile to a wave 298; with 2 or 8
 //                  waves to a workgroup 261 or 211 (131000 positions of one sequence, one each: 37 or 39 for 33); without
 //                  the matrix instructions first (s_setprio) 194.
+#include <math.h>
+
 #include <type_traits>
 
 #include "kv8.h"
@@ -161,7 +163,8 @@ struct AttnArgs {
   KvRows q, out;
   int seq0, n_seqs, g, n, splits, tiles;
   int vec;        // bit 0: q can be loaded 16 bytes at a time, bit 1: out can be stored so
-  float kf;       // |scale| log2 e
+  float kf;       // |scale| log2 e, less 2^ke
+  int ke;
   uint32_t sign;  // of the scale
   float* part;    // [sequence, KV head, column][split][D]
   float2* ml;     // [sequence, KV head, column][split]: M + L, sum
@@ -232,6 +235,7 @@ __global__ __launch_bounds__(kWaves * 64, NT == 1 && D == 64 ? 4 : 2) void k_kv8
   auto scales = [&]() {
     // a V that is not finite makes the scores NaN, not the scale: columns that see none of the block are masked there
     if (vs_l != vs_l) ks_l = vs_l, vs_l = 1.0f;
+    ks_l *= a.kf;
     lvs_l = __builtin_amdgcn_logf(vs_l);
     ivs_l = 1.0f / vs_l;
   };
@@ -265,7 +269,7 @@ __global__ __launch_bounds__(kWaves * 64, NT == 1 && D == 64 ? 4 : 2) void k_kv8
 
   // queries and the rows that each column sees
   h8 qh[NT][KS], ql[NT][F16 ? 1 : KS];
-  float kf[NT];
+  int qe[NT];  // log2 of what is still to be multiplied by: ke, and what queries of f32 were divided by
   int sees[NT];
 #pragma unroll
   for (int t = 0; t < NT; t++) {
@@ -282,7 +286,7 @@ __global__ __launch_bounds__(kWaves * 64, NT == 1 && D == 64 ? 4 : 2) void k_kv8
         if constexpr (F16) x[k][j] += x[k][j] - x[k][j];  // inf to NaN, as the difference of f32's halves makes it
       }
     }
-    kf[t] = a.kf;
+    qe[t] = a.ke;
     if constexpr (!F16) {
       float m = 0.0f;
 #pragma unroll
@@ -298,7 +302,7 @@ __global__ __launch_bounds__(kWaves * 64, NT == 1 && D == 64 ? 4 : 2) void k_kv8
       for (int k = 0; k < KS; k++)
 #pragma unroll
         for (int j = 0; j < 8; j++) x[k][j] = __builtin_amdgcn_ldexpf(__builtin_amdgcn_ldexpf(x[k][j], e1), e2);
-      kf[t] = __builtin_amdgcn_ldexpf(a.kf, e - 10);
+      qe[t] += e - 10;
     }
 #pragma unroll
     for (int k = 0; k < KS; k++)
@@ -328,10 +332,12 @@ __global__ __launch_bounds__(kWaves * 64, NT == 1 && D == 64 ? 4 : 2) void k_kv8
   float vref = kNone;  // the largest log2 of a scale of V that came with a move of M
   float none = -__builtin_inff();  // opaque, so that eight maxima with it are four instructions
   asm("" : "+s"(none));
-  // One block: kop(half, k), vop(u) give the operands, then() runs behind the scores. masked: some column does not see all of it (S is -inf there,
-  // which moves no maximum; NaN with a scale of 0, which moves none either), or `bad` names poisoned rows, of the tail.
+  // One block: kop(half, k), vop(u) give the operands, then() runs behind the scores; ks is the scale of K with that of
+  // the scores in it, lvs and ivs log2 and inverse of the scale of V. masked: 0, or 1 where some column does not see all
+  // of it (S is -inf there, which moves no maximum; NaN with a scale of 0, which moves none either), or 2 for the tail,
+  // whose poisoned rows `bad` names.
   auto block = [&](auto masked, auto kop, auto vop, auto then, float ks, float lvs, float ivs, int b, uint32_t bad) {
-    constexpr bool MASKED = decltype(masked)::value;
+    constexpr bool MASKED = decltype(masked)::value != 0, TAIL = decltype(masked)::value == 2;
     f4 S[NT][2];
     if constexpr (NT > 1) __builtin_amdgcn_s_setprio(1);
 #pragma unroll
@@ -366,7 +372,13 @@ __global__ __launch_bounds__(kWaves * 64, NT == 1 && D == 64 ? 4 : 2) void k_kv8
     bool move = false;
 #pragma unroll
     for (int t = 0; t < NT; t++) {
-      f[t] = kf[t] * ks;
+      // the three scales of a score meet here, with their exponents in one: no two of them leave f32 where all three
+      // do not. The tail has no scale of K that says how small it is: its scores come in 2^24 times.
+      if constexpr (TAIL) {
+#pragma unroll
+        for (int x = 0; x < 8; x++) S[t][x >> 2][x & 3] *= 0x1p24f;
+      }
+      f[t] = __builtin_amdgcn_ldexpf(ks, TAIL ? qe[t] - 24 : qe[t]);
       mx[t] = none;
 #pragma unroll
       for (int x = 0; x < 8; x++) mx[t] = __builtin_fmaxf(mx[t], S[t][x >> 2][x & 3]);
@@ -504,14 +516,14 @@ __global__ __launch_bounds__(kWaves * 64, NT == 1 && D == 64 ? 4 : 2) void k_kv8
     for (int x = 0; x < whole; x += PF) {
 #pragma unroll
       for (int p = 0; p < PF; p++) {
-        if (x + p < whole) run(std::false_type(), p, x + p, [&]() { if constexpr (EARLY) fetch_k(p, x + p + PF); });
+        if (x + p < whole) run(std::integral_constant<int, 0>(), p, x + p, [&]() { if constexpr (EARLY) fetch_k(p, x + p + PF); });
         if constexpr (EARLY) fetch_v(p, x + p + PF);
         else fetch(p, x + p + PF);
       }
     }
     for (int x = whole; x < count; x++) {
       if (x) fetch(0, x);
-      run(std::true_type(), 0, x, []() {});
+      run(std::integral_constant<int, 1>(), 0, x, []() {});
     }
   }
   if (seen > full && full % step == b0) {  // the tail, in fp16
@@ -529,7 +541,7 @@ __global__ __launch_bounds__(kWaves * 64, NT == 1 && D == 64 ? 4 : 2) void k_kv8
         v[j] = use >> (G * 4 + (j & 3) + 16 * (j >> 2)) & 1 ? v[j] : (_Float16)0.0f;
       return v;
     };
-    block(std::true_type(), kop, vop, []() {}, 1.0f, 0.0f, 1.0f, full, bad);
+    block(std::integral_constant<int, 2>(), kop, vop, []() {}, a.kf, 0.0f, 1.0f, full, bad);
   }
 
   // the waves' shares, tile by tile
@@ -788,10 +800,12 @@ hipError_t attend(hipStream_t s, AttnArgs a, float decay) {
 hipError_t launch_kv8_attend(hipStream_t s, const Kv8Dev& c, int seq0, int n_seqs, int heads, int n, float scale,
                              KvRows q, KvRows out, float decay, void* ws) {
   const bool track = decay >= 0.0f;
+  int ke;
+  const float kf = frexpf(__builtin_fabsf(scale), &ke) * kLog2e;
   const KvAttnPlan p = kv8_attn_plan(c, n_seqs, heads, n, track);
   char* w = (char*)ws;
   AttnArgs a{c, q, out, seq0, n_seqs, heads / c.kvh, n, p.splits, 1, wide_rows(q) | wide_rows(out) << 1,
-             __builtin_fabsf(scale) * kLog2e, scale < 0.0f ? 0x80000000u : 0u, (float*)(w + p.parts), (float2*)(w + p.ml), (float*)(w + p.tot),
+             kf, ke, scale < 0.0f ? 0x80000000u : 0u, (float*)(w + p.parts), (float2*)(w + p.ml), (float*)(w + p.tot),
              track ? (float*)(w + p.lse) : nullptr};
 #define ATT(DD, FF) \
   if (c.d == DD && q.f16 == FF) return track ? attend<DD, FF, true>(s, a, decay) : attend<DD, FF, false>(s, a, decay);

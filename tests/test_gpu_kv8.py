@@ -956,3 +956,24 @@ def test_scores_of_any_size(hip, dtype, max_len, n):
                         if decay is not None:
                             mass = np.stack([dev.mass(0, h, -(-rows // B)) for h in range(2)])
                             assert np.isfinite(mass).all() and (mass >= 0).all() and (mass <= 2 * n).all(), (kind, size)
+
+
+def test_factors_of_a_score_that_leave_f32_together(hip):
+    """Queries of 3e38 beside keys of 1e-6, scales from 1e-30 to 1e36: the scores are numbers, whatever two of their
+    three factors make. All the weight is on the row of the largest one."""
+    rng = np.random.default_rng(32)
+    d, rows = 64, 300
+    dev, ref = both(hip, 1, 1, d, 512)
+    k, v = np.zeros((1, rows, 1, d), np.float32), normal(rng, 1, rows, 1, d)
+    k[..., 0] = rng.integers(1, 100, (1, rows, 1)) * 2.0 ** -20
+    k[0, 130, 0, 0] = 127 * 2.0 ** -20
+    dev.append(k, v)
+    ref.append(k, v)
+    want = ref.rows(0, 0)[1][130]
+    for n in (1, 20):
+        for size, scale in ((3e38, 1e3), (3e38, 1.0), (3e38, 1e-30), (1e20, 1e15), (1e3, 1e36), (1e-3, 1e30)):
+            q = np.zeros((1, n, 2, d), np.float32)
+            q[..., 0] = size
+            for out in (dev.attend(q, scale), dev.attend(q, scale, decay=0.5)):
+                # two halves of a weight, scales and sums: 16 roundings at most
+                assert (np.abs(out - want) <= 2.0 ** -20 * np.abs(want).max()).all(), (n, size, scale)
