@@ -977,3 +977,24 @@ def test_factors_of_a_score_that_leave_f32_together(hip):
             for out in (dev.attend(q, scale), dev.attend(q, scale, decay=0.5)):
                 # two halves of a weight, scales and sums: 16 roundings at most
                 assert (np.abs(out - want) <= 2.0 ** -20 * np.abs(want).max()).all(), (n, size, scale)
+
+
+@pytest.mark.parametrize("n", [1, 20])
+@pytest.mark.parametrize("dtype", [moert.F32, moert.F16])
+def test_subnormal_fp16_counts(hip, dtype, n):
+    """Queries, rows of K and rows of V that fp16 holds as subnormals, coded and in the tail, with scales that make
+    ordinary scores of them."""
+    rng = np.random.default_rng(33)
+    for rows in (20, 75):
+        for size_q, size_k, size_v in ((2.0 ** -20, 1.0, 1.0), (1.0, 2.0 ** -20, 1.0), (1.0, 1.0, 2.0 ** -20),
+                                       (2.0 ** -20, 2.0 ** -20, 2.0 ** -20)):
+            dev, ref = both(hip, 1, 2, 64, 128)
+            k, v = normal(rng, 1, rows, 2, 64, scale=size_k), normal(rng, 1, rows, 2, 64, scale=size_v)
+            dev.append(k, v)
+            ref.append(k, v)
+            q = normal(rng, 1, n, 6, 64, scale=size_q).astype(np.float16)
+            scale = float(np.float32(0.125 / (size_q * size_k)))
+            want = ref.attend(q, scale)
+            off = weights_bound(ref, q, scale, dtype == moert.F16)
+            got = dev.attend(q, scale, dtype).astype(np.float64)
+            assert (np.abs(got - want) <= off).all(), (rows, size_q, size_k, size_v, (np.abs(got - want) / off).max())

@@ -16,7 +16,7 @@ STAND_IN = r"""
 #include <string.h>
 typedef struct { uint32_t x, y, z; } dim3;
 static struct { const void* f; char name[256]; } known[4096];
-static int n_known, last, launches, fail_at = -1;
+static int n_known, last, launches, fail_at = -1, device, at_device;
 static dim3 g, b;
 static size_t shm;
 static void* stream;
@@ -46,10 +46,11 @@ int hipLaunchKernel(const void* f, dim3 grid, dim3 block, void** a, size_t s, vo
 }
 int hipGetLastError(void) { const int e = last; last = 0; return e; }
 const char* hipGetErrorString(int e) { return "told to fail"; }
-int hipGetDevice(int* d) { *d = 0; return 0; }
-int hipSetDevice(int d) { return 0; }
+void stand_in_device(int d) { at_device = d; }
+int hipGetDevice(int* d) { *d = device; return 0; }
+int hipSetDevice(int d) { device = d; fprintf(out, "device %d 0 0 0\n", d); return 0; }
 /* type (2: device memory), device, then pointers */
-int hipPointerGetAttributes(int* a, const void* p) { memset(a, 0, 16); a[0] = 2; return 0; }
+int hipPointerGetAttributes(int* a, const void* p) { memset(a, 0, 16); a[0] = 2; a[1] = at_device; return 0; }
 """
 
 CHILD = r"""
@@ -61,6 +62,7 @@ import moert
 path, cases, results = sys.argv[2].encode(), json.loads(sys.argv[4]), []
 for c in cases:
     shim.stand_in(path, c.get("fail", -1), c.get("stale", 0))
+    shim.stand_in_device(c.get("device", 0))
     at = {n[:-4]: 0x10000 for n, _ in moert.moert_kv8._fields_[4:]}
     kv = moert.Kv8(*c["cache"], at)
     call = dict(c["kw"])
@@ -152,3 +154,13 @@ def test_an_error_of_an_earlier_call_is_not_the_launchs(launches):
     that did not fit, say) makes no call fail, and leaves none half done."""
     for (c, want), got in zip(FORMS, launches([dict(c, stale=2) for c, _ in FORMS])):
         assert got[0] == 0 and kinds(got) == want, (c, got)
+
+
+def test_calls_run_on_the_buffers_device_and_leave_the_current_one(launches):
+    """Also where a launch fails."""
+    for fail in (-1, 0):
+        for (c, want), got in zip(FORMS, launches([dict(c, device=3, fail=fail) for c, _ in FORMS])):
+            lines = [(line[0], line[1]) for line in got[1]]
+            assert lines[0] == ("device", 3) and lines[-1] == ("device", 0), (c, got)
+            assert len(lines) == 2 + (len(want) if fail < 0 else 1) and got[0] == (0 if fail < 0 else -1), (c, got)
+            assert all(name != "device" for name, _ in lines[1:-1]), (c, got)
