@@ -21,9 +21,9 @@
 //                hold of P here when the positions of V are taken in that order: v_place lays V out so, and p never
 //                leaves its lane.
 // f32 queries enter as two fp16 (their row scaled by a power of two to below 2^10). p is taken as two fp16 for f32 outputs,
-// and for fp16 ones of a single tile, where that is free (step after 131000 positions 32.9 us, of eight sequences 125 ->
-// 125.2) and brings them from 2.2-2.4e-4 off to the 2.0-2.2e-4 of their own rounding. Wider ones round p once: bound by the
-// vector unit, 1000 positions after 16001 would take 245 us for 194, to be 2.1e-4 off for 2.4e-4.
+// and for fp16 ones of a single tile, where that is free (a pass over 131000 positions 33.8 us, over eight sequences 125,
+// as with one) and brings them from 2.2-2.4e-4 off to the 2.0-2.2e-4 of their own rounding. Wider ones round p once: bound
+// by the vector unit, 1000 positions after 16001 would take 242 us for 192, to be 2.1e-4 off for 2.4e-4.
 //
 // The waves of a workgroup take the blocks of their tile in turn and join in LDS; where the tiles are too few for the
 // device, several workgroups share a tile (splits) and a second launch joins them. For eviction each block's sum goes
@@ -32,12 +32,12 @@
 // What bounds it, measured on one MI355X (3B shape: 8 KV heads of 64, 3 query heads each):
 //   one position   the cache's bytes: 134 MB of one sequence in 26 us (5.2 TB/s), 565 MB of eight in 110 us (5.2; blocks
 //                  in any order; a streaming read of 512 MiB reaches 5.7). Short caches: launches (5.6 us for 100 rows).
-//   many           the vector unit: 1000 positions after 16001, 101 GFLOP, in about 170 us in fp16. A block of two tiles
-//                  is 16 MFMAs of 16 cycles beside some 170 vector instructions, 64 of them the conversion of the codes,
-//                  16 exps at a quarter of the rate; the vector unit issues in 83% of the time, the matrix cores are busy
-//                  in 25%, 2.4 waves are on a SIMD. The whole call is 189 us, with one tile to a wave 298; with 2 or 8
-//                  waves to a workgroup 261 or 211 (131000 positions of one sequence, one each: 37 or 39 for 33); without
-//                  the matrix instructions first (s_setprio) 194.
+//   many           the vector unit: 1000 positions after 16001, 101 GFLOP, in about 172 us in fp16. A block of two tiles
+//                  is 16 MFMAs of 16 cycles beside 174 vector instructions, 64 of them the conversion of the codes, 16
+//                  exps at a quarter of the rate; the vector unit issues in 83% of the time, the matrix cores are busy
+//                  in 25%, 2.4 waves are on a SIMD. The whole pass is 192 us, with one tile to a wave 311; with 2 or 8
+//                  waves to a workgroup 266 or 215 (131000 positions of one sequence, one each: 40 or 43 for 34);
+//                  without the matrix instructions first (s_setprio) 195.5.
 #include <math.h>
 
 #include <type_traits>
@@ -190,12 +190,12 @@ __global__ __launch_bounds__(kWaves * 64, NT == 1 && D == 64 ? 4 : 2) void k_kv8
   constexpr int RP = 16 / (U / 2);
   auto elem = [](int u, int i) { return (u / 2 * RP + i % RP) * U + 2 * (i / RP) + u % 2; };
   // blocks in flight: with two tiles, or the 8 KB blocks of wide heads, the other waves cover the loads (with two: sixteen
-  // sequences of wide heads 34.7 us a pass for 32.7, one of 30000 positions 22.0 for 20.0; narrow ones gain with two where
-  // waves are few: 131000 positions of one sequence 33.3 for 33.7 with one, of eight 124.5 for 122.3)
+  // sequences of wide heads 34.5 us a pass for 32.6, one of 30000 positions 22.0 for 20.2; narrow ones gain with two where
+  // waves are few: 131000 positions of one sequence 33.7 for 34.0 with one, of eight 124.8 for 123.1)
   constexpr int PF = NT == 1 && D == 64 ? 2 : 1;
   // One block in flight: the next one's K is asked for once this one's scores are there, not behind its products of V
-  // (sixteen sequences of wide heads 35.3 -> 32.7 us a pass, 1000 positions after 16001 192 -> 189). With two in flight
-  // that is late already (131000 positions 33.3 -> 33.8).
+  // (sixteen sequences of wide heads 35.0 -> 32.6 us a pass, 1000 positions after 16001 197.5 -> 192). With two in flight
+  // that is late already (131000 positions 33.7 -> 34.4).
   constexpr bool EARLY = PF == 1;
   __shared__ __align__(16) float Os[kWaves][16][D + 4];
   __shared__ float2 Ms[kWaves][16];
@@ -739,8 +739,8 @@ KvAttnPlan kv8_attn_plan(const Kv8Dev& c, int n_seqs, int heads, int n, bool tra
   const long long units = (long long)n_seqs * c.kvh * tiles;
   // Splits cost a second launch and the partials' way through memory: one workgroup for each of 256 compute units, and
   // more (up to 1024, four to a unit) only while a wave keeps 16 blocks of a full cache; never fewer than 3 a wave. With
-  // 1024 workgroups wherever they could be had, a pass over sixteen sequences of wide heads takes 39 us for 32.7, 300
-  // positions after 1000 in f32 39 for 30.6; with 256 at most, eight sequences of up to 100003 take 161 for 124.5, though
+  // 1024 workgroups wherever they could be had, a pass over sixteen sequences of wide heads takes 39 us for 32.6, 300
+  // positions after 1000 in f32 39.7 for 30.8; with 256 at most, eight sequences of up to 100003 take 162 for 125, though
   // 200 positions after 4000 of wide heads 54 for 64.
   const int cap = c.slots / (kWaves * 3), most = cap < 1 ? 1 : cap > kMaxSplits ? kMaxSplits : cap;
   long long s = 256 / units > 1 ? 256 / units : 1;
@@ -767,8 +767,8 @@ hipError_t attend(hipStream_t s, AttnArgs a, float decay) {
   const long long units = (long long)a.n_seqs * a.c.kvh * a.splits;
   const long long grid = (units < 8 ? units : (units + 7) / 8 * 8) * a.tiles;  // below 2^23 (256 threads each: 2^31)
   // A layer's cache of 96 MB and more is streamed past the others: three of them outgrow the 256 MB last-level cache, and
-  // a model has more. 565 MB of eight sequences 138 -> 124.5 us a pass, 134 MB of one 35.3 -> 33.3; where three caches
-  // still fit (68 MB in use of 134 each), a pass loses what it would find there, 32.5 -> 32.9.
+  // a model has more. 565 MB of eight sequences 138 -> 125 us a pass, 134 MB of one 35.7 -> 33.7; where three caches
+  // still fit (68 MB in use of 134 each), a pass loses what it would find there, 31.5 -> 32.6.
   const bool stream = nt == 1 && 2ll * a.n_seqs * a.c.kvh * a.c.max_len * D >= 96ll << 20;
   if (stream) klaunch(k_kv8_attend<D, F16, 1, TRACK, true>, (unsigned)grid, kWaves * 64, 0, s, a);
   else if (nt == 1) klaunch(k_kv8_attend<D, F16, 1, TRACK, false>, (unsigned)grid, kWaves * 64, 0, s, a);
