@@ -307,7 +307,7 @@ def _plan(case, c, st):
     # the others, in order, while there are pages
     n = new.clamp(min=0)
     end = torch.cumsum(n, 0)
-    ok = (end <= T) & (rows + n <= M * P)
+    ok = (n == 0) | (end <= T) & (rows + n <= M * P)
     need = torch.where(ok, (rows + n + P - 1) // P - held, 0)
     upto = torch.cumsum(need, 0)
     ok = ok & ((need == 0) | (upto <= count))
@@ -419,7 +419,7 @@ def _plan_by_steps(case, st):
     for s, n in enumerate(max(x, 0) for x in new):
         rows = state[s][0]
         held, need = -(-rows // P), -(-(rows + n) // P) - -(-rows // P)
-        fits = len(slots) + n <= T and rows + n <= case["max_pages"] * P
+        fits = n == 0 or len(slots) + n <= T and rows + n <= case["max_pages"] * P
         if fits and need and (out_of_pages or need > free[0]):
             fits, out_of_pages = False, True
         if fits:
