@@ -40,8 +40,8 @@ enum {
   MOERT_E_RANGE = -5     /* token or index out of range (rust/moe-rt/src/gpu_model.rs:255-257) */
 };
 
-/* MOERT_F16 is a type of rows (moert_rows), not of matrices. */
-typedef enum { MOERT_F32 = 0, MOERT_Q8_0 = 1, MOERT_Q4_0 = 2, MOERT_F16 = 3 } moert_dtype;
+/* MOERT_F16 and MOERT_BF16 are types of rows (moert_rows) and of the paged cache, not of matrices. */
+typedef enum { MOERT_F32 = 0, MOERT_Q8_0 = 1, MOERT_Q4_0 = 2, MOERT_F16 = 3, MOERT_BF16 = 4 } moert_dtype;
 
 /* Model constants; mirrors `Config` (rust/moe-rt/src/model.rs:14-31). */
 typedef struct {
@@ -423,8 +423,8 @@ typedef struct {
 } moert_kv8;
 
 /* Rows in device memory: element e of head h of position i of the call's sequence s lies at
- * data[s * seq_stride + i * pos_stride + h * head_stride + e]. Strides are in elements; MOERT_F32 or MOERT_F16, the
- * pointer aligned to the element. Rows that a call writes must not overlap each other. */
+ * data[s * seq_stride + i * pos_stride + h * head_stride + e]. Strides are in elements; MOERT_F32 or MOERT_F16 (with the
+ * paged cache MOERT_BF16 too), the pointer aligned to the element. Rows that a call writes must not overlap each other. */
 typedef struct {
   void* data_dev;
   int dtype;
@@ -475,6 +475,92 @@ int moert_kv8_read(const moert_kv8* c, int seq0, int n_seqs, int pos, int n, con
 /* Lengths of the sequences, once the stream has come to this call (synchronises it; not under capture).
  * MOERT_E_FULL, with the lengths, where rows were dropped since the sequence was cleared. */
 int moert_kv8_lengths(const moert_kv8* c, int seq0, int n_seqs, int* lengths, void* stream);
+
+/* ---------------------------------------------------------------------------------------------------------
+ * Paged 16-bit K/V cache, in the caller's device buffers (no reference counterpart: the reference serves one sequence,
+ * whose cache is as long as it may become). Many sequences share one pool of pages: a plan on the device gives each
+ * step's sequences the pages that they lack and takes back those of sequences that have ended, rows are appended by the
+ * slots that it names, and attention reads them there, of one new position each (a decoding step, split along the
+ * cache) or of whole prompts. One plan, table and state serve all layers of a model; each layer has its K and V.
+ *
+ * A step: moert_pages_plan with the number of new rows of each sequence; per layer moert_pages_append of their K and V,
+ * packed one sequence behind the other, and moert_pages_prompt; or, where every sequence has one row, or none,
+ * moert_pages_attend. Both together, the prompt with least = 2, serve a step that mixes the two.
+ *
+ * Buffers, all of the device:
+ *   k, v   fp16 or bf16 (dtype: MOERT_F16, MOERT_BF16) [pages][kv_heads][page / 32][32 * head_dim]; may be NULL in calls
+ *          that neither append nor attend. Of a block of 32 positions, position t and element e lie
+ *            K at ((e / 8) * 32 + t) * 8 + e % 8
+ *            V at ((t / 16 * 2 + t % 8 / 4) * head_dim + e) * 8 + t % 4 + 4 * (t % 16 / 8)
+ *   table  i32 [seqs][max_pages]  pages of each sequence, in order
+ *   state  i32 [seqs][4]  rows of the sequence, rows refused for want of room (2^31 - 1: or more), the position of the
+ *          last plan's first row (-1: that plan has refused the sequence), 0
+ *   free   i32 [pages + 1]  how many pages are free, and which; the last of them is given first
+ * moert_pages_clear makes them an empty cache. Lengths are on the device, so that a captured graph of these calls can be
+ * replayed. Pages that several sequences share may be put into the table by the caller; a plan knows nothing of it and
+ * gives them back with each. Kernels keep to the buffers whatever table, state, free, starts and slots hold.
+ *
+ * Rows are of the cache's type, or f32 (rounded to nearest, ties to even) for a cache in fp16. A row of K or V that is
+ * not finite in the cache's type makes NaN of every output that sees it, and of no other. Memory behind a sequence's
+ * rows may hold anything.
+ *
+ * Limits: head_dim 64 or 128; page 32, 64, 128 or 256; max_pages * page at most 2^20, pages * page at most 2^30 and with
+ * kv_heads 2^35; at most 65535 sequences, 256 KV heads, 2^20 KV heads and 2^30 table entries of all sequences, 2^24 rows
+ * in a call, 64 query heads to a KV head, 2^24 query heads of all sequences and 2^27 of all rows of an attention. Calls
+ * enqueue on `stream` (a hipStream_t of the buffers' device, NULL for its default stream), allocate nothing and do not
+ * synchronise, except moert_pages_lengths. Calls on one cache are ordered by the caller (one stream, or events);
+ * attentions may overlap, each with a workspace of its own.
+ * ------------------------------------------------------------------------------------------------------- */
+enum { MOERT_PAGES_BLOCK = 32 };
+typedef struct {
+  int seqs, kv_heads, head_dim, page, pages, max_pages, dtype;
+  uint16_t *k_dev, *v_dev;
+  int *table_dev, *state_dev, *free_dev;
+} moert_pages;
+
+/* Empties the cache: no rows, all pages free, the first one given first. */
+int moert_pages_clear(const moert_pages* c, void* stream);
+
+/* Plans a step: new_dev [seqs] has the number of new rows of each sequence, negative for one that has ended (it becomes
+ * empty and its pages free, before any are given). starts_dev [seqs + 1] receives the packed rows of each sequence,
+ * [starts[s], starts[s + 1]), slots_dev [tokens] the slot of each row, page * (positions of a page) + place in it, and
+ * positions_dev [tokens], unless it is NULL, its position in the sequence; both are -1 behind the last row. `tokens` is
+ * the room for rows. The sequences get their pages in order. One whose rows do not fit into `tokens` or max_pages, or
+ * that lacks more pages than are left, stays as it is, and so do those behind it that lack any: their rows have slot
+ * -1, their positions see nothing until a plan takes them again, and moert_pages_lengths reports them. */
+int moert_pages_plan(const moert_pages* c, const int* new_dev, int tokens, int* starts_dev, int* slots_dev,
+                     int* positions_dev, void* stream);
+
+/* Writes `tokens` rows of K and V (of one type; seq_stride is not used) into their slots; no row where the slot is no
+ * slot of the pool. No two rows have the same slot. */
+int moert_pages_append(const moert_pages* c, const moert_rows* k, const moert_rows* v, const int* slots_dev,
+                       int tokens, void* stream);
+
+/* Bytes of workspace for attentions of `heads` query heads. Nothing in it has to be kept or cleared between calls. */
+int moert_pages_workspace(const moert_pages* c, int heads, size_t* bytes);
+
+/* Attention of one new position of every sequence over all rows of its own, its new one among them (appended before).
+ * Row starts[s] of q and out is that of sequence s where starts_dev gives it exactly one; the others are left out, and
+ * their rows of `out` as they were. Without starts (NULL) row s is, and tokens = seqs. Query head h reads KV head
+ * h / (heads / kv_heads). out = sum_t p_t v_t, p = softmax(scale * q . k); a position that sees no row gets 0, a query
+ * row that is not finite NaN. q and out are of one type, seq_stride is not used. Scores, weights and sums are f32, a
+ * weight as good as its score, an f32; outputs are finite as long as head_dim * max|q| * max|k|, and |scale| times
+ * that, are below 10^38, and max|v| below 2^90. The weights enter the second product as the sum of two numbers of the
+ * cache's type, off by 2^-22 (bf16 2^-16) of themselves or 2^-30 of the row's largest. out may be q itself, with the
+ * same strides; otherwise they do not overlap. ws: moert_pages_workspace bytes, aligned to 16. */
+int moert_pages_attend(const moert_pages* c, int heads, float scale, const moert_rows* q, const moert_rows* out,
+                       const int* starts_dev, int tokens, void* ws_dev, size_t ws_bytes, void* stream);
+
+/* Attention of the new rows of every sequence that has at least `least` (>= 1) of them, packed as starts_dev says, each
+ * over its own row and those before it: row i of n in a sequence of len rows sees the first len - n + 1 + i. As
+ * moert_pages_attend otherwise, but 16-bit rows' weights are rounded once to the cache's type. The rows of the other
+ * sequences, and those behind the last, stay as they were in `out`. */
+int moert_pages_prompt(const moert_pages* c, int heads, float scale, const moert_rows* q, const moert_rows* out,
+                       const int* starts_dev, int tokens, int least, void* stream);
+
+/* Lengths of the sequences, once the stream has come to this call (synchronises it; not under capture). MOERT_E_FULL,
+ * with the lengths, where rows were refused since a sequence began. */
+int moert_pages_lengths(const moert_pages* c, int seq0, int n_seqs, int* lengths, void* stream);
 
 /* Achievable HBM bandwidth reference: mean microseconds of one device-to-device streaming copy of `bytes`
  * (multiple of 16) over `iters` launches, each timed by its own dispatch events. No reference counterpart (the

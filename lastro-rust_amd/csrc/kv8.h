@@ -24,7 +24,7 @@ struct Kv8Dev {
 // moert_rows on the device; strides in elements.
 struct KvRows {
   void* p;
-  int f16;
+  int f16;  // 0 f32, 1 fp16, 2 bf16 (of the paged cache only)
   long long seq, pos, head;
 };
 

@@ -3,10 +3,9 @@
 
 #include "../../include/moert.h"
 #include "launch.h"
+#include "rows_api.h"
 
 namespace moert {
-
-int set_error(int code, const char* fmt, ...);
 
 namespace {
 
@@ -458,24 +457,7 @@ using namespace moert;
 
 namespace {
 
-#define KV_CFG(cond, ...) \
-  do {                    \
-    if (!(cond)) return set_error(MOERT_E_CONFIG, __VA_ARGS__); \
-  } while (0)
-
-#define KV_HIP(expr)                                                                                            \
-  do {                                                                                                          \
-    const hipError_t e_ = (expr);                                                                               \
-    if (e_ != hipSuccess)                                                                                       \
-      return set_error(MOERT_E_DEVICE, "%s failed: %s (%s:%d)", #expr, hipGetErrorString(e_), __FILE__, __LINE__); \
-  } while (0)
-
-#define KV_TRY(expr)             \
-  do {                           \
-    const int rc_ = (expr);      \
-    if (rc_ != MOERT_OK) return rc_; \
-  } while (0)
-
+constexpr int kOf8Bits = 1 << MOERT_F32 | 1 << MOERT_F16;
 constexpr int kKvMaxLen = 1 << 20, kKvMaxSeqs = 65535, kKvMaxHeads = 256;
 
 int view(const char* what, const moert_kv8* c, int seq0, int n_seqs, bool mass, Kv8Dev* d) {
@@ -501,65 +483,6 @@ int view(const char* what, const moert_kv8* c, int seq0, int n_seqs, bool mass, 
   return MOERT_OK;
 }
 
-// Rows that a call reads or (out) writes.
-int rows(const char* what, const moert_rows* r, int n_seqs, int n, int heads, int d, bool out, KvRows* k) {
-  KV_CFG(r && r->data_dev, "%s: null rows", what);
-  KV_CFG(r->dtype == MOERT_F32 || r->dtype == MOERT_F16, "%s: rows of dtype %d", what, r->dtype);
-  KV_CFG((uintptr_t)r->data_dev % (r->dtype == MOERT_F32 ? 4 : 2) == 0, "%s: rows not aligned to their type", what);
-  if (out) {
-    // each axis, from the one with the least stride on, has to clear all that the ones before it span
-    struct Axis {
-      long long stride;
-      int count;
-    } a[3] = {{r->seq_stride, n_seqs}, {r->pos_stride, n}, {r->head_stride, heads}};
-    for (int i = 0; i < 2; i++)
-      for (int j = 0; j < 2 - i; j++)
-        if (a[j].stride > a[j + 1].stride) {
-          const Axis t = a[j];
-          a[j] = a[j + 1];
-          a[j + 1] = t;
-        }
-    __int128 span = d;
-    for (const Axis& x : a)
-      if (x.count > 1) {
-        KV_CFG(x.stride >= span, "%s: rows to be written overlap (strides %lld, %lld, %lld)", what, r->seq_stride,
-               r->pos_stride, r->head_stride);
-        span += (__int128)x.stride * (x.count - 1);
-      }
-  }
-  *k = KvRows{r->data_dev, r->dtype == MOERT_F16, r->seq_stride, r->pos_stride, r->head_stride};
-  return MOERT_OK;
-}
-
-// Makes the buffers' device the current one while the call lasts. An error that an earlier call of the caller's has
-// left in the thread is dropped: the launchers ask for the last error, and it would pass for a launch's.
-class OnDevice {
- public:
-  ~OnDevice() {
-    if (back_ >= 0) (void)hipSetDevice(back_);
-  }
-  int enter(const char* what, const void* p) {
-    (void)hipGetLastError();
-    hipPointerAttribute_t a;
-    if (hipPointerGetAttributes(&a, p) != hipSuccess) {
-      (void)hipGetLastError();  // an address that the runtime does not know is no device error
-      return set_error(MOERT_E_CONFIG, "%s: the cache is not in device memory", what);
-    }
-    KV_CFG(a.type == hipMemoryTypeDevice || a.type == hipMemoryTypeManaged, "%s: the cache is not in device memory",
-           what);
-    int now = -1;
-    KV_HIP(hipGetDevice(&now));
-    if (now != a.device) {
-      KV_HIP(hipSetDevice(a.device));
-      back_ = now;
-    }
-    return MOERT_OK;
-  }
-
- private:
-  int back_ = -1;
-};
-
 }  // namespace
 
 extern "C" {
@@ -579,8 +502,8 @@ int moert_kv8_append(const moert_kv8* c, int seq0, int n_seqs, const moert_rows*
   KvRows kr, vr;
   KV_TRY(view("kv8_append", c, seq0, n_seqs, false, &d));
   KV_CFG(n >= 1 && n <= d.max_len, "kv8_append: %d rows, max_len %d", n, d.max_len);
-  KV_TRY(rows("kv8_append", k, n_seqs, n, d.kvh, d.d, false, &kr));
-  KV_TRY(rows("kv8_append", v, n_seqs, n, d.kvh, d.d, false, &vr));
+  KV_TRY(rows("kv8_append", k, kOf8Bits, n_seqs, n, d.kvh, d.d, false, &kr));
+  KV_TRY(rows("kv8_append", v, kOf8Bits, n_seqs, n, d.kvh, d.d, false, &vr));
   OnDevice on;
   KV_TRY(on.enter("kv8_append", d.kc));
   KV_HIP(launch_kv8_append((hipStream_t)stream, d, seq0, n_seqs, kr, vr, n));
@@ -594,8 +517,8 @@ int moert_kv8_read(const moert_kv8* c, int seq0, int n_seqs, int pos, int n, con
   KV_TRY(view("kv8_read", c, seq0, n_seqs, false, &d));
   KV_CFG(n >= 1 && n <= d.max_len && pos >= -d.max_len && pos < d.max_len, "kv8_read: %d positions from %d, max_len %d",
          n, pos, d.max_len);
-  KV_TRY(rows("kv8_read", k, n_seqs, n, d.kvh, d.d, true, &kr));
-  KV_TRY(rows("kv8_read", v, n_seqs, n, d.kvh, d.d, true, &vr));
+  KV_TRY(rows("kv8_read", k, kOf8Bits, n_seqs, n, d.kvh, d.d, true, &kr));
+  KV_TRY(rows("kv8_read", v, kOf8Bits, n_seqs, n, d.kvh, d.d, true, &vr));
   KV_CFG(k->data_dev != v->data_dev, "kv8_read: K and V to one address");
   OnDevice on;
   KV_TRY(on.enter("kv8_read", d.kc));
@@ -640,8 +563,8 @@ int moert_kv8_attend(const moert_kv8* c, int seq0, int n_seqs, int heads, int n,
   KV_TRY(view("kv8_attend", c, seq0, n_seqs, track, &d));
   KV_TRY(attend_shape("kv8_attend", d, n_seqs, heads, n));
   KV_CFG(scale - scale == 0.0f, "kv8_attend: scale %g", (double)scale);
-  KV_TRY(rows("kv8_attend", q, n_seqs, n, heads, d.d, false, &qr));
-  KV_TRY(rows("kv8_attend", out, n_seqs, n, heads, d.d, true, &orow));
+  KV_TRY(rows("kv8_attend", q, kOf8Bits, n_seqs, n, heads, d.d, false, &qr));
+  KV_TRY(rows("kv8_attend", out, kOf8Bits, n_seqs, n, heads, d.d, true, &orow));
   KV_CFG(q->dtype == out->dtype, "kv8_attend: q of dtype %d, out of %d", q->dtype, out->dtype);
   const KvAttnPlan p = kv8_attn_plan(d, n_seqs, heads, n, track);
   KV_CFG(ws_dev && (uintptr_t)ws_dev % 16 == 0 && ws_bytes >= p.bytes,

@@ -22,7 +22,7 @@ from typing import List, Optional
 
 import numpy as np
 
-F32, Q8_0, Q4_0, F16 = 0, 1, 2, 3  # F16: a type of rows (Kv8), not of matrices
+F32, Q8_0, Q4_0, F16, BF16 = 0, 1, 2, 3, 4  # F16, BF16: types of rows and caches (Kv8, Pages), not of matrices
 DTYPE_NAMES = {F32: "f32", Q8_0: "q8_0", Q4_0: "q4_0"}
 
 (K_EMBED, K_QKV, K_ATTN_SPLIT, K_ATTN_COMBINE, K_OPROJ, K_ROUTE_UP, K_EXPERT_DOWN, K_HEAD,
@@ -102,6 +102,11 @@ class moert_kv8(ctypes.Structure):
                 ("k_codes", "v_codes", "k_scale", "v_scale", "k_tail", "v_tail", "tail_bad", "table", "mass", "state")]
 
 
+class moert_pages(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int) for n in ("seqs", "kv_heads", "head_dim", "page", "pages", "max_pages", "dtype")] + \
+               [(n + "_dev", ctypes.c_void_p) for n in ("k", "v", "table", "state", "free")]
+
+
 _ROWS = struct.Struct("@Piqqq")  # moert_rows: address, dtype, strides; packing one takes a third of a Structure's time
 
 
@@ -179,6 +184,13 @@ def lib() -> ctypes.CDLL:
             "moert_kv8_evict": (i, [vp, i, i, i, i, i, vp]),
             "moert_kv8_read": (i, [vp, i, i, i, i, vp, vp, vp]),
             "moert_kv8_lengths": (i, [vp, i, i, vp, vp]),
+            "moert_pages_clear": (i, [vp, vp]),
+            "moert_pages_plan": (i, [vp, vp, i, vp, vp, vp, vp]),
+            "moert_pages_append": (i, [vp, vp, vp, vp, i, vp]),
+            "moert_pages_workspace": (i, [vp, i, ctypes.POINTER(sz)]),
+            "moert_pages_attend": (i, [vp, i, f, vp, vp, vp, i, vp, sz, vp]),
+            "moert_pages_prompt": (i, [vp, i, f, vp, vp, vp, i, i, vp]),
+            "moert_pages_lengths": (i, [vp, i, i, vp, vp]),
             "moert_exp_device": (i, [vp, vp, i]),
             "moert_copy_probe": (i, [sz, i, ctypes.POINTER(ctypes.c_double)]),
             "moert_read_probe": (i, [sz, i, ctypes.POINTER(ctypes.c_double)]),
@@ -253,7 +265,9 @@ EXPORTED = ["moert_last_error", "moert_device_info", "moert_model_create", "moer
             "moert_block_experts_in_step", "moert_block_batched_kernel", "moert_block_fault_inject", "moert_block_time_batched", "moert_router_topk", "moert_argmax", "moert_gemv",
             "moert_dequant", "moert_rmsnorm", "moert_rope", "moert_attn_decode", "moert_attn_decode_noalloc",
             "moert_kv8_clear", "moert_kv8_append", "moert_kv8_workspace", "moert_kv8_attend", "moert_kv8_evict",
-            "moert_kv8_read", "moert_kv8_lengths", "moert_exp_device",
+            "moert_kv8_read", "moert_kv8_lengths", "moert_pages_clear", "moert_pages_plan", "moert_pages_append",
+            "moert_pages_workspace", "moert_pages_attend", "moert_pages_prompt", "moert_pages_lengths",
+            "moert_exp_device",
             "moert_copy_probe", "moert_read_probe", "moert_h2d_probe", "moert_quantize", "moert_dtype_bytes", "moert_synth_normal", "moert_synth_quantized",
             "moert_synth_fp16", "moert_config_from_json", "moert_checkpoint_open", "moert_checkpoint_close",
             "moert_checkpoint_tensor", "moert_checkpoint_read_bf16", "moert_checkpoint_load", "moert_host_model_weights",
@@ -960,6 +974,91 @@ class Kv8:
         out = np.empty(max(1, self._n(seq0, n_seqs)), np.int32)
         try:
             check(self._lib.moert_kv8_lengths(self._p, seq0, self._n(seq0, n_seqs), ptr(out), stream))
+        except MoertError as e:
+            if e.code == E_FULL:
+                e.lengths = out
+            raise
+        return out
+
+
+# ---- paged 16-bit K/V cache --------------------------------------------------------------------------------------
+PAGES_BLOCK = 32  # positions of a block of a page
+
+
+def pages_shapes(seqs: int, kv_heads: int, head_dim: int, page: int, pages: int, max_pages: int) -> dict:
+    """The buffers of a paged K/V cache (moert_pages): name -> (shape, numpy dtype); k and v as bits."""
+    pool = (pages, kv_heads, page // PAGES_BLOCK, PAGES_BLOCK * head_dim)
+    return {"k": (pool, np.uint16), "v": (pool, np.uint16), "table": ((seqs, max_pages), np.int32),
+            "state": ((seqs, 4), np.int32), "free": ((pages + 1,), np.int32)}
+
+
+class Pages:
+    """Paged 16-bit K/V cache of one layer over the caller's device buffers (moert_pages_*): `buffers` gives the device
+    address of each name of pages_shapes (k and v may be left out where nothing appends or attends; layers share the
+    others). dtype, F16 or BF16, is the cache's. Arrays, rows, queries and outputs are device addresses too; rows are of
+    the cache's type, or F32 with one in F16, packed [row, head, element] or with `strides` (elements between rows and
+    heads). Calls enqueue on `stream` (a hipStream_t address, 0 = default stream)."""
+
+    def __init__(self, seqs: int, kv_heads: int, head_dim: int, page: int, pages: int, max_pages: int, buffers: dict,
+                 dtype: int = F16):
+        names = [n[:-4] for n, _ in moert_pages._fields_[7:]]
+        unknown = set(buffers) - set(names)
+        if unknown:
+            raise ValueError(f"no such buffers: {sorted(unknown)}")
+        self.seqs, self.kv_heads, self.head_dim, self.dtype = seqs, kv_heads, head_dim, dtype
+        self.page, self.pages, self.max_pages = page, pages, max_pages
+        self._c = moert_pages(seqs, kv_heads, head_dim, page, pages, max_pages, dtype,
+                              *[buffers.get(n) for n in names])
+        self._p = ctypes.addressof(self._c)
+        self._lib = lib()
+
+    def _rows(self, at, dtype, strides, heads):
+        r, h = strides or (heads * self.head_dim, self.head_dim)
+        return _ROWS.pack(at or 0, self.dtype if dtype is None else dtype, 0, r, h)
+
+    def clear(self, stream: int = 0) -> None:
+        """Empties the cache: all pages free."""
+        check(self._lib.moert_pages_clear(self._p, stream))
+
+    def plan(self, new: int, tokens: int, starts: int, slots: int, positions: int = 0, stream: int = 0) -> None:
+        """Plans a step of new[s] rows of each sequence (negative: it has ended): starts of the packed rows, and the
+        slot and position of each of `tokens`."""
+        check(self._lib.moert_pages_plan(self._p, new, tokens, starts, slots, positions, stream))
+
+    def append(self, k: int, v: int, slots: int, tokens: int, dtype: Optional[int] = None,
+               strides: Optional[tuple] = None, stream: int = 0) -> None:
+        """Writes rows into their slots."""
+        kr, vr = self._rows(k, dtype, strides, self.kv_heads), self._rows(v, dtype, strides, self.kv_heads)
+        check(self._lib.moert_pages_append(self._p, kr, vr, slots, tokens, stream))
+
+    def workspace(self, heads: int) -> int:
+        """Bytes of workspace of an attention of one position of every sequence."""
+        b = ctypes.c_size_t(0)
+        check(self._lib.moert_pages_workspace(self._p, heads, ctypes.byref(b)))
+        return b.value
+
+    def attend(self, q: int, out: int, heads: int, scale: float, ws: int, ws_bytes: int, starts: int = 0,
+               tokens: Optional[int] = None, dtype: Optional[int] = None, q_strides: Optional[tuple] = None,
+               out_strides: Optional[tuple] = None, stream: int = 0) -> None:
+        """Attention of the new position of every sequence that has one, over all its rows."""
+        qr, orow = self._rows(q, dtype, q_strides, heads), self._rows(out, dtype, out_strides, heads)
+        check(self._lib.moert_pages_attend(self._p, heads, scale, qr, orow, starts,
+                                           self.seqs if tokens is None else tokens, ws, ws_bytes, stream))
+
+    def prompt(self, q: int, out: int, heads: int, scale: float, starts: int, tokens: int, least: int = 1,
+               dtype: Optional[int] = None, q_strides: Optional[tuple] = None, out_strides: Optional[tuple] = None,
+               stream: int = 0) -> None:
+        """Attention of the new rows of every sequence that has at least `least`, each over its row and those before."""
+        qr, orow = self._rows(q, dtype, q_strides, heads), self._rows(out, dtype, out_strides, heads)
+        check(self._lib.moert_pages_prompt(self._p, heads, scale, qr, orow, starts, tokens, least, stream))
+
+    def lengths(self, seq0: int = 0, n_seqs: Optional[int] = None, stream: int = 0) -> np.ndarray:
+        """Lengths of the sequences (synchronises the stream); raises E_FULL, with the lengths in the error's `lengths`,
+        where rows were refused."""
+        n = self.seqs - seq0 if n_seqs is None else n_seqs
+        out = np.empty(max(1, n), np.int32)
+        try:
+            check(self._lib.moert_pages_lengths(self._p, seq0, n, ptr(out), stream))
         except MoertError as e:
             if e.code == E_FULL:
                 e.lengths = out
