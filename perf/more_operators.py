@@ -245,8 +245,8 @@ def prepare(case, seed):
                             {name: t.data_ptr() for name, t in state["c"].items()},
                             dtype=moert.BF16 if dtype == "bf16" else moert.F16)
         state.update(cache=cache, rows={"f32": moert.F32, "f16": moert.F16, "bf16": moert.BF16}[dtype])
-        if kind == "step":
-            size = cache.workspace(case["kv_heads"] * case["group"])
+        if kind in ("step", "prompt"):
+            size = cache.workspace(case["kv_heads"] * case["group"], state["tokens"] if kind == "prompt" else 0)
             state.update(ws=torch.empty(size, dtype=torch.uint8, device="cuda"), ws_bytes=size)
     return state
 
@@ -273,8 +273,8 @@ def run(state):
                          dtype=state["rows"], stream=stream)
         else:
             cache.prompt(state["q"].data_ptr(), state["out"].data_ptr(), case["kv_heads"] * case["group"],
-                         case["dim"] ** -0.5, state["starts"].data_ptr(), state["tokens"], dtype=state["rows"],
-                         stream=stream)
+                         case["dim"] ** -0.5, state["starts"].data_ptr(), state["tokens"], state["ws"].data_ptr(),
+                         state["ws_bytes"], dtype=state["rows"], stream=stream)
     elif kind == "plan":
         _plan(case, c, state)
     elif kind == "append":
