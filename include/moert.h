@@ -536,8 +536,9 @@ int moert_pages_plan(const moert_pages* c, const int* new_dev, int tokens, int* 
 int moert_pages_append(const moert_pages* c, const moert_rows* k, const moert_rows* v, const int* slots_dev,
                        int tokens, void* stream);
 
-/* Bytes of workspace for attentions of `heads` query heads. Nothing in it has to be kept or cleared between calls. */
-int moert_pages_workspace(const moert_pages* c, int heads, size_t* bytes);
+/* Bytes of workspace for attentions of `heads` query heads: of one position of each sequence, and of prompts of `tokens`
+ * rows (0: none). Nothing in it has to be kept or cleared between calls. */
+int moert_pages_workspace(const moert_pages* c, int heads, int tokens, size_t* bytes);
 
 /* Attention of one new position of every sequence over all rows of its own, its new one among them (appended before).
  * Row starts[s] of q and out is that of sequence s where starts_dev gives it exactly one; the others are left out, and
@@ -547,16 +548,16 @@ int moert_pages_workspace(const moert_pages* c, int heads, size_t* bytes);
  * weight as good as its score, an f32; outputs are finite as long as head_dim * max|q| * max|k|, and |scale| times
  * that, are below 10^38, and max|v| below 2^90. The weights enter the second product as the sum of two numbers of the
  * cache's type, off by 2^-22 (bf16 2^-16) of themselves or 2^-30 of the row's largest. out may be q itself, with the
- * same strides; otherwise they do not overlap. ws: moert_pages_workspace bytes, aligned to 16. */
+ * same strides; otherwise they do not overlap. ws: moert_pages_workspace bytes (tokens 0), aligned to 16. */
 int moert_pages_attend(const moert_pages* c, int heads, float scale, const moert_rows* q, const moert_rows* out,
                        const int* starts_dev, int tokens, void* ws_dev, size_t ws_bytes, void* stream);
 
 /* Attention of the new rows of every sequence that has at least `least` (>= 1) of them, packed as starts_dev says, each
  * over its own row and those before it: row i of n in a sequence of len rows sees the first len - n + 1 + i. As
  * moert_pages_attend otherwise, but 16-bit rows' weights are rounded once to the cache's type. The rows of the other
- * sequences, and those behind the last, stay as they were in `out`. */
+ * sequences, and those behind the last, stay as they were in `out`. ws: moert_pages_workspace bytes of `tokens`. */
 int moert_pages_prompt(const moert_pages* c, int heads, float scale, const moert_rows* q, const moert_rows* out,
-                       const int* starts_dev, int tokens, int least, void* stream);
+                       const int* starts_dev, int tokens, int least, void* ws_dev, size_t ws_bytes, void* stream);
 
 /* Lengths of the sequences, once the stream has come to this call (synchronises it; not under capture). MOERT_E_FULL,
  * with the lengths, where rows were refused since a sequence began. */

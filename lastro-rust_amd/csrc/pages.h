@@ -50,7 +50,7 @@ __device__ __forceinline__ int2 pg_span(const int* starts, int s, int tokens) {
   return make_int2(lo, hi);
 }
 
-size_t pages_workspace(const PagesDev& c, int heads);
+size_t pages_workspace(const PagesDev& c, int heads, int tokens);
 
 hipError_t launch_pages_clear(hipStream_t s, const PagesDev& c);
 hipError_t launch_pages_plan(hipStream_t s, const PagesDev& c, const int* fresh, int tokens, int* starts, int* slots,
@@ -59,6 +59,6 @@ hipError_t launch_pages_append(hipStream_t s, const PagesDev& c, KvRows k, KvRow
 hipError_t launch_pages_attend(hipStream_t s, const PagesDev& c, int heads, float scale, KvRows q, KvRows out,
                                const int* starts, int tokens, void* ws);
 hipError_t launch_pages_prompt(hipStream_t s, const PagesDev& c, int heads, float scale, KvRows q, KvRows out,
-                               const int* starts, int tokens, int least);
+                               const int* starts, int tokens, int least, void* ws);
 
 }  // namespace moert

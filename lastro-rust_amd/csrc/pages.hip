@@ -255,10 +255,18 @@ int tokens_ok(const char* what, int tokens) {
   return MOERT_OK;
 }
 
-int heads_ok(const char* what, const PagesDev& d, int heads) {
+int heads_ok(const char* what, const PagesDev& d, int heads, int tokens) {
   KV_CFG(heads >= 1 && heads % d.kvh == 0 && heads / d.kvh <= 64, "%s: %d query heads over %d KV heads", what, heads,
          d.kvh);
   KV_CFG((long long)d.seqs * heads <= 1 << 24, "%s: %d sequences x %d heads", what, d.seqs, heads);
+  KV_TRY(tokens_ok(what, tokens));
+  KV_CFG((long long)tokens * heads <= 1 << 27, "%s: %d rows x %d heads", what, tokens, heads);
+  return MOERT_OK;
+}
+
+int workspace_ok(const char* what, size_t need, const void* ws, size_t bytes) {
+  KV_CFG(bytes >= need && (!need || (ws && (uintptr_t)ws % 16 == 0)),
+         "%s: a workspace of %zu bytes aligned to 16 is needed, got %zu", what, need, bytes);
   return MOERT_OK;
 }
 
@@ -270,9 +278,7 @@ int ints_ok(const char* what, const int* p) {
 // What an attention is called with.
 int queries(const char* what, const PagesDev& d, int heads, float scale, const moert_rows* q, const moert_rows* out,
             int tokens, KvRows* qr, KvRows* orow) {
-  KV_TRY(heads_ok(what, d, heads));
-  KV_TRY(tokens_ok(what, tokens));
-  KV_CFG((long long)tokens * heads <= 1 << 27, "%s: %d rows x %d heads", what, tokens, heads);
+  KV_TRY(heads_ok(what, d, heads, tokens));
   KV_CFG(scale - scale == 0.0f, "%s: scale %g", what, (double)scale);
   KV_TRY(rows(what, q, types_of(d), 1, tokens, heads, d.d, false, qr));
   KV_TRY(rows(what, out, types_of(d), 1, tokens, heads, d.d, true, orow));
@@ -325,12 +331,12 @@ int moert_pages_append(const moert_pages* c, const moert_rows* k, const moert_ro
   return MOERT_OK;
 }
 
-int moert_pages_workspace(const moert_pages* c, int heads, size_t* bytes) {
+int moert_pages_workspace(const moert_pages* c, int heads, int tokens, size_t* bytes) {
   PagesDev d;
   KV_TRY(view("pages_workspace", c, 0, &d));
   KV_CFG(bytes, "pages_workspace: null bytes");
-  KV_TRY(heads_ok("pages_workspace", d, heads));
-  *bytes = pages_workspace(d, heads);
+  KV_TRY(heads_ok("pages_workspace", d, heads, tokens));
+  *bytes = pages_workspace(d, heads, tokens);
   return MOERT_OK;
 }
 
@@ -342,9 +348,7 @@ int moert_pages_attend(const moert_pages* c, int heads, float scale, const moert
   KV_TRY(queries("pages_attend", d, heads, scale, q, out, tokens, &qr, &orow));
   if (starts_dev) KV_TRY(ints_ok("pages_attend", starts_dev));
   else KV_CFG(tokens == d.seqs, "pages_attend: %d rows of %d sequences, without starts", tokens, d.seqs);
-  const size_t need = pages_workspace(d, heads);
-  KV_CFG(ws_bytes >= need && (!need || (ws_dev && (uintptr_t)ws_dev % 16 == 0)),
-         "pages_attend: a workspace of %zu bytes aligned to 16 is needed, got %zu", need, ws_bytes);
+  KV_TRY(workspace_ok("pages_attend", pages_workspace(d, heads, 0), ws_dev, ws_bytes));
   if (!tokens) return MOERT_OK;
   OnDevice on;
   KV_TRY(on.enter("pages_attend", d.k));
@@ -353,17 +357,18 @@ int moert_pages_attend(const moert_pages* c, int heads, float scale, const moert
 }
 
 int moert_pages_prompt(const moert_pages* c, int heads, float scale, const moert_rows* q, const moert_rows* out,
-                       const int* starts_dev, int tokens, int least, void* stream) {
+                       const int* starts_dev, int tokens, int least, void* ws_dev, size_t ws_bytes, void* stream) {
   PagesDev d;
   KvRows qr, orow;
   KV_TRY(view("pages_prompt", c, PG_POOL | PG_TABLE, &d));
   KV_TRY(queries("pages_prompt", d, heads, scale, q, out, tokens, &qr, &orow));
   KV_TRY(ints_ok("pages_prompt", starts_dev));
   KV_CFG(least >= 1, "pages_prompt: sequences of at least %d rows", least);
+  KV_TRY(workspace_ok("pages_prompt", pages_workspace(d, heads, tokens), ws_dev, ws_bytes));
   if (!tokens) return MOERT_OK;
   OnDevice on;
   KV_TRY(on.enter("pages_prompt", d.k));
-  KV_HIP(launch_pages_prompt((hipStream_t)stream, d, heads, scale, qr, orow, starts_dev, tokens, least));
+  KV_HIP(launch_pages_prompt((hipStream_t)stream, d, heads, scale, qr, orow, starts_dev, tokens, least, ws_dev));
   return MOERT_OK;
 }
 

@@ -1,6 +1,5 @@
 // Attention over the paged 16-bit K/V cache (pages.h).
-#include "launch.h"
-#include "pages.h"
+#include "pages_dev.h"
 
 namespace moert {
 
@@ -81,9 +80,21 @@ hipError_t rows_of(hipStream_t s, const PagesDev& c, int heads, float scale, KvR
   return hipGetLastError();
 }
 
+PgArgs args(const PagesDev& c, int heads, float scale, KvRows q, KvRows out, const int* starts, int tokens, int least,
+            int most) {
+  PgArgs a{};
+  a.c = c, a.q = q, a.out = out, a.starts = starts;
+  a.tokens = tokens, a.heads = heads, a.g = heads / c.kvh;
+  a.least = least, a.most = most;
+  a.vec = wide_rows(q) | wide_rows(out) << 1;
+  a.kf = frexpf(__builtin_fabsf(scale), &a.ke) * kPgLog2e;
+  a.sign = scale < 0.0f ? 0x80000000u : 0u;
+  return a;
+}
+
 }  // namespace
 
-size_t pages_workspace(const PagesDev& c, int heads) { return 0; }
+size_t pages_workspace(const PagesDev& c, int heads, int tokens) { return 0; }
 
 hipError_t launch_pages_attend(hipStream_t s, const PagesDev& c, int heads, float scale, KvRows q, KvRows out,
                                const int* starts, int tokens, void* ws) {
@@ -91,8 +102,8 @@ hipError_t launch_pages_attend(hipStream_t s, const PagesDev& c, int heads, floa
 }
 
 hipError_t launch_pages_prompt(hipStream_t s, const PagesDev& c, int heads, float scale, KvRows q, KvRows out,
-                               const int* starts, int tokens, int least) {
-  return rows_of(s, c, heads, scale, q, out, starts, tokens, 0, least);
+                               const int* starts, int tokens, int least, void* ws) {
+  return launch_pages_tiles(s, args(c, heads, scale, q, out, starts, tokens, least, 1 << 30));
 }
 
 }  // namespace moert

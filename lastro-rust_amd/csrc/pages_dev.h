@@ -1,0 +1,187 @@
+// What both attention kernels of the paged cache share (pages.h): types, queries, outputs, which rows a workgroup has.
+#pragma once
+#include <math.h>
+
+#include "launch.h"
+#include "pages.h"
+
+namespace moert {
+
+// Types of rows.
+enum { PG_F32 = 0, PG_F16 = 1, PG_BF16 = 2 };
+
+typedef _Float16 pg_h8 __attribute__((ext_vector_type(8)));
+typedef __bf16 pg_b8 __attribute__((ext_vector_type(8)));
+typedef _Float16 pg_h2 __attribute__((ext_vector_type(2)));
+typedef __bf16 pg_b2 __attribute__((ext_vector_type(2)));
+typedef float pg_f2 __attribute__((ext_vector_type(2)));
+typedef float pg_f4 __attribute__((ext_vector_type(4)));
+typedef float pg_f16 __attribute__((ext_vector_type(16)));
+
+constexpr float kPgNone = -3.4e38f;  // maximum of what has no score yet; finite, so that differences with it are
+constexpr float kPgSlack = 8.0f;     // log2 of how far a weight may lie above 1 before the maximum moves
+constexpr float kPgFar = 1048576.0f;  // scores beyond it lose 2^-5 in a product less a maximum: differences come first
+constexpr int kPgMaxSplits = 64;     // one lane each in the combine
+constexpr float kPgLog2e = 1.44269504088896341f;
+
+template <int T>
+__device__ __forceinline__ uint32_t pg_pack(float a, float b) {
+  const pg_f2 x = {a, b};
+  if constexpr (T == PG_BF16) return __builtin_bit_cast(uint32_t, __builtin_convertvector(x, pg_b2));
+  else return __builtin_bit_cast(uint32_t, __builtin_convertvector(x, pg_h2));
+}
+// The two numbers of a pair, as floats.
+template <int T>
+__device__ __forceinline__ pg_f2 pg_unpack(uint32_t w) {
+  if constexpr (T == PG_BF16) return pg_f2{__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)};
+  else return __builtin_convertvector(__builtin_bit_cast(pg_h2, w), pg_f2);
+}
+
+// D = A B + C on the matrix cores, A and B in 16 bits, 8 elements of a lane each.
+template <int T>
+__device__ __forceinline__ pg_f4 pg_mfma(uint4 a, uint4 b, pg_f4 c) {
+  if constexpr (T == PG_BF16)
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(pg_b8, a), __builtin_bit_cast(pg_b8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(pg_h8, a), __builtin_bit_cast(pg_h8, b), c, 0, 0, 0);
+}
+template <int T>
+__device__ __forceinline__ pg_f16 pg_mfma(uint4 a, uint4 b, pg_f16 c) {
+  if constexpr (T == PG_BF16)
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(pg_b8, a), __builtin_bit_cast(pg_b8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(pg_h8, a), __builtin_bit_cast(pg_h8, b), c, 0, 0, 0);
+}
+
+struct PgArgs {
+  PagesDev c;
+  KvRows q, out;
+  const int* starts;
+  int tokens, heads, g, splits, tiles;
+  int least, most;  // sequences of so many rows are attended
+  int vec;          // bit 0: q can be loaded 16 bytes at a time, bit 1: out can be stored so
+  float kf;         // |scale| log2 e, less 2^ke
+  int ke;
+  uint32_t sign;    // of the scale
+  float* part;      // [KV head][tile][row of it][split][D]
+  float2* ml;       // [KV head][tile][row of it][split]: maximum, sum
+};
+
+// Eight elements of a query from element `at` on, of a scale's sign.
+template <int T>
+__device__ __forceinline__ void pg_query(const PgArgs& a, long long at, float* x) {
+  if constexpr (T == PG_F32) {
+    const float* p = (const float*)a.q.p + at;
+    if (a.vec & 1) {
+      const float4 u = gload_f4(p), v = gload_f4(p + 4);
+      x[0] = u.x, x[1] = u.y, x[2] = u.z, x[3] = u.w, x[4] = v.x, x[5] = v.y, x[6] = v.z, x[7] = v.w;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; j++) x[j] = gmem(p)[j];
+    }
+#pragma unroll
+    for (int j = 0; j < 8; j++) x[j] = __uint_as_float(__float_as_uint(x[j]) ^ a.sign);
+  }
+}
+template <int T>
+__device__ __forceinline__ uint4 pg_query16(const PgArgs& a, long long at) {
+  const uint16_t* p = (const uint16_t*)a.q.p + at;
+  uint32_t w[4];
+  if (a.vec & 1) {
+    const uint4 v = gload_u4(p);
+    w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; j++) w[j] = (uint32_t)gmem(p)[2 * j] | (uint32_t)gmem(p)[2 * j + 1] << 16;
+  }
+  const uint32_t flip = a.sign ? 0x80008000u : 0u;
+  return make_uint4(w[0] ^ flip, w[1] ^ flip, w[2] ^ flip, w[3] ^ flip);
+}
+
+// An output is a mean of fp16 values: what roundings bring beyond the largest of them is cut.
+template <int T>
+__device__ __forceinline__ float pg_clip(float x) {
+  if constexpr (T == PG_F16) return x > 65504.0f ? 65504.0f : x < -65504.0f ? -65504.0f : x;
+  return x;
+}
+
+// N (4 or 8) elements of an output from element `at` on.
+template <int T, int N>
+__device__ __forceinline__ void pg_store(const PgArgs& a, long long at, const float* x) {
+  if constexpr (T == PG_F32) {
+    float* p = (float*)a.out.p + at;
+    if (a.vec & 2) {
+#pragma unroll
+      for (int j = 0; j < N; j += 4) *reinterpret_cast<pg_f4*>(p + j) = pg_f4{x[j], x[j + 1], x[j + 2], x[j + 3]};
+    } else {
+#pragma unroll
+      for (int j = 0; j < N; j++) p[j] = x[j];
+    }
+  } else {
+    uint16_t* p = (uint16_t*)a.out.p + at;
+    uint32_t w[N / 2];
+#pragma unroll
+    for (int j = 0; j < N / 2; j++) w[j] = pg_pack<T>(pg_clip<T>(x[2 * j]), pg_clip<T>(x[2 * j + 1]));
+    if (a.vec & 2) {
+      if constexpr (N == 8) *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+      else *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < N; j++) p[j] = (uint16_t)(w[j >> 1] >> (16 * (j & 1)));
+    }
+  }
+}
+
+// Tiles of W rows (a row: one query head of the group at one position, position by position) in a packed batch: those of
+// sequence s are counted from floor(starts[s] g / W) + s on, which leaves room for all of them, the last not full one
+// too, without anybody adding up. So tile y is the sequence's that is the last to begin at or before y: 64 candidates at
+// a time, one to a lane.
+__device__ __forceinline__ int pg_first_tile(const PgArgs& a, int s, int w) {
+  return min(max(gmem(a.starts)[s], 0), a.tokens) * a.g / w + s;
+}
+__device__ __forceinline__ int pg_find(const PgArgs& a, int y, int w) {
+  const int lane = threadIdx.x & 63;
+  int lo = 0, len = a.c.seqs;
+  while (len > 1) {
+    const int step = (len + 63) / 64, i = lane * step;
+    const bool in = i < len && pg_first_tile(a, lo + min(i, len - 1), w) <= y;
+    const unsigned long long m = __ballot(in);
+    const int x = m ? 63 - __builtin_clzll(m) : 0;
+    lo += x * step;
+    len = min(step, len - x * step);
+  }
+  return lo;
+}
+
+// What a tile has to do.
+struct PgTile {
+  int s, row0, rows, lo;  // sequence, its first row, rows of the sequence, place of the sequence in the batch
+  int sees0;              // rows that the sequence's first position sees
+};
+__device__ __forceinline__ bool pg_tile(const PgArgs& a, int y, int w, PgTile* t) {
+  int s, first;
+  if (a.starts) {
+    s = pg_find(a, y, w);
+    first = pg_first_tile(a, s, w);
+  } else {
+    const int per = (a.g + w - 1) / w;  // one position of each sequence
+    s = y / per;
+    first = s * per;
+  }
+  const int2 span = pg_span(a.starts, s, a.tokens);
+  const int n = span.y - span.x;
+  t->s = s;
+  t->lo = span.x;
+  t->rows = n * a.g;
+  t->row0 = (y - first) * w;
+  t->sees0 = pg_seen(a.c, s) - n + 1;
+  return n >= a.least && n <= a.most && t->row0 < t->rows;
+}
+// Tiles that a batch may have.
+inline int pg_tiles(const PgArgs& a, int w) {
+  return a.starts ? (int)((long long)a.tokens * a.g / w) + a.c.seqs : a.c.seqs * ((a.g + w - 1) / w);
+}
+
+hipError_t launch_pages_tiles(hipStream_t s, PgArgs a);
+
+}  // namespace moert

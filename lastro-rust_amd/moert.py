@@ -187,9 +187,9 @@ def lib() -> ctypes.CDLL:
             "moert_pages_clear": (i, [vp, vp]),
             "moert_pages_plan": (i, [vp, vp, i, vp, vp, vp, vp]),
             "moert_pages_append": (i, [vp, vp, vp, vp, i, vp]),
-            "moert_pages_workspace": (i, [vp, i, ctypes.POINTER(sz)]),
+            "moert_pages_workspace": (i, [vp, i, i, ctypes.POINTER(sz)]),
             "moert_pages_attend": (i, [vp, i, f, vp, vp, vp, i, vp, sz, vp]),
-            "moert_pages_prompt": (i, [vp, i, f, vp, vp, vp, i, i, vp]),
+            "moert_pages_prompt": (i, [vp, i, f, vp, vp, vp, i, i, vp, sz, vp]),
             "moert_pages_lengths": (i, [vp, i, i, vp, vp]),
             "moert_exp_device": (i, [vp, vp, i]),
             "moert_copy_probe": (i, [sz, i, ctypes.POINTER(ctypes.c_double)]),
@@ -1031,10 +1031,10 @@ class Pages:
         kr, vr = self._rows(k, dtype, strides, self.kv_heads), self._rows(v, dtype, strides, self.kv_heads)
         check(self._lib.moert_pages_append(self._p, kr, vr, slots, tokens, stream))
 
-    def workspace(self, heads: int) -> int:
-        """Bytes of workspace of an attention of one position of every sequence."""
+    def workspace(self, heads: int, tokens: int = 0) -> int:
+        """Bytes of workspace of attentions of one position of every sequence, and of prompts of `tokens` rows."""
         b = ctypes.c_size_t(0)
-        check(self._lib.moert_pages_workspace(self._p, heads, ctypes.byref(b)))
+        check(self._lib.moert_pages_workspace(self._p, heads, tokens, ctypes.byref(b)))
         return b.value
 
     def attend(self, q: int, out: int, heads: int, scale: float, ws: int, ws_bytes: int, starts: int = 0,
@@ -1045,12 +1045,12 @@ class Pages:
         check(self._lib.moert_pages_attend(self._p, heads, scale, qr, orow, starts,
                                            self.seqs if tokens is None else tokens, ws, ws_bytes, stream))
 
-    def prompt(self, q: int, out: int, heads: int, scale: float, starts: int, tokens: int, least: int = 1,
-               dtype: Optional[int] = None, q_strides: Optional[tuple] = None, out_strides: Optional[tuple] = None,
-               stream: int = 0) -> None:
+    def prompt(self, q: int, out: int, heads: int, scale: float, starts: int, tokens: int, ws: int, ws_bytes: int,
+               least: int = 1, dtype: Optional[int] = None, q_strides: Optional[tuple] = None,
+               out_strides: Optional[tuple] = None, stream: int = 0) -> None:
         """Attention of the new rows of every sequence that has at least `least`, each over its row and those before."""
         qr, orow = self._rows(q, dtype, q_strides, heads), self._rows(out, dtype, out_strides, heads)
-        check(self._lib.moert_pages_prompt(self._p, heads, scale, qr, orow, starts, tokens, least, stream))
+        check(self._lib.moert_pages_prompt(self._p, heads, scale, qr, orow, starts, tokens, least, ws, ws_bytes, stream))
 
     def lengths(self, seq0: int = 0, n_seqs: Optional[int] = None, stream: int = 0) -> np.ndarray:
         """Lengths of the sequences (synchronises the stream); raises E_FULL, with the lengths in the error's `lengths`,

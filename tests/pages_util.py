@@ -176,8 +176,8 @@ class Device:
         at = slots if isinstance(slots, int) else self.hip.upload(np.asarray(slots, np.int32))
         self.c.append(self.hip.upload(k), self.hip.upload(v), at, k.shape[0], dtype=dtype, **kw)
 
-    def workspace(self, heads):
-        size = self.c.workspace(heads)
+    def workspace(self, heads, tokens=0):
+        size = self.c.workspace(heads, tokens)
         return self.hip.upload(np.full(max(size, 16), 0xFF, np.uint8)), size
 
     def _out(self, q, dtype):
@@ -194,8 +194,9 @@ class Device:
 
     def prompt(self, q, scale, dtype, starts, **kw):
         out = self._out(q, dtype)
+        ws, size = self.workspace(q.shape[1], q.shape[0])
         self.c.prompt(self.hip.upload(q), out, q.shape[1], scale, self.hip.upload(np.asarray(starts, np.int32)),
-                      q.shape[0], dtype=dtype, **kw)
+                      q.shape[0], ws, size, dtype=dtype, **kw)
         self.hip.sync()
         return self.hip.get(out, q.shape, q.dtype)
 

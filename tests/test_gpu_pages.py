@@ -203,8 +203,9 @@ def test_strides(hip, dtype, shift, row, head):
     dev.set("state", [128, 0, 128 - n, 0])
     out = np.full(size, 7.0, np.float32) if dtype == F32 else np.full(size, 0x4321, np.uint16)
     po = hip.upload(out)
+    ws, ws_bytes = dev.workspace(heads, n)
     dev.c.prompt(hip.upload(k) + first * item, po + first * item, heads, 0.125, hip.upload(np.int32(starts)), n,
-                 dtype=dtype, q_strides=(row, head), out_strides=(row, head)) if min(row, head) > 0 else None
+                 ws, ws_bytes, dtype=dtype, q_strides=(row, head), out_strides=(row, head)) if min(row, head) > 0 else None
     hip.sync()
     got = hip.get(po, out.shape, out.dtype)
     if min(row, head) > 0:
@@ -398,13 +399,13 @@ def test_a_server(hip, dtype):
     dev, ref = both(hip, S, H, d, 32, 14, 8, dtype=cache_type(dtype))
     new, starts, slots, pos = (hip.upload(np.zeros(n, np.int32)) for n in (S, S + 1, T, T))
     k, v, q = (hip.upload(np.zeros((T, n, d), t)) for n in (H, H, heads))
-    ws, size = dev.workspace(heads)
+    ws, size = dev.workspace(heads, T)
     stream = hip.stream()
 
     def calls():
         dev.c.plan(new, T, starts, slots, pos, stream=stream)
         dev.c.append(k, v, slots, T, dtype=dtype, stream=stream)
-        dev.c.prompt(q, q, heads, 0.125, starts, T, least=2, dtype=dtype, stream=stream)
+        dev.c.prompt(q, q, heads, 0.125, starts, T, ws, size, least=2, dtype=dtype, stream=stream)
         dev.c.attend(q, q, heads, 0.125, ws, size, starts=starts, tokens=T, dtype=dtype, stream=stream)
 
     graph = hip.capture(stream, calls)

@@ -27,7 +27,7 @@ CALLS = {
     "attend": lambda c, **kw: c.attend(**{**dict(q=0x20000, out=0x20000, heads=4, scale=0.125, ws=0x30000,
                                                  ws_bytes=1 << 40), **kw}),
     "prompt": lambda c, **kw: c.prompt(**{**dict(q=0x20000, out=0x20000, heads=4, scale=0.125, starts=0x30000,
-                                                 tokens=5), **kw}),
+                                                 tokens=5, ws=0x40000, ws_bytes=1 << 40), **kw}),
     "lengths": lambda c, **kw: c.lengths(**kw),
 }
 USES = {"clear": "free state", "plan": "free state table", "append": "state k v", "workspace": "state",
@@ -66,12 +66,12 @@ def test_a_null_cache_and_unknown_buffers_are_refused():
     assert moert.lib().moert_pages_clear(None, None) == moert.E_CONFIG
     with pytest.raises(ValueError):
         cache({"keys": 1})
-    assert moert.lib().moert_pages_workspace(cache()._p, 4, None) == moert.E_CONFIG
+    assert moert.lib().moert_pages_workspace(cache()._p, 4, 0, None) == moert.E_CONFIG
 
 
 def test_bad_arrays_and_rows_are_refused():
     c = cache()
-    for name in ("plan", "append", "attend", "prompt"):
+    for name in ("plan", "append", "attend", "prompt", "workspace"):
         for n in (-1, (1 << 24) + 1):
             refused(lambda: CALLS[name](c, tokens=n), "rows")
     for bad in (dict(new=0), dict(new=0x20001), dict(starts=0), dict(starts=0x20002), dict(slots=0), dict(slots=0x20003),
@@ -159,7 +159,7 @@ def test_definition_attends():
     for i in (0, 7, 39):
         w = np.exp(0.125 * kk[:i + 1] @ q[i, 1])
         assert np.allclose(out[i, 1], w @ vv[:i + 1] / w.sum(), rtol=1e-12)
-    assert wrote.all() and (off > 0).all() and (off < 1e-4).all()
+    assert wrote.all() and (off > 0).all() and (off < 1e-3).all()
 
 
 @pytest.mark.parametrize("dtype", [F16, BF16])
