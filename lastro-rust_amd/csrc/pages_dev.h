@@ -98,6 +98,31 @@ __device__ __forceinline__ uint4 pg_query16(const PgArgs& a, long long at) {
   return make_uint4(w[0] ^ flip, w[1] ^ flip, w[2] ^ flip, w[3] ^ flip);
 }
 
+// f32 queries enter as two fp16: their row by a power of two to below 2^10, then what the first rounding leaves. So they
+// are off by 2^-22 of themselves. pg_split_exp: log2 of what the row has been divided by; m: its largest magnitude.
+__device__ __forceinline__ int pg_split_exp(float m) {
+  return (m > 0.0f && m < __int_as_float(0x7f800000) ? __builtin_amdgcn_frexp_expf(m) : 0) - 10;
+}
+template <int T>
+__device__ __forceinline__ void pg_split(const float* x, int e, uint4* hi, uint4* lo) {
+  const int e1 = -e / 2, e2 = -e - e1;  // in two factors: either alone could leave the type
+  uint32_t h[4], l[4];
+#pragma unroll
+  for (int j = 0; j < 4; j++) {
+    const float p = __builtin_amdgcn_ldexpf(__builtin_amdgcn_ldexpf(x[2 * j], e1), e2);
+    const float q = __builtin_amdgcn_ldexpf(__builtin_amdgcn_ldexpf(x[2 * j + 1], e1), e2);
+    h[j] = pg_pack<T>(p, q);
+    const pg_f2 back = pg_unpack<T>(h[j]);
+    l[j] = pg_pack<T>(p - back.x, q - back.y);
+  }
+  *hi = make_uint4(h[0], h[1], h[2], h[3]);
+  *lo = make_uint4(l[0], l[1], l[2], l[3]);
+}
+// What a sum of products is multiplied by; never 0: what is masked has to stay -inf.
+__device__ __forceinline__ float pg_factor(const PgArgs& a, int qe) {
+  return __builtin_fmaxf(__builtin_amdgcn_ldexpf(a.kf, a.ke + qe), 0x1p-126f);
+}
+
 // An output is a mean of fp16 values: what roundings bring beyond the largest of them is cut.
 template <int T>
 __device__ __forceinline__ float pg_clip(float x) {
@@ -160,11 +185,11 @@ struct PgTile {
 };
 __device__ __forceinline__ bool pg_tile(const PgArgs& a, int y, int w, PgTile* t) {
   int s, first;
-  if (a.starts) {
+  if (a.most > 1) {
     s = pg_find(a, y, w);
     first = pg_first_tile(a, s, w);
-  } else {
-    const int per = (a.g + w - 1) / w;  // one position of each sequence
+  } else {  // one position of each sequence
+    const int per = (a.g + w - 1) / w;
     s = y / per;
     first = s * per;
   }
@@ -179,9 +204,17 @@ __device__ __forceinline__ bool pg_tile(const PgArgs& a, int y, int w, PgTile* t
 }
 // Tiles that a batch may have.
 inline int pg_tiles(const PgArgs& a, int w) {
-  return a.starts ? (int)((long long)a.tokens * a.g / w) + a.c.seqs : a.c.seqs * ((a.g + w - 1) / w);
+  return a.most > 1 ? (int)((long long)a.tokens * a.g / w) + a.c.seqs : a.c.seqs * ((a.g + w - 1) / w);
 }
 
+// Splits of a tile of 128 rows that have work, of `blocks` blocks.
+__device__ __forceinline__ int pg_tiles_used(const PgArgs& a, int blocks) {
+  return max(1, min(a.splits, (blocks + 7) / 8));
+}
+
+// a.tiles and a.splits say how; launch_pages_join joins the splits of tiles of `width` rows.
 hipError_t launch_pages_tiles(hipStream_t s, PgArgs a);
+hipError_t launch_pages_cols(hipStream_t s, PgArgs a);
+hipError_t launch_pages_join(hipStream_t s, PgArgs a, int width);
 
 }  // namespace moert

@@ -43,7 +43,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void k_pages_tiles(PgArgs a) {
   if (!pg_tile(a, y, W, &t)) return;
   const int row1 = min(t.row0 + W, t.rows);
   const int seen = max(0, t.sees0 + (row1 - 1) / a.g), blocks = (seen + kPgBlock - 1) / kPgBlock;
-  const int stages = (blocks + kStage - 1) / kStage, used = max(1, min(a.splits, stages / 4));
+  const int stages = (blocks + kStage - 1) / kStage, used = pg_tiles_used(a, blocks);
   if (split >= used) return;
 
   // queries, and the rows that each column sees
@@ -65,30 +65,14 @@ __global__ __launch_bounds__(kWaves * 64, 2) void k_pages_tiles(PgArgs a) {
 #pragma unroll
         for (int j = 0; j < 8; j++) m = __builtin_fmaxf(m, __builtin_fabsf(v[k][j]));
       }
-      m = max_stage<32>(m);
-      const int e = m > 0.0f && m < __int_as_float(0x7f800000) ? __builtin_amdgcn_frexp_expf(m) : 0;
-      const int e1 = (10 - e) / 2, e2 = 10 - e - e1;  // in two factors: either alone could leave the type
-      qe = e - 10;
+      qe = pg_split_exp(max_stage<32>(m));
 #pragma unroll
-      for (int k = 0; k < KS; k++) {
-        uint32_t hi[4], lo[4];
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-          const float p = __builtin_amdgcn_ldexpf(__builtin_amdgcn_ldexpf(v[k][2 * j], e1), e2);
-          const float q = __builtin_amdgcn_ldexpf(__builtin_amdgcn_ldexpf(v[k][2 * j + 1], e1), e2);
-          hi[j] = pg_pack<T>(p, q);
-          const pg_f2 back = pg_unpack<T>(hi[j]);
-          lo[j] = pg_pack<T>(p - back.x, q - back.y);
-        }
-        qh[x][k] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-        ql[x][k] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-      }
+      for (int k = 0; k < KS; k++) pg_split<T>(v[k], qe, &qh[x][k], &ql[x][k]);
     } else {
 #pragma unroll
       for (int k = 0; k < KS; k++) qh[x][k] = pg_query16<T>(a, at + k * 16);
     }
-    // never 0: what is masked has to stay -inf
-    f[x] = __builtin_fmaxf(__builtin_amdgcn_ldexpf(a.kf, a.ke + qe), 0x1p-126f);
+    f[x] = pg_factor(a, qe);
   }
   const int least = t.sees0 + min(mine, t.rows - 1) / a.g;                     // rows that the wave's first column sees
   const int most = t.sees0 + min(mine + 32 * Q - 1, t.rows - 1) / a.g;         // and its last
@@ -280,8 +264,6 @@ __global__ __launch_bounds__(kWaves * 64, 2) void k_pages_tiles(PgArgs a) {
 }  // namespace
 
 hipError_t launch_pages_tiles(hipStream_t s, PgArgs a) {
-  a.tiles = pg_tiles(a, 128);
-  a.splits = 1;
   const unsigned grid = (unsigned)a.tiles * a.c.kvh * a.splits;
 #define TILES(DD, TT) \
   if (a.c.d == DD && a.q.f16 == TT) klaunch(k_pages_tiles<DD, TT, 1>, grid, kWaves * 64, 0, s, a);

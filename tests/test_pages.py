@@ -116,6 +116,18 @@ def test_bad_attentions_are_refused():
         refused(lambda: c.lengths(*seqs), "sequences")
 
 
+def test_workspaces():
+    """A workspace that is too small or not aligned is refused; none is needed where sequences are never split."""
+    for kw in (dict(max_pages=4096, pages=5000, seqs=1), dict(max_pages=64, seqs=4)):
+        c = cache(**kw)
+        size = c.workspace(4)
+        assert size > 0
+        refused(lambda: CALLS["attend"](c, ws_bytes=size - 1), "workspace")
+        refused(lambda: CALLS["attend"](c, ws=0x30008, ws_bytes=size), "workspace")
+        refused(lambda: CALLS["attend"](c, ws=0, ws_bytes=size), "workspace")
+    assert cache(max_pages=1).workspace(4) == 0
+
+
 def test_no_rows_need_nothing():
     c = cache()
     CALLS["append"](c, tokens=0, slots=0)
