@@ -57,8 +57,8 @@ hipError_t launch_pages_plan(hipStream_t s, const PagesDev& c, const int* fresh,
                              int* positions);
 hipError_t launch_pages_append(hipStream_t s, const PagesDev& c, KvRows k, KvRows v, const int* slots, int tokens);
 hipError_t launch_pages_attend(hipStream_t s, const PagesDev& c, int heads, float scale, KvRows q, KvRows out,
-                               const int* starts, int tokens, void* ws);
+                               const int* starts, int tokens, void* ws, size_t ws_bytes);
 hipError_t launch_pages_prompt(hipStream_t s, const PagesDev& c, int heads, float scale, KvRows q, KvRows out,
-                               const int* starts, int tokens, int least, void* ws);
+                               const int* starts, int tokens, int least, void* ws, size_t ws_bytes);
 
 }  // namespace moert

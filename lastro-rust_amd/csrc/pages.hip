@@ -352,7 +352,7 @@ int moert_pages_attend(const moert_pages* c, int heads, float scale, const moert
   if (!tokens) return MOERT_OK;
   OnDevice on;
   KV_TRY(on.enter("pages_attend", d.k));
-  KV_HIP(launch_pages_attend((hipStream_t)stream, d, heads, scale, qr, orow, starts_dev, tokens, ws_dev));
+  KV_HIP(launch_pages_attend((hipStream_t)stream, d, heads, scale, qr, orow, starts_dev, tokens, ws_dev, ws_bytes));
   return MOERT_OK;
 }
 
@@ -368,7 +368,8 @@ int moert_pages_prompt(const moert_pages* c, int heads, float scale, const moert
   if (!tokens) return MOERT_OK;
   OnDevice on;
   KV_TRY(on.enter("pages_prompt", d.k));
-  KV_HIP(launch_pages_prompt((hipStream_t)stream, d, heads, scale, qr, orow, starts_dev, tokens, least, ws_dev));
+  KV_HIP(launch_pages_prompt((hipStream_t)stream, d, heads, scale, qr, orow, starts_dev, tokens, least, ws_dev,
+                              ws_bytes));
   return MOERT_OK;
 }
 

@@ -27,38 +27,71 @@ int cols_splits(const PagesDev& c, long long units) {
   return (int)(s < most ? s : most);
 }
 
+constexpr int kTilesAtOnce = 512;
+
+// Tiles of 128 rows, where there are fewer than two workgroups to a unit: splits, of at least 16 blocks of a full table
+// each. (64 positions after 16000, 8 KV heads of 128: 407 us without splits, 59, 47 and 42 with 256, 512 and 768 workgroups
+// at most; 16 sequences of up to 100 after 500, 3 query heads each: 19.5 us without, 19.8 with 512, 26.7 with 768.)
+int tiles_splits(const PagesDev& c, long long units) {
+  const int blocks = c.max_pages << (c.lp - 5), cap = blocks / 16;
+  const int most = cap < 1 ? 1 : cap > kPgMaxSplits ? kPgMaxSplits : cap;
+  const long long s = kTilesAtOnce / units;
+  return (int)(s < 1 ? 1 : s < most ? s : most);
+}
+
+// Whether the tiles of 16 rows that the waves of a workgroup share do better than those of 128 rows that they split: up to
+// 32 rows of a sequence on average. (One sequence of 4000 positions, 8 KV heads of 64, 3 query heads: 24 rows 12.0 us in the
+// one, 17.5 in the other; of 32000, 33 rows: 23.3 and 22.2; 64 of 1000, of 128, 44 rows: 60.0 and 53.5.)
+bool few_rows(const PgArgs& a) { return (long long)a.tokens * a.g <= 32ll * a.c.seqs; }
+
 size_t up(size_t x) { return (x + 255) / 256 * 256; }
 size_t share_bytes(const PagesDev& c, size_t rows) { return up(rows * 8) + up(rows * c.d * 4); }
 
-void place(PgArgs* a, void* ws, int width) {
-  if (a->splits == 1) return;
+// Whether the workspace does for the splits; where it lies for them.
+bool place(PgArgs* a, void* ws, size_t bytes, int width) {
+  if (a->splits == 1) return true;
+  const size_t rows = (size_t)a->tiles * a->c.kvh * width * a->splits;
   a->ml = (float2*)ws;
-  a->part = (float*)((char*)ws + up((size_t)a->tiles * a->c.kvh * width * a->splits * 8));
+  a->part = (float*)((char*)ws + up(rows * 8));
+  return share_bytes(a->c, rows) <= bytes;
 }
 
 }  // namespace
 
 size_t pages_workspace(const PagesDev& c, int heads, int tokens) {
-  const int tiles = c.seqs * ((heads / c.kvh + 15) / 16), splits = cols_splits(c, (long long)tiles * c.kvh);
-  return splits > 1 ? share_bytes(c, (size_t)tiles * c.kvh * 16 * splits) : 0;
+  const int g = heads / c.kvh, tiles = c.seqs * ((g + 15) / 16), splits = cols_splits(c, (long long)tiles * c.kvh);
+  size_t rows = splits > 1 ? (size_t)tiles * c.kvh * 16 * splits : 0;
+  if (tokens) {  // of as many rows and of fewer: never less than for fewer
+    const size_t most = (size_t)(c.max_pages << (c.lp - 5)) / 8 < kPgMaxSplits ? (c.max_pages << (c.lp - 5)) / 8 : kPgMaxSplits;
+    const size_t few = ((size_t)tokens * g / 16 + c.seqs) * c.kvh, many = ((size_t)tokens * g / 128 + c.seqs) * c.kvh;
+    const size_t a = few * most < 1024 ? few * most : 1024, b = many * most < kTilesAtOnce ? many * most : kTilesAtOnce;
+    if (most > 1 && rows < a * 16) rows = a * 16;
+    if (most > 1 && rows < b * 128) rows = b * 128;
+  }
+  return rows ? share_bytes(c, rows) : 0;
 }
 
 hipError_t launch_pages_attend(hipStream_t s, const PagesDev& c, int heads, float scale, KvRows q, KvRows out,
-                               const int* starts, int tokens, void* ws) {
+                               const int* starts, int tokens, void* ws, size_t ws_bytes) {
   PgArgs a = args(c, heads, scale, q, out, starts, tokens, 1, 1);
   a.tiles = pg_tiles(a, 16);
   a.splits = cols_splits(c, (long long)a.tiles * c.kvh);
-  place(&a, ws, 16);
+  if (!place(&a, ws, ws_bytes, 16)) return hipErrorInvalidValue;
   if (const hipError_t e = launch_pages_cols(s, a)) return e;
   return a.splits > 1 ? launch_pages_join(s, a, 16) : hipSuccess;
 }
 
 hipError_t launch_pages_prompt(hipStream_t s, const PagesDev& c, int heads, float scale, KvRows q, KvRows out,
-                               const int* starts, int tokens, int least, void* ws) {
+                               const int* starts, int tokens, int least, void* ws,
+                               size_t ws_bytes) {
   PgArgs a = args(c, heads, scale, q, out, starts, tokens, least, 1 << 30);
-  a.tiles = pg_tiles(a, 128);
-  a.splits = 1;
-  return launch_pages_tiles(s, a);
+  const int width = few_rows(a) ? 16 : 128;
+  a.tiles = pg_tiles(a, width);
+  const long long units = (long long)a.tiles * c.kvh;
+  a.splits = width == 16 ? cols_splits(c, units) : tiles_splits(c, units);
+  if (!place(&a, ws, ws_bytes, width)) return hipErrorInvalidValue;
+  if (const hipError_t e = width == 16 ? launch_pages_cols(s, a) : launch_pages_tiles(s, a)) return e;
+  return a.splits > 1 ? launch_pages_join(s, a, width) : hipSuccess;
 }
 
 }  // namespace moert

@@ -32,11 +32,12 @@ __device__ __forceinline__ int cols_used(const PgArgs& a, int blocks) {
   return max(1, min(a.splits, (blocks + kWaves - 1) / kWaves));
 }
 
-template <int D, int T>
-__global__ __launch_bounds__(kWaves * 64, D == 64 ? 4 : 2) void k_pages_cols(PgArgs a) {
-  constexpr int KS = D / 32, U = D / 16, PF = D == 64 ? 2 : 1;  // blocks in flight
-  constexpr bool LO = T == PG_F32;                              // queries as two fp16
-  __shared__ __align__(16) float Os[kWaves][16][D + 4];
+template <int D, int T, bool STREAM>
+__global__ __launch_bounds__(kWaves * 64, D == 64 ? 2 : 1) void k_pages_cols(PgArgs a) {
+  constexpr int KS = D / 32, U = D / 16, RING = 2;             // blocks in flight, and being worked on
+  constexpr int kBytes = 64 * D, kCopies = 2 * kBytes / 1024;  // of a block of K or V; of both
+  constexpr bool LO = T == PG_F32;                                                     // queries as two fp16
+  __shared__ __align__(16) uint8_t ring[kWaves][RING][2][kBytes];
   __shared__ float2 Ms[kWaves][16];
   const PagesDev& c = a.c;
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, G = lane >> 4;
@@ -45,40 +46,26 @@ __global__ __launch_bounds__(kWaves * 64, D == 64 ? 4 : 2) void k_pages_cols(PgA
   if (!pg_tile(a, y, 16, &t)) return;
   const int blocks = tile_blocks(a, t, 16), used = cols_used(a, blocks);
   if (split >= used) return;
-  const int b0 = split * kWaves + w, step = a.splits * kWaves;  // this wave's first block, and on to the next
-
-  // the wave's blocks, 64 at a time, lane x holding the x-th one's place in the pool
+  // this wave's blocks: b0, b0 + step, ..; lane x holds the place in the pool of the x-th of 64
+  const int b0 = split * kWaves + w, step = a.splits * kWaves, count = max(0, (blocks - b0 + step - 1) / step);
   const int* table = c.table + (size_t)t.s * c.max_pages;
-  const int lb = c.lp - 5;
-  int block_l = 0, count = 0;
-  uint4 kb[PF][2 * KS], vb[PF][U];
-  auto batch = [&](int base) {
-    const int b = min(base + lane * step, blocks - 1);
-    block_l = pg_block(c, pg_page(c, gmem(table)[b >> lb]), h, b);
-    count = min(64, (blocks - base + step - 1) / step);
-  };
-  auto fetch_k = [&](int p, int x) {
-    const int b = __builtin_amdgcn_readlane(block_l, min(x, count - 1));
-    const uint16_t* at = c.k + (size_t)b * (kPgBlock * D) + (G * kPgBlock + col / 8 * 16 + col % 8) * 8;
-#pragma unroll
-    for (int z = 0; z < 2; z++)
-#pragma unroll
-      for (int k = 0; k < KS; k++) kb[p][z * KS + k] = gload_u4(at + (k * 4 * kPgBlock + z * 8) * 8);
-  };
-  auto fetch_v = [&](int p, int x) {
-    const int b = __builtin_amdgcn_readlane(block_l, min(x, count - 1));
-    const uint16_t* at = c.v + (size_t)b * (kPgBlock * D) + (G * D + col) * 8;
-#pragma unroll
-    for (int u = 0; u < U; u++) vb[p][u] = gload_u4(at + u * 128);
-  };
-  if (b0 < blocks) {
-    batch(b0);
-#pragma unroll
-    for (int p = 0; p < PF; p++) {
-      fetch_k(p, p);
-      fetch_v(p, p);
+  int place = 0;
+  auto fetch = [&](int x) {
+    if (x % 64 == 0) {
+      const int b = min(b0 + (x + lane) * step, blocks - 1);
+      place = pg_block(c, pg_page(c, gmem(table)[b >> (c.lp - 5)]), h, b);
     }
-  }
+    const size_t at = (size_t)__builtin_amdgcn_readlane(place, x % 64) * kBytes + lane * 16;
+    uint8_t* to = &ring[w][x % RING][0][0];
+#pragma unroll
+    for (int i = 0; i < kCopies / 2; i++) pg_copy_to_lds<STREAM>((const uint8_t*)c.k + at + i * 1024, to + i * 1024);
+#pragma unroll
+    for (int i = 0; i < kCopies / 2; i++)
+      pg_copy_to_lds<STREAM>((const uint8_t*)c.v + at + i * 1024, to + kBytes + i * 1024);
+  };
+#pragma unroll
+  for (int x = 0; x < RING; x++)
+    if (x < count) fetch(x);
 
   // queries, and the rows that each column sees
   const int row = min(t.row0 + col, t.rows - 1), i = row / a.g;
@@ -114,7 +101,7 @@ __global__ __launch_bounds__(kWaves * 64, D == 64 ? 4 : 2) void k_pages_cols(PgA
   float none = -__builtin_inff();
   asm("" : "+s"(none));
 
-  auto block = [&](auto masked, int p, int b, int next) {
+  auto block = [&](auto masked, const uint8_t* kp, const uint8_t* vp, int b) {
     constexpr bool MASKED = decltype(masked)::value;
     pg_f4 S[2];
 #pragma unroll
@@ -122,8 +109,9 @@ __global__ __launch_bounds__(kWaves * 64, D == 64 ? 4 : 2) void k_pages_cols(PgA
       S[z] = pg_f4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
       for (int k = 0; k < KS; k++) {
-        S[z] = pg_mfma<T>(kb[p][z * KS + k], qh[k], S[z]);
-        if constexpr (LO) S[z] = pg_mfma<T>(kb[p][z * KS + k], ql[k], S[z]);
+        const uint4 ka = *reinterpret_cast<const uint4*>(kp + ((4 * k + G) * kPgBlock + col / 8 * 16 + col % 8 + 8 * z) * 16);
+        S[z] = pg_mfma<T>(ka, qh[k], S[z]);
+        if constexpr (LO) S[z] = pg_mfma<T>(ka, ql[k], S[z]);
       }
     }
     const int t0 = b * kPgBlock + G / 2 * 16 + G % 2 * 4;  // the lane's first position
@@ -132,7 +120,6 @@ __global__ __launch_bounds__(kWaves * 64, D == 64 ? 4 : 2) void k_pages_cols(PgA
       for (int z = 0; z < 8; z++)
         if (t0 + z / 4 * 8 + z % 4 >= sees) S[z / 4][z % 4] = -__builtin_inff();
     }
-    if (next < count) fetch_k(p, next);
     float mx = none;
 #pragma unroll
     for (int z = 0; z < 8; z++) mx = __builtin_fmaxf(mx, S[z / 4][z % 4]);
@@ -175,38 +162,33 @@ __global__ __launch_bounds__(kWaves * 64, D == 64 ? 4 : 2) void k_pages_cols(PgA
     }
 #pragma unroll
     for (int u = 0; u < U; u++) {
-      uint4 va = vb[p][u];
+      uint4 va = *reinterpret_cast<const uint4*>(vp + (G * D + 16 * u + col) * 16);
       if constexpr (MASKED) va = make_uint4(va.x & keep[0], va.y & keep[1], va.z & keep[2], va.w & keep[3]);
       O[u] = pg_mfma<T>(va, ph, O[u]);
       O[u] = pg_mfma<T>(va, pl, O[u]);
     }
-    if (next < count) fetch_v(p, next);
   };
 
-  for (int base = b0; base < blocks; base += 64 * step) {
-    if (base != b0) {
-      batch(base);
-#pragma unroll
-      for (int p = 0; p < PF; p++) {
-        fetch_k(p, p);
-        fetch_v(p, p);
-      }
-    }
-    for (int x = 0; x < count; x += PF) {
-#pragma unroll
-      for (int p = 0; p < PF; p++) {
-        const int b = base + (x + p) * step;
-        if (PF > 1 && x + p >= count) break;
-        if ((b + 1) * kPgBlock > least) block(std::true_type{}, p, b, x + p + PF);
-        else block(std::false_type{}, p, b, x + p + PF);
-      }
+  for (int x = 0; x < count; x++) {
+    if (x + RING <= count) pg_wait_copies<(RING - 1) * kCopies>();
+    else pg_wait_copies<0>();
+    const int b = b0 + x * step;
+    const uint8_t *kp = ring[w][x % RING][0], *vp = ring[w][x % RING][1];
+    if ((b + 1) * kPgBlock > least) block(std::true_type{}, kp, vp, b);
+    else block(std::false_type{}, kp, vp, b);
+    if (x + RING < count) {
+      pg_wait_reads();
+      fetch(x + RING);
     }
   }
 
   // the waves' shares; a wave without blocks has none
   l = sum16(l);
+  auto shares = [&](int x) { return reinterpret_cast<float(*)[D + 4]>(&ring[x]); };  // of a wave, where its blocks were
+  static_assert(sizeof(float) * 16 * (D + 4) <= RING * 2 * kBytes, "");
+  pg_wait_reads();
 #pragma unroll
-  for (int u = 0; u < U; u++) *reinterpret_cast<pg_f4*>(&Os[w][col][16 * u + 4 * G]) = O[u];
+  for (int u = 0; u < U; u++) *reinterpret_cast<pg_f4*>(&shares(w)[col][16 * u + 4 * G]) = O[u];
   if (G == 0) Ms[w][col] = make_float2(M, l);
   __syncthreads();
   const int cl = threadIdx.x / 16, e0 = threadIdx.x % 16 * U, r = t.row0 + cl;
@@ -220,7 +202,7 @@ __global__ __launch_bounds__(kWaves * 64, D == 64 ? 4 : 2) void k_pages_cols(PgA
     const float al = __builtin_amdgcn_exp2f(Ms[x][cl].x - m);
     sum = __builtin_fmaf(Ms[x][cl].y, al, sum);
 #pragma unroll
-    for (int e = 0; e < U; e++) o[e] = __builtin_fmaf(Os[x][cl][e0 + e], al, o[e]);
+    for (int e = 0; e < U; e++) o[e] = __builtin_fmaf(shares(x)[cl][e0 + e], al, o[e]);
   }
   if (used == 1) {
     const float inv = t.sees0 + r / a.g > 0 ? 1.0f / sum : 0.0f;
@@ -236,38 +218,65 @@ __global__ __launch_bounds__(kWaves * 64, D == 64 ? 4 : 2) void k_pages_cols(PgA
   }
 }
 
-// The splits' shares of 16 rows of a tile of W, a wave to four of them.
-template <int D, int T, int W>
-__global__ __launch_bounds__(256) void k_pages_join(PgArgs a) {
-  constexpr int E = D / 64, P = W / 16;
+// The splits' shares of a tile's rows. C = 4: a workgroup to a row, its waves take every fourth split; C = 1, up to 8 splits:
+// 16 rows to a workgroup, a wave takes one at a time. All products are asked for at once and before it is known which
+// splits have any: the others lie in the workspace too, and are not looked at.
+template <int D, int T, int W, int C>
+__global__ __launch_bounds__(256) void k_pages_join(PgArgs a, int groups) {
+  constexpr int E = D / 64, N = C == 4 ? kPgMaxSplits / 4 : 8, R = C == 4 ? 1 : 4;
+  __shared__ float Os[4][D];
   const PagesDev& c = a.c;
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int id = blockIdx.x, h = id % c.kvh, part = id / c.kvh % P, y = id / c.kvh / P;
+  const int id = blockIdx.x, h = id % c.kvh, x0 = id / c.kvh % groups * (C == 4 ? 1 : 16) + (C == 4 ? 0 : w * R);
+  const int y = id / c.kvh / groups, s0 = C == 4 ? w : 0;
+  const size_t row0 = ((size_t)h * a.tiles + y) * W + x0;
+  float2 ml[R];
+  float p[R][N][E];
+#pragma unroll
+  for (int i = 0; i < R; i++) {
+    ml[i] = a.ml[(row0 + i) * a.splits + min(lane, a.splits - 1)];
+#pragma unroll
+    for (int j = 0; j < N; j++)
+#pragma unroll
+      for (int e = 0; e < E; e++)
+        if (s0 + C * j < a.splits) p[i][j][e] = gmem(a.part)[((row0 + i) * a.splits + s0 + C * j) * D + e * 64 + lane];
+  }
   PgTile t;
   if (!pg_tile(a, y, W, &t)) return;
   const int blocks = tile_blocks(a, t, W), used = W == 16 ? cols_used(a, blocks) : pg_tiles_used(a, blocks);
   if (used == 1) return;
-  for (int j = 0; j < 4; j++) {
-    const int x = part * 16 + w * 4 + j, r = t.row0 + x;
-    if (r >= t.rows) return;
-    const size_t wc = (((size_t)h * a.tiles + y) * W + x) * a.splits;
-    const float2 ml = a.ml[wc + min(lane, used - 1)];
-    const float m = group_max(lane < used ? ml.x : kPgNone);
-    const float al = lane < used ? __builtin_amdgcn_exp2f(ml.x - m) : 0.0f;
-    const float sum = group_sum(lane < used ? ml.y * al : 0.0f);
-    float o[E] = {};
-#pragma unroll 8
-    for (int s = 0; s < used; s++) {
-      const float f = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(al), s));
 #pragma unroll
-      for (int e = 0; e < E; e++) o[e] = __builtin_fmaf(gmem(a.part)[(wc + s) * D + lane * E + e], f, o[e]);
+  for (int i = 0; i < R; i++) {
+    const int r = t.row0 + x0 + i;
+    if (r >= t.rows) return;
+    const float m = group_max(lane < used ? ml[i].x : kPgNone);
+    const float al = lane < used ? __builtin_amdgcn_exp2f(ml[i].x - m) : 0.0f;
+    const float sum = group_sum(lane < used ? ml[i].y * al : 0.0f);
+    float o[E] = {};
+#pragma unroll
+    for (int j = 0; j < N; j++) {
+      const int s = s0 + C * j;
+      if (s < used) {
+        const float f = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(al), s));
+#pragma unroll
+        for (int e = 0; e < E; e++) o[e] = __builtin_fmaf(p[i][j][e], f, o[e]);
+      }
+    }
+    if constexpr (C == 4) {
+#pragma unroll
+      for (int e = 0; e < E; e++) Os[w][e * 64 + lane] = o[e];
+      __syncthreads();
+      if (w) return;
+#pragma unroll
+      for (int e = 0; e < E; e++)
+        o[e] = (o[e] + Os[1][e * 64 + lane]) + (Os[2][e * 64 + lane] + Os[3][e * 64 + lane]);
     }
     const float inv = t.sees0 + r / a.g > 0 ? 1.0f / sum : 0.0f;
-    const long long at = (long long)(t.lo + r / a.g) * a.out.pos + (long long)(h * a.g + r % a.g) * a.out.head + lane * E;
+    const long long at = (long long)(t.lo + r / a.g) * a.out.pos + (long long)(h * a.g + r % a.g) * a.out.head + lane;
 #pragma unroll
     for (int e = 0; e < E; e++) {
-      if constexpr (T == PG_F32) ((float*)a.out.p)[at + e] = o[e] * inv;
-      else ((uint16_t*)a.out.p)[at + e] = (uint16_t)pg_pack<T>(pg_clip<T>(o[e] * inv), 0.0f);
+      if constexpr (T == PG_F32) ((float*)a.out.p)[at + e * 64] = o[e] * inv;
+      else ((uint16_t*)a.out.p)[at + e * 64] = (uint16_t)pg_pack<T>(pg_clip<T>(o[e] * inv), 0.0f);
     }
   }
 }
@@ -276,21 +285,32 @@ __global__ __launch_bounds__(256) void k_pages_join(PgArgs a) {
 
 hipError_t launch_pages_cols(hipStream_t s, PgArgs a) {
   const unsigned grid = (unsigned)a.tiles * a.c.kvh * a.splits;
-#define COLS(DD, TT) \
-  if (a.c.d == DD && a.q.f16 == TT) klaunch(k_pages_cols<DD, TT>, grid, kWaves * 64, 0, s, a);
+  // Two blocks to a wave: with four narrow ones 42 us for 38.7 (131000 positions of 8 heads of 64), with one wide one 154
+  // for 147 (64 sequences, 973 MB). Caches that outgrow the last-level cache in three layers are streamed past it: 174.8 us
+  // with one wide block without, 153.8 with the hint; rows whose tiles read the cache again find it there.
+  const PagesDev& c = a.c;
+  const long long held = (long long)(c.pages < (long long)c.seqs * c.max_pages ? c.pages : (long long)c.seqs * c.max_pages);
+  const bool stream = a.most == 1 && a.g <= 16 && ((held * c.kvh * c.d) << c.lp) * 4 >= 96ll << 20;
+#define COLS(DD, TT)                                                                              \
+  if (c.d == DD && a.q.f16 == TT) {                                                               \
+    if (stream) klaunch(k_pages_cols<DD, TT, true>, grid, kWaves * 64, 0, s, a);                  \
+    else klaunch(k_pages_cols<DD, TT, false>, grid, kWaves * 64, 0, s, a);                        \
+  }
   COLS(64, 0) COLS(64, 1) COLS(64, 2) COLS(128, 0) COLS(128, 1) COLS(128, 2)
 #undef COLS
   return hipGetLastError();
 }
 
 hipError_t launch_pages_join(hipStream_t s, PgArgs a, int width) {
-  const unsigned grid = (unsigned)a.tiles * a.c.kvh * (width / 16);
-#define JOIN(DD, TT)                                                                   \
-  if (a.c.d == DD && a.q.f16 == TT) {                                                  \
-    if (width == 16) klaunch(k_pages_join<DD, TT, 16>, grid, 256, 0, s, a);            \
-    else klaunch(k_pages_join<DD, TT, 128>, grid, 256, 0, s, a);                       \
-  }
-  JOIN(64, 0) JOIN(64, 1) JOIN(64, 2) JOIN(128, 0) JOIN(128, 1) JOIN(128, 2)
+  const int rows = a.most > 1 || a.g > width ? width : a.g;  // of one position there are no more
+  const int wide = a.splits > 8, groups = wide ? rows : (rows + 15) / 16;
+  const unsigned grid = (unsigned)a.tiles * a.c.kvh * groups;
+#define JOIN(DD, TT, WW, CC) \
+  if (a.c.d == DD && a.q.f16 == TT && width == WW && wide == (CC == 4)) \
+    klaunch(k_pages_join<DD, TT, WW, CC>, grid, 256, 0, s, a, groups);
+#define JOINS(DD, TT) JOIN(DD, TT, 16, 1) JOIN(DD, TT, 16, 4) JOIN(DD, TT, 128, 1) JOIN(DD, TT, 128, 4)
+  JOINS(64, 0) JOINS(64, 1) JOINS(64, 2) JOINS(128, 0) JOINS(128, 1) JOINS(128, 2)
+#undef JOINS
 #undef JOIN
   return hipGetLastError();
 }

@@ -37,6 +37,15 @@ __device__ __forceinline__ pg_f2 pg_unpack(uint32_t w) {
   else return __builtin_convertvector(__builtin_bit_cast(pg_h2, w), pg_f2);
 }
 
+// x + a pair's sum.
+template <int T>
+__device__ __forceinline__ float pg_add(uint32_t w, float x) {
+  if constexpr (T == PG_BF16)
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(pg_b2, w), pg_b2{(__bf16)1.0f, (__bf16)1.0f}, x, false);
+  else
+    return __builtin_amdgcn_fdot2(__builtin_bit_cast(pg_h2, w), pg_h2{(_Float16)1.0f, (_Float16)1.0f}, x, false);
+}
+
 // D = A B + C on the matrix cores, A and B in 16 bits, 8 elements of a lane each.
 template <int T>
 __device__ __forceinline__ pg_f4 pg_mfma(uint4 a, uint4 b, pg_f4 c) {
@@ -97,6 +106,25 @@ __device__ __forceinline__ uint4 pg_query16(const PgArgs& a, long long at) {
   const uint32_t flip = a.sign ? 0x80008000u : 0u;
   return make_uint4(w[0] ^ flip, w[1] ^ flip, w[2] ^ flip, w[3] ^ flip);
 }
+
+// 16 bytes of each lane to LDS, in a row from `dst` (the wave's) on, without a way through registers. Not by the builtin:
+// the compiler cannot tell the buffer that is filled from the one being read, and would wait for the copy before each read.
+// Whoever reads them waits by pg_wait_copies first: for all but the last N copies and loads of the wave (loads of the
+// compiler's among them only make it wait for more). STREAM: with the non-temporal hint.
+template <bool STREAM>
+__device__ __forceinline__ void pg_copy_to_lds(const uint8_t* src, uint8_t* dst) {
+  const uint32_t at = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)dst);
+  if constexpr (STREAM)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off nt" : : "s"(at), "v"(src) : "memory", "m0");
+  else
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(at), "v"(src) : "memory", "m0");
+}
+template <int N>
+__device__ __forceinline__ void pg_wait_copies() {
+  asm volatile("s_waitcnt vmcnt(%0)" : : "n"(N) : "memory");
+}
+// The wave's reads of LDS have their data: copies may go over what they read.
+__device__ __forceinline__ void pg_wait_reads() { asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory"); }
 
 // f32 queries enter as two fp16: their row by a power of two to below 2^10, then what the first rounding leaves. So they
 // are off by 2^-22 of themselves. pg_split_exp: log2 of what the row has been divided by; m: its largest magnitude.

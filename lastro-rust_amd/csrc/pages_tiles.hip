@@ -21,17 +21,9 @@ namespace {
 constexpr int kWaves = 4;
 constexpr int kStage = 2;  // blocks staged together
 
-// 16 bytes of each lane to LDS, in a row from `dst` (the wave's) on, without a way through registers. Not by the builtin:
-// the compiler cannot tell the buffer that it fills from the one being read, and would wait for the copy before each read.
-// Whoever reads them waits for vmcnt 0 and a barrier first.
-__device__ __forceinline__ void pg_copy_to_lds(const uint8_t* src, uint8_t* dst) {
-  const uint32_t at = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)dst);
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(at), "v"(src) : "memory", "m0");
-}
-
-template <int D, int T, int Q>
-__global__ __launch_bounds__(kWaves * 64, 2) void k_pages_tiles(PgArgs a) {
-  constexpr int KS = D / 16, U = D / 32, W = 32 * Q * kWaves, kBytes = 64 * D;  // of a block of K or V
+template <int D, int T>
+__global__ __launch_bounds__(kWaves * 64, D == 64 ? 3 : 2) void k_pages_tiles(PgArgs a) {
+  constexpr int KS = D / 16, U = D / 32, W = 32 * kWaves, kBytes = 64 * D;  // of a block of K or V
   constexpr bool LO = T == PG_F32;  // queries and weights as two fp16
   __shared__ __align__(16) uint8_t lds[2][kStage][2][kBytes];
   const PagesDev& c = a.c;
@@ -46,17 +38,38 @@ __global__ __launch_bounds__(kWaves * 64, 2) void k_pages_tiles(PgArgs a) {
   const int stages = (blocks + kStage - 1) / kStage, used = pg_tiles_used(a, blocks);
   if (split >= used) return;
 
-  // queries, and the rows that each column sees
-  uint4 qh[Q][KS], ql[Q][LO ? KS : 1];
-  float f[Q];
-  int sees[Q];
-  const int mine = t.row0 + w * 32 * Q;  // the wave's first row
+  // this split's stages: split, split + used, ..; wave w copies K (even) or V (odd) of block w / 2 of a stage
+  const int* table = c.table + (size_t)t.s * c.max_pages;
+  const int block_w = w >> 1, last = blocks - 1, lb = c.lp - 5;
+  const uint16_t* pool = w & 1 ? c.v : c.k;
+  auto page_of = [&](int st) { return pg_page(c, gmem(table)[min(st * kStage + block_w, last) >> lb]); };
+  auto copy = [&](int st, int buf, int page) {
+    const int b = min(st * kStage + block_w, last);
+    const uint8_t* src = (const uint8_t*)(pool + (size_t)pg_block(c, __builtin_amdgcn_readfirstlane(page), h, b) *
+                                                     (kPgBlock * D));
+    uint8_t* dst = &lds[buf][block_w][w & 1][0];
 #pragma unroll
-  for (int x = 0; x < Q; x++) {
-    const int row = min(mine + x * 32 + col, t.rows - 1), i = row / a.g;
-    sees[x] = t.sees0 + i;
+    for (int i = 0; i < kBytes / 1024; i++) pg_copy_to_lds<false>(src + i * 1024 + lane * 16, dst + i * 1024);
+  };
+  int st = split, buf = 0, page = 0;
+  if (blocks > 0) {
+    copy(st, 0, page_of(st));
+    page = page_of(st + used);
+  }
+  // the stage's copies have come, from all waves, which are done with the one before; the next one's set out
+  auto arrive = [&]() {
+    pg_wait_copies<0>();
+    __syncthreads();
+    if (st + used < stages) copy(st + used, buf ^ 1, page);
+    page = page_of(st + 2 * used);
+  };
+
+  // queries, and the rows that the wave's columns see
+  uint4 qh[KS], ql[LO ? KS : 1];
+  const int mine = t.row0 + w * 32, row = min(mine + col, t.rows - 1), i = row / a.g, sees = t.sees0 + i;
+  int qe = 0;
+  {
     const long long at = (long long)(t.lo + i) * a.q.pos + (long long)(h * a.g + row % a.g) * a.q.head + G * 8;
-    int qe = 0;
     if constexpr (LO) {
       float v[KS][8], m = 0.0f;
 #pragma unroll
@@ -67,130 +80,79 @@ __global__ __launch_bounds__(kWaves * 64, 2) void k_pages_tiles(PgArgs a) {
       }
       qe = pg_split_exp(max_stage<32>(m));
 #pragma unroll
-      for (int k = 0; k < KS; k++) pg_split<T>(v[k], qe, &qh[x][k], &ql[x][k]);
+      for (int k = 0; k < KS; k++) pg_split<T>(v[k], qe, &qh[k], &ql[k]);
     } else {
 #pragma unroll
-      for (int k = 0; k < KS; k++) qh[x][k] = pg_query16<T>(a, at + k * 16);
+      for (int k = 0; k < KS; k++) qh[k] = pg_query16<T>(a, at + k * 16);
     }
-    f[x] = pg_factor(a, qe);
   }
-  const int least = t.sees0 + min(mine, t.rows - 1) / a.g;                     // rows that the wave's first column sees
-  const int most = t.sees0 + min(mine + 32 * Q - 1, t.rows - 1) / a.g;         // and its last
+  const float f = pg_factor(a, qe);
   const bool idle = mine >= t.rows;
-  const int len = t.sees0 + t.rows / a.g - 1;  // rows of the sequence
+  const int least = t.sees0 + min(mine, t.rows - 1) / a.g;             // rows that the wave's first column sees
+  const int most = idle ? 0 : t.sees0 + min(mine + 31, t.rows - 1) / a.g;  // and its last
+  const int len = t.sees0 + t.rows / a.g - 1;                          // rows of the sequence
 
-  float Sm[Q], M[Q], l[Q];  // the maximum as a sum of products, and times f; a lane's own sum
-  pg_f16 O[Q][U];
+  float Sm = kPgNone, M = kPgNone, l = 0.0f;  // the maximum as a sum of products, and times f; a lane's own sum
+  pg_f16 O[U];
 #pragma unroll
-  for (int x = 0; x < Q; x++) {
-    Sm[x] = kPgNone;
-    M[x] = kPgNone;
-    l[x] = 0.0f;
+  for (int u = 0; u < U; u++)
 #pragma unroll
-    for (int u = 0; u < U; u++)
-#pragma unroll
-      for (int i = 0; i < 16; i++) O[x][u][i] = 0.0f;
-  }
-  bool far = false;
-  float none = -__builtin_inff();
-  asm("" : "+s"(none));
+    for (int x = 0; x < 16; x++) O[u][x] = 0.0f;
 
-  // this split's stages: split, split + used, ..
-  const int* table = c.table + (size_t)t.s * c.max_pages;
-  const int block_w = w >> 1, last = blocks - 1, lb = c.lp - 5;
-  const uint16_t* pool = w & 1 ? c.v : c.k;
-  // wave w copies K (even) or V (odd) of block w / 2 of a stage
-  auto page_of = [&](int st) { return pg_page(c, gmem(table)[min(st * kStage + block_w, last) >> lb]); };
-  auto stage = [&](int st, int buf, int page) {
-    const int b = min(st * kStage + block_w, last);
-    const uint8_t* src = (const uint8_t*)(pool + (size_t)pg_block(c, __builtin_amdgcn_readfirstlane(page), h, b) *
-                                                     (kPgBlock * D));
-    uint8_t* dst = &lds[buf][block_w][w & 1][0];
+  auto scores = [&](const uint8_t* kp, pg_f16& S) {
 #pragma unroll
-    for (int i = 0; i < kBytes / 1024; i++)
-      pg_copy_to_lds(src + i * 1024 + lane * 16, dst + i * 1024);
-  };
-
-  auto block = [&](auto masked, const uint8_t* kp, const uint8_t* vp, int b) {
-    constexpr bool MASKED = decltype(masked)::value;
-    pg_f16 S[Q];
-#pragma unroll
-    for (int x = 0; x < Q; x++)
-#pragma unroll
-      for (int i = 0; i < 16; i++) S[x][i] = 0.0f;
+    for (int x = 0; x < 16; x++) S[x] = 0.0f;
 #pragma unroll
     for (int k = 0; k < KS; k++) {
       const uint4 ka = *reinterpret_cast<const uint4*>(kp + k * 1024 + lane * 16);
-#pragma unroll
-      for (int x = 0; x < Q; x++) {
-        S[x] = pg_mfma<T>(ka, qh[x][k], S[x]);
-        if constexpr (LO) S[x] = pg_mfma<T>(ka, ql[x][k], S[x]);
-      }
+      S = pg_mfma<T>(ka, qh[k], S);
+      if constexpr (LO) S = pg_mfma<T>(ka, ql[k], S);
     }
-    if constexpr (MASKED) {
+  };
+  // A block's weights, and their sum. Of 16 bits the sum is that of the rounded ones, a pair to an instruction.
+  auto weights = [&](auto far, const pg_f16& S, uint4* ph, uint4* pl, float sum) {
 #pragma unroll
-      for (int x = 0; x < Q; x++)
+    for (int s2 = 0; s2 < 2; s2++) {
+      uint32_t hi[4], lo[4];
 #pragma unroll
-        for (int i = 0; i < 16; i++)
-          if (b * kPgBlock + 8 * (i / 4) + 4 * G + i % 4 >= sees[x]) S[x][i] = -__builtin_inff();
-    }
-    float mx[Q];
-    bool move = false;
+      for (int j = 0; j < 4; j++) {
+        float p[2];
 #pragma unroll
-    for (int x = 0; x < Q; x++) {
-      mx[x] = none;
-#pragma unroll
-      for (int i = 0; i < 16; i++) mx[x] = __builtin_fmaxf(mx[x], S[x][i]);
-      move |= __builtin_fmaf(mx[x], f[x], -M[x]) > kPgSlack;
-    }
-    if (__any(move)) {
-#pragma unroll
-      for (int x = 0; x < Q; x++) {
-        const float m = __builtin_fmaxf(Sm[x], max_stage<32>(mx[x]));
-        const float al = __builtin_amdgcn_exp2f((Sm[x] - m) * f[x]);
-        Sm[x] = m;
-        M[x] = __builtin_fmaxf(m * f[x], kPgNone);  // finite where nothing is seen yet
-        far |= __any(__builtin_fabsf(M[x]) > kPgFar && m > kPgNone);
-        l[x] *= al;
-#pragma unroll
-        for (int u = 0; u < U; u++)
-#pragma unroll
-          for (int i = 0; i < 16; i++) O[x][u][i] *= al;
-      }
-    }
-    uint4 ph[Q][2], pl[Q][LO ? 2 : 1];
-    auto weights = [&](auto is_far) {
-#pragma unroll
-      for (int x = 0; x < Q; x++)
-#pragma unroll
-        for (int s2 = 0; s2 < 2; s2++) {
-          uint32_t hi[4], lo[4];
-#pragma unroll
-          for (int j = 0; j < 4; j++) {
-            float p[2];
-#pragma unroll
-            for (int z = 0; z < 2; z++) {
-              const float sc = S[x][s2 * 8 + j * 2 + z];
-              p[z] = __builtin_amdgcn_exp2f(decltype(is_far)::value ? (sc - Sm[x]) * f[x]
-                                                                    : __builtin_fmaf(sc, f[x], -M[x]));
-              l[x] += p[z];
-            }
-            hi[j] = pg_pack<T>(p[0], p[1]);
-            if constexpr (LO) {
-              const pg_f2 back = pg_unpack<T>(hi[j]);
-              lo[j] = pg_pack<T>(p[0] - back.x, p[1] - back.y);
-            }
-          }
-          ph[x][s2] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-          if constexpr (LO) pl[x][s2] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+        for (int z = 0; z < 2; z++) {
+          const float sc = S[s2 * 8 + j * 2 + z];
+          p[z] = __builtin_amdgcn_exp2f(decltype(far)::value ? (sc - Sm) * f : __builtin_fmaf(sc, f, -M));
         }
-    };
-    if (far) weights(std::true_type{});
-    else weights(std::false_type{});
+        hi[j] = pg_pack<T>(p[0], p[1]);
+        if constexpr (LO) {
+          const pg_f2 back = pg_unpack<T>(hi[j]);
+          lo[j] = pg_pack<T>(p[0] - back.x, p[1] - back.y);
+          sum += p[0];
+          sum += p[1];
+        } else {
+          sum = pg_add<T>(hi[j], sum);
+        }
+      }
+      ph[s2] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+      if constexpr (LO) pl[s2] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+    }
+    return sum;
+  };
+  auto rescale = [&](float m) {
+    const float al = __builtin_amdgcn_exp2f((Sm - m) * f);
+    Sm = m;
+    M = __builtin_fmaxf(m * f, kPgNone);  // finite where nothing is seen yet
+    l *= al;
+#pragma unroll
+    for (int u = 0; u < U; u++)
+#pragma unroll
+      for (int x = 0; x < 16; x++) O[u][x] *= al;
+  };
+  auto is_far = [&](float m) { return __any(__builtin_fabsf(m * f) > kPgFar && m > kPgNone); };
+  auto outputs = [&](auto masked, const uint8_t* vp, const uint4* ph, const uint4* pl, int b) {
 #pragma unroll
     for (int s2 = 0; s2 < 2; s2++) {
       uint32_t keep[4];  // memory behind the sequence's rows may hold anything, and 0 times that would be NaN
-      if constexpr (MASKED) {
+      if constexpr (decltype(masked)::value) {
 #pragma unroll
         for (int j = 0; j < 4; j++) {
           const int at = b * kPgBlock + 16 * s2 + 4 * G + j % 2 * 2 + j / 2 * 8;
@@ -200,64 +162,92 @@ __global__ __launch_bounds__(kWaves * 64, 2) void k_pages_tiles(PgArgs a) {
 #pragma unroll
       for (int u = 0; u < U; u++) {
         uint4 va = *reinterpret_cast<const uint4*>(vp + ((2 * s2 + G) * D + 32 * u + col) * 16);
-        if constexpr (MASKED) va = make_uint4(va.x & keep[0], va.y & keep[1], va.z & keep[2], va.w & keep[3]);
-#pragma unroll
-        for (int x = 0; x < Q; x++) {
-          O[x][u] = pg_mfma<T>(va, ph[x][s2], O[x][u]);
-          if constexpr (LO) O[x][u] = pg_mfma<T>(va, pl[x][s2], O[x][u]);
-        }
+        if constexpr (decltype(masked)::value)
+          va = make_uint4(va.x & keep[0], va.y & keep[1], va.z & keep[2], va.w & keep[3]);
+        O[u] = pg_mfma<T>(va, ph[s2], O[u]);
+        if constexpr (LO) O[u] = pg_mfma<T>(va, pl[s2], O[u]);
       }
     }
   };
 
-  if (blocks > 0) {
-    int page = page_of(split);
-    stage(split, 0, page);
-    page = page_of(split + used);
-    for (int st = split, buf = 0; st < stages; st += used, buf ^= 1) {
-      __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): this wave's part of the stage has come
-      __syncthreads();
-      if (st + used < stages) stage(st + used, buf ^ 1, page);
-      page = page_of(st + 2 * used);
-#pragma unroll 1
-      for (int j = 0; j < kStage; j++) {
-        const int b = st * kStage + j;
-        if (!idle && b * kPgBlock < most) {
-          if ((b + 1) * kPgBlock > least) block(std::true_type{}, lds[buf][j][0], lds[buf][j][1], b);
-          else block(std::false_type{}, lds[buf][j][0], lds[buf][j][1], b);
-        }
+  // Stages that all columns of the wave see whole. Weights come before any maximum is looked at: only where their sum says
+  // that one is above 2^8 or so, the maximum moves and they are taken again. Scores far from 0 are left to what follows.
+  bool arrived = false;
+  for (const int full = min(stages, max(least, 0) / (kStage * kPgBlock)); st < full; st += used, buf ^= 1) {
+    arrive();
+    pg_f16 S[kStage];
+    uint4 ph[kStage][2], pl[kStage][LO ? 2 : 1];
+#pragma unroll
+    for (int j = 0; j < kStage; j++) scores(lds[buf][j][0], S[j]);
+    float sum = 0.0f;
+#pragma unroll
+    for (int j = 0; j < kStage; j++) sum = weights(std::false_type{}, S[j], ph[j], pl[j], sum);
+    if (__any(!(sum <= 256.0f))) {
+      float m = -__builtin_inff();
+#pragma unroll
+      for (int j = 0; j < kStage; j++)
+#pragma unroll
+        for (int x = 0; x < 16; x++) m = __builtin_fmaxf(m, S[j][x]);
+      m = __builtin_fmaxf(Sm, max_stage<32>(m));
+      if (is_far(m)) {
+        arrived = true;
+        break;
       }
+      rescale(m);
+      sum = 0.0f;
+#pragma unroll
+      for (int j = 0; j < kStage; j++) sum = weights(std::false_type{}, S[j], ph[j], pl[j], sum);
+    }
+    l += sum;
+#pragma unroll
+    for (int j = 0; j < kStage; j++) outputs(std::false_type{}, lds[buf][j][1], ph[j], pl[j], 0);
+  }
+  // The others, and all that comes after scores far from 0: differences of scores before products.
+  for (; st < stages; st += used, buf ^= 1) {
+    if (!arrived) arrive();
+    arrived = false;
+#pragma unroll 1
+    for (int j = 0; j < kStage; j++) {
+      const int b = st * kStage + j;
+      if (b * kPgBlock >= most) break;
+      pg_f16 S;
+      uint4 ph[2], pl[LO ? 2 : 1];
+      scores(lds[buf][j][0], S);
+      float m = -__builtin_inff();
+#pragma unroll
+      for (int x = 0; x < 16; x++) {
+        if (b * kPgBlock + 8 * (x / 4) + 4 * G + x % 4 >= sees) S[x] = -__builtin_inff();
+        m = __builtin_fmaxf(m, S[x]);
+      }
+      m = __builtin_fmaxf(Sm, max_stage<32>(m));
+      if (__any(m > Sm)) rescale(m);
+      l = weights(std::true_type{}, S, ph, pl, l);
+      outputs(std::true_type{}, lds[buf][j][1], ph, pl, b);
     }
   }
   if (idle) return;
+  l += partner<32>(l);
+  if (mine + col >= t.rows) return;
+  if (used == 1) {
+    const float inv = sees > 0 ? 1.0f / l : 0.0f;
+    const long long at = (long long)(t.lo + i) * a.out.pos + (long long)(h * a.g + row % a.g) * a.out.head + 4 * G;
 #pragma unroll
-  for (int x = 0; x < Q; x++) {
-    const int row = mine + x * 32 + col;
-    const float sum = l[x] + partner<32>(l[x]);
-    if (row >= t.rows) continue;
-    const int i = row / a.g;
-    if (used == 1) {
-      const float inv = sees[x] > 0 ? 1.0f / sum : 0.0f;
-      const long long at = (long long)(t.lo + i) * a.out.pos + (long long)(h * a.g + row % a.g) * a.out.head + 4 * G;
+    for (int u = 0; u < U; u++)
 #pragma unroll
-      for (int u = 0; u < U; u++)
+      for (int r = 0; r < 4; r++) {
+        const float o[4] = {O[u][4 * r] * inv, O[u][4 * r + 1] * inv, O[u][4 * r + 2] * inv, O[u][4 * r + 3] * inv};
+        pg_store<T, 4>(a, at + 32 * u + 8 * r, o);
+      }
+  } else {
+    const size_t wc = (((size_t)h * a.tiles + y) * W + (row - t.row0)) * a.splits + split;
+    float* po = a.part + wc * D + 4 * G;
 #pragma unroll
-        for (int r = 0; r < 4; r++) {
-          const float o[4] = {O[x][u][4 * r] * inv, O[x][u][4 * r + 1] * inv, O[x][u][4 * r + 2] * inv,
-                              O[x][u][4 * r + 3] * inv};
-          pg_store<T, 4>(a, at + 32 * u + 8 * r, o);
-        }
-    } else {
-      const size_t wc = (((size_t)h * a.tiles + y) * W + (row - t.row0)) * a.splits + split;
-      float* po = a.part + wc * D + 4 * G;
+    for (int u = 0; u < U; u++)
 #pragma unroll
-      for (int u = 0; u < U; u++)
-#pragma unroll
-        for (int r = 0; r < 4; r++)
-          *reinterpret_cast<pg_f4*>(po + 32 * u + 8 * r) =
-              pg_f4{O[x][u][4 * r], O[x][u][4 * r + 1], O[x][u][4 * r + 2], O[x][u][4 * r + 3]};
-      if (G == 0) a.ml[wc] = make_float2(M[x], sum);
-    }
+      for (int r = 0; r < 4; r++)
+        *reinterpret_cast<pg_f4*>(po + 32 * u + 8 * r) =
+            pg_f4{O[u][4 * r], O[u][4 * r + 1], O[u][4 * r + 2], O[u][4 * r + 3]};
+    if (G == 0) a.ml[wc] = make_float2(M, l);
   }
 }
 
@@ -266,7 +256,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void k_pages_tiles(PgArgs a) {
 hipError_t launch_pages_tiles(hipStream_t s, PgArgs a) {
   const unsigned grid = (unsigned)a.tiles * a.c.kvh * a.splits;
 #define TILES(DD, TT) \
-  if (a.c.d == DD && a.q.f16 == TT) klaunch(k_pages_tiles<DD, TT, 1>, grid, kWaves * 64, 0, s, a);
+  if (a.c.d == DD && a.q.f16 == TT) klaunch(k_pages_tiles<DD, TT>, grid, kWaves * 64, 0, s, a);
   TILES(64, 0) TILES(64, 1) TILES(64, 2) TILES(128, 0) TILES(128, 1) TILES(128, 2)
 #undef TILES
   return hipGetLastError();
