@@ -1,6 +1,6 @@
 // Attention of many rows over the paged 16-bit K/V cache (pages.h), on the matrix cores with f32 sums.
 //
-// A row is one query head at one position; the rows of a KV head's group, position by position, go in tiles of 128 Q, 32 Q
+// A row is one query head at one position; the rows of a KV head's group, position by position, go in tiles of 128, 32
 // to each of four waves. Per block of 32 positions of the cache, for 32 rows:
 //   S = K Q^T    MFMA 32x32x16, rows = positions, columns = rows of the tile
 //   softmax      p = 2^(S f - M), f = scale log2 e. The running maximum M moves only where it has to (a weight above
@@ -19,13 +19,21 @@ namespace moert {
 namespace {
 
 constexpr int kWaves = 4;
-constexpr int kStage = 2;  // blocks staged together
+
+// Blocks of a stage, stages in LDS, and waves to a SIMD. Wide heads of 16 bits fit three waves with one block to a stage
+// (twelve prompts of 128: 355 us, with two blocks and two waves 377); f32 would spill there.
+template <int D, int T>
+struct Shape {
+  static constexpr bool kTight = D == 128 && T != PG_F32;
+  static constexpr int kStage = kTight ? 1 : 2, kStages = kTight ? 3 : 2, kPerSimd = D == 64 || kTight ? 3 : 2;
+};
 
 template <int D, int T>
-__global__ __launch_bounds__(kWaves * 64, D == 64 ? 3 : 2) void k_pages_tiles(PgArgs a) {
+__global__ __launch_bounds__(kWaves * 64, (Shape<D, T>::kPerSimd)) void k_pages_tiles(PgArgs a) {
+  constexpr int kStage = Shape<D, T>::kStage, NB = Shape<D, T>::kStages;
   constexpr int KS = D / 16, U = D / 32, W = 32 * kWaves, kBytes = 64 * D;  // of a block of K or V
   constexpr bool LO = T == PG_F32;  // queries and weights as two fp16
-  __shared__ __align__(16) uint8_t lds[2][kStage][2][kBytes];
+  __shared__ __align__(16) uint8_t lds[NB][kStage][2][kBytes];
   const PagesDev& c = a.c;
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 31, G = lane >> 5;
   // the tiles of a KV head run on one XCD (workgroups go round them in turn) where there are eight of them, the last ones
@@ -38,30 +46,35 @@ __global__ __launch_bounds__(kWaves * 64, D == 64 ? 3 : 2) void k_pages_tiles(Pg
   const int stages = (blocks + kStage - 1) / kStage, used = pg_tiles_used(a, blocks);
   if (split >= used) return;
 
-  // this split's stages: split, split + used, ..; wave w copies K (even) or V (odd) of block w / 2 of a stage
+  // this split's stages: split, split + used, ..; each wave copies a quarter of one. Lane x holds the place in the pool of
+  // the wave's block of the x-th of 64
+  constexpr int kPart = kStage * 2 * kBytes / kWaves, kCopies = kPart / 1024;
   const int* table = c.table + (size_t)t.s * c.max_pages;
-  const int block_w = w >> 1, last = blocks - 1, lb = c.lp - 5;
-  const uint16_t* pool = w & 1 ? c.v : c.k;
-  auto page_of = [&](int st) { return pg_page(c, gmem(table)[min(st * kStage + block_w, last) >> lb]); };
-  auto copy = [&](int st, int buf, int page) {
-    const int b = min(st * kStage + block_w, last);
-    const uint8_t* src = (const uint8_t*)(pool + (size_t)pg_block(c, __builtin_amdgcn_readfirstlane(page), h, b) *
-                                                     (kPgBlock * D));
-    uint8_t* dst = &lds[buf][block_w][w & 1][0];
+  const int from = w * kPart, block_w = from / (2 * kBytes), in_w = from % kBytes, last = blocks - 1;
+  const uint8_t* pool = (const uint8_t*)(from / kBytes % 2 ? c.v : c.k) + in_w + lane * 16;
+  const int count = max(0, (stages - split + used - 1) / used);
+  int place = 0;
+  auto copy = [&](int x) {
+    if (x % 64 == 0) {
+      const int b = min((split + (x + lane) * used) * kStage + block_w, last);
+      place = pg_block(c, pg_page(c, gmem(table)[b >> (c.lp - 5)]), h, b);
+    }
+    const uint8_t* src = pool + (size_t)__builtin_amdgcn_readlane(place, x % 64) * kBytes;
+    uint8_t* dst = &lds[0][0][0][0] + x % NB * (kStage * 2 * kBytes) + from;
 #pragma unroll
-    for (int i = 0; i < kBytes / 1024; i++) pg_copy_to_lds<false>(src + i * 1024 + lane * 16, dst + i * 1024);
+    for (int i = 0; i < kCopies; i++) pg_copy_to_lds<false>(src + i * 1024, dst + i * 1024);
   };
-  int st = split, buf = 0, page = 0;
-  if (blocks > 0) {
-    copy(st, 0, page_of(st));
-    page = page_of(st + used);
-  }
-  // the stage's copies have come, from all waves, which are done with the one before; the next one's set out
-  auto arrive = [&]() {
-    pg_wait_copies<0>();
-    __syncthreads();
-    if (st + used < stages) copy(st + used, buf ^ 1, page);
-    page = page_of(st + 2 * used);
+#pragma unroll
+  for (int x = 0; x < NB - 1; x++)
+    if (x < count) copy(x);
+  // the x-th stage's copies have come, from all waves, which are done with the one before; another one's set out
+  auto arrive = [&](int x) {
+    if (x + NB - 1 <= count) pg_wait_copies<(NB - 2) * kCopies>();
+    else pg_wait_copies<0>();
+    pg_wait_reads();
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" : : : "memory");
+    if (x + NB - 1 < count) copy(x + NB - 1);
   };
 
   // queries, and the rows that the wave's columns see
@@ -102,15 +115,18 @@ __global__ __launch_bounds__(kWaves * 64, D == 64 ? 3 : 2) void k_pages_tiles(Pg
   auto scores = [&](const uint8_t* kp, pg_f16& S) {
 #pragma unroll
     for (int x = 0; x < 16; x++) S[x] = 0.0f;
+    uint4 ka[KS];
+#pragma unroll
+    for (int k = 0; k < KS; k++) ka[k] = *reinterpret_cast<const uint4*>(kp + k * 1024 + lane * 16);
 #pragma unroll
     for (int k = 0; k < KS; k++) {
-      const uint4 ka = *reinterpret_cast<const uint4*>(kp + k * 1024 + lane * 16);
-      S = pg_mfma<T>(ka, qh[k], S);
-      if constexpr (LO) S = pg_mfma<T>(ka, ql[k], S);
+      S = pg_mfma<T>(ka[k], qh[k], S);
+      if constexpr (LO) S = pg_mfma<T>(ka[k], ql[k], S);
     }
   };
   // A block's weights, and their sum. Of 16 bits the sum is that of the rounded ones, a pair to an instruction.
   auto weights = [&](auto far, const pg_f16& S, uint4* ph, uint4* pl, float sum) {
+    float part[4] = {sum, 0.0f, 0.0f, 0.0f};  // sums that do not wait for each other
 #pragma unroll
     for (int s2 = 0; s2 < 2; s2++) {
       uint32_t hi[4], lo[4];
@@ -126,16 +142,16 @@ __global__ __launch_bounds__(kWaves * 64, D == 64 ? 3 : 2) void k_pages_tiles(Pg
         if constexpr (LO) {
           const pg_f2 back = pg_unpack<T>(hi[j]);
           lo[j] = pg_pack<T>(p[0] - back.x, p[1] - back.y);
-          sum += p[0];
-          sum += p[1];
+          part[j] += p[0];
+          part[j] += p[1];
         } else {
-          sum = pg_add<T>(hi[j], sum);
+          part[j] = pg_add<T>(hi[j], part[j]);
         }
       }
       ph[s2] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
       if constexpr (LO) pl[s2] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
     }
-    return sum;
+    return (part[0] + part[1]) + (part[2] + part[3]);
   };
   auto rescale = [&](float m) {
     const float al = __builtin_amdgcn_exp2f((Sm - m) * f);
@@ -173,12 +189,14 @@ __global__ __launch_bounds__(kWaves * 64, D == 64 ? 3 : 2) void k_pages_tiles(Pg
   // Stages that all columns of the wave see whole. Weights come before any maximum is looked at: only where their sum says
   // that one is above 2^8 or so, the maximum moves and they are taken again. Scores far from 0 are left to what follows.
   bool arrived = false;
-  for (const int full = min(stages, max(least, 0) / (kStage * kPgBlock)); st < full; st += used, buf ^= 1) {
-    arrive();
+  int x = 0, st = split;
+  for (const int full = min(stages, max(least, 0) / (kStage * kPgBlock)); st < full; st += used, x++) {
+    arrive(x);
+    uint8_t(*at)[2][kBytes] = lds[x % NB];
     pg_f16 S[kStage];
     uint4 ph[kStage][2], pl[kStage][LO ? 2 : 1];
 #pragma unroll
-    for (int j = 0; j < kStage; j++) scores(lds[buf][j][0], S[j]);
+    for (int j = 0; j < kStage; j++) scores(at[j][0], S[j]);
     float sum = 0.0f;
 #pragma unroll
     for (int j = 0; j < kStage; j++) sum = weights(std::false_type{}, S[j], ph[j], pl[j], sum);
@@ -200,11 +218,12 @@ __global__ __launch_bounds__(kWaves * 64, D == 64 ? 3 : 2) void k_pages_tiles(Pg
     }
     l += sum;
 #pragma unroll
-    for (int j = 0; j < kStage; j++) outputs(std::false_type{}, lds[buf][j][1], ph[j], pl[j], 0);
+    for (int j = 0; j < kStage; j++) outputs(std::false_type{}, at[j][1], ph[j], pl[j], 0);
   }
   // The others, and all that comes after scores far from 0: differences of scores before products.
-  for (; st < stages; st += used, buf ^= 1) {
-    if (!arrived) arrive();
+  for (; st < stages; st += used, x++) {
+    if (!arrived) arrive(x);
+    uint8_t(*at)[2][kBytes] = lds[x % NB];
     arrived = false;
 #pragma unroll 1
     for (int j = 0; j < kStage; j++) {
@@ -212,7 +231,7 @@ __global__ __launch_bounds__(kWaves * 64, D == 64 ? 3 : 2) void k_pages_tiles(Pg
       if (b * kPgBlock >= most) break;
       pg_f16 S;
       uint4 ph[2], pl[LO ? 2 : 1];
-      scores(lds[buf][j][0], S);
+      scores(at[j][0], S);
       float m = -__builtin_inff();
 #pragma unroll
       for (int x = 0; x < 16; x++) {
@@ -222,7 +241,7 @@ __global__ __launch_bounds__(kWaves * 64, D == 64 ? 3 : 2) void k_pages_tiles(Pg
       m = __builtin_fmaxf(Sm, max_stage<32>(m));
       if (__any(m > Sm)) rescale(m);
       l = weights(std::true_type{}, S, ph, pl, l);
-      outputs(std::true_type{}, lds[buf][j][1], ph, pl, b);
+      outputs(std::true_type{}, at[j][1], ph, pl, b);
     }
   }
   if (idle) return;
