@@ -17,11 +17,14 @@ PgArgs args(const PagesDev& c, int heads, float scale, KvRows q, KvRows out, con
   return a;
 }
 
-// Splits cost a second launch and the partials' way through memory: one workgroup for each of 256 compute units, and more
-// (up to 1024, four to a unit) only while a wave keeps 16 blocks of a full table; never fewer than 3 a wave.
+// Splits cost a second launch and the partials' way through memory, about what a wave takes for 7 blocks: none where a wave
+// of a full table keeps at most 24 (1000 of 1280 positions, 8 KV heads: 8.6 us without, 10.9 with 3; sixteen sequences of up
+// to 2000 of 2560: 13.7 without, 15.9 with 2; 4097 of 4608: 24.1 without, 11.5 with 12). Then one workgroup for each of 256
+// compute units, and more (up to 1024, four to a unit) only while a wave keeps 16 blocks; never fewer than 3 a wave. (131000
+// positions, 8 KV heads: 43.1 us with 64 splits, 44.1 with 32, 50.6 with 16.)
 int cols_splits(const PagesDev& c, long long units) {
-  const int blocks = c.max_pages << (c.lp - 5), cap = blocks / 12;
-  const int most = cap < 1 ? 1 : cap > kPgMaxSplits ? kPgMaxSplits : cap;
+  const int blocks = c.max_pages << (c.lp - 5), cap = blocks / 12, most = cap > kPgMaxSplits ? kPgMaxSplits : cap;
+  if (blocks <= 24 * 4) return 1;
   long long s = 256 / units > 1 ? 256 / units : 1;
   while (2 * s * units <= 1024 && blocks / (8 * s) >= 16) s *= 2;
   return (int)(s < most ? s : most);

@@ -125,10 +125,11 @@ __global__ __launch_bounds__(kWaves * 64, D == 64 ? 2 : 1) void k_pages_cols(PgA
     for (int z = 0; z < 8; z++) mx = __builtin_fmaxf(mx, S[z / 4][z % 4]);
     if (__any(__builtin_fmaf(mx, f, -M) > kPgSlack)) {
       const float m = __builtin_fmaxf(Sm, max_stage<32>(max_stage<16>(mx)));
-      const float al = __builtin_amdgcn_exp2f((Sm - m) * f);
+      const float to = __builtin_fmaxf(m * f, kPgNone);  // finite where nothing is seen yet
+      far |= __any(__builtin_fabsf(to) > kPgFar && m > kPgNone);
+      const float al = __builtin_amdgcn_exp2f(far ? (Sm - m) * f : M - to);  // as the weights were taken
       Sm = m;
-      M = __builtin_fmaxf(m * f, kPgNone);  // finite where nothing is seen yet
-      far |= __any(__builtin_fabsf(M) > kPgFar && m > kPgNone);
+      M = to;
       l *= al;
 #pragma unroll
       for (int u = 0; u < U; u++) O[u] *= al;
@@ -218,67 +219,94 @@ __global__ __launch_bounds__(kWaves * 64, D == 64 ? 2 : 1) void k_pages_cols(PgA
   }
 }
 
-// The splits' shares of a tile's rows. C = 4: a workgroup to a row, its waves take every fourth split; C = 1, up to 8 splits:
-// 16 rows to a workgroup, a wave takes one at a time. All products are asked for at once and before it is known which
-// splits have any: the others lie in the workspace too, and are not looked at.
-template <int D, int T, int W, int C>
-__global__ __launch_bounds__(256) void k_pages_join(PgArgs a, int groups) {
-  constexpr int E = D / 64, N = C == 4 ? kPgMaxSplits / 4 : 8, R = C == 4 ? 1 : 4;
+// The splits' shares of a row, more than 8 of them: a workgroup to a row, its waves take every fourth split. All products
+// are asked for at once and before it is known which splits have any: the others lie in the workspace too, and are not
+// looked at.
+template <int D, int T, int W>
+__global__ __launch_bounds__(256) void k_pages_join(PgArgs a, int rows) {
+  constexpr int E = D / 64, N = kPgMaxSplits / 4;
   __shared__ float Os[4][D];
   const PagesDev& c = a.c;
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int id = blockIdx.x, h = id % c.kvh, x0 = id / c.kvh % groups * (C == 4 ? 1 : 16) + (C == 4 ? 0 : w * R);
-  const int y = id / c.kvh / groups, s0 = C == 4 ? w : 0;
-  const size_t row0 = ((size_t)h * a.tiles + y) * W + x0;
-  float2 ml[R];
-  float p[R][N][E];
+  const int id = blockIdx.x, h = id % c.kvh, x = id / c.kvh % rows, y = id / c.kvh / rows;
+  const size_t wc = (((size_t)h * a.tiles + y) * W + x) * a.splits;
+  const float2 ml = a.ml[wc + min(lane, a.splits - 1)];
+  float p[N][E];
 #pragma unroll
-  for (int i = 0; i < R; i++) {
-    ml[i] = a.ml[(row0 + i) * a.splits + min(lane, a.splits - 1)];
+  for (int j = 0; j < N; j++)
 #pragma unroll
-    for (int j = 0; j < N; j++)
-#pragma unroll
-      for (int e = 0; e < E; e++)
-        if (s0 + C * j < a.splits) p[i][j][e] = gmem(a.part)[((row0 + i) * a.splits + s0 + C * j) * D + e * 64 + lane];
-  }
+    for (int e = 0; e < E; e++)
+      if (w + 4 * j < a.splits) p[j][e] = gmem(a.part)[(wc + w + 4 * j) * D + e * 64 + lane];
   PgTile t;
   if (!pg_tile(a, y, W, &t)) return;
   const int blocks = tile_blocks(a, t, W), used = W == 16 ? cols_used(a, blocks) : pg_tiles_used(a, blocks);
-  if (used == 1) return;
+  const int r = t.row0 + x;
+  if (used == 1 || r >= t.rows) return;
+  const float m = group_max(lane < used ? ml.x : kPgNone);
+  const float al = lane < used ? __builtin_amdgcn_exp2f(ml.x - m) : 0.0f;
+  const float sum = group_sum(lane < used ? ml.y * al : 0.0f);
+  float o[E] = {};
 #pragma unroll
-  for (int i = 0; i < R; i++) {
-    const int r = t.row0 + x0 + i;
-    if (r >= t.rows) return;
-    const float m = group_max(lane < used ? ml[i].x : kPgNone);
-    const float al = lane < used ? __builtin_amdgcn_exp2f(ml[i].x - m) : 0.0f;
-    const float sum = group_sum(lane < used ? ml[i].y * al : 0.0f);
-    float o[E] = {};
+  for (int j = 0; j < N; j++) {
+    const int s = w + 4 * j;
+    if (s < used) {
+      const float f = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(al), s));
 #pragma unroll
-    for (int j = 0; j < N; j++) {
-      const int s = s0 + C * j;
-      if (s < used) {
-        const float f = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(al), s));
-#pragma unroll
-        for (int e = 0; e < E; e++) o[e] = __builtin_fmaf(p[i][j][e], f, o[e]);
-      }
-    }
-    if constexpr (C == 4) {
-#pragma unroll
-      for (int e = 0; e < E; e++) Os[w][e * 64 + lane] = o[e];
-      __syncthreads();
-      if (w) return;
-#pragma unroll
-      for (int e = 0; e < E; e++)
-        o[e] = (o[e] + Os[1][e * 64 + lane]) + (Os[2][e * 64 + lane] + Os[3][e * 64 + lane]);
-    }
-    const float inv = t.sees0 + r / a.g > 0 ? 1.0f / sum : 0.0f;
-    const long long at = (long long)(t.lo + r / a.g) * a.out.pos + (long long)(h * a.g + r % a.g) * a.out.head + lane;
-#pragma unroll
-    for (int e = 0; e < E; e++) {
-      if constexpr (T == PG_F32) ((float*)a.out.p)[at + e * 64] = o[e] * inv;
-      else ((uint16_t*)a.out.p)[at + e * 64] = (uint16_t)pg_pack<T>(pg_clip<T>(o[e] * inv), 0.0f);
+      for (int e = 0; e < E; e++) o[e] = __builtin_fmaf(p[j][e], f, o[e]);
     }
   }
+#pragma unroll
+  for (int e = 0; e < E; e++) Os[w][e * 64 + lane] = o[e];
+  __syncthreads();
+  if (w) return;
+  const float inv = t.sees0 + r / a.g > 0 ? 1.0f / sum : 0.0f;
+  const long long at = (long long)(t.lo + r / a.g) * a.out.pos + (long long)(h * a.g + r % a.g) * a.out.head + lane;
+#pragma unroll
+  for (int e = 0; e < E; e++) {
+    const float v = ((o[e] + Os[1][e * 64 + lane]) + (Os[2][e * 64 + lane] + Os[3][e * 64 + lane])) * inv;
+    if constexpr (T == PG_F32) ((float*)a.out.p)[at + e * 64] = v;
+    else ((uint16_t*)a.out.p)[at + e * 64] = (uint16_t)pg_pack<T>(pg_clip<T>(v), 0.0f);
+  }
+}
+
+// The same for up to 8 splits: a lane to four elements of a row, 1024 / D rows to a workgroup.
+template <int D, int T, int W>
+__global__ __launch_bounds__(256) void k_pages_join_few(PgArgs a, int rows) {
+  constexpr int L = D / 4, R = 256 / L, N = 8;
+  const PagesDev& c = a.c;
+  const int per = (rows + R - 1) / R, id = blockIdx.x, h = id % c.kvh, y = id / c.kvh / per;
+  const int x = id / c.kvh % per * R + threadIdx.x / L, e = threadIdx.x % L * 4;
+  const size_t wc = (((size_t)h * a.tiles + y) * W + min(x, W - 1)) * a.splits;
+  float2 ml[N];
+  float4 p[N];
+#pragma unroll
+  for (int j = 0; j < N; j++)
+    if (j < a.splits) {
+      ml[j] = a.ml[wc + j];
+      p[j] = gload_f4(a.part + (wc + j) * D + e);
+    }
+  PgTile t;
+  if (!pg_tile(a, y, W, &t)) return;
+  const int blocks = tile_blocks(a, t, W), used = W == 16 ? cols_used(a, blocks) : pg_tiles_used(a, blocks);
+  const int r = t.row0 + x;
+  if (used == 1 || x >= rows || r >= t.rows) return;
+  float m = ml[0].x;
+#pragma unroll
+  for (int j = 1; j < N; j++)
+    if (j < used) m = __builtin_fmaxf(m, ml[j].x);
+  float sum = 0.0f, o[4] = {};
+#pragma unroll
+  for (int j = 0; j < N; j++)
+    if (j < used) {
+      const float al = __builtin_amdgcn_exp2f(ml[j].x - m);
+      sum = __builtin_fmaf(ml[j].y, al, sum);
+      o[0] = __builtin_fmaf(p[j].x, al, o[0]), o[1] = __builtin_fmaf(p[j].y, al, o[1]);
+      o[2] = __builtin_fmaf(p[j].z, al, o[2]), o[3] = __builtin_fmaf(p[j].w, al, o[3]);
+    }
+  const float inv = t.sees0 + r / a.g > 0 ? 1.0f / sum : 0.0f;
+#pragma unroll
+  for (int i = 0; i < 4; i++) o[i] *= inv;
+  pg_store<T, 4>(a, (long long)(t.lo + r / a.g) * a.out.pos + (long long)(h * a.g + r % a.g) * a.out.head + e, o);
 }
 
 }  // namespace
@@ -303,12 +331,14 @@ hipError_t launch_pages_cols(hipStream_t s, PgArgs a) {
 
 hipError_t launch_pages_join(hipStream_t s, PgArgs a, int width) {
   const int rows = a.most > 1 || a.g > width ? width : a.g;  // of one position there are no more
-  const int wide = a.splits > 8, groups = wide ? rows : (rows + 15) / 16;
-  const unsigned grid = (unsigned)a.tiles * a.c.kvh * groups;
-#define JOIN(DD, TT, WW, CC) \
-  if (a.c.d == DD && a.q.f16 == TT && width == WW && wide == (CC == 4)) \
-    klaunch(k_pages_join<DD, TT, WW, CC>, grid, 256, 0, s, a, groups);
-#define JOINS(DD, TT) JOIN(DD, TT, 16, 1) JOIN(DD, TT, 16, 4) JOIN(DD, TT, 128, 1) JOIN(DD, TT, 128, 4)
+  const int per = a.splits > 8 ? rows : (rows * a.c.d / 4 + 255) / 256;
+  const unsigned grid = (unsigned)a.tiles * a.c.kvh * per;
+#define JOIN(DD, TT, WW)                                                                 \
+  if (a.c.d == DD && a.q.f16 == TT && width == WW) {                                     \
+    if (a.splits > 8) klaunch(k_pages_join<DD, TT, WW>, grid, 256, 0, s, a, rows);       \
+    else klaunch(k_pages_join_few<DD, TT, WW>, grid, 256, 0, s, a, rows);                \
+  }
+#define JOINS(DD, TT) JOIN(DD, TT, 16) JOIN(DD, TT, 128)
   JOINS(64, 0) JOINS(64, 1) JOINS(64, 2) JOINS(128, 0) JOINS(128, 1) JOINS(128, 2)
 #undef JOINS
 #undef JOIN

@@ -105,7 +105,7 @@ __global__ __launch_bounds__(kWaves * 64, (Shape<D, T>::kPerSimd)) void k_pages_
   const int most = idle ? 0 : t.sees0 + min(mine + 31, t.rows - 1) / a.g;  // and its last
   const int len = t.sees0 + t.rows / a.g - 1;                          // rows of the sequence
 
-  float Sm = kPgNone, M = kPgNone, l = 0.0f;  // the maximum as a sum of products, and times f; a lane's own sum
+  float Sm = kPgNone, M = kPgNone, rest = 0.0f, l = 0.0f;  // the maximum as a sum of products, and times f; a lane's own sum
   pg_f16 O[U];
 #pragma unroll
   for (int u = 0; u < U; u++)
@@ -136,7 +136,7 @@ __global__ __launch_bounds__(kWaves * 64, (Shape<D, T>::kPerSimd)) void k_pages_
 #pragma unroll
         for (int z = 0; z < 2; z++) {
           const float sc = S[s2 * 8 + j * 2 + z];
-          p[z] = __builtin_amdgcn_exp2f(decltype(far)::value ? (sc - Sm) * f : __builtin_fmaf(sc, f, -M));
+          p[z] = __builtin_amdgcn_exp2f(decltype(far)::value ? __builtin_fmaf(sc - Sm, f, rest) : __builtin_fmaf(sc, f, -M));
         }
         hi[j] = pg_pack<T>(p[0], p[1]);
         if constexpr (LO) {
@@ -153,10 +153,15 @@ __global__ __launch_bounds__(kWaves * 64, (Shape<D, T>::kPerSimd)) void k_pages_
     }
     return (part[0] + part[1]) + (part[2] + part[3]);
   };
+  // Moves the maximum to m. Weights are taken of S f - M, M rounded, and so is what they are multiplied by; far from 0,
+  // where that rounding is more than a small part of a weight, of (S - Sm) f: rest is 0 there, and otherwise Sm f - M.
   auto rescale = [&](float m) {
-    const float al = __builtin_amdgcn_exp2f((Sm - m) * f);
+    const float to = __builtin_fmaxf(m * f, kPgNone);  // finite where nothing is seen yet
+    const bool far = __builtin_fabsf(to) > kPgFar;
+    const float al = __builtin_amdgcn_exp2f(far ? (Sm - m) * f : M - to);
     Sm = m;
-    M = __builtin_fmaxf(m * f, kPgNone);  // finite where nothing is seen yet
+    M = to;
+    rest = far ? 0.0f : __builtin_fmaf(m, f, -to);
     l *= al;
 #pragma unroll
     for (int u = 0; u < U; u++)
