@@ -228,7 +228,8 @@ __device__ __forceinline__ bool pg_tile(const PgArgs& a, int y, int w, PgTile* t
   t->rows = n * a.g;
   t->row0 = (y - first) * w;
   t->sees0 = pg_seen(a.c, s) - n + 1;
-  return n >= a.least && n <= a.most && t->row0 < t->rows;
+  // starts that do not begin at 0, or fall, leave tiles before the sequence's first
+  return n >= a.least && n <= a.most && t->row0 >= 0 && t->row0 < t->rows;
 }
 // Tiles that a batch may have.
 inline int pg_tiles(const PgArgs& a, int w) {

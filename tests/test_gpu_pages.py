@@ -506,3 +506,40 @@ def test_calls_of_no_rows(hip):
     dev.append(z, z, [0], F32)
     dev.prompt(z, 0.125, F32, [0, 0, 0])
     assert dev.attend(z, 0.125, F32, starts=[0, 0, 0]).size == 0
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+def test_rows_before_the_first_sequence(hip, dtype):
+    """Starts that begin behind rows of no sequence: those stay as they were."""
+    rng = np.random.default_rng(25)
+    for n, before in ((200, 100), (9, 40), (1, 7)):
+        dev, ref = both(hip, 3, 2, 64, 32, 40, 12, dtype=cache_type(dtype))
+        step(dev, ref, rng, [n, 0, n + 3], dtype)
+        starts = before + np.array([0, n, n, 2 * n + 3])
+        q, x = queries(rng, dtype, starts[-1] + 5, 6, 64)
+        pu.check(dev.prompt(q, 0.125, dtype, starts), ref.attend(x, starts, 0.125, dtype), dtype)
+        starts = before + np.array([0, 1, 1, 2])
+        pu.check(dev.attend(q, 0.125, dtype, starts=starts), ref.attend(x, starts, 0.125, dtype), dtype)
+
+
+@pytest.mark.parametrize("tokens", [3, 40, 700])
+def test_broken_starts_write_nothing_outside_the_rows(hip, tokens):
+    """Known bytes before and behind the outputs of a batch, in whose starts is anything."""
+    rng = np.random.default_rng(tokens)
+    dev, ref = both(hip, 9, 2, 64, 32, 40, 30)
+    k = pu.to_bits(normal(rng, 40 * 32, 2, 64), F16)
+    dev.append(k, k, np.arange(40 * 32), F16)
+    dev.set("table", rng.integers(0, 40, 9 * 30))
+    dev.set("state", np.stack([rng.integers(0, 960, 9), np.zeros(9), np.zeros(9), np.zeros(9)], 1))
+    pad, row = 5000 * 4 * 64, 4 * 64
+    ws, size = dev.workspace(4, tokens)
+    q = hip.upload(pu.to_bits(normal(rng, tokens * row + 2 * pad), F16)) + 2 * pad
+    for i in range(12):
+        starts = rng.choice([-2 ** 31, -1, 0, 1, 2, tokens // 2, tokens - 1, tokens, tokens + 1, 2 ** 31 - 1], 10)
+        out = hip.upload(np.full(tokens * row + 2 * pad, 0x4321, np.uint16))
+        at = hip.upload(starts.astype(np.int32))
+        dev.c.prompt(q, out + 2 * pad, 4, 0.125, at, tokens, ws, size)
+        dev.c.attend(q, out + 2 * pad, 4, 0.125, ws, size, starts=at, tokens=tokens)
+        hip.sync()
+        got = hip.get(out, (tokens * row + 2 * pad,), np.uint16)
+        assert (got[:pad] == 0x4321).all() and (got[-pad:] == 0x4321).all()
