@@ -43,9 +43,10 @@ int tiles_splits(const PagesDev& c, long long units) {
 }
 
 // Whether the tiles of 16 rows that the waves of a workgroup share do better than those of 128 rows that they split: up to
-// 32 rows of a sequence on average. (One sequence of 4000 positions, 8 KV heads of 64, 3 query heads: 24 rows 12.0 us in the
-// one, 17.5 in the other; of 32000, 33 rows: 23.3 and 22.2; 64 of 1000, of 128, 44 rows: 60.0 and 53.5.)
-bool few_rows(const PgArgs& a) { return (long long)a.tokens * a.g <= 32ll * a.c.seqs; }
+// 48 rows of a sequence on average, of wide heads 32. (8 KV heads of 64, 48 rows: 4000 positions 11.4 us in the one, 14.1 in
+// the other, 32000 25.5 and 21.7, of eight sequences of 4000 17.5 and 23.4; of 128, 32 rows: 12.4 and 18.8, 33.5 and 30.5,
+// 25.5 and 30.3, but 44 rows of 64 sequences of 1000 59.3 and 42.5.)
+bool few_rows(const PgArgs& a) { return (long long)a.tokens * a.g <= (a.c.d == 64 ? 48ll : 32ll) * a.c.seqs; }
 
 size_t up(size_t x) { return (x + 255) / 256 * 256; }
 size_t share_bytes(const PagesDev& c, size_t rows) { return up(rows * 8) + up(rows * c.d * 4); }

@@ -49,19 +49,17 @@ __global__ __launch_bounds__(kWaves * 64, D == 64 ? 2 : 1) void k_pages_cols(PgA
   // this wave's blocks: b0, b0 + step, ..; lane x holds the place in the pool of the x-th of 64
   const int b0 = split * kWaves + w, step = a.splits * kWaves, count = max(0, (blocks - b0 + step - 1) / step);
   const int* table = c.table + (size_t)t.s * c.max_pages;
+  const uint32_t into = pg_lds(ring[w]);
   int place = 0;
   auto fetch = [&](int x) {
     if (x % 64 == 0) {
       const int b = min(b0 + (x + lane) * step, blocks - 1);
       place = pg_block(c, pg_page(c, gmem(table)[b >> (c.lp - 5)]), h, b);
     }
-    const size_t at = (size_t)__builtin_amdgcn_readlane(place, x % 64) * kBytes + lane * 16;
-    uint8_t* to = &ring[w][x % RING][0][0];
-#pragma unroll
-    for (int i = 0; i < kCopies / 2; i++) pg_copy_to_lds<STREAM>((const uint8_t*)c.k + at + i * 1024, to + i * 1024);
-#pragma unroll
-    for (int i = 0; i < kCopies / 2; i++)
-      pg_copy_to_lds<STREAM>((const uint8_t*)c.v + at + i * 1024, to + kBytes + i * 1024);
+    const size_t at = (size_t)__builtin_amdgcn_readlane(place, x % 64) * kBytes;
+    const uint32_t to = into + x % RING * (2 * kBytes);
+    pg_copy_to_lds<kCopies / 2, STREAM>((const uint8_t*)c.k + at, lane * 16, to);
+    pg_copy_to_lds<kCopies / 2, STREAM>((const uint8_t*)c.v + at, lane * 16, to + kBytes);
   };
 #pragma unroll
   for (int x = 0; x < RING; x++)

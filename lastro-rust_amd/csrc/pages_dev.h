@@ -107,17 +107,41 @@ __device__ __forceinline__ uint4 pg_query16(const PgArgs& a, long long at) {
   return make_uint4(w[0] ^ flip, w[1] ^ flip, w[2] ^ flip, w[3] ^ flip);
 }
 
-// 16 bytes of each lane to LDS, in a row from `dst` (the wave's) on, without a way through registers. Not by the builtin:
-// the compiler cannot tell the buffer that is filled from the one being read, and would wait for the copy before each read.
+// N KB of memory to LDS, 16 bytes of each lane at a time, without a way through registers; `src` and `dst` (a place in LDS)
+// are the wave's, `lane` 16 times the lane. The instruction's offset counts on both sides. Not by the builtin: the
+// compiler cannot tell the buffer that is filled from the one being read, and would wait for the copy before each read.
 // Whoever reads them waits by pg_wait_copies first: for all but the last N copies and loads of the wave (loads of the
 // compiler's among them only make it wait for more). STREAM: with the non-temporal hint.
-template <bool STREAM>
-__device__ __forceinline__ void pg_copy_to_lds(const uint8_t* src, uint8_t* dst) {
-  const uint32_t at = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)dst);
-  if constexpr (STREAM)
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off nt" : : "s"(at), "v"(src) : "memory", "m0");
-  else
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(at), "v"(src) : "memory", "m0");
+template <int N, bool STREAM>
+__device__ __forceinline__ void pg_copy_to_lds(const uint8_t* src, uint32_t lane, uint32_t dst) {
+  if constexpr (N > 4) {
+    pg_copy_to_lds<4, STREAM>(src, lane, dst);
+    pg_copy_to_lds<N - 4, STREAM>(src + 4096, lane, dst + 4096);
+  } else {
+    static_assert(N == 2 || N == 4, "");
+    dst = __builtin_amdgcn_readfirstlane(dst);
+#define PG_COPY(HINT)                                                                                                \
+  if constexpr (N == 4)                                                                                              \
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" HINT                              \
+                 "\n\tglobal_load_lds_dwordx4 %1, %2 offset:1024" HINT                                              \
+                 "\n\tglobal_load_lds_dwordx4 %1, %2 offset:2048" HINT                                              \
+                 "\n\tglobal_load_lds_dwordx4 %1, %2 offset:3072" HINT                                              \
+                 : : "s"(dst), "v"(lane), "s"(src) : "memory", "m0");                                                \
+  else                                                                                                               \
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" HINT                              \
+                 "\n\tglobal_load_lds_dwordx4 %1, %2 offset:1024" HINT                                              \
+                 : : "s"(dst), "v"(lane), "s"(src) : "memory", "m0");
+    if constexpr (STREAM) {
+      PG_COPY(" nt")
+    } else {
+      PG_COPY("")
+    }
+#undef PG_COPY
+  }
+}
+// A place in LDS as a copy takes it.
+__device__ __forceinline__ uint32_t pg_lds(const void* p) {
+  return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)p;
 }
 template <int N>
 __device__ __forceinline__ void pg_wait_copies() {

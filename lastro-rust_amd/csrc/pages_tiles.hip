@@ -51,7 +51,8 @@ __global__ __launch_bounds__(kWaves * 64, (Shape<D, T>::kPerSimd)) void k_pages_
   constexpr int kPart = kStage * 2 * kBytes / kWaves, kCopies = kPart / 1024;
   const int* table = c.table + (size_t)t.s * c.max_pages;
   const int from = w * kPart, block_w = from / (2 * kBytes), in_w = from % kBytes, last = blocks - 1;
-  const uint8_t* pool = (const uint8_t*)(from / kBytes % 2 ? c.v : c.k) + in_w + lane * 16;
+  const uint8_t* pool = (const uint8_t*)(from / kBytes % 2 ? c.v : c.k) + in_w;
+  const uint32_t into = pg_lds(lds) + from;
   const int count = max(0, (stages - split + used - 1) / used);
   int place = 0;
   auto copy = [&](int x) {
@@ -60,9 +61,7 @@ __global__ __launch_bounds__(kWaves * 64, (Shape<D, T>::kPerSimd)) void k_pages_
       place = pg_block(c, pg_page(c, gmem(table)[b >> (c.lp - 5)]), h, b);
     }
     const uint8_t* src = pool + (size_t)__builtin_amdgcn_readlane(place, x % 64) * kBytes;
-    uint8_t* dst = &lds[0][0][0][0] + x % NB * (kStage * 2 * kBytes) + from;
-#pragma unroll
-    for (int i = 0; i < kCopies; i++) pg_copy_to_lds<false>(src + i * 1024, dst + i * 1024);
+    pg_copy_to_lds<kCopies, false>(src, lane * 16, into + x % NB * (kStage * 2 * kBytes));
   };
 #pragma unroll
   for (int x = 0; x < NB - 1; x++)

@@ -85,7 +85,7 @@ FORMS = [
     (case("attend", heads=16, tokens=4), ["cols", "join_few"]),
     (case("attend", cache=(4, 1, 64, 64, 500, 100), heads=4, tokens=4), ["cols", "join"]),
     (case("attend", cache=(4, 8, 64, 64, 500, 40), heads=16, tokens=4), ["cols"]),
-    (case("prompt", heads=16, tokens=40), ["cols", "join_few"]),
+    (case("prompt", heads=16, tokens=90), ["cols", "join_few"]),
     (case("prompt", cache=(1, 1, 128, 64, 500, 100), heads=4, tokens=8), ["cols", "join"]),
     (case("prompt", heads=16, tokens=400), ["tiles", "join_few"]),
     (case("prompt", cache=(1, 1, 128, 64, 500, 200), heads=4, tokens=50), ["tiles", "join"]),
