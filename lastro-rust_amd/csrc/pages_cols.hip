@@ -147,8 +147,7 @@ __global__ __launch_bounds__(kWaves * 64, D == 64 ? 2 : 1) void k_pages_cols(PgA
       l += pa;
       l += pb;
       hi[j] = pg_pack<T>(pa, pb);
-      const pg_f2 back = pg_unpack<T>(hi[j]);
-      lo[j] = pg_pack<T>(pa - back.x, pb - back.y);
+      lo[j] = pg_rest<T>(hi[j], pa, pb);
     }
     const uint4 ph = make_uint4(hi[0], hi[1], hi[2], hi[3]), pl = make_uint4(lo[0], lo[1], lo[2], lo[3]);
     uint32_t keep[4];  // memory behind the sequence's rows may hold anything, and 0 times that would be NaN

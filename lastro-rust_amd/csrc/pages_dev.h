@@ -30,11 +30,15 @@ __device__ __forceinline__ uint32_t pg_pack(float a, float b) {
   if constexpr (T == PG_BF16) return __builtin_bit_cast(uint32_t, __builtin_convertvector(x, pg_b2));
   else return __builtin_bit_cast(uint32_t, __builtin_convertvector(x, pg_h2));
 }
-// The two numbers of a pair, as floats.
+// What rounding to the pair `w` has left of a and b, as a pair.
 template <int T>
-__device__ __forceinline__ pg_f2 pg_unpack(uint32_t w) {
-  if constexpr (T == PG_BF16) return pg_f2{__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)};
-  else return __builtin_convertvector(__builtin_bit_cast(pg_h2, w), pg_f2);
+__device__ __forceinline__ uint32_t pg_rest(uint32_t w, float a, float b) {
+  if constexpr (T == PG_BF16) {
+    return pg_pack<T>(a - __uint_as_float(w << 16), b - __uint_as_float(w & 0xffff0000u));
+  } else {
+    const pg_h2 h = __builtin_bit_cast(pg_h2, w);
+    return pg_pack<T>(a - (float)h.x, b - (float)h.y);
+  }
 }
 
 // x + a pair's sum.
@@ -164,8 +168,7 @@ __device__ __forceinline__ void pg_split(const float* x, int e, uint4* hi, uint4
     const float p = __builtin_amdgcn_ldexpf(__builtin_amdgcn_ldexpf(x[2 * j], e1), e2);
     const float q = __builtin_amdgcn_ldexpf(__builtin_amdgcn_ldexpf(x[2 * j + 1], e1), e2);
     h[j] = pg_pack<T>(p, q);
-    const pg_f2 back = pg_unpack<T>(h[j]);
-    l[j] = pg_pack<T>(p - back.x, q - back.y);
+    l[j] = pg_rest<T>(h[j], p, q);
   }
   *hi = make_uint4(h[0], h[1], h[2], h[3]);
   *lo = make_uint4(l[0], l[1], l[2], l[3]);

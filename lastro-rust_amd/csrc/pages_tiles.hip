@@ -139,8 +139,7 @@ __global__ __launch_bounds__(kWaves * 64, (Shape<D, T>::kPerSimd)) void k_pages_
         }
         hi[j] = pg_pack<T>(p[0], p[1]);
         if constexpr (LO) {
-          const pg_f2 back = pg_unpack<T>(hi[j]);
-          lo[j] = pg_pack<T>(p[0] - back.x, p[1] - back.y);
+          lo[j] = pg_rest<T>(hi[j], p[0], p[1]);
           part[j] += p[0];
           part[j] += p[1];
         } else {
@@ -202,9 +201,13 @@ __global__ __launch_bounds__(kWaves * 64, (Shape<D, T>::kPerSimd)) void k_pages_
 #pragma unroll
     for (int j = 0; j < kStage; j++) scores(at[j][0], S[j]);
     float sum = 0.0f;
+    bool move = x == 0;  // there is no maximum yet
+    if (!move) {
 #pragma unroll
-    for (int j = 0; j < kStage; j++) sum = weights(std::false_type{}, S[j], ph[j], pl[j], sum);
-    if (__any(!(sum <= 256.0f))) {
+      for (int j = 0; j < kStage; j++) sum = weights(std::false_type{}, S[j], ph[j], pl[j], sum);
+      move = __any(!(sum <= 256.0f));
+    }
+    if (move) {
       float m = -__builtin_inff();
 #pragma unroll
       for (int j = 0; j < kStage; j++)

@@ -543,3 +543,59 @@ def test_broken_starts_write_nothing_outside_the_rows(hip, tokens):
         hip.sync()
         got = hip.get(out, (tokens * row + 2 * pad,), np.uint16)
         assert (got[:pad] == 0x4321).all() and (got[-pad:] == 0x4321).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("q_strides,out_strides", [((4 * 64 + 1, 64), (4 * 64, 64)), ((4 * 64, 64), (300, 67)),
+                                                   ((-4 * 64, 64), (64, 64 * 50))])
+def test_strides_of_queries_and_outputs(hip, dtype, q_strides, out_strides):
+    """Each with its own, of one position and of prompts."""
+    rng = np.random.default_rng(27)
+    n, heads, d, item = 46, 4, 64, 4 if dtype == F32 else 2
+    dev, ref = both(hip, 3, 2, d, 32, 12, 8, dtype=cache_type(dtype))
+    starts = step(dev, ref, rng, [40, 5, 1], dtype)
+
+    def places(strides):
+        first = max(0, -strides[0]) * n
+        return first, first + np.arange(n)[:, None, None] * strides[0] + np.arange(heads)[None, :, None] * strides[1] + np.arange(d)
+
+    (q0, q_at), (o0, o_at) = places(q_strides), places(out_strides)
+    q = pu.to_bits(normal(rng, q_at.max() + 9, scale=2.0), dtype)
+    ws, size = dev.workspace(heads, n)
+    for call, which in (("prompt", lambda m: m >= 1), ("attend", lambda m: m == 1)):
+        out = np.full(o_at.max() + 9, pu.untouched(dtype))
+        at = hip.upload(out)
+        kw = dict(starts=hip.upload(starts.astype(np.int32)), tokens=n, ws=ws, ws_bytes=size, dtype=dtype,
+                  q_strides=q_strides, out_strides=out_strides)
+        getattr(dev.c, call)(hip.upload(q) + q0 * item, at + o0 * item, heads, 0.125, **kw)
+        hip.sync()
+        got = hip.get(at, out.shape, out.dtype)
+        pu.check(got[o_at], ref.attend(pu.from_bits(q[q_at], dtype), starts, 0.125, dtype, which), dtype)
+        rest = np.ones(out.size, bool)
+        rest[o_at.reshape(-1)] = False
+        assert (got[rest] == pu.untouched(dtype)).all()
+
+
+@pytest.mark.parametrize("new", [3, 40])
+def test_prompts_of_many_sequences(hip, new):
+    """More sequences than a wave looks at together, many of them without rows: few rows each, and more."""
+    rng = np.random.default_rng(new)
+    S = 150
+    dev, ref = both(hip, S, 1, 64, 32, 400, 5)
+    step(dev, ref, rng, rng.integers(0, 40, S), F16)
+    counts = np.where(rng.random(S) < 0.5, 0, rng.integers(1, new + 1, S))
+    starts = step(dev, ref, rng, counts, F16, tokens=int(counts.sum()) + 9)
+    q, x = queries(rng, F16, int(counts.sum()) + 9, 3, 64)
+    pu.check(dev.prompt(q, 0.125, F16, starts), ref.attend(x, starts, 0.125, F16), F16)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_a_batch_in_which_one_sequence_is_long(hip, dtype):
+    """Few rows on average, but one prompt among single rows, and the other way round: whatever the choice, the same."""
+    rng = np.random.default_rng(29)
+    dev, ref = both(hip, 20, 1, 64, 32, 60, 20, dtype=cache_type(dtype))
+    step(dev, ref, rng, [20] * 20, dtype)
+    for new in ([300] + [1] * 19, [1] * 19 + [100]):
+        starts = step(dev, ref, rng, new, dtype)
+        q, x = queries(rng, dtype, sum(new), 2, 64)
+        pu.check(dev.prompt(q, 0.125, dtype, starts), ref.attend(x, starts, 0.125, dtype), dtype)
