@@ -7,7 +7,7 @@
 //   S = K Q^T    MFMA 16x16x32, rows = positions, columns = rows of the tile. Row i of product x is position
 //                16 (i / 8) + 8 x + i % 8, so that a lane of group G = lane / 16 gets the 8 positions that lie side by
 //                side in V: 16 (G / 2) + 4 (G % 2) + 0 .. 3, and 8 on.
-//   softmax      p = 2^(S f - M), f = scale log2 e; the running maximum M moves only for weights above 2^8.
+//   softmax      p = 2^(S f - M), f = scale log2 e; M, the running maximum less 7, moves only for weights above 2^15.
 //   O += V^T P^T MFMA 16x16x32, rows = elements; p, as two numbers of the cache's type, never leaves its lane.
 #include <type_traits>
 
@@ -123,7 +123,7 @@ __global__ __launch_bounds__(kWaves * 64, D == 64 ? 2 : 1) void k_pages_cols(PgA
     for (int z = 0; z < 8; z++) mx = __builtin_fmaxf(mx, S[z / 4][z % 4]);
     if (__any(__builtin_fmaf(mx, f, -M) > kPgSlack)) {
       const float m = __builtin_fmaxf(Sm, max_stage<32>(max_stage<16>(mx)));
-      const float to = __builtin_fmaxf(m * f, kPgNone);  // finite where nothing is seen yet
+      const float to = __builtin_fmaxf(__builtin_fmaf(m, f, -kPgShift), kPgNone);  // finite where nothing is seen yet
       far |= __any(__builtin_fabsf(to) > kPgFar && m > kPgNone);
       const float al = __builtin_amdgcn_exp2f(far ? (Sm - m) * f : M - to);  // as the weights were taken
       Sm = m;
@@ -135,7 +135,7 @@ __global__ __launch_bounds__(kWaves * 64, D == 64 ? 2 : 1) void k_pages_cols(PgA
     float x[8];
     if (far) {
 #pragma unroll
-      for (int z = 0; z < 8; z++) x[z] = (S[z / 4][z % 4] - Sm) * f;
+      for (int z = 0; z < 8; z++) x[z] = __builtin_fmaf(S[z / 4][z % 4] - Sm, f, kPgShift);
     } else {
 #pragma unroll
       for (int z = 0; z < 8; z++) x[z] = __builtin_fmaf(S[z / 4][z % 4], f, -M);

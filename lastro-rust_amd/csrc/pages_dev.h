@@ -19,7 +19,9 @@ typedef float pg_f4 __attribute__((ext_vector_type(4)));
 typedef float pg_f16 __attribute__((ext_vector_type(16)));
 
 constexpr float kPgNone = -3.4e38f;  // maximum of what has no score yet; finite, so that differences with it are
-constexpr float kPgSlack = 8.0f;     // log2 of how far a weight may lie above 1 before the maximum moves
+// Weights are 2^7 for the maximum that they are taken of, which moves only for weights above 2^15: fp16 has 11 bits for them
+// down to 2^-21 of the largest, and stops at 2^-31.
+constexpr float kPgShift = 7.0f, kPgSlack = 15.0f;
 constexpr float kPgFar = 1048576.0f;  // scores beyond it lose 2^-5 in a product less a maximum: differences come first
 constexpr int kPgMaxSplits = 64;     // one lane each in the combine
 constexpr float kPgLog2e = 1.44269504088896341f;

@@ -3,8 +3,8 @@
 // A row is one query head at one position; the rows of a KV head's group, position by position, go in tiles of 128, 32
 // to each of four waves. Per block of 32 positions of the cache, for 32 rows:
 //   S = K Q^T    MFMA 32x32x16, rows = positions, columns = rows of the tile
-//   softmax      p = 2^(S f - M), f = scale log2 e. The running maximum M moves only where it has to (a weight above
-//                2^8), so most blocks cost no exchange between lanes and leave O alone.
+//   softmax      p = 2^(S f - M), f = scale log2 e. M, the running maximum less 7, moves only where it has to (a weight
+//                above 2^15), so most blocks cost no exchange between lanes and leave O alone.
 //   O += V^T P^T MFMA 32x32x16, rows = elements. A lane of S holds, of its column, the positions 8 (r / 4) + 4 (lane / 32)
 //                + r % 4, which is what it has to hold of P here when V's positions are taken in that order: V lies so in
 //                the pool, and p never leaves its lane.
@@ -152,14 +152,14 @@ __global__ __launch_bounds__(kWaves * 64, (Shape<D, T>::kPerSimd)) void k_pages_
     return (part[0] + part[1]) + (part[2] + part[3]);
   };
   // Moves the maximum to m. Weights are taken of S f - M, M rounded, and so is what they are multiplied by; far from 0,
-  // where that rounding is more than a small part of a weight, of (S - Sm) f: rest is 0 there, and otherwise Sm f - M.
+  // where that rounding is more than a small part of a weight, of (S - Sm) f + 7: rest is 7 there, and otherwise Sm f - M.
   auto rescale = [&](float m) {
-    const float to = __builtin_fmaxf(m * f, kPgNone);  // finite where nothing is seen yet
+    const float to = __builtin_fmaxf(__builtin_fmaf(m, f, -kPgShift), kPgNone);  // finite where nothing is seen yet
     const bool far = __builtin_fabsf(to) > kPgFar;
     const float al = __builtin_amdgcn_exp2f(far ? (Sm - m) * f : M - to);
     Sm = m;
     M = to;
-    rest = far ? 0.0f : __builtin_fmaf(m, f, -to);
+    rest = far ? kPgShift : __builtin_fmaf(m, f, -to);
     l *= al;
 #pragma unroll
     for (int u = 0; u < U; u++)
@@ -190,7 +190,7 @@ __global__ __launch_bounds__(kWaves * 64, (Shape<D, T>::kPerSimd)) void k_pages_
   };
 
   // Stages that all columns of the wave see whole. Weights come before any maximum is looked at: only where their sum says
-  // that one is above 2^8 or so, the maximum moves and they are taken again. Scores far from 0 are left to what follows.
+  // that one is above 2^15 or so, the maximum moves and they are taken again. Scores far from 0 are left to what follows.
   bool arrived = false;
   int x = 0, st = split;
   for (const int full = min(stages, max(least, 0) / (kStage * kPgBlock)); st < full; st += used, x++) {
@@ -205,7 +205,7 @@ __global__ __launch_bounds__(kWaves * 64, (Shape<D, T>::kPerSimd)) void k_pages_
     if (!move) {
 #pragma unroll
       for (int j = 0; j < kStage; j++) sum = weights(std::false_type{}, S[j], ph[j], pl[j], sum);
-      move = __any(!(sum <= 256.0f));
+      move = __any(!(sum <= 32768.0f));
     }
     if (move) {
       float m = -__builtin_inff();
