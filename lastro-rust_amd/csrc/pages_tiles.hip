@@ -123,9 +123,9 @@ __global__ __launch_bounds__(kWaves * 64, (Shape<D, T>::kPerSimd)) void k_pages_
       if constexpr (LO) S = pg_mfma<T>(ka[k], ql[k], S);
     }
   };
-  // A block's weights, and their sum. Of 16 bits the sum is that of the rounded ones, a pair to an instruction.
-  auto weights = [&](auto far, const pg_f16& S, uint4* ph, uint4* pl, float sum) {
-    float part[4] = {sum, 0.0f, 0.0f, 0.0f};  // sums that do not wait for each other
+  // A block's weights; part takes their sums, two that do not wait for each other. Of 16 bits they are those of the rounded
+  // ones, a pair to an instruction.
+  auto weights = [&](auto far, const pg_f16& S, uint4* ph, uint4* pl, float* part) {
 #pragma unroll
     for (int s2 = 0; s2 < 2; s2++) {
       uint32_t hi[4], lo[4];
@@ -140,16 +140,15 @@ __global__ __launch_bounds__(kWaves * 64, (Shape<D, T>::kPerSimd)) void k_pages_
         hi[j] = pg_pack<T>(p[0], p[1]);
         if constexpr (LO) {
           lo[j] = pg_rest<T>(hi[j], p[0], p[1]);
-          part[j] += p[0];
-          part[j] += p[1];
+          part[0] += p[0];
+          part[1] += p[1];
         } else {
-          part[j] = pg_add<T>(hi[j], part[j]);
+          part[j % 2] = pg_add<T>(hi[j], part[j % 2]);
         }
       }
       ph[s2] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
       if constexpr (LO) pl[s2] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
     }
-    return (part[0] + part[1]) + (part[2] + part[3]);
   };
   // Moves the maximum to m. Weights are taken of S f - M, M rounded, and so is what they are multiplied by; far from 0,
   // where that rounding is more than a small part of a weight, of (S - Sm) f + 7: rest is 7 there, and otherwise Sm f - M.
@@ -200,12 +199,12 @@ __global__ __launch_bounds__(kWaves * 64, (Shape<D, T>::kPerSimd)) void k_pages_
     uint4 ph[kStage][2], pl[kStage][LO ? 2 : 1];
 #pragma unroll
     for (int j = 0; j < kStage; j++) scores(at[j][0], S[j]);
-    float sum = 0.0f;
+    float part[2] = {0.0f, 0.0f};
     bool move = x == 0;  // there is no maximum yet
     if (!move) {
 #pragma unroll
-      for (int j = 0; j < kStage; j++) sum = weights(std::false_type{}, S[j], ph[j], pl[j], sum);
-      move = __any(!(sum <= 32768.0f));
+      for (int j = 0; j < kStage; j++) weights(std::false_type{}, S[j], ph[j], pl[j], part);
+      move = __any(!(part[0] + part[1] <= 32768.0f));
     }
     if (move) {
       float m = -__builtin_inff();
@@ -219,11 +218,11 @@ __global__ __launch_bounds__(kWaves * 64, (Shape<D, T>::kPerSimd)) void k_pages_
         break;
       }
       rescale(m);
-      sum = 0.0f;
+      part[0] = part[1] = 0.0f;
 #pragma unroll
-      for (int j = 0; j < kStage; j++) sum = weights(std::false_type{}, S[j], ph[j], pl[j], sum);
+      for (int j = 0; j < kStage; j++) weights(std::false_type{}, S[j], ph[j], pl[j], part);
     }
-    l += sum;
+    l += part[0] + part[1];
 #pragma unroll
     for (int j = 0; j < kStage; j++) outputs(std::false_type{}, at[j][1], ph[j], pl[j], 0);
   }
@@ -247,7 +246,9 @@ __global__ __launch_bounds__(kWaves * 64, (Shape<D, T>::kPerSimd)) void k_pages_
       }
       m = __builtin_fmaxf(Sm, max_stage<32>(m));
       if (__any(m > Sm)) rescale(m);
-      l = weights(std::true_type{}, S, ph, pl, l);
+      float part[2] = {0.0f, 0.0f};
+      weights(std::true_type{}, S, ph, pl, part);
+      l += part[0] + part[1];
       outputs(std::true_type{}, at[j][1], ph, pl, b);
     }
   }
