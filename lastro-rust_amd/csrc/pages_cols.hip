@@ -2,13 +2,21 @@
 // splits.
 //
 // A row is one query head at one position; the rows of a KV head's group, position by position, go in tiles of 16. The
-// waves of a workgroup take the blocks of 32 positions in turn, straight from memory into registers, and join in LDS;
+// waves of a workgroup take the blocks of 32 positions in turn, each for itself, and join in LDS;
 // where tiles are too few for the device several workgroups share one (splits) and a second launch joins them. Per block:
 //   S = K Q^T    MFMA 16x16x32, rows = positions, columns = rows of the tile. Row i of product x is position
 //                16 (i / 8) + 8 x + i % 8, so that a lane of group G = lane / 16 gets the 8 positions that lie side by
 //                side in V: 16 (G / 2) + 4 (G % 2) + 0 .. 3, and 8 on.
 //   softmax      p = 2^(S f - M), f = scale log2 e; M, the running maximum less 7, moves only for weights above 2^15.
 //   O += V^T P^T MFMA 16x16x32, rows = elements; p, as two numbers of the cache's type, never leaves its lane.
+// A wave's blocks go to its own ring in LDS, one being worked on while the next is on its way; nobody waits for another
+// wave. (Straight into registers, where the compiler kept one in flight, 131000 positions of 8 KV heads of 64 took 87 us for
+// 39.)
+//
+// What bounds it, measured on one MI355X: the cache's bytes. 973 MB of 43 sequences (8 KV heads of 128, bf16) in 146 us, 6.6
+// TB/s (a copy of 1 GiB reaches 5.2, reading and writing); 268 MB of one in 39, part of it from the last-level cache. Short
+// caches: launches and four loads that wait for each other (4.6 us for 100 rows). Reads of K take two turns in LDS for one
+// (rows 8 apart share banks), a third of its cycles, which nothing waits for.
 #include <type_traits>
 
 #include "pages_dev.h"
