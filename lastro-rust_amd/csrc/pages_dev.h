@@ -126,17 +126,17 @@ __device__ __forceinline__ void pg_copy_to_lds(const uint8_t* src, uint32_t lane
   } else {
     static_assert(N == 2 || N == 4, "");
     dst = __builtin_amdgcn_readfirstlane(dst);
-#define PG_COPY(HINT)                                                                                                \
-  if constexpr (N == 4)                                                                                              \
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" HINT                              \
-                 "\n\tglobal_load_lds_dwordx4 %1, %2 offset:1024" HINT                                              \
-                 "\n\tglobal_load_lds_dwordx4 %1, %2 offset:2048" HINT                                              \
-                 "\n\tglobal_load_lds_dwordx4 %1, %2 offset:3072" HINT                                              \
-                 : : "s"(dst), "v"(lane), "s"(src) : "memory", "m0");                                                \
-  else                                                                                                               \
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" HINT                              \
-                 "\n\tglobal_load_lds_dwordx4 %1, %2 offset:1024" HINT                                              \
-                 : : "s"(dst), "v"(lane), "s"(src) : "memory", "m0");
+#define PG_COPY(HINT)                                                                                        \
+  if constexpr (N == 4)                                                                                      \
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" HINT                      \
+                 "\n\tglobal_load_lds_dwordx4 %1, %2 offset:%3" HINT                                        \
+                 "\n\tglobal_load_lds_dwordx4 %1, %2 offset:%4" HINT                                        \
+                 "\n\tglobal_load_lds_dwordx4 %1, %2 offset:%5" HINT                                        \
+                 : : "s"(dst), "v"(lane), "s"(src), "n"(1 * 1024), "n"(2 * 1024), "n"(3 * 1024) : "memory", "m0"); \
+  else                                                                                                       \
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" HINT                      \
+                 "\n\tglobal_load_lds_dwordx4 %1, %2 offset:%3" HINT                                        \
+                 : : "s"(dst), "v"(lane), "s"(src), "n"(1 * 1024) : "memory", "m0");
     if constexpr (STREAM) {
       PG_COPY(" nt")
     } else {
@@ -175,9 +175,11 @@ __device__ __forceinline__ void pg_split(const float* x, int e, uint4* hi, uint4
   *hi = make_uint4(h[0], h[1], h[2], h[3]);
   *lo = make_uint4(l[0], l[1], l[2], l[3]);
 }
-// What a sum of products is multiplied by; never 0: what is masked has to stay -inf.
+// What a sum of products is multiplied by. Never 0: what is masked has to stay -inf. Nor infinite, where it leaves f32
+// without the scores (of keys that are small): sums that differ do so by 2^-58 or more there, and 2^127 of that is all the
+// weight or none, as more of it would be.
 __device__ __forceinline__ float pg_factor(const PgArgs& a, int qe) {
-  return __builtin_fmaxf(__builtin_amdgcn_ldexpf(a.kf, a.ke + qe), 0x1p-126f);
+  return __builtin_fminf(__builtin_fmaxf(__builtin_amdgcn_ldexpf(a.kf, a.ke + qe), 0x1p-126f), 0x1p127f);
 }
 
 // An output is a mean of fp16 values: what roundings bring beyond the largest of them is cut.

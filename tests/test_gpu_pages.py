@@ -599,3 +599,202 @@ def test_a_batch_in_which_one_sequence_is_long(hip, dtype):
         starts = step(dev, ref, rng, new, dtype)
         q, x = queries(rng, dtype, sum(new), 2, 64)
         pu.check(dev.prompt(q, 0.125, dtype, starts), ref.attend(x, starts, 0.125, dtype), dtype)
+
+
+# ---- scores of any size ----------------------------------------------------------------------------------------------
+def one_sequence(hip, dtype, k, v, max_pages=None):
+    """A cache of one sequence with the given rows (f32 values)."""
+    rows, H, d = k.shape
+    pages = -(-rows // 64)
+    dev, ref = both(hip, 1, H, d, 64, pages, max_pages or pages, dtype=cache_type(dtype))
+    step(dev, ref, np.random.default_rng(0), [rows], dtype, k=k.astype(np.float32), v=v.astype(np.float32))
+    return dev, ref
+
+
+def both_ways(dev, q, scale, dtype):
+    """The last positions' outputs, of prompts of few rows and of many (with the queries behind others), and of the last
+    position alone."""
+    n = q.shape[0]
+    yield n, dev.prompt(q, scale, dtype, [0, n])
+    more = np.concatenate([np.repeat(q[:1], 60, 0), q])
+    yield n, dev.prompt(more, scale, dtype, [0, 60 + n])[60:]
+    yield 1, dev.attend(q[-1:], scale, dtype)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("max_pages", [11, 256])
+def test_scores_of_any_size(hip, dtype, max_pages):
+    """Scores of 10^4 to 10^30, far beyond the steps of exponents: all the weight on one row, or shared by every 37th in
+    equal parts."""
+    rng = np.random.default_rng(31)
+    d, rows, n = 64, 700, 12
+    v = normal(rng, rows, 2, d)
+    for every in (rows, 37):
+        k = np.zeros((rows, 2, d), np.float32)
+        k[..., 0], k[..., 1] = rng.integers(20, 100, (rows, 2)), 127.0
+        k[20::every, :, 0] = 127.0
+        dev, ref = one_sequence(hip, dtype, k, v, max_pages)
+        at = np.arange(20, rows, every)
+        for size in (1e4, 1e5, 1e6, 1e7, 1e9, 1e12, 1e30):
+            for sign in (1.0, -1.0):
+                q = np.zeros((n, 4, d), np.float32)
+                q[..., 0] = 16.0
+                if sign < 0:  # every score below 0, the same ones apart
+                    q[..., 1] = -32.0
+                for m, out in both_ways(dev, pu.to_bits(q, dtype), size / (16.0 * 127.0), dtype):
+                    for i in range(m):
+                        for a in range(4):
+                            x = ref.kv(0, a // 2, rows)[1][at[at < rows - m + 1 + i]]
+                            want = x.mean(0)
+                            # weights of one size, rounded alike; sums and products in f32, the output
+                            off = 2.0 ** -19 * np.abs(x).mean(0) + pu.HALF[dtype] * (np.abs(want) + 2.0 ** -13)
+                            if dtype == BF16:  # two numbers of 8 bits
+                                off = off + 2.0 ** -15 * np.abs(x).mean(0)
+                            err = np.abs(pu.from_bits(out, dtype)[i, a] - want)
+                            assert (err <= off).all(), (every, size, sign, m, i, a, (err / off).max())
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_scores_near_f32s_lowest(hip, dtype):
+    """Scores of about -1e36, apart by 1e34 and more: all the weight is on the least negative one that is seen."""
+    rng = np.random.default_rng(33)
+    d, rows = 64, 500
+    k, v = np.zeros((rows, 1, d)), normal(rng, rows, 1, d)
+    k[..., 0] = 127.0
+    k[340, 0, 0] = 100.0
+    dev, ref = one_sequence(hip, dtype, k, v)
+    q = np.zeros((9, 2, d), np.float32)
+    q[..., 0] = -1e34
+    want = ref.kv(0, 0, rows)[1][340]
+    for _, out in both_ways(dev, pu.to_bits(q, dtype), 1.0, dtype):
+        assert (np.abs(pu.from_bits(out, dtype) - want) <= (pu.HALF[dtype] + 2.0 ** -22) * np.abs(want)).all()
+
+
+def test_factors_of_a_score_that_leave_f32_together(hip):
+    """Queries of 3e38 beside keys of 1e-6, scales from 1e-30 to 1e36: the scores are numbers, whatever two of their
+    three factors make. All the weight is on the row of the largest one."""
+    rng = np.random.default_rng(35)
+    d, rows = 64, 300
+    k, v = np.zeros((rows, 1, d)), normal(rng, rows, 1, d)
+    k[..., 0] = rng.integers(1, 100, (rows, 1)) * 2.0 ** -20
+    k[130, 0, 0] = 127 * 2.0 ** -20
+    dev, ref = one_sequence(hip, F32, k, v)
+    want = ref.kv(0, 0, rows)[1][130]
+    for size, scale in ((3e38, 1e3), (3e38, 1.0), (3e38, 1e-30), (1e20, 1e15), (1e3, 1e36), (1e-3, 1e30)):
+        q = np.zeros((9, 2, d), np.float32)
+        q[..., 0] = size
+        for _, out in both_ways(dev, q, scale, F32):
+            assert (np.abs(out - want) <= 2.0 ** -20 * np.abs(want)).all(), (size, scale)
+
+
+@pytest.mark.parametrize("max_pages", [6, 200])
+def test_the_largest_values_stay_finite(hip, max_pages):
+    """V of fp16's largest magnitude, weights whose rounding to fp16 has one sign in all rows that count."""
+    d, rows = 64, 384
+    k, v = np.zeros((rows, 1, d)), np.full((rows, 1, d), 65504.0)
+    k[rows // 2:, :, 0] = 1.0
+    v[..., 1::2] = -65504.0
+    dev, ref = one_sequence(hip, F16, k, v, max_pages)
+    q = np.zeros((3, 64, d), np.float32)
+    q[..., 0] = 0.7 + np.arange(64) / 14.5
+    for m, out in both_ways(dev, pu.to_bits(q, F16), 1.0, F16):
+        got = pu.from_bits(out, F16)
+        assert np.isfinite(got).all() and (np.abs(got - v[0, 0]) <= 65504.0 * 2.0 ** -11).all()
+
+
+@pytest.mark.parametrize("size_q,size_k,size_v", [(2.0 ** -20, 1.0, 1.0), (1.0, 2.0 ** -20, 1.0), (1.0, 1.0, 2.0 ** -20),
+                                                  (2.0 ** -20,) * 3])
+@pytest.mark.parametrize("dtype", [F32, F16])
+def test_subnormal_fp16_counts(hip, dtype, size_q, size_k, size_v):
+    rng = np.random.default_rng(37)
+    rows, n = 200, 9
+    dev, ref = one_sequence(hip, dtype, normal(rng, rows, 2, 64, scale=size_k), normal(rng, rows, 2, 64, scale=size_v))
+    q = pu.to_bits(normal(rng, n, 6, 64, scale=size_q), dtype)
+    scale = float(np.float32(0.125 / (size_q * size_k)))
+    for m, out in both_ways(dev, q, scale, dtype):
+        want = ref.attend(pu.from_bits(q[-m:], dtype), [0, m], scale, dtype)
+        pu.check(out, want, dtype)
+
+
+# ---- more calls ------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+def test_outputs_in_place_of_the_queries(hip, dtype):
+    """out = q, of the same strides: every row of q is read before its output is written, with and without splits."""
+    rng = np.random.default_rng(39)
+    for max_pages in (20, 300):
+        dev, ref = both(hip, 2, 2, 64, 32, 60, max_pages, dtype=cache_type(dtype))
+        step(dev, ref, rng, [500, 333], dtype)
+        ws, size = dev.workspace(6, 400)
+        for starts in ([0, 5, 9], [0, 150, 300]):
+            q, _ = queries(rng, dtype, starts[-1], 6, 64)
+            want, at = dev.prompt(q, 0.125, dtype, starts), hip.upload(q)
+            dev.c.prompt(at, at, 6, 0.125, hip.upload(np.int32(starts)), len(q), ws, size, dtype=dtype)
+            hip.sync()
+            assert np.array_equal(hip.get(at, q.shape, q.dtype), want)
+        q, _ = queries(rng, dtype, 2, 6, 64)
+        want, at = dev.attend(q, 0.125, dtype), hip.upload(q)
+        dev.c.attend(at, at, 6, 0.125, ws, size, dtype=dtype)
+        hip.sync()
+        assert np.array_equal(hip.get(at, q.shape, q.dtype), want)
+
+
+def test_two_graphs_of_one_cache_and_workspace(hip):
+    """A step of single rows and one of prompts, captured apart, replayed in turn with eager work in between."""
+    rng = np.random.default_rng(41)
+    S, H, heads, d, T = 3, 1, 4, 64, 150
+    dev, ref = both(hip, S, H, d, 32, 64, 128, dtype=F16)
+    new, starts, slots = (hip.upload(np.zeros(n, np.int32)) for n in (S, S + 1, T))
+    rows, q, out = (hip.upload(np.zeros((T, n, d), np.uint16)) for n in (H, heads, heads))
+    ws, size = dev.workspace(heads, T)
+    stream = hip.stream()
+
+    def calls(single):
+        dev.c.plan(new, T, starts, slots, stream=stream)
+        dev.c.append(rows, rows, slots, T, stream=stream)
+        if single:
+            dev.c.attend(q, out, heads, 0.125, ws, size, starts=starts, tokens=T, stream=stream)
+        else:
+            dev.c.prompt(q, out, heads, 0.125, starts, T, ws, size, stream=stream)
+
+    graphs = [hip.capture(stream, lambda: calls(single)) for single in (False, True)]
+    for want in ([100, 1, 40], [1, 1, 1], [1, 0, 1], [20, 60, 0], [1, 1, 1], [0, 1, 1], [50, 50, 50]):
+        single = max(want) == 1
+        kk = pu.to_bits(normal(rng, T, H, d), F16)
+        qq, x = queries(rng, F16, T, heads, d)
+        hip.put(new, np.array(want, np.int32)), hip.put(rows, kk), hip.put(q, qq)
+        hip.put(out, np.full((T, heads, d), 0x4321, np.uint16))
+        hip.sync()
+        hip.launch(graphs[single], stream)
+        hip.sync()
+        at, sl, _ = ref.plan(want, T)
+        ref.append(kk, kk, sl, F16)
+        pu.assert_planned(dev, ref)
+        pu.check(hip.get(out, (T, heads, d), np.uint16), ref.attend(x, at, 0.125, F16), F16)
+        assert dev.attend(qq[:3], 0.125, F16).size  # eager work on the default stream in between
+
+
+def test_lengths_are_not_read_under_capture(hip):
+    dev, _ = both(hip, 1, 1, 64, 32, 2, 2)
+    stream = hip.stream()
+    with pytest.raises(moert.MoertError) as e:
+        hip.capture(stream, lambda: dev.c.lengths(stream=stream))
+    assert "captured" in str(e.value)
+
+
+def test_the_most_sequences_and_the_longest(hip):
+    """65535 sequences in one plan; one sequence of 2^20 rows."""
+    rng = np.random.default_rng(43)
+    dev, ref = both(hip, 65535, 1, 64, 32, 50000, 3)
+    for new in (rng.choice([0, 0, 1, 33], 65535), rng.choice([-1, 0, 1, 40], 65535)):
+        tokens = int(np.maximum(new, 0).sum()) + 5
+        want = ref.plan(new, tokens)
+        got, _ = dev.plan(new, tokens)
+        assert all(np.array_equal(a, b) for a, b in zip(got, want))
+        pu.assert_planned(dev, ref)
+    dev, ref = both(hip, 2, 1, 64, 256, 5000, 4096)
+    for new in ([2 ** 20, 5], [1, 1], [-1, 0]):
+        tokens = max(0, new[0]) + max(0, new[1])
+        want = ref.plan(new, tokens)
+        got, _ = dev.plan(new, tokens)
+        assert all(np.array_equal(a, b) for a, b in zip(got, want))
+        pu.assert_planned(dev, ref)
