@@ -9,7 +9,7 @@ PgArgs args(const PagesDev& c, int heads, float scale, KvRows q, KvRows out, con
             int most) {
   PgArgs a{};
   a.c = c, a.q = q, a.out = out, a.starts = starts;
-  a.tokens = tokens, a.heads = heads, a.g = heads / c.kvh;
+  a.tokens = tokens, a.g = heads / c.kvh;
   a.least = least, a.most = most;
   a.vec = wide_rows(q) | wide_rows(out) << 1;
   a.kf = frexpf(__builtin_fabsf(scale), &a.ke) * kPgLog2e;
@@ -86,8 +86,7 @@ hipError_t launch_pages_attend(hipStream_t s, const PagesDev& c, int heads, floa
 }
 
 hipError_t launch_pages_prompt(hipStream_t s, const PagesDev& c, int heads, float scale, KvRows q, KvRows out,
-                               const int* starts, int tokens, int least, void* ws,
-                               size_t ws_bytes) {
+                               const int* starts, int tokens, int least, void* ws, size_t ws_bytes) {
   PgArgs a = args(c, heads, scale, q, out, starts, tokens, least, 1 << 30);
   const int width = few_rows(a) ? 16 : 128;
   a.tiles = pg_tiles(a, width);

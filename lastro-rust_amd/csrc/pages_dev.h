@@ -72,7 +72,7 @@ struct PgArgs {
   PagesDev c;
   KvRows q, out;
   const int* starts;
-  int tokens, heads, g, splits, tiles;
+  int tokens, g, splits, tiles;  // g: query heads to a KV head
   int least, most;  // sequences of so many rows are attended
   int vec;          // bit 0: q can be loaded 16 bytes at a time, bit 1: out can be stored so
   float kf;         // |scale| log2 e, less 2^ke
@@ -113,10 +113,10 @@ __device__ __forceinline__ uint4 pg_query16(const PgArgs& a, long long at) {
   return make_uint4(w[0] ^ flip, w[1] ^ flip, w[2] ^ flip, w[3] ^ flip);
 }
 
-// N KB of memory to LDS, 16 bytes of each lane at a time, without a way through registers; `src` and `dst` (a place in LDS)
+// N KB (a multiple of 4) of memory to LDS, 16 bytes of each lane at a time, without a way through registers; `src` and `dst` (a place in LDS)
 // are the wave's, `lane` 16 times the lane. The instruction's offset counts on both sides. Not by the builtin: the
 // compiler cannot tell the buffer that is filled from the one being read, and would wait for the copy before each read.
-// Whoever reads them waits by pg_wait_copies first: for all but the last N copies and loads of the wave (loads of the
+// Whoever reads them waits by pg_wait_copies<M> first: for all but the last M copies and loads of the wave (loads of the
 // compiler's among them only make it wait for more). STREAM: with the non-temporal hint.
 template <int N, bool STREAM>
 __device__ __forceinline__ void pg_copy_to_lds(const uint8_t* src, uint32_t lane, uint32_t dst) {
@@ -124,19 +124,14 @@ __device__ __forceinline__ void pg_copy_to_lds(const uint8_t* src, uint32_t lane
     pg_copy_to_lds<4, STREAM>(src, lane, dst);
     pg_copy_to_lds<N - 4, STREAM>(src + 4096, lane, dst + 4096);
   } else {
-    static_assert(N == 2 || N == 4, "");
+    static_assert(N == 4, "");
     dst = __builtin_amdgcn_readfirstlane(dst);
 #define PG_COPY(HINT)                                                                                        \
-  if constexpr (N == 4)                                                                                      \
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" HINT                      \
-                 "\n\tglobal_load_lds_dwordx4 %1, %2 offset:%3" HINT                                        \
-                 "\n\tglobal_load_lds_dwordx4 %1, %2 offset:%4" HINT                                        \
-                 "\n\tglobal_load_lds_dwordx4 %1, %2 offset:%5" HINT                                        \
-                 : : "s"(dst), "v"(lane), "s"(src), "n"(1 * 1024), "n"(2 * 1024), "n"(3 * 1024) : "memory", "m0"); \
-  else                                                                                                       \
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" HINT                      \
-                 "\n\tglobal_load_lds_dwordx4 %1, %2 offset:%3" HINT                                        \
-                 : : "s"(dst), "v"(lane), "s"(src), "n"(1 * 1024) : "memory", "m0");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" HINT                        \
+               "\n\tglobal_load_lds_dwordx4 %1, %2 offset:%3" HINT                                          \
+               "\n\tglobal_load_lds_dwordx4 %1, %2 offset:%4" HINT                                          \
+               "\n\tglobal_load_lds_dwordx4 %1, %2 offset:%5" HINT                                          \
+               : : "s"(dst), "v"(lane), "s"(src), "n"(1 * 1024), "n"(2 * 1024), "n"(3 * 1024) : "memory", "m0");
     if constexpr (STREAM) {
       PG_COPY(" nt")
     } else {
