@@ -497,8 +497,9 @@ int moert_kv8_lengths(const moert_kv8* c, int seq0, int n_seqs, int* lengths, vo
  *          last plan's first row (-1: that plan has refused the sequence), 0
  *   free   i32 [pages + 1]  how many pages are free, and which; the last of them is given first
  * moert_pages_clear makes them an empty cache. Lengths are on the device, so that a captured graph of these calls can be
- * replayed. Pages that several sequences share may be put into the table by the caller; a plan knows nothing of it and
- * gives them back with each. Kernels keep to the buffers whatever table, state, free, starts and slots hold.
+ * replayed. The caller may put pages that several sequences share into the table; a plan knows nothing of it and gives
+ * them back with each, so they have to be taken out of `free` again before the next one. Kernels keep to the buffers
+ * whatever table, state, free, starts and slots hold.
  *
  * Rows are of the cache's type, or f32 (rounded to nearest, ties to even) for a cache in fp16. A row of K or V that is
  * not finite in the cache's type makes NaN of every output that sees it, and of no other. Memory behind a sequence's
@@ -540,8 +541,8 @@ int moert_pages_append(const moert_pages* c, const moert_rows* k, const moert_ro
  * rows (0: none). Nothing in it has to be kept or cleared between calls. */
 int moert_pages_workspace(const moert_pages* c, int heads, int tokens, size_t* bytes);
 
-/* Attention of one new position of every sequence over all rows of its own, its new one among them (appended before).
- * Row starts[s] of q and out is that of sequence s where starts_dev gives it exactly one; the others are left out, and
+/* Attention of one new position of every sequence over all rows of its own, its new one among them (appended before). q
+ * and out have `tokens` rows. Row starts[s] of q and out is that of sequence s where starts_dev gives it exactly one; the others are left out, and
  * their rows of `out` as they were. Without starts (NULL) row s is, and tokens = seqs. Query head h reads KV head
  * h / (heads / kv_heads). out = sum_t p_t v_t, p = softmax(scale * q . k); a position that sees no row gets 0, a query
  * row that is not finite NaN. q and out are of one type, seq_stride is not used. Scores, weights and sums are f32, a
@@ -554,13 +555,14 @@ int moert_pages_attend(const moert_pages* c, int heads, float scale, const moert
 
 /* Attention of the new rows of every sequence that has at least `least` (>= 1) of them, packed as starts_dev says, each
  * over its own row and those before it: row i of n in a sequence of len rows sees the first len - n + 1 + i. As
- * moert_pages_attend otherwise, but 16-bit rows' weights are rounded once to the cache's type. The rows of the other
+ * moert_pages_attend otherwise, but the weights of 16-bit rows may be rounded once to the cache's type: which kernel runs,
+ * and so the last bits, goes by tokens, seqs, heads and max_pages, not by what the batch holds. The rows of the other
  * sequences, and those behind the last, stay as they were in `out`. ws: moert_pages_workspace bytes of `tokens`. */
 int moert_pages_prompt(const moert_pages* c, int heads, float scale, const moert_rows* q, const moert_rows* out,
                        const int* starts_dev, int tokens, int least, void* ws_dev, size_t ws_bytes, void* stream);
 
 /* Lengths of the sequences, once the stream has come to this call (synchronises it; not under capture). MOERT_E_FULL,
- * with the lengths, where rows were refused since a sequence began. */
+ * with the lengths, where rows were refused since a sequence began, whether a later plan took them or not. */
 int moert_pages_lengths(const moert_pages* c, int seq0, int n_seqs, int* lengths, void* stream);
 
 /* Achievable HBM bandwidth reference: mean microseconds of one device-to-device streaming copy of `bytes`
