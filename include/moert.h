@@ -557,7 +557,8 @@ int moert_pages_attend(const moert_pages* c, int heads, float scale, const moert
  * over its own row and those before it: row i of n in a sequence of len rows sees the first len - n + 1 + i. As
  * moert_pages_attend otherwise, but the weights of 16-bit rows may be rounded once to the cache's type: which kernel runs,
  * and so the last bits, goes by tokens, seqs, heads and max_pages, not by what the batch holds. The rows of the other
- * sequences, and those behind the last, stay as they were in `out`. ws: moert_pages_workspace bytes of `tokens`. */
+ * sequences, and those behind the last, stay as they were in `out`. Fastest where the batch's longest sequences come
+ * first. ws: moert_pages_workspace bytes of `tokens`. */
 int moert_pages_prompt(const moert_pages* c, int heads, float scale, const moert_rows* q, const moert_rows* out,
                        const int* starts_dev, int tokens, int least, void* ws_dev, size_t ws_bytes, void* stream);
 

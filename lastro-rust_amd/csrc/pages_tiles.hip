@@ -44,9 +44,8 @@ __global__ __launch_bounds__(kWaves * 64, (Shape<D, T>::kPerSimd)) void k_pages_
   __shared__ __align__(16) uint8_t lds[NB][kStage][2][kBytes];
   const PagesDev& c = a.c;
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 31, G = lane >> 5;
-  // the tiles of a KV head run on one XCD (workgroups go round them in turn) where there are eight of them, the last ones
-  // of a sequence, which see the most, first
-  const int id = blockIdx.x, h = id % c.kvh, split = id / c.kvh % a.splits, y = a.tiles - 1 - id / c.kvh / a.splits;
+  // the tiles of a KV head run on one XCD (workgroups go round them in turn) where there are eight of them
+  const int id = blockIdx.x, h = id % c.kvh, split = id / c.kvh % a.splits, y = id / c.kvh / a.splits;
   PgTile t;
   if (!pg_tile(a, y, W, &t)) return;
   const int row1 = min(t.row0 + W, t.rows);

@@ -28,8 +28,8 @@ def tile(starts, tokens, g, y, w, seqs):
     s = find(starts, tokens, g, y, w, seqs)
     lo = min(max(starts[s], 0), tokens)
     n = min(max(starts[s + 1], lo), tokens) - lo
-    row0 = (y - first_tile(starts, tokens, g, s, w)) * w
-    return (s, lo, row0, n * g) if n >= 1 and 0 <= row0 < n * g else None
+    at = -(-n * g // w) - 1 - (y - first_tile(starts, tokens, g, s, w))  # the last ones first
+    return (s, lo, at * w, n * g) if n >= 1 and 0 <= at < -(-n * g // w) else None
 
 
 def tiles(tokens, g, w, seqs):
