@@ -7,7 +7,8 @@
 //   S = K Q^T    MFMA 16x16x32, rows = positions, columns = rows of the tile. Row i of product x is position
 //                16 (i / 8) + 8 x + i % 8, so that a lane of group G = lane / 16 gets the 8 positions that lie side by
 //                side in V: 16 (G / 2) + 4 (G % 2) + 0 .. 3, and 8 on.
-//   softmax      p = 2^(S f - M), f = scale log2 e; M, the running maximum less 7, moves only for weights above 2^15.
+//   softmax      p = 2^(S f - M), f = scale log2 e; M, the running maximum less 7, moves only for weights above 2^15 (or, where
+//                scores are far from 0, above 2^7).
 //   O += V^T P^T MFMA 16x16x32, rows = elements; p, as two numbers of the cache's type, never leaves its lane.
 // A wave's blocks go to its own ring in LDS, one being worked on while the next is on its way; nobody waits for another
 // wave. (Straight into registers, where the compiler kept one in flight, 131000 positions of 8 KV heads of 64 took 87 us for
@@ -129,7 +130,8 @@ __global__ __launch_bounds__(kWaves * 64, D == 64 ? 2 : 1) void k_pages_cols(PgA
     float mx = none;
 #pragma unroll
     for (int z = 0; z < 8; z++) mx = __builtin_fmaxf(mx, S[z / 4][z % 4]);
-    if (__any(__builtin_fmaf(mx, f, -M) > kPgSlack)) {
+    // Far from 0 the maximum moves for any score above it: there M is rounded by more than the slack leaves.
+    if (__any(far ? mx > Sm : __builtin_fmaf(mx, f, -M) > kPgSlack)) {
       const float m = __builtin_fmaxf(Sm, max_stage<32>(max_stage<16>(mx)));
       const float to = __builtin_fmaxf(__builtin_fmaf(m, f, -kPgShift), kPgNone);  // finite where nothing is seen yet
       far |= __any(__builtin_fabsf(to) > kPgFar && m > kPgNone);

@@ -1,0 +1,54 @@
+"""Attention over the paged K/V cache where its scores are hardest: large ones a few steps of f32 apart, factors beyond
+f32's exponents, weights whose rounding shows. Bounds follow from the roundings that include/moert.h states."""
+import numpy as np
+import pytest
+
+import pages_util as pu
+from pages_util import BF16, F16, F32
+from test_gpu_pages import both_ways, hip, normal, one_sequence  # noqa: F401 (hip: a fixture)
+
+pytestmark = pytest.mark.gpu
+
+TWO = {F32: 2.0 ** -21, F16: 2.0 ** -21, BF16: 2.0 ** -15}  # weights as two numbers of the cache's type, and their sum
+
+
+def weight_error(dtype, m):
+    """Of a weight, relative: as two numbers (one position), or rounded once and its sum with it (prompts)."""
+    return TWO[dtype] if m == 1 or dtype == F32 else 2 * pu.HALF[dtype]
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("first", [0, 200])
+def test_large_scores_a_few_steps_apart(hip, dtype, d, sign, first):  # noqa: F811
+    """Four rows of about 2^24 as sums of products, 0 to 9 steps of f32 apart, in blocks that one wave takes one after the
+    other, times factors that make scores of 2^16 to 2^44 and of 10^35 of them, many of them where one step is about what
+    moves a maximum; the others are far below. Their differences are exact, and so the weights differ by little more than
+    their roundings: of the factor and the exponent, 2^-22 of an exponent below 32 (a smaller weight is below 2^-24), of
+    exp2, of sums, and of what the second product takes. From row 200 on the prompts' waves have been through stages of
+    small scores before."""
+    rng = np.random.default_rng(51)
+    rows, n, heads = first + 3 * 128 + 40, 7, 4
+    at = first + 128 * np.arange(4)
+    v = normal(rng, rows, 1, d)
+    few = [m * 2.0 ** e for e in range(-8, 20) for m in (1.0, 1.37)] + [1e27, 1.1e28]
+    many = [(1 + m / 64) * 2.0 ** e for e in range(9) for m in range(64)]
+    for step, order, scales in ((1, (0, 1, 2, 3), many), (3, (0, 1, 2, 3), few), (1, (1, 0, 3, 2), few)):
+        q, k = np.zeros((n, heads, d), np.float32), np.zeros((rows, 1, d), np.float32)
+        q[..., 0], q[..., 1] = sign * 4080.0, step
+        k[:, 0, 0] = 0.0 if sign > 0 else 4096.0
+        k[at, 0, 0], k[at, 0, 1] = 4080.0, order
+        b = pu.to_bits(q, dtype)
+        dev, ref = one_sequence(hip, dtype, k, v)
+        x = ref.kv(0, 0, rows)[1][at]
+        for scale in np.float32(scales).tolist():
+            s = scale * step * np.array(order, np.float64)
+            p = np.exp(s - s.max())
+            p /= p.sum()
+            want = p @ x
+            for m, out in both_ways(dev, b, scale, dtype):
+                off = (2.0 ** -16 + weight_error(dtype, m)) * (p @ np.abs(x)) + 2.0 ** -20 * np.abs(x).max() + \
+                    pu.HALF[dtype] * np.abs(want)
+                err = np.abs(pu.from_bits(out, dtype) - want)
+                assert (err <= off).all(), (scale, step, order, m, (err / off).max())
