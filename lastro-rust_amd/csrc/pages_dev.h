@@ -170,11 +170,11 @@ __device__ __forceinline__ void pg_split(const float* x, int e, uint4* hi, uint4
   *hi = make_uint4(h[0], h[1], h[2], h[3]);
   *lo = make_uint4(l[0], l[1], l[2], l[3]);
 }
-// What a sum of products is multiplied by. Never 0: what is masked has to stay -inf. Nor infinite, where it leaves f32
-// without the scores (of keys that are small): sums that differ do so by 2^-58 or more there, and 2^127 of that is all the
-// weight or none, as more of it would be.
+// What a sum of products is multiplied by. Never 0: what is masked has to stay -inf, and f32's smallest number, 2^-149, of a
+// sum below 10^38 is no score. Nor infinite, where it leaves f32 without the scores (of keys that are small): sums that differ
+// do so by 2^-58 or more there, and 2^127 of that is all the weight or none, as more of it would be.
 __device__ __forceinline__ float pg_factor(const PgArgs& a, int qe) {
-  return __builtin_fminf(__builtin_fmaxf(__builtin_amdgcn_ldexpf(a.kf, a.ke + qe), 0x1p-126f), 0x1p127f);
+  return __builtin_fminf(__builtin_fmaxf(__builtin_amdgcn_ldexpf(a.kf, a.ke + qe), 0x1p-149f), 0x1p127f);
 }
 
 // An output is a mean of fp16 values: what roundings bring beyond the largest of them is cut.

@@ -52,3 +52,21 @@ def test_large_scores_a_few_steps_apart(hip, dtype, d, sign, first):  # noqa: F8
                     pu.HALF[dtype] * np.abs(want)
                 err = np.abs(pu.from_bits(out, dtype) - want)
                 assert (err <= off).all(), (scale, step, order, m, (err / off).max())
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("scale", [0.0, 1e-45, 1e-40, -1e-39, 3e-39, -1e-38])
+def test_scales_without_a_normal_factor(hip, dtype, d, scale):  # noqa: F811
+    """Scales of 0 and of f32's smallest, beside the largest products that the type lets through (bf16: of 10^38): the
+    products of scale 0 all weigh the same."""
+    rng = np.random.default_rng(53)
+    rows, n = 333, 7
+    big = {F32: (1e38 / 60000.0 / d, 60000.0), F16: (60000.0, 60000.0), BF16: (2.0 ** 60, 1e38 / 2.0 ** 60 / d)}[dtype]
+    q = np.full((n, 4, d), big[0], np.float32)
+    k = (rng.choice([-1.0, -0.5, 0.0, 0.5, 1.0], (rows, 1, 1)) * big[1] * 0.99 * np.ones(d)).astype(np.float32)
+    dev, ref = one_sequence(hip, dtype, k, normal(rng, rows, 1, d))
+    b = pu.to_bits(q, dtype)
+    scale = float(np.float32(scale))
+    for m, out in both_ways(dev, b, scale, dtype):
+        pu.check(out, ref.attend(pu.from_bits(b[-m:], dtype), [0, m], scale, dtype), dtype)
