@@ -5,7 +5,7 @@ import pytest
 
 import pages_util as pu
 from pages_util import BF16, F16, F32
-from test_gpu_pages import both_ways, hip, normal, one_sequence  # noqa: F401 (hip: a fixture)
+from test_gpu_pages import both_ways, cache_type, hip, normal, one_sequence  # noqa: F401 (hip: a fixture)
 
 pytestmark = pytest.mark.gpu
 
@@ -70,3 +70,47 @@ def test_scales_without_a_normal_factor(hip, dtype, d, scale):  # noqa: F811
     scale = float(np.float32(scale))
     for m, out in both_ways(dev, b, scale, dtype):
         pu.check(out, ref.attend(pu.from_bits(b[-m:], dtype), [0, m], scale, dtype), dtype)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("max_pages", [7, 256])
+def test_one_positions_weights_are_two_numbers(hip, dtype, d, max_pages):  # noqa: F811
+    """Half of the rows weigh 1, half exp(-s), s of 1/16 to 4; their V cancel for one element of each head, so that an
+    output's own rounding does not hide a weight's, which has one sign in all rows. Scores are exact; the factor, the
+    exponent, exp2 and sums bring 2^-19 at most (of exponents below 13 their f32 roundings, 2^-20)."""
+    rows, heads = 400, 64
+    s = (1 + np.arange(heads)) / 16
+    k, v = np.zeros((rows, 1, d), np.float32), np.ones((rows, 1, d), np.float32)
+    k[1::2, 0, 0] = -1.0
+    cancel = pu.from_bits(pu.to_bits(np.exp(s[np.arange(d) % heads]), cache_type(dtype)), cache_type(dtype))
+    v[1::2, 0] = -cancel
+    dev, ref = one_sequence(hip, dtype, k, v, max_pages)
+    q = np.zeros((1, heads, d), np.float32)
+    q[..., 0] = s
+    w = np.exp(-s)[:, None]
+    want = (1 - w * cancel) / (1 + w)
+    size = (1 + w * cancel) / (1 + w)
+    off = (2.0 ** -19 + TWO[dtype]) * size + pu.HALF[dtype] * np.abs(want) + (2.0 ** -24 if dtype == F16 else 0.0)
+    once = pu.from_bits(pu.to_bits(w, cache_type(dtype)), cache_type(dtype))
+    assert (np.abs((1 - once * cancel) / (1 + w) - want) > 4 * off).any()  # weights rounded once would show
+    err = np.abs(pu.from_bits(dev.attend(pu.to_bits(q, dtype), 1.0, dtype), dtype)[0] - want)
+    assert (err <= off).all(), (err / off).max()
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("d", [64, 128])
+def test_many_small_weights(hip, dtype, d):  # noqa: F811
+    """20000 rows of 2^-18 to 2^-24 of the largest weight, as 16-bit numbers below fp16's normal ones: all V are 1, and so is
+    the output, as long as sums and products hold the same weights. What a weight below fp16's steps (2^-31 of the largest)
+    loses is 2^-17 of the output at most, in one of the two."""
+    rows, n = 20000, 7
+    k = np.zeros((rows, 1, d), np.float32)
+    k[1:, 0, 0] = -1.0
+    dev, ref = one_sequence(hip, dtype, k, np.ones((rows, 1, d)))
+    for power in (18.0, 20.5, 21.25, 22.0, 24.0):
+        q = np.zeros((n, 4, d), np.float32)
+        q[..., 0] = power
+        for m, out in both_ways(dev, pu.to_bits(q, dtype), float(np.float32(np.log(2))), dtype):
+            err = np.abs(pu.from_bits(out, dtype) - 1.0)
+            assert (err <= pu.HALF[dtype] + 2.0 ** -16).all(), (power, m, err.max())
