@@ -114,3 +114,30 @@ def test_many_small_weights(hip, dtype, d):  # noqa: F811
         for m, out in both_ways(dev, pu.to_bits(q, dtype), float(np.float32(np.log(2))), dtype):
             err = np.abs(pu.from_bits(out, dtype) - 1.0)
             assert (err <= pu.HALF[dtype] + 2.0 ** -16).all(), (power, m, err.max())
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("kind", ["subnormal", "large", "falling", "rising", "equal"])
+def test_extremes_of_wide_heads(hip, dtype, kind):  # noqa: F811
+    """Heads of 128: values at the ends of their types, scores that fall or rise all along by up to 900, and equal ones of
+    10^9, in caches that are split and not."""
+    rng = np.random.default_rng(55)
+    rows, n, d = 700, 7, 128
+    k, v, q, scale = normal(rng, rows, 1, d), normal(rng, rows, 1, d), normal(rng, n, 4, d), 0.0625
+    if kind == "subnormal":
+        k, v, q, scale = k * 3e-6, v * 3e-6, q * 3e-6, 1e10
+    elif kind == "large":
+        k, v = np.clip(k, -1, 1) * 60000, np.clip(v * 4, -1, 1) * 65504
+        q, scale = q * 1e3, 1e-8
+    elif kind in ("falling", "rising"):
+        k = np.broadcast_to(np.linspace(0, 7, rows)[:, None, None], k.shape)
+        k = k[::-1] if kind == "falling" else k
+        q, scale = np.ones_like(q), 1.0
+    else:
+        k, q, scale = np.full_like(k, 300.0), np.full_like(q, 500.0), 52.0
+    for max_pages in (11, 256):
+        dev, ref = one_sequence(hip, dtype, k, v, max_pages)
+        b = pu.to_bits(q, dtype)
+        for m, out in both_ways(dev, b, scale, dtype):
+            want = ref.attend(pu.from_bits(b[-m:], dtype), [0, m], 0.0 if kind == "equal" else scale, dtype)
+            pu.check(out, want, dtype)
