@@ -499,7 +499,9 @@ int moert_kv8_lengths(const moert_kv8* c, int seq0, int n_seqs, int* lengths, vo
  * moert_pages_clear makes them an empty cache. Lengths are on the device, so that a captured graph of these calls can be
  * replayed. The caller may put pages that several sequences share into the table; a plan knows nothing of it and gives
  * them back with each, so they have to be taken out of `free` again before the next one. Kernels keep to the buffers
- * whatever table, state, free, starts and slots hold.
+ * whatever table, state, free, starts and slots hold. An attention may be called of some sequences that follow each
+ * other: seqs is their number, table_dev, state_dev and the call's starts_dev are at the first of them, tokens stays the
+ * batch's, the workspace is that of these sequences.
  *
  * Rows are of the cache's type, or f32 (rounded to nearest, ties to even) for a cache in fp16. A row of K or V that is
  * not finite in the cache's type makes NaN of every output that sees it, and of no other. Memory behind a sequence's
@@ -507,10 +509,10 @@ int moert_kv8_lengths(const moert_kv8* c, int seq0, int n_seqs, int* lengths, vo
  *
  * Limits: head_dim 64 or 128; page 32, 64, 128 or 256; max_pages * page at most 2^20, pages * page at most 2^30 and with
  * kv_heads 2^35; at most 65535 sequences, 256 KV heads, 2^20 KV heads and 2^30 table entries of all sequences, 2^24 rows
- * in a call, 64 query heads to a KV head, 2^24 query heads of all sequences and 2^27 of all rows of an attention. Calls
- * enqueue on `stream` (a hipStream_t of the buffers' device, NULL for its default stream), allocate nothing and do not
- * synchronise, except moert_pages_lengths. Calls on one cache are ordered by the caller (one stream, or events);
- * attentions may overlap, each with a workspace of its own.
+ * in a call, 2^27 KV heads of all rows of an append, 64 query heads to a KV head, 2^24 query heads of all sequences and
+ * 2^27 of all rows of an attention. Calls enqueue on `stream` (a hipStream_t of the buffers' device, NULL for its default
+ * stream), allocate nothing and do not synchronise, except moert_pages_lengths. Calls on one cache are ordered by the
+ * caller (one stream, or events); attentions may overlap, each with a workspace of its own.
  * ------------------------------------------------------------------------------------------------------- */
 enum { MOERT_PAGES_BLOCK = 32 };
 typedef struct {
@@ -527,8 +529,9 @@ int moert_pages_clear(const moert_pages* c, void* stream);
  * [starts[s], starts[s + 1]), slots_dev [tokens] the slot of each row, page * (positions of a page) + place in it, and
  * positions_dev [tokens], unless it is NULL, its position in the sequence; both are -1 behind the last row. `tokens` is
  * the room for rows. The sequences get their pages in order. One whose rows do not fit into `tokens` or max_pages, or
- * that lacks more pages than are left, stays as it is, and so do those behind it that lack any: their rows have slot
- * -1, their positions see nothing until a plan takes them again, and moert_pages_lengths reports them. */
+ * that lacks more pages than are left, stays as it is, and behind one that lacks too many so does every one that lacks
+ * any: their rows have slot -1, their positions see nothing until a plan takes them again, and moert_pages_lengths
+ * reports them. */
 int moert_pages_plan(const moert_pages* c, const int* new_dev, int tokens, int* starts_dev, int* slots_dev,
                      int* positions_dev, void* stream);
 
@@ -542,13 +545,15 @@ int moert_pages_append(const moert_pages* c, const moert_rows* k, const moert_ro
 int moert_pages_workspace(const moert_pages* c, int heads, int tokens, size_t* bytes);
 
 /* Attention of one new position of every sequence over all rows of its own, its new one among them (appended before). q
- * and out have `tokens` rows. Row starts[s] of q and out is that of sequence s where starts_dev gives it exactly one; the others are left out, and
- * their rows of `out` as they were. Without starts (NULL) row s is, and tokens = seqs. Query head h reads KV head
- * h / (heads / kv_heads). out = sum_t p_t v_t, p = softmax(scale * q . k); a position that sees no row gets 0, a query
- * row that is not finite NaN. q and out are of one type, seq_stride is not used. Scores, weights and sums are f32, a
- * weight as good as its score, an f32; outputs are finite as long as head_dim * max|q| * max|k|, and |scale| times
- * that, are below 10^38, and max|v| below 2^90. The weights enter the second product as the sum of two numbers of the
- * cache's type, off by 2^-22 (bf16 2^-16) of themselves or 2^-30 of the row's largest. out may be q itself, with the
+ * and out have `tokens` rows. Row starts[s] of q and out is that of sequence s where starts_dev gives it exactly one; the
+ * others are left out, and their rows of `out` as they were. Without starts (NULL) row s is, and tokens = seqs. Query
+ * head h reads KV head h / (heads / kv_heads). out = sum_t p_t v_t, p = softmax(scale * q . k); a position that sees no
+ * row gets 0, a query row that is not finite NaN. q and out are of one type, seq_stride is not used. Scores, weights and
+ * sums are f32, a weight as good as its score, an f32; outputs are finite as long as head_dim * max|q| * max|k|, and
+ * |scale| times that, are below 10^38, and max|v| below 2^90. f32 queries enter the first product as the sum of two fp16
+ * numbers and a power of two of the row's, off by 2^-22 of an element or 2^-34 of the row's largest; the weights enter
+ * the second as the sum of two numbers of the cache's type, off by 2^-22 (bf16 2^-16) of themselves or 2^-30 of the
+ * row's largest. More than 16 query heads to a KV head read the cache once for each 16. out may be q itself, with the
  * same strides; otherwise they do not overlap. ws: moert_pages_workspace bytes (tokens 0), aligned to 16. */
 int moert_pages_attend(const moert_pages* c, int heads, float scale, const moert_rows* q, const moert_rows* out,
                        const int* starts_dev, int tokens, void* ws_dev, size_t ws_bytes, void* stream);
@@ -556,9 +561,10 @@ int moert_pages_attend(const moert_pages* c, int heads, float scale, const moert
 /* Attention of the new rows of every sequence that has at least `least` (>= 1) of them, packed as starts_dev says, each
  * over its own row and those before it: row i of n in a sequence of len rows sees the first len - n + 1 + i. As
  * moert_pages_attend otherwise, but the weights of 16-bit rows may be rounded once to the cache's type: which kernel runs,
- * and so the last bits, goes by tokens, seqs, heads and max_pages, not by what the batch holds. The rows of the other
- * sequences, and those behind the last, stay as they were in `out`. Fastest where the batch's longest sequences come
- * first. ws: moert_pages_workspace bytes of `tokens`. */
+ * and so the last bits, goes by tokens, seqs, heads and max_pages, not by what the batch holds. So a long prompt beside
+ * many short or idle sequences, or after a long text, runs as few rows do, slower than by itself; a caller who knows of
+ * it calls for its sequence alone (see above). The rows of the other sequences, and those behind the last, stay as they
+ * were in `out`. Fastest where the batch's longest sequences come first. ws: moert_pages_workspace bytes of `tokens`. */
 int moert_pages_prompt(const moert_pages* c, int heads, float scale, const moert_rows* q, const moert_rows* out,
                        const int* starts_dev, int tokens, int least, void* ws_dev, size_t ws_bytes, void* stream);
 

@@ -45,7 +45,12 @@ int tiles_splits(const PagesDev& c, long long units) {
 // Whether the tiles of 16 rows that the waves of a workgroup share do better than those of 128 rows that they split: up to
 // 48 rows of a sequence on average, of wide heads 32. (8 KV heads of 64, 48 rows: 4000 positions 11.4 us in the one, 14.1 in
 // the other, 32000 25.5 and 21.7, of eight sequences of 4000 17.5 and 23.4; of 128, 32 rows: 12.4 and 18.8, 33.5 and 30.5,
-// 25.5 and 30.3, but 44 rows of 64 sequences of 1000 59.3 and 42.5.)
+// 25.5 and 30.3, but 44 rows of 64 sequences of 1000 59.3 and 42.5.) The average is all that the host knows, and the rule
+// holds for what is like it: after long texts 128 rows would do better (the two figures at 32000), and where one sequence
+// has the rows and most have few or none, it runs as one of few rows does. (3 heads of 64 in fp16, 4 of 128 in bf16; the
+// sequence's rows in 128 and beside other sequences' single rows in 16: 300 rows beside 63 8.7 and 6.8 us, 12.1 and 14.8;
+// 900, 440 of wide heads, 16.1 and 18.9, 15.0 and 21.7; 300 after 16000 59 and 105, 113 and 337; 5000 beside 999 106 and
+// 280, 218 and 819.) A caller who knows of one calls for it alone.
 bool few_rows(const PgArgs& a) { return (long long)a.tokens * a.g <= (a.c.d == 64 ? 48ll : 32ll) * a.c.seqs; }
 
 size_t up(size_t x) { return (x + 255) / 256 * 256; }

@@ -113,8 +113,8 @@ __device__ __forceinline__ uint4 pg_query16(const PgArgs& a, long long at) {
   return make_uint4(w[0] ^ flip, w[1] ^ flip, w[2] ^ flip, w[3] ^ flip);
 }
 
-// N KB (a multiple of 4) of memory to LDS, 16 bytes of each lane at a time, without a way through registers; `src` and `dst` (a place in LDS)
-// are the wave's, `lane` 16 times the lane. The instruction's offset counts on both sides. Not by the builtin: the
+// N KB (a multiple of 4) of memory to LDS, 16 bytes of each lane at a time, without a way through registers; `src` and
+// `dst` (a place in LDS) are the wave's, `lane` 16 times the lane. The instruction's offset counts on both sides. Not by the builtin: the
 // compiler cannot tell the buffer that is filled from the one being read, and would wait for the copy before each read.
 // Whoever reads them waits by pg_wait_copies<M> first: for all but the last M copies and loads of the wave (loads of the
 // compiler's among them only make it wait for more). STREAM: with the non-temporal hint.
@@ -152,7 +152,7 @@ __device__ __forceinline__ void pg_wait_copies() {
 __device__ __forceinline__ void pg_wait_reads() { asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory"); }
 
 // f32 queries enter as two fp16: their row by a power of two to below 2^10, then what the first rounding leaves. So they
-// are off by 2^-22 of themselves. pg_split_exp: log2 of what the row has been divided by; m: its largest magnitude.
+// are off by 2^-22 of themselves, or by half of fp16's least step, 2^-34 of the row's largest. pg_split_exp: log2 of what the row has been divided by; m: its largest magnitude.
 __device__ __forceinline__ int pg_split_exp(float m) {
   return (m > 0.0f && m < __int_as_float(0x7f800000) ? __builtin_amdgcn_frexp_expf(m) : 0) - 10;
 }

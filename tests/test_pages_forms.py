@@ -23,3 +23,10 @@ def test_forms_take_their_kernels(launches, d):  # noqa: F811
 def test_every_kernel_of_an_attention_is_in_a_form():
     taken = {pf.kernel(k, d, dtype) for *_, kernels in pf.FORMS.values() for k in kernels for d in (64, 128) for dtype in pf.TYPES}
     assert len(taken) == 6 * (2 + 1 + 4)
+
+
+def test_a_part_of_the_sequences_takes_kernels_of_its_own(launches):  # noqa: F811
+    """A prompt of 900 rows beside 63 single rows: tiles of 16 rows in a call for all sequences, of 128 in one for its own."""
+    whole, part = (dict(call="prompt", cache=(seqs, 8, 64, 64, 500, 100), kw=dict(heads=24, tokens=963, least=2)) for seqs in (64, 1))
+    got = launches([whole, part])
+    assert "k_pages_cols" in got[0][1][0][0] and "k_pages_tiles" in got[1][1][0][0]
