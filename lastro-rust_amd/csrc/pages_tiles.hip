@@ -12,9 +12,9 @@
 // straight copies of 16 bytes a lane, past the registers, while those before them are worked on.
 //
 // What bounds it, measured on one MI355X: the chip's power, between the matrix cores and the vector unit. 16384 positions,
-// 8 KV heads of 64 with 3 query heads each, fp16, 825 GFLOP: 876 us, 941 TFLOP/s, at 1.77 GHz, the matrix cores busy in 45%
-// of the cycles and vector instructions issuing in 60% (a library product of 8192 x 8192 x 8192: 1070 TFLOP/s at 1.58 GHz,
-// 70% and 28%). A block of 32 x 32 scores is 8 MFMAs of 32 cycles beside 48 vector instructions, 16 of them exponentials at
+// 8 KV heads of 64 with 3 query heads each, fp16, 825 GFLOP: 876 us, 941 TFLOP/s (on another such device 936 us, 881
+// TFLOP/s), at 1.77 GHz, the matrix cores busy in 45% of the cycles and vector instructions issuing in 60% (a library
+// product of 8192 x 8192 x 8192: 1070 TFLOP/s at 1.58 GHz, 70% and 28%). A block of 32 x 32 scores is 8 MFMAs of 32 cycles beside 48 vector instructions, 16 of them exponentials at
 // half the rate, and 5 others. Measured on the way, same case: the maximum looked at in every block, through a second copy
 // of the accumulators, 1084; two blocks a stage without it 916; copies by one base 888; two running sums, not four, 870. Two
 // tiles of rows to a wave 956 for 934, priorities for the MFMAs or three stages in LDS within 1%.
