@@ -141,3 +141,28 @@ def test_extremes_of_wide_heads(hip, dtype, kind):  # noqa: F811
         for m, out in both_ways(dev, b, scale, dtype):
             want = ref.attend(pu.from_bits(b[-m:], dtype), [0, m], 0.0 if kind == "equal" else scale, dtype)
             pu.check(out, want, dtype)
+
+
+@pytest.mark.parametrize("power", [4, 8, 12, 16, 20])
+def test_small_elements_of_f32_queries(hip, power):  # noqa: F811
+    """All of a score comes from an element of 2^-power of its row's largest, which meets zeros: as two fp16 it is off by
+    2^-22 of itself, or by 2^-34 of the largest. A weight is off by the factor of its own score's and of the sum's; exp2,
+    the factor, exponents below 16 and sums bring 2^-18."""
+    rng = np.random.default_rng(57)
+    rows, n, d = 300, 7, 64
+    x = 1.37 * 2.0 ** -power
+    scale = float(np.float32(4.0 / (60000.0 * x)))
+    k = np.zeros((rows, 1, d), np.float32)
+    k[..., 1] = rng.uniform(-60000, 60000, (rows, 1))
+    dev, ref = one_sequence(hip, F32, k, normal(rng, rows, 1, d))
+    q = np.zeros((n, 4, d), np.float32)
+    q[..., 0], q[..., 1] = 1.0, x
+    off = 2 * scale * 60000.0 * (2.0 ** -22 * x + 2.0 ** -34) + 2.0 ** -18 + TWO[F32]
+    for m, out in both_ways(dev, q, scale, F32):
+        for i in range(m):
+            kk, vv = ref.kv(0, 0, rows - m + 1 + i)
+            s = scale * np.float64(np.float32(x)) * kk[:, 1]
+            p = np.exp(s - s.max())
+            p /= p.sum()
+            err = np.abs(out[i] - p @ vv)
+            assert (err <= off * (p @ np.abs(vv)) + 2.0 ** -24 * np.abs(vv).max()).all(), (m, i, err.max())
